@@ -44,6 +44,7 @@ typedef struct llambda_hip_moe_session llambda_hip_moe_session;
 typedef struct llambda_hip_llama_session llambda_hip_llama_session;
 typedef struct llambda_hip_sampler llambda_hip_sampler;
 typedef struct llambda_hip_gguf llambda_hip_gguf;
+typedef struct llambda_hip_ssm_session llambda_hip_ssm_session;
 
 /* ---- probe, versions, errors -------------------------------------- */
 
@@ -357,6 +358,105 @@ int llambda_hip_llama_session_read_kv(llambda_hip_llama_session* session, int64_
 
 /* Wait for `stream` (null = the session's stream). */
 int llambda_hip_llama_session_sync(llambda_hip_llama_session* session, void* stream);
+
+/* ---- Mamba-2 mixers ------------------------------------------------------- */
+
+/* One recurrent layer of a Nemotron-H model (tensors blk.N.<name>, host
+ * memory, copied at creation) between its projections ssm_in and ssm_out: the
+ * short causal convolution, the selective state space scan and the gated
+ * group norm.  A row of the input is a row of ssm_in's output,
+ *   [z: heads * head_dim | x: heads * head_dim | B: groups * state |
+ *    C: groups * state | dt: heads],
+ * a row of the output, heads * head_dim wide, is ssm_out's input.  Per token,
+ * with u = silu(conv(x | B | C)), dt = softplus(dt + ssm_dt), per head
+ *   s = exp(dt ssm_a) s + dt u_x u_B^T,   y = s u_C + ssm_d u_x,
+ * then v = y silu(z) and, per group of heads, v / sqrt(mean(v^2) + epsilon)
+ * times ssm_norm.  All fp32; logarithms of decays are summed in 64 bits. */
+typedef struct llambda_hip_ssm_desc {
+  int64_t heads;
+  int64_t head_dim;           /* a multiple of 16, 16 to 128 */
+  int64_t groups;             /* divides heads; at most 16384 channels each */
+  int64_t state;              /* 16, 32, 64, 128 or 256 */
+  int64_t conv_width;         /* taps, 2 to 4 */
+  const float* conv_weight;   /* ssm_conv1d.weight [channels][conv_width], oldest tap
+                                 first; channels = heads * head_dim + 2 * groups * state */
+  const float* conv_bias;     /* ssm_conv1d.bias [channels], NULL = zeros */
+  const float* dt_bias;       /* ssm_dt.bias [heads] */
+  const float* a;             /* ssm_a [heads], finite, not positive */
+  const float* d;             /* ssm_d [heads] */
+  const float* norm;          /* ssm_norm [heads * head_dim] */
+  float norm_epsilon;
+  int64_t slots;              /* sequences whose states the pool holds */
+  int64_t max_tokens;         /* most tokens of one call (sizes the workspace) */
+  int64_t max_sequences;      /* most sequences of one call */
+  /* The pool, in device memory (16-byte aligned): [slots][conv_width - 1]
+   * [channels], the last rows of x | B | C before the convolution, oldest
+   * first, and [slots][heads][head_dim][state].  Both NULL: the session
+   * allocates it, zeroed. */
+  float* conv_states;
+  float* ssm_states;
+} llambda_hip_ssm_desc;
+
+/* Upload a layer.  No counterpart in the reference's bridge: it is the
+ * per-layer hook for the recurrent layers of its Nemotron-H step function
+ * (llambda.lisp:5768-5825, 6020-6128). */
+int llambda_hip_ssm_session_create(const llambda_hip_ssm_desc* desc,
+                                   llambda_hip_ssm_session** result);
+void llambda_hip_ssm_session_destroy(llambda_hip_ssm_session* session);
+
+/* Elements of an input and an output row; 0 for null. */
+size_t llambda_hip_ssm_session_input_element_count(const llambda_hip_ssm_session* session);
+size_t llambda_hip_ssm_session_output_element_count(const llambda_hip_ssm_session* session);
+
+/* `tokens` rows of one sequence, host memory, synchronous: continues from the
+ * state in `slot` and leaves the new state there. */
+int llambda_hip_ssm_session_run(llambda_hip_ssm_session* session, int64_t slot,
+                                const float* input, size_t input_element_count, float* output,
+                                size_t output_element_count, size_t tokens);
+
+/* Device-resident form over several sequences; every pointer is device
+ * memory.  Rows [offsets[i], offsets[i + 1]) of `input` (`tokens` rows in all)
+ * are sequence i's; offsets[sequences + 1] ascends, a sequence may be empty,
+ * and rows that belong to none are left as they are in `output`.  Sequence i
+ * continues from the state in slot from_slots[i] (-1: a new sequence, zeros)
+ * and leaves its state in slot to_slots[i] (-1: nowhere); the two may be equal.
+ * Null lists mean slot i.  input and output do not overlap.
+ * What only the device can see is checked there, before anything is written:
+ * offsets that do not ascend within the call's tokens (nothing of the call is
+ * run), slots outside the pool, and a to-slot that another sequence of the
+ * call reads or writes (the sequence is not run: its rows and slots stay as
+ * they are).  llambda_hip_ssm_session_sync reports them.
+ * Enqueued on `stream` (null = the session's stream), not waited for, with no
+ * allocation.  The calls of a session share its workspace: each waits on the
+ * device for the one before, whatever stream it ran on.  Under stream capture
+ * no wait or record is made: the graph orders its own calls, and replays of
+ * graphs that hold calls of one session must not overlap. */
+int llambda_hip_ssm_session_run_device(llambda_hip_ssm_session* session, const float* input,
+                                       float* output, size_t tokens, const int32_t* offsets,
+                                       size_t sequences, const int32_t* from_slots,
+                                       const int32_t* to_slots, void* stream);
+
+/* One token of each sequence: row i of `input` is sequence i's next token.
+ * Slots, checks and stream as above; it uses no workspace, so steps need no
+ * order but that of the slots they share. */
+int llambda_hip_ssm_session_step_device(llambda_hip_ssm_session* session, const float* input,
+                                        float* output, size_t sequences,
+                                        const int32_t* from_slots, const int32_t* to_slots,
+                                        void* stream);
+
+/* Wait for `stream` (null = the session's stream) and report, once, any
+ * sequence that was refused on the device since the last report. */
+int llambda_hip_ssm_session_sync(llambda_hip_ssm_session* session, void* stream);
+
+/* Zero slot `slot`, or copy its state (conv [conv_width - 1][channels], ssm
+ * [heads][head_dim][state]) in or out; host memory, or device memory for write
+ * when on_device = 1.  Synchronous; calls on other streams that use the slot
+ * have to have ended. */
+int llambda_hip_ssm_session_reset(llambda_hip_ssm_session* session, int64_t slot);
+int llambda_hip_ssm_session_write_state(llambda_hip_ssm_session* session, int64_t slot,
+                                        const float* conv, const float* ssm, int on_device);
+int llambda_hip_ssm_session_read_state(llambda_hip_ssm_session* session, int64_t slot,
+                                       float* conv, float* ssm);
 
 /* ---- sampling ------------------------------------------------------------ */
 

@@ -28,6 +28,7 @@
 #include "moe.h"
 #include "sample.h"
 #include "sha256.h"
+#include "ssm.h"
 
 using namespace llhip;
 
@@ -1469,6 +1470,328 @@ int llambda_hip_llama_session_sync(llambda_hip_llama_session* s, void* stream) {
     if (!s) failf("llama sync: null session");
     HIPC(hipStreamSynchronize(stream ? static_cast<hipStream_t>(stream) : s->stream));
     HIPC(hipEventSynchronize(s->done));
+  });
+}
+
+}  // extern "C"
+
+// ----------------------------------------------------------- Mamba-2 mixers
+
+struct llambda_hip_ssm_session {
+  std::mutex run_mutex;
+  int device = 0;
+  hipStream_t stream = nullptr;
+  SsmLayerPlan plan{};
+  DevBuf weights, pool_conv, pool_ssm, error;
+  DevBuf sequences, segments, chunks, counts, bc, decay, seg_states, seg_decay;
+  DevBuf x, y, lists;  // device staging of the host-pointer runs; lists: offsets, slot
+  size_t staged_tokens = 0;
+  // recorded after every call that uses the workspace; the next one waits
+  hipEvent_t done = nullptr;
+  ~llambda_hip_ssm_session() {
+    if (done) (void)hipEventDestroy(done);
+    if (stream) (void)hipStreamDestroy(stream);
+  }
+  int64_t channels() const {
+    return (int64_t)plan.heads * plan.head_dim + 2 * (int64_t)plan.groups * plan.state;
+  }
+  size_t row() const { return (size_t)ssm_row(plan); }
+  size_t inner() const { return (size_t)plan.heads * plan.head_dim; }
+  size_t conv_elements() const { return (size_t)(plan.conv - 1) * channels(); }
+  size_t ssm_elements() const { return inner() * plan.state; }
+  void raise_error(hipStream_t s) {
+    int flag = 0;
+    HIPC(hipMemcpyAsync(&flag, plan.error, sizeof flag, hipMemcpyDeviceToHost, s));
+    HIPC(hipStreamSynchronize(s));
+    if (!flag) return;
+    HIPC(ssm_reset_error_launch(plan, s));
+    HIPC(hipStreamSynchronize(s));
+    failf("ssm: a call was refused on the device:%s%s%s",
+          flag & kSsmErrOffsets ? " offsets do not ascend within its tokens;" : "",
+          flag & kSsmErrSlot ? " a slot lies outside the pool;" : "",
+          flag & kSsmErrConflict ? " a slot is written by one sequence and used by another;" : "");
+  }
+};
+
+namespace {
+
+bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + nb && y < x + na;
+}
+
+void check_ssm_call(const llambda_hip_ssm_session* s, const char* what, const float* input,
+                    const float* output, size_t tokens, size_t sequences, const int32_t* from,
+                    const int32_t* to) {
+  const SsmLayerPlan& p = s->plan;
+  if (!input || !output) failf("%s: null input or output", what);
+  if (sequences == 0 || sequences > (size_t)p.max_sequences)
+    failf("%s: %zu sequences are not in 1..%d", what, sequences, p.max_sequences);
+  if (tokens == 0 || tokens > (size_t)p.max_tokens)
+    failf("%s: %zu tokens are not in 1..%d", what, tokens, p.max_tokens);
+  if ((!from || !to) && sequences > (size_t)p.slots)
+    failf("%s: %zu sequences without a slot list, but %d slots", what, sequences, p.slots);
+  if ((reinterpret_cast<uintptr_t>(input) | reinterpret_cast<uintptr_t>(output) |
+       reinterpret_cast<uintptr_t>(from) | reinterpret_cast<uintptr_t>(to)) & 3u)
+    failf("%s: pointers must be 4-byte aligned", what);
+  if (overlap(input, tokens * s->row() * sizeof(float), output, tokens * s->inner() * sizeof(float)))
+    failf("%s: input and output overlap", what);
+}
+
+void ssm_enqueue(llambda_hip_ssm_session* s, const SsmCall& c, hipStream_t st) {
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  HIPC(hipStreamIsCapturing(st, &capture));
+  const bool ordered = capture == hipStreamCaptureStatusNone;
+  if (ordered) HIPC(hipStreamWaitEvent(st, s->done, 0));
+  HIPC(ssm_run_launch(s->plan, c, st));
+  if (ordered) HIPC(hipEventRecord(s->done, st));
+}
+
+}  // namespace
+
+extern "C" {
+
+int llambda_hip_ssm_session_create(const llambda_hip_ssm_desc* d,
+                                   llambda_hip_ssm_session** result) {
+  return guarded([&] {
+    if (!result) failf("ssm_session_create: null result pointer");
+    *result = nullptr;
+    if (!d) failf("ssm_session_create: null description");
+    auto in = [&](int64_t v, int64_t lo, int64_t hi, const char* what) {
+      if (v < lo || v > hi)
+        failf("ssm_session_create: %s %lld is not in %lld..%lld", what, (long long)v, (long long)lo,
+              (long long)hi);
+    };
+    in(d->heads, 1, 4096, "heads");
+    in(d->head_dim, 16, kSsmMaxHeadDim, "head_dim");
+    if (d->head_dim % 16) failf("ssm_session_create: head_dim %lld is not a multiple of 16", (long long)d->head_dim);
+    in(d->groups, 1, d->heads, "groups");
+    if (d->heads % d->groups)
+      failf("ssm_session_create: %lld groups do not divide %lld heads", (long long)d->groups,
+            (long long)d->heads);
+    in(d->state, 16, kSsmMaxState, "state");
+    if (d->state & (d->state - 1)) failf("ssm_session_create: state %lld is not a power of two", (long long)d->state);
+    in(d->conv_width, 2, kSsmMaxConv, "conv_width");
+    in(d->heads / d->groups * d->head_dim, 1, kSsmMaxNormWidth, "channels of a norm group");
+    in(d->heads * d->head_dim * d->state, 1, 1 << 25, "state elements of a sequence");
+    in(d->slots, 1, 1 << 20, "slots");
+    in(d->max_tokens, 1, 1 << 20, "max_tokens");
+    in(d->max_sequences, 1, 65535, "max_sequences");
+    if (!d->conv_weight || !d->dt_bias || !d->a || !d->d || !d->norm)
+      failf("ssm_session_create: null weights");
+    if (!(d->norm_epsilon >= 0.f && std::isfinite(d->norm_epsilon)))
+      failf("ssm_session_create: norm_epsilon %g", (double)d->norm_epsilon);
+    for (int64_t h = 0; h < d->heads; ++h)
+      if (!(d->a[h] <= 0.f && std::isfinite(d->a[h])))
+        failf("ssm_session_create: ssm_a[%lld] is %g: it must be finite and not positive", (long long)h,
+              (double)d->a[h]);
+    if (!d->conv_states != !d->ssm_states) failf("ssm_session_create: one state pool without the other");
+    if ((reinterpret_cast<uintptr_t>(d->conv_states) | reinterpret_cast<uintptr_t>(d->ssm_states)) & 15u)
+      failf("ssm_session_create: state pools must be 16-byte aligned");
+    std::unique_ptr<llambda_hip_ssm_session> s(new llambda_hip_ssm_session());
+    s->device = current_device_checked();
+    SsmLayerPlan& p = s->plan;
+    p.heads = (int)d->heads;
+    p.head_dim = (int)d->head_dim;
+    p.groups = (int)d->groups;
+    p.state = (int)d->state;
+    p.conv = (int)d->conv_width;
+    p.slots = (int)d->slots;
+    p.max_tokens = (int)d->max_tokens;
+    p.max_sequences = (int)d->max_sequences;
+    p.epsilon = d->norm_epsilon;
+    HIPC(hipStreamCreateWithFlags(&s->stream, hipStreamNonBlocking));
+    HIPC(hipEventCreateWithFlags(&s->done, hipEventDisableTiming));
+    // the weights in one buffer; the taps transposed, so that neighbouring
+    // channels' taps are neighbours
+    const size_t C = (size_t)s->channels(), W = (size_t)p.conv, H = (size_t)p.heads, I = s->inner();
+    const size_t C4 = (C + 3) & ~(size_t)3, H4 = (H + 3) & ~(size_t)3;
+    std::vector<float> w(W * C4 + C4 + 3 * H4 + I, 0.f);
+    float* at = w.data();
+    for (size_t c = 0; c < C; ++c)
+      for (size_t k = 0; k < W; ++k) at[k * C + c] = d->conv_weight[c * W + k];
+    if (d->conv_bias) std::copy_n(d->conv_bias, C, at + W * C4);
+    std::copy_n(d->dt_bias, H, at + W * C4 + C4);
+    std::copy_n(d->a, H, at + W * C4 + C4 + H4);
+    std::copy_n(d->d, H, at + W * C4 + C4 + 2 * H4);
+    std::copy_n(d->norm, I, at + W * C4 + C4 + 3 * H4);
+    s->weights.alloc(w.size() * sizeof(float), "ssm weights");
+    HIPC(hipMemcpyAsync(s->weights.ptr, w.data(), w.size() * sizeof(float), hipMemcpyHostToDevice, s->stream));
+    const float* dw = s->weights.as<float>();
+    p.conv_weight = dw;
+    p.conv_bias = dw + W * C4;
+    p.dt_bias = p.conv_bias + C4;
+    p.a = p.dt_bias + H4;
+    p.d = p.a + H4;
+    p.norm = p.d + H4;
+    if (d->conv_states) {
+      p.conv_states = d->conv_states;
+      p.ssm_states = d->ssm_states;
+    } else {
+      const size_t nc = (size_t)p.slots * s->conv_elements() * sizeof(float);
+      const size_t ns = (size_t)p.slots * s->ssm_elements() * sizeof(float);
+      s->pool_conv.alloc(nc, "convolution states");
+      s->pool_ssm.alloc(ns, "ssm states");
+      HIPC(hipMemsetAsync(s->pool_conv.ptr, 0, nc, s->stream));
+      HIPC(hipMemsetAsync(s->pool_ssm.ptr, 0, ns, s->stream));
+      p.conv_states = s->pool_conv.as<float>();
+      p.ssm_states = s->pool_ssm.as<float>();
+    }
+    const size_t chunks = (size_t)ssm_max_chunks(p.max_tokens, p.max_sequences);
+    const size_t segments = (size_t)ssm_max_segments(p, p.max_tokens, p.max_sequences);
+    s->error.alloc(sizeof(int), "error flag");
+    s->counts.alloc(2 * sizeof(int), "segment and chunk counts");
+    s->sequences.alloc((size_t)p.max_sequences * sizeof(SsmSequence), "sequence table");
+    s->segments.alloc(segments * sizeof(int2), "segment table");
+    s->chunks.alloc(chunks * sizeof(int2), "chunk table");
+    s->bc.alloc(chunks * 2 * p.groups * p.state * kSsmChunk * sizeof(float), "convolved B and C");
+    s->decay.alloc(chunks * 3 * H * kSsmChunk * sizeof(float), "decays");
+    const size_t states = (size_t)ssm_max_states(p, p.max_tokens);
+    s->seg_states.alloc(states * s->ssm_elements() * sizeof(float), "segment states");
+    s->seg_decay.alloc(states * H * sizeof(float), "segment decays");
+    p.error = s->error.as<int>();
+    p.counts = s->counts.as<int>();
+    p.sequences = s->sequences.as<SsmSequence>();
+    p.segments = s->segments.as<int2>();
+    p.chunks = s->chunks.as<int2>();
+    p.bc = s->bc.as<float>();
+    p.decay = s->decay.as<float>();
+    p.seg_states = s->seg_states.as<float>();
+    p.seg_decay = s->seg_decay.as<float>();
+    HIPC(ssm_reset_error_launch(p, s->stream));
+    HIPC(hipStreamSynchronize(s->stream));
+    *result = s.release();
+  });
+}
+
+void llambda_hip_ssm_session_destroy(llambda_hip_ssm_session* session) { delete session; }
+
+size_t llambda_hip_ssm_session_input_element_count(const llambda_hip_ssm_session* s) {
+  return s ? s->row() : 0;
+}
+size_t llambda_hip_ssm_session_output_element_count(const llambda_hip_ssm_session* s) {
+  return s ? s->inner() : 0;
+}
+
+int llambda_hip_ssm_session_run(llambda_hip_ssm_session* s, int64_t slot, const float* input,
+                                size_t n_in, float* output, size_t n_out, size_t tokens) {
+  return guarded([&] {
+    if (!s) failf("ssm_session_run: null session");
+    if (!input || !output) failf("ssm_session_run: null input or output");
+    if (slot < 0 || slot >= s->plan.slots)
+      failf("ssm_session_run: slot %lld is not in 0..%d", (long long)slot, s->plan.slots - 1);
+    if (tokens == 0 || tokens > (size_t)s->plan.max_tokens)
+      failf("ssm_session_run: %zu tokens are not in 1..%d", tokens, s->plan.max_tokens);
+    if (n_in != tokens * s->row() || n_out != tokens * s->inner())
+      failf("ssm_session_run: element counts %zu/%zu do not match %zu rows of %zu and %zu", n_in, n_out,
+            tokens, s->row(), s->inner());
+    std::lock_guard<std::mutex> lock(s->run_mutex);
+    HIPC(hipSetDevice(s->device));
+    if (tokens > s->staged_tokens) {
+      s->staged_tokens = 0;
+      s->x.alloc(tokens * s->row() * sizeof(float), "ssm input");
+      s->y.alloc(tokens * s->inner() * sizeof(float), "ssm output");
+      s->staged_tokens = tokens;
+    }
+    if (!s->lists.ptr) s->lists.alloc(3 * sizeof(int32_t), "ssm slot list");
+    const int32_t lists[3] = {0, (int32_t)tokens, (int32_t)slot};
+    HIPC(hipMemcpyAsync(s->lists.ptr, lists, sizeof lists, hipMemcpyHostToDevice, s->stream));
+    HIPC(hipMemcpyAsync(s->x.ptr, input, n_in * sizeof(float), hipMemcpyHostToDevice, s->stream));
+    const int* dl = s->lists.as<int>();
+    SsmCall c{s->x.as<float>(), s->y.as<float>(), (int)tokens, 1, tokens == 1 ? nullptr : dl, dl + 2, dl + 2};
+    if (tokens == 1) {
+      HIPC(ssm_step_launch(s->plan, c, s->stream));
+    } else {
+      ssm_enqueue(s, c, s->stream);
+    }
+    HIPC(hipMemcpyAsync(output, s->y.ptr, n_out * sizeof(float), hipMemcpyDeviceToHost, s->stream));
+    HIPC(hipStreamSynchronize(s->stream));
+  });
+}
+
+int llambda_hip_ssm_session_run_device(llambda_hip_ssm_session* s, const float* input,
+                                       float* output, size_t tokens, const int32_t* offsets,
+                                       size_t sequences, const int32_t* from_slots,
+                                       const int32_t* to_slots, void* stream) {
+  return guarded([&] {
+    if (!s) failf("ssm_session_run_device: null session");
+    if (!offsets) failf("ssm_session_run_device: null offsets");
+    if (reinterpret_cast<uintptr_t>(offsets) & 3u) failf("ssm_session_run_device: offsets must be 4-byte aligned");
+    check_ssm_call(s, "ssm_session_run_device", input, output, tokens, sequences, from_slots, to_slots);
+    std::lock_guard<std::mutex> lock(s->run_mutex);
+    HIPC(hipSetDevice(s->device));
+    SsmCall c{input, output, (int)tokens, (int)sequences, offsets, from_slots, to_slots};
+    ssm_enqueue(s, c, stream ? static_cast<hipStream_t>(stream) : s->stream);
+  });
+}
+
+int llambda_hip_ssm_session_step_device(llambda_hip_ssm_session* s, const float* input,
+                                        float* output, size_t sequences, const int32_t* from_slots,
+                                        const int32_t* to_slots, void* stream) {
+  return guarded([&] {
+    if (!s) failf("ssm_session_step_device: null session");
+    check_ssm_call(s, "ssm_session_step_device", input, output, sequences, sequences, from_slots, to_slots);
+    std::lock_guard<std::mutex> lock(s->run_mutex);
+    HIPC(hipSetDevice(s->device));
+    SsmCall c{input, output, (int)sequences, (int)sequences, nullptr, from_slots, to_slots};
+    HIPC(ssm_step_launch(s->plan, c, stream ? static_cast<hipStream_t>(stream) : s->stream));
+  });
+}
+
+int llambda_hip_ssm_session_sync(llambda_hip_ssm_session* s, void* stream) {
+  return guarded([&] {
+    if (!s) failf("ssm_session_sync: null session");
+    std::lock_guard<std::mutex> lock(s->run_mutex);
+    HIPC(hipSetDevice(s->device));
+    s->raise_error(stream ? static_cast<hipStream_t>(stream) : s->stream);
+  });
+}
+
+int llambda_hip_ssm_session_reset(llambda_hip_ssm_session* s, int64_t slot) {
+  return guarded([&] {
+    if (!s) failf("ssm_session_reset: null session");
+    if (slot < 0 || slot >= s->plan.slots)
+      failf("ssm_session_reset: slot %lld is not in 0..%d", (long long)slot, s->plan.slots - 1);
+    std::lock_guard<std::mutex> lock(s->run_mutex);
+    HIPC(hipSetDevice(s->device));
+    const size_t nc = s->conv_elements(), ns = s->ssm_elements();
+    HIPC(hipStreamWaitEvent(s->stream, s->done, 0));
+    HIPC(hipMemsetAsync(s->plan.conv_states + slot * nc, 0, nc * sizeof(float), s->stream));
+    HIPC(hipMemsetAsync(s->plan.ssm_states + slot * ns, 0, ns * sizeof(float), s->stream));
+    HIPC(hipStreamSynchronize(s->stream));
+  });
+}
+
+int llambda_hip_ssm_session_write_state(llambda_hip_ssm_session* s, int64_t slot, const float* conv,
+                                        const float* ssm, int on_device) {
+  return guarded([&] {
+    if (!s || !conv || !ssm) failf("ssm_session_write_state: null argument");
+    if (slot < 0 || slot >= s->plan.slots)
+      failf("ssm_session_write_state: slot %lld is not in 0..%d", (long long)slot, s->plan.slots - 1);
+    std::lock_guard<std::mutex> lock(s->run_mutex);
+    HIPC(hipSetDevice(s->device));
+    const size_t nc = s->conv_elements(), ns = s->ssm_elements();
+    const hipMemcpyKind kind = on_device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice;
+    HIPC(hipStreamWaitEvent(s->stream, s->done, 0));
+    HIPC(hipMemcpyAsync(s->plan.conv_states + slot * nc, conv, nc * sizeof(float), kind, s->stream));
+    HIPC(hipMemcpyAsync(s->plan.ssm_states + slot * ns, ssm, ns * sizeof(float), kind, s->stream));
+    HIPC(hipStreamSynchronize(s->stream));
+  });
+}
+
+int llambda_hip_ssm_session_read_state(llambda_hip_ssm_session* s, int64_t slot, float* conv,
+                                       float* ssm) {
+  return guarded([&] {
+    if (!s || !conv || !ssm) failf("ssm_session_read_state: null argument");
+    if (slot < 0 || slot >= s->plan.slots)
+      failf("ssm_session_read_state: slot %lld is not in 0..%d", (long long)slot, s->plan.slots - 1);
+    std::lock_guard<std::mutex> lock(s->run_mutex);
+    HIPC(hipSetDevice(s->device));
+    const size_t nc = s->conv_elements(), ns = s->ssm_elements();
+    HIPC(hipStreamWaitEvent(s->stream, s->done, 0));
+    HIPC(hipMemcpyAsync(conv, s->plan.conv_states + slot * nc, nc * sizeof(float), hipMemcpyDeviceToHost, s->stream));
+    HIPC(hipMemcpyAsync(ssm, s->plan.ssm_states + slot * ns, ns * sizeof(float), hipMemcpyDeviceToHost, s->stream));
+    HIPC(hipStreamSynchronize(s->stream));
   });
 }
 

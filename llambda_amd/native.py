@@ -97,6 +97,19 @@ class Sampling(ctypes.Structure):
                 ("random_value", ctypes.c_float)]
 
 
+class SsmDesc(ctypes.Structure):
+    """llambda_hip_ssm_desc."""
+    _fields_ = [
+        ("heads", c_i64), ("head_dim", c_i64), ("groups", c_i64), ("state", c_i64),
+        ("conv_width", c_i64),
+        ("conv_weight", c_void_p), ("conv_bias", c_void_p), ("dt_bias", c_void_p),
+        ("a", c_void_p), ("d", c_void_p), ("norm", c_void_p),
+        ("norm_epsilon", ctypes.c_float),
+        ("slots", c_i64), ("max_tokens", c_i64), ("max_sequences", c_i64),
+        ("conv_states", c_void_p), ("ssm_states", c_void_p),
+    ]
+
+
 class GgufTensor(ctypes.Structure):
     """llambda_hip_gguf_tensor."""
     _fields_ = [("name", c_void_p), ("name_length", c_size), ("dimension_count", ctypes.c_uint32),
@@ -156,6 +169,20 @@ SIGNATURES = {
     "llambda_hip_llama_session_read_kv": (c_int, [c_void_p, c_i64, c_i64, c_i64, c_void_p,
                                                   c_void_p]),
     "llambda_hip_llama_session_sync": (c_int, [c_void_p, c_void_p]),
+    "llambda_hip_ssm_session_create": (c_int, [ctypes.POINTER(SsmDesc), ctypes.POINTER(c_void_p)]),
+    "llambda_hip_ssm_session_destroy": (None, [c_void_p]),
+    "llambda_hip_ssm_session_input_element_count": (c_size, [c_void_p]),
+    "llambda_hip_ssm_session_output_element_count": (c_size, [c_void_p]),
+    "llambda_hip_ssm_session_run": (c_int, [c_void_p, c_i64, c_void_p, c_size, c_void_p, c_size,
+                                            c_size]),
+    "llambda_hip_ssm_session_run_device": (c_int, [c_void_p, c_void_p, c_void_p, c_size, c_void_p,
+                                                   c_size, c_void_p, c_void_p, c_void_p]),
+    "llambda_hip_ssm_session_step_device": (c_int, [c_void_p, c_void_p, c_void_p, c_size, c_void_p,
+                                                    c_void_p, c_void_p]),
+    "llambda_hip_ssm_session_sync": (c_int, [c_void_p, c_void_p]),
+    "llambda_hip_ssm_session_reset": (c_int, [c_void_p, c_i64]),
+    "llambda_hip_ssm_session_write_state": (c_int, [c_void_p, c_i64, c_void_p, c_void_p, c_int]),
+    "llambda_hip_ssm_session_read_state": (c_int, [c_void_p, c_i64, c_void_p, c_void_p]),
     "llambda_hip_sampler_create": (c_int, [c_size, ctypes.POINTER(c_void_p)]),
     "llambda_hip_sampler_destroy": (None, [c_void_p]),
     "llambda_hip_sampler_sample": (c_int, [c_void_p, c_void_p, c_size, c_int,

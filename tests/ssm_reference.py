@@ -1,0 +1,66 @@
+"""The mixer's recurrence in 64 bits, token by token, with bounds on what
+single precision may differ by.
+
+bound(): every product and sum of an fp32 evaluation rounds by at most u =
+2^-24 of its value, and what it rounds is at most the same expression over
+absolute values.  An output's longest chain is: the convolution and silu of
+x, B and C (conv_width + 8 roundings each), dt (its relative error of about 8 u
+moves a decay e^-c by 8 u c e^-c < 3 u), the sum over the state (N, or N / 2
+with fewer), the sum over a chunk of 32 tokens, one product with a decay per
+chunk and segment, and the skip.  K roundings move it by at most K u of the
+absolute expression (to first order, K u < 1e-3 here).
+"""
+import numpy as np
+
+U = 2.0 ** -24
+
+
+def _silu(v):
+    return v / (1 + np.exp(-v))
+
+
+def _softplus(v):
+    return np.maximum(v, 0) + np.log1p(np.exp(-np.abs(v)))
+
+
+def sequence(layer, x, conv, ssm):
+    """One sequence: (y, conv, ssm, y's bound, ssm's bound) for rows x [T][row] from a state."""
+    L, H, P, G, N, W = layer, layer.heads, layer.head_dim, layer.groups, layer.state, layer.conv_width
+    x = x.astype(np.float64)
+    T, inner, channels = x.shape[0], L.inner, L.channels
+    raw = np.concatenate([conv.astype(np.float64), x[:, inner:inner + channels]])
+    bias = np.zeros(channels) if L.conv_bias is None else L.conv_bias.astype(np.float64)
+    w = L.conv_weight.astype(np.float64)
+    s = ssm.astype(np.float64)
+    s_abs = np.abs(s)
+    y, y_abs = np.empty((T, inner)), np.empty((T, inner))
+    share = H // G
+    a, d = L.a.astype(np.float64), L.d.astype(np.float64)
+    for t in range(T):
+        taps = raw[t:t + W]
+        pre = bias + (w.T * taps).sum(0)
+        # |silu'| <= 1.1, so the convolution's roundings reach u by the taps' absolute sum
+        u, u_abs = _silu(pre), np.abs(bias) + (np.abs(w.T) * np.abs(taps)).sum(0)
+        dt = _softplus(x[t, inner + channels:] + L.dt_bias.astype(np.float64))
+        e = np.exp(dt * a)
+        xs = u[:inner].reshape(H, P)
+        bs = np.repeat(u[inner:inner + G * N].reshape(G, N), share, 0)
+        cs = np.repeat(u[inner + G * N:].reshape(G, N), share, 0)
+        xa = u_abs[:inner].reshape(H, P)
+        ba = np.repeat(u_abs[inner:inner + G * N].reshape(G, N), share, 0)
+        ca = np.repeat(u_abs[inner + G * N:].reshape(G, N), share, 0)
+        s = e[:, None, None] * s + (dt[:, None] * xs)[:, :, None] * bs[:, None, :]
+        s_abs = e[:, None, None] * s_abs + (dt[:, None] * xa)[:, :, None] * ba[:, None, :]
+        y[t] = ((s * cs[:, None, :]).sum(-1) + d[:, None] * xs).reshape(-1)
+        y_abs[t] = ((s_abs * ca[:, None, :]).sum(-1) + np.abs(d)[:, None] * xa).reshape(-1)
+    K = 3 * (W + 8) + N + 32 + T // 16 + 32
+    z = _silu(x[:, :inner])
+    v, dv = y * z, K * U * y_abs * np.abs(z) + 8 * U * np.abs(y * z)
+    vg, dg = v.reshape(T, G, inner // G), dv.reshape(T, G, inner // G)
+    r = 1 / np.sqrt((vg * vg).mean(-1, keepdims=True) + float(np.float32(L.norm_epsilon)))
+    norm = L.norm.astype(np.float64)
+    out = (vg * r).reshape(T, inner) * norm
+    # d(1 / rms) / (1 / rms) <= |dv| / |v| in the 2-norm over the group, and its own roundings
+    rel = np.sqrt((dg * dg).sum(-1, keepdims=True)) * r / np.sqrt(vg.shape[-1]) + 24 * U
+    bound = (r * (dg + np.abs(vg) * rel)).reshape(T, inner) * np.abs(norm)
+    return out, raw[T:].astype(np.float32), s, bound, K * U * s_abs

@@ -1,0 +1,358 @@
+"""Mamba-2 mixer sessions (llambda_hip_ssm_session_*) against the recurrence
+in 64 bits (ssm_reference.py, which derives the bounds)."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import ssm_reference
+from llambda_amd import native
+from llambda_amd.hip_backend import HipBackendError
+from llambda_amd.ssm import HipSsmSession, synthetic_ssm
+
+pytestmark = pytest.mark.gpu
+
+LAYOUTS = {
+    "hybrid": dict(heads=64, head_dim=64, groups=8, state=128, conv_width=4),
+    "one_group": dict(heads=6, head_dim=80, groups=1, state=64, conv_width=3),
+    "wide": dict(heads=4, head_dim=128, groups=2, state=256, conv_width=4),
+    "narrow": dict(heads=8, head_dim=32, groups=2, state=16, conv_width=2),
+    "thin": dict(heads=3, head_dim=16, groups=3, state=32, conv_width=4),
+    "odd": dict(heads=5, head_dim=48, groups=1, state=128, conv_width=4, conv_bias=False),
+    "broad_norm": dict(heads=48, head_dim=96, groups=1, state=16, conv_width=4),
+}
+
+
+class Case:
+    """A session over tensors on the device, and the reference's answer to the same call."""
+
+    def __init__(self, layout, lengths, seed, old=None, new=None, slots=None, extra_rows=0, layer=None):
+        import torch
+        self.torch = torch
+        rng = np.random.default_rng(seed)
+        self.layer = layer or synthetic_ssm(rng, **LAYOUTS[layout])
+        L = self.layer
+        self.lengths, n = lengths, len(lengths)
+        self.tokens = sum(lengths) + extra_rows
+        self.x = rng.normal(size=(self.tokens, L.row)).astype(np.float32)
+        self.old = np.arange(n) if old is None else np.asarray(old)
+        self.new = np.arange(n) if new is None else np.asarray(new)
+        self.slots = slots or int(max(self.old.max(), self.new.max(), 0)) + 1
+        self.conv = rng.normal(size=(self.slots, L.conv_width - 1, L.channels)).astype(np.float32)
+        self.ssm = rng.normal(size=(self.slots, L.heads, L.head_dim, L.state)).astype(np.float32)
+        self.offsets = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32)
+
+    def device(self, max_tokens=None):
+        torch = self.torch
+        t = torch.from_numpy
+        self.dx, self.dconv, self.dssm = t(self.x).cuda(), t(self.conv).cuda(), t(self.ssm).cuda()
+        self.doff = t(self.offsets).cuda()
+        self.dold = t(self.old.astype(np.int32)).cuda()
+        self.dnew = t(self.new.astype(np.int32)).cuda()
+        self.dy = torch.full((self.tokens, self.layer.inner), 7.25, device="cuda")
+        self.session = HipSsmSession(self.layer, slots=self.slots, max_tokens=max_tokens or self.tokens,
+                                     max_sequences=len(self.lengths), conv_states_ptr=self.dconv.data_ptr(),
+                                     ssm_states_ptr=self.dssm.data_ptr())
+        torch.cuda.synchronize()
+        return self
+
+    def run(self, stream=0, lists=True):
+        s, n = self.session, len(self.lengths)
+        old, new = (self.dold.data_ptr(), self.dnew.data_ptr()) if lists else (0, 0)
+        s.run_device(self.dx.data_ptr(), self.dy.data_ptr(), self.tokens, self.doff.data_ptr(), n, old, new, stream)
+
+    def step(self, stream=0, lists=True):
+        old, new = (self.dold.data_ptr(), self.dnew.data_ptr()) if lists else (0, 0)
+        self.session.step_device(self.dx.data_ptr(), self.dy.data_ptr(), len(self.lengths), old, new, stream)
+
+    def reference(self):
+        """Per sequence what ssm_reference.sequence returns."""
+        L, out = self.layer, []
+        for i, old in enumerate(self.old):
+            conv = self.conv[old] if old >= 0 else np.zeros((L.conv_width - 1, L.channels), np.float32)
+            ssm = self.ssm[old] if old >= 0 else np.zeros((L.heads, L.head_dim, L.state), np.float32)
+            out.append(ssm_reference.sequence(L, self.x[self.offsets[i]:self.offsets[i + 1]], conv, ssm))
+        return out
+
+    def check(self, refused=()):
+        y, conv, ssm = (a.cpu().numpy() for a in (self.dy, self.dconv, self.dssm))
+        want_conv, written = self.conv.copy(), set()
+        for i, (out, taps, state, bound, state_bound) in enumerate(self.reference()):
+            rows = slice(self.offsets[i], self.offsets[i + 1])
+            if i in refused:
+                assert np.all(y[rows] == 7.25), f"sequence {i}: rows of a refused sequence"
+                continue
+            far = np.abs(y[rows] - out) - bound
+            assert not far.size or far.max() <= 0, (
+                f"sequence {i} of {self.lengths[i]}: row {far.max(1).argmax()} is {far.max():.3g} outside")
+            if self.new[i] < 0:
+                continue
+            written.add(int(self.new[i]))
+            want_conv[self.new[i]] = taps
+            far = np.abs(ssm[self.new[i]] - state) - state_bound
+            assert far.max() <= 0, f"sequence {i}: state {far.max():.3g} outside"
+        assert np.array_equal(conv, want_conv)
+        for k in range(self.slots):
+            if k not in written:
+                assert np.array_equal(ssm[k], self.ssm[k]), f"slot {k} changed"
+        assert np.all(y[self.offsets[-1]:] == 7.25), "rows behind the last sequence"
+
+
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+@pytest.mark.parametrize("lengths", [[1], [2, 31, 32, 33], [0, 65, 0, 1, 5], [129, 300]], ids=str)
+def test_prompts(hip, layout, lengths):
+    n = len(lengths)
+    rng = np.random.default_rng(n)
+    old = rng.permutation(n)
+    old[::2] = -1
+    new = n + rng.permutation(n)
+    c = Case(layout, lengths, 11, old, new, slots=2 * n, extra_rows=3).device()
+    c.run()
+    c.session.sync()
+    c.check()
+
+
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+@pytest.mark.parametrize("n", [1, 7])
+def test_steps(hip, layout, n):
+    rng = np.random.default_rng(n)
+    c = Case(layout, [1] * n, 12, rng.permutation(n), n + rng.permutation(n), slots=2 * n).device()
+    c.step()
+    c.session.sync()
+    c.check()
+
+
+def test_steps_in_place_new_and_dropped(hip):
+    c = Case("hybrid", [1] * 5, 13, [3, -1, 2, 6, -1], [3, 0, 2, -1, -1], slots=7).device()
+    c.step()
+    c.session.sync()
+    c.check()
+
+
+def test_prompts_in_place_new_and_dropped(hip):
+    c = Case("one_group", [200, 3, 0, 40, 17], 14, [3, -1, 2, 6, -1], [3, 0, 2, -1, -1], slots=7).device()
+    c.run()
+    c.session.sync()
+    c.check()
+
+
+def test_without_lists_sequence_i_is_slot_i(hip):
+    c = Case("narrow", [4, 150, 1], 15, slots=4).device()
+    c.run(lists=False)
+    c.session.sync()
+    c.check()
+    c = Case("narrow", [1, 1, 1], 16, slots=4).device()
+    c.step(lists=False)
+    c.session.sync()
+    c.check()
+
+
+def test_one_state_read_by_several(hip):
+    """A prefix's state continued in several ways."""
+    c = Case("thin", [40, 200, 3], 17, [0, 0, 0], [1, 2, 3], slots=4).device()
+    c.run()
+    c.session.sync()
+    c.check()
+
+
+def test_long_sequence_of_many_segments(hip):
+    c = Case("narrow", [5003, 64], 18, [0, 1], [0, 2], slots=3).device()
+    c.run()
+    c.session.sync()
+    c.check()
+
+
+def test_misaligned_rows_and_buffers(hip):
+    """Rows of an odd length from a pointer that is only 4-byte aligned."""
+    import torch
+    c = Case("thin", [50, 9], 19).device()
+    flat = torch.empty(c.dx.numel() + 1, device="cuda")
+    flat[1:] = c.dx.reshape(-1)
+    out = torch.full((c.dy.numel() + 1,), 7.25, device="cuda")
+    torch.cuda.synchronize()
+    c.session.run_device(flat.data_ptr() + 4, out.data_ptr() + 4, c.tokens, c.doff.data_ptr(), 2)
+    c.session.sync()
+    c.dy = out[1:].reshape(c.dy.shape)
+    c.check()
+
+
+def test_strong_decays_and_large_steps(hip):
+    """Decays that leave nothing beside decays that keep all: exponents far beyond single precision's range."""
+    rng = np.random.default_rng(20)
+    layer = synthetic_ssm(rng, **LAYOUTS["narrow"])
+    layer.a[:] = [-1e4, -16, -1e-6, 0, -50, -1, -3e3, -8]
+    c = Case("narrow", [97, 260], 21, layer=layer)
+    c.x[:, -layer.heads:] *= 4
+    c.x[::13, -layer.heads:] = 60
+    c.device().run()
+    c.session.sync()
+    c.check()
+
+
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+def test_non_finite_rows_reach_no_earlier_token_and_no_other_sequence(hip, value):
+    import torch
+    c = Case("narrow", [70, 90, 20], 22)
+    L = c.layer
+    clean = c.reference()
+    at, ch = 41, 5
+    c.x[c.offsets[1] + at, L.inner + ch] = value  # an x channel of head 0 in the second sequence
+    c.device().run()
+    c.session.sync()
+    y = c.dy.cpu().numpy()
+    for i in (0, 2):
+        out, _, _, bound, _ = clean[i]
+        assert np.all(np.abs(y[c.offsets[i]:c.offsets[i + 1]] - out) <= bound)
+    out, _, _, bound, _ = clean[1]
+    rows = y[c.offsets[1]:c.offsets[2]]
+    assert np.all(np.abs(rows[:at] - out[:at]) <= bound[:at])
+    width = L.inner // L.groups
+    assert np.all(~np.isfinite(rows[at:, ch])) and np.all(~np.isfinite(rows[at:, :width]))
+    other = slice(width, None)  # the other group's channels do not know
+    assert np.all(np.abs(rows[:, other] - out[:, other]) <= bound[:, other])
+    # B of one token: its group's states from there on
+    c = Case("narrow", [70, 90, 20], 22)
+    c.x[c.offsets[1] + at, L.inner + L.inner + 3] = value
+    c.device().run()
+    c.session.sync()
+    rows = c.dy.cpu().numpy()[c.offsets[1]:c.offsets[2]]
+    assert np.all(np.abs(rows[:at] - out[:at]) <= bound[:at])
+    assert not np.isfinite(rows[at + 1:, :width]).any()
+    assert np.all(np.abs(rows[:, other] - out[:, other]) <= bound[:, other])
+    torch.cuda.synchronize()
+
+
+def test_refused_on_the_device(hip):
+    import torch
+    # slot 2 is written twice; slot 0 is written by 3 and read by 4; slot 9 does not exist
+    c = Case("one_group", [40, 5, 130, 7, 8, 2], 23, [3, 4, 1, -1, 0, 5], [2, 6, 2, 0, 7, 5], slots=8).device()
+    c.dold[5] = 9
+    torch.cuda.synchronize()
+    c.run()
+    with pytest.raises(HipBackendError, match="outside the pool.*written by one sequence"):
+        c.session.sync()
+    c.session.sync()  # reported once
+    c.check(refused=(0, 2, 3, 5))
+    c = Case("one_group", [1] * 6, 24, [3, 4, 1, -1, 0, 5], [2, 6, 2, 0, 7, 5], slots=8).device()
+    c.dnew[5] = -2
+    torch.cuda.synchronize()
+    c.step()
+    with pytest.raises(HipBackendError, match="outside the pool.*written by one sequence"):
+        c.session.sync()
+    c.check(refused=(0, 2, 3, 5))
+
+
+@pytest.mark.parametrize("offsets", [[0, 5, 3, 12], [0, 5, 12, 13], [-1, 5, 6, 12], [0, 12, 0, 12]])
+def test_offsets_that_do_not_ascend(hip, offsets):
+    import torch
+    c = Case("thin", [5, 3, 4], 25).device()
+    c.doff.copy_(torch.tensor(offsets, dtype=torch.int32))
+    torch.cuda.synchronize()
+    c.run()
+    with pytest.raises(HipBackendError, match="offsets do not ascend"):
+        c.session.sync()
+    assert bool((c.dy == 7.25).all()) and np.array_equal(c.dssm.cpu().numpy(), c.ssm)
+    assert np.array_equal(c.dconv.cpu().numpy(), c.conv)
+    # the session goes on
+    c.doff.copy_(torch.from_numpy(c.offsets))
+    torch.cuda.synchronize()
+    c.run()
+    c.session.sync()
+    c.check()
+
+
+def test_captured_calls_replay(hip):
+    """A prompt and a step in one graph, replayed between eager calls of another session."""
+    import torch
+    c = Case("hybrid", [70, 1, 33], 26, [0, 1, 2], [3, 4, 5], slots=6).device()
+    e = Case("hybrid", [70, 1, 33], 27, [0, 1, 2], [3, 4, 5], slots=6).device()
+    d = Case("hybrid", [1] * 9, 28, np.arange(9), 9 + np.arange(9), slots=18).device()
+    stream = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream, capture_error_mode="relaxed"):
+        c.run(stream.cuda_stream)
+        d.step(stream.cuda_stream)
+    rng = np.random.default_rng(29)
+    for _ in range(4):
+        for k in (c, d):
+            k.x = rng.normal(size=k.x.shape).astype(np.float32)
+            k.dx.copy_(torch.from_numpy(k.x))
+            k.dy.fill_(7.25)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        e.run()
+        torch.cuda.synchronize()
+        for k in (c, d, e):
+            k.session.sync()
+            k.check()
+            k.dssm.copy_(torch.from_numpy(k.ssm))
+            k.dconv.copy_(torch.from_numpy(k.conv))
+
+
+def test_calls_on_several_streams_share_the_workspace(hip):
+    """Each call waits for the one before, whatever its stream."""
+    import torch
+    c = Case("narrow", [900, 700], 30, [0, 1], [2, 3], slots=4).device()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = [torch.full_like(c.dy, 7.25) for _ in range(6)]
+    torch.cuda.synchronize()
+    for k, out in enumerate(outs):
+        c.session.run_device(c.dx.data_ptr(), out.data_ptr(), c.tokens, c.doff.data_ptr(), 2, c.dold.data_ptr(),
+                             c.dnew.data_ptr(), streams[k % 3].cuda_stream)
+    torch.cuda.synchronize()
+    c.session.sync()
+    c.dy = outs[0]
+    c.check()
+    for out in outs[1:]:
+        assert torch.equal(out, outs[0])
+
+
+def test_host_runs_and_states(hip):
+    rng = np.random.default_rng(31)
+    layer = synthetic_ssm(rng, **LAYOUTS["one_group"])
+    x = rng.normal(size=(45, layer.row)).astype(np.float32)
+    s = HipSsmSession(layer, slots=3, max_tokens=64)
+    assert (s.input_element_count, s.output_element_count) == (layer.row, layer.inner)
+    conv = np.zeros((layer.conv_width - 1, layer.channels), np.float32)
+    ssm = np.zeros((layer.heads, layer.head_dim, layer.state), np.float32)
+    out, taps, state, bound, state_bound = ssm_reference.sequence(layer, x, conv, ssm)
+    y = np.concatenate([s.run(x[:30], slot=1), s.run(x[30:31], slot=1), s.run(x[31:], slot=1)])
+    assert np.all(np.abs(y - out) <= bound)
+    got_conv, got_ssm = s.read_state(1)
+    assert np.array_equal(got_conv, taps) and np.all(np.abs(got_ssm - state) <= state_bound)
+    for k in (0, 2):
+        assert not any(a.any() for a in s.read_state(k))
+    s.write_state(2, got_conv, got_ssm)
+    assert np.array_equal(s.run(x[:9], slot=2), s.run(x[:9], slot=1))
+    s.reset(1)
+    assert np.all(np.abs(s.run(x, slot=1) - out) <= bound)
+    with pytest.raises(HipBackendError, match="slot 3 is not in 0..2"):
+        s.run(x, slot=3)
+    with pytest.raises(HipBackendError, match="65 tokens are not in 1..64"):
+        s.run(np.zeros((65, layer.row), np.float32))
+    s.close()
+    with pytest.raises(HipBackendError, match="closed"):
+        s.run(x)
+
+
+def test_refused_on_the_host(hip):
+    c = Case("thin", [5, 3], 32, slots=2).device()
+    s, x, y, o = c.session, c.dx.data_ptr(), c.dy.data_ptr(), c.doff.data_ptr()
+    for args, text in [((0, y, 8, o, 2), "null input"), ((x, 0, 8, o, 2), "null input"),
+                       ((x, y, 8, 0, 2), "null offsets"), ((x, y, 9, o, 2), "9 tokens"),
+                       ((x, y, 0, o, 2), "0 tokens"), ((x, y, 8, o, 3), "3 sequences"),
+                       ((x, y, 8, o, 0), "0 sequences"), ((x + 2, y, 8, o, 2), "aligned"),
+                       ((x, x + 4, 8, o, 2), "overlap")]:
+        with pytest.raises(HipBackendError, match=text):
+            s.run_device(*args)
+    with pytest.raises(HipBackendError, match="3 sequences"):
+        s.step_device(x, y, 3)
+    few = HipSsmSession(c.layer, slots=1, max_tokens=8, max_sequences=2)
+    with pytest.raises(HipBackendError, match="without a slot list"):
+        few.step_device(x, y, 2)
+    L = native.lib()
+    assert L.llambda_hip_ssm_session_run_device(None, x, y, 8, o, 2, None, None, None) == -1
+    assert L.llambda_hip_ssm_session_read_state(s.pointer, 0, None, None) == -1
+    assert L.llambda_hip_ssm_session_sync(None, None) == -1
+    assert L.llambda_hip_ssm_session_create(None, ctypes.byref(ctypes.c_void_p())) == -1
