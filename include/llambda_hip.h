@@ -45,6 +45,8 @@ typedef struct llambda_hip_llama_session llambda_hip_llama_session;
 typedef struct llambda_hip_sampler llambda_hip_sampler;
 typedef struct llambda_hip_gguf llambda_hip_gguf;
 typedef struct llambda_hip_ssm_session llambda_hip_ssm_session;
+typedef struct llambda_hip_router llambda_hip_router;
+typedef struct llambda_hip_batch_sampler llambda_hip_batch_sampler;
 
 /* ---- probe, versions, errors -------------------------------------- */
 
@@ -249,6 +251,61 @@ int llambda_hip_moe_session_run_device_noalloc(llambda_hip_moe_session* session,
  * unfilled slots (-1, -FLT_MAX).  Host pointers, synchronous, on the device. */
 int llambda_hip_select_top_k(const float* logits, size_t n, size_t k, size_t batch,
                              int64_t* top_indices, float* top_logits);
+
+/* ---- routers ------------------------------------------------------------ */
+
+enum {
+  LLAMBDA_HIP_ROUTE_SOFTMAX = 0, /* softmax over all experts */
+  LLAMBDA_HIP_ROUTE_SIGMOID = 1
+};
+
+/* Routing as MoE checkpoints define it, where it differs from the reference's
+ * gating (which adds Nemotron-H's bias to the logits and takes the sigmoid of
+ * the sums, llambda.lisp:5892-5913).  Per token, in 64 bits, with logits l:
+ *   s = softmax(l) or sigmoid(l);  c = s + bias
+ *   a group, expert_count / groups neighbours, scores the sum of its
+ *   group_rank highest c; the experts of the top_groups highest groups stay
+ *   the top_k highest c among them, lower index first among equals
+ *   weights: s of those, over their sum when weights_norm (and the sum is
+ *   positive), times weights_scale
+ * NaN logits and logits <= -FLT_MAX are never chosen and add nothing to a
+ * softmax; places left unfilled hold (-1, 0). */
+typedef struct llambda_hip_router_desc {
+  int score;                  /* LLAMBDA_HIP_ROUTE_* */
+  int64_t expert_count;       /* 1..1024 */
+  int64_t top_k;              /* 1..64, at most the open groups' experts */
+  int64_t groups;             /* 1..64, divides expert_count; 1 = no groups */
+  int64_t top_groups;
+  int64_t group_rank;         /* 1 or 2 */
+  const float* bias;          /* host, [expert_count], NULL = none; copied */
+  int weights_norm;
+  float weights_scale;
+} llambda_hip_router_desc;
+
+/* No counterpart in the reference's bridge (it routes in Lisp). */
+int llambda_hip_router_create(const llambda_hip_router_desc* desc, llambda_hip_router** result);
+void llambda_hip_router_destroy(llambda_hip_router* router);
+
+/* Host pointers, synchronous: logits [batch][expert_count] -> top_indices,
+ * top_weights [batch][top_k]. */
+int llambda_hip_router_run(llambda_hip_router* router, const float* logits, size_t count,
+                           int64_t* top_indices, float* top_weights, size_t batch);
+
+/* Device-resident form, one launch on `stream` (null = the router's own), not
+ * waited for.  Calls share nothing: they may run at once and be captured. */
+int llambda_hip_router_run_device(llambda_hip_router* router, const float* logits,
+                                  int32_t* top_indices, float* top_weights, size_t batch,
+                                  void* stream);
+
+/* Let a MoE layer's later runs gate with `router` (copied: it may be destroyed)
+ * in place of the reference's gating; NULL restores that.  The router's
+ * expert_count and top_k are the layer's.  Logits that a run returns are then
+ * the router tensor's products alone, the shared expert's gate stays as it is,
+ * and the run's input errors are raised as before (unfilled places; with
+ * weights_norm a sum that is not positive).  Graphs captured before the change
+ * keep the gating they hold and have to be captured anew. */
+int llambda_hip_moe_session_set_router(llambda_hip_moe_session* session,
+                                       llambda_hip_router* router);
 
 /* ---- measurement ------------------------------------------------------ */
 
@@ -494,6 +551,48 @@ int llambda_hip_sampler_sample(llambda_hip_sampler* sampler, const float* logits
 int llambda_hip_llama_session_sample(llambda_hip_llama_session* session,
                                      llambda_hip_sampler* sampler,
                                      const llambda_hip_sampling* params, int64_t* token);
+
+/* ---- sampling of a batch --------------------------------------------------- */
+
+/* The parameters of each row, [rows] each (device memory for the device form,
+ * host memory for the host form).  NULL: that parameter's default for all. */
+typedef struct llambda_hip_batch_sampling {
+  const float* temperature;   /* >= 0, finite; default 1; 0 takes the highest logit */
+  const int32_t* top_k;       /* >= 0; default 0 = off */
+  const float* top_p;         /* (0, 1]; default 1 = off */
+  const float* min_p;         /* [0, 1]; default 0 = off */
+  const float* random_value;  /* [0, 1); required */
+} llambda_hip_batch_sampling;
+
+/* Workspace for up to max_rows rows of up to `vocab` logits (at most 262144).
+ * No counterpart in the reference, which samples one row at a time. */
+int llambda_hip_batch_sampler_create(size_t vocab, size_t max_rows,
+                                     llambda_hip_batch_sampler** result);
+void llambda_hip_batch_sampler_destroy(llambda_hip_batch_sampler* sampler);
+
+/* One token per row of logits[rows][count], all device memory, on `stream`
+ * (null = the sampler's), not waited for, with no allocation.  Per row, in 64
+ * bits, with x = logit / temperature: weights are exp(x - max x); ranks go by
+ * logit, the lower index first among equals.  Kept are the top_k first ranks;
+ * of those the shortest run from the first whose weights reach top_p of their
+ * total; of those the weights of at least min_p (the largest weight is 1).
+ * The token is the first, by index, at which the running sum of kept weights
+ * exceeds random_value times their total.  (sample-token-id-from-logits, which
+ * llambda_hip_sampler_sample follows, keeps ties at the top-k cutoff and takes
+ * the temperature last.)
+ * A row gets -1 where a logit is NaN, none lies above -inf, or its parameters
+ * are out of range.  The calls of a sampler share its workspace and are
+ * ordered as llambda_hip_ssm_session_run_device's, under capture too. */
+int llambda_hip_batch_sampler_sample_device(llambda_hip_batch_sampler* sampler,
+                                            const float* logits, size_t count, size_t rows,
+                                            const llambda_hip_batch_sampling* params,
+                                            int32_t* tokens, void* stream);
+
+/* Host pointers, synchronous; parameters out of range and rows without a token
+ * are errors. */
+int llambda_hip_batch_sampler_sample(llambda_hip_batch_sampler* sampler, const float* logits,
+                                     size_t count, size_t rows,
+                                     const llambda_hip_batch_sampling* params, int64_t* tokens);
 
 /* ---- GGUF files ------------------------------------------------------------ */
 

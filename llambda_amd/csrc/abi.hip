@@ -27,6 +27,7 @@
 #include "gguf.h"
 #include "moe.h"
 #include "sample.h"
+#include "sample_batch.h"
 #include "sha256.h"
 #include "ssm.h"
 
@@ -505,6 +506,20 @@ static MoeScratchBytes moe_scratch_bytes(const MoePlan& p, size_t T) {
   return b;
 }
 
+struct llambda_hip_router {
+  std::mutex run_mutex;
+  int device = 0;
+  hipStream_t stream = nullptr;
+  RouteSpec spec{};
+  std::vector<float> host_bias;
+  DevBuf bias;
+  DevBuf logits, indices, weights;  // device staging of the host-pointer runs
+  size_t staged_tokens = 0;
+  ~llambda_hip_router() {
+    if (stream) (void)hipStreamDestroy(stream);
+  }
+};
+
 struct llambda_hip_moe_session {
   std::mutex run_mutex;
   int device = 0;
@@ -512,6 +527,7 @@ struct llambda_hip_moe_session {
   MoePlan plan{};
   DevBuf router, bias, gate, up, down, sh_gate, sh_up, sh_down, lat_down, lat_up;
   DevBuf up_g, down_g, sh_up_g, sh_down_g;  // stage-major copies (group pipeline)
+  DevBuf route_bias;
   DevBuf logits, router_part, top_idx, top_w, shared_w, perm, chunks, chunk_counts,
       down_out, error, xq, xsum, aq, asum, lat, lq, lsum, lat_y;
   DevBuf x, y;     // device staging for the host-pointer runs
@@ -1053,6 +1069,119 @@ int llambda_hip_select_top_k(const float* logits, size_t n, size_t k, size_t bat
     HIPC(hipMemcpyAsync(top_logits, dv.ptr, batch * k * sizeof(float), hipMemcpyDeviceToHost, stream));
     HIPC(hipStreamSynchronize(stream));
     for (size_t i = 0; i < idx.size(); ++i) top_indices[i] = idx[i];
+  });
+}
+
+}  // extern "C"
+
+// ----------------------------------------------------------------- routers
+
+extern "C" {
+
+int llambda_hip_router_create(const llambda_hip_router_desc* d, llambda_hip_router** result) {
+  return guarded([&] {
+    if (!result) failf("router_create: null result pointer");
+    *result = nullptr;
+    if (!d) failf("router_create: null description");
+    if (d->score != LLAMBDA_HIP_ROUTE_SOFTMAX && d->score != LLAMBDA_HIP_ROUTE_SIGMOID)
+      failf("router_create: unknown score %d", d->score);
+    auto in = [&](int64_t v, int64_t lo, int64_t hi, const char* what) {
+      if (v < lo || v > hi)
+        failf("router_create: %s %lld is not in %lld..%lld", what, (long long)v, (long long)lo, (long long)hi);
+    };
+    in(d->expert_count, 1, kMoeMaxExperts, "expert_count");
+    in(d->groups, 1, std::min<int64_t>(kRouteMaxGroups, d->expert_count), "groups");
+    if (d->expert_count % d->groups)
+      failf("router_create: %lld groups do not divide %lld experts", (long long)d->groups,
+            (long long)d->expert_count);
+    in(d->top_groups, 1, d->groups, "top_groups");
+    in(d->group_rank, 1, 2, "group_rank");
+    in(d->top_k, 1, std::min<int64_t>(kMoeMaxTopK, d->top_groups * (d->expert_count / d->groups)), "top_k");
+    if (!std::isfinite(d->weights_scale)) failf("router_create: weights_scale %g", (double)d->weights_scale);
+    std::unique_ptr<llambda_hip_router> r(new llambda_hip_router());
+    r->device = current_device_checked();
+    HIPC(hipStreamCreateWithFlags(&r->stream, hipStreamNonBlocking));
+    if (d->bias) {
+      r->host_bias.assign(d->bias, d->bias + d->expert_count);
+      r->bias.alloc(r->host_bias.size() * sizeof(float), "router bias");
+      HIPC(hipMemcpyAsync(r->bias.ptr, d->bias, r->host_bias.size() * sizeof(float), hipMemcpyHostToDevice, r->stream));
+      HIPC(hipStreamSynchronize(r->stream));
+    }
+    r->spec = RouteSpec{r->bias.as<float>(), (int)d->expert_count, (int)d->top_k, (int)d->groups,
+                        (int)d->top_groups, (int)d->group_rank, d->score == LLAMBDA_HIP_ROUTE_SIGMOID,
+                        d->weights_norm != 0, d->weights_scale};
+    *result = r.release();
+  });
+}
+
+void llambda_hip_router_destroy(llambda_hip_router* router) { delete router; }
+
+int llambda_hip_router_run_device(llambda_hip_router* r, const float* logits, int32_t* top_indices,
+                                  float* top_weights, size_t batch, void* stream) {
+  return guarded([&] {
+    if (!r) failf("router_run_device: null router");
+    if (!logits || !top_indices || !top_weights) failf("router_run_device: null argument");
+    if (batch == 0 || batch > (1u << 24)) failf("router_run_device: bad batch %zu", batch);
+    if ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(top_indices) |
+         reinterpret_cast<uintptr_t>(top_weights)) & 3u)
+      failf("router_run_device: pointers must be 4-byte aligned");
+    HIPC(hipSetDevice(r->device));
+    HIPC(route_launch(r->spec, logits, (int)batch, top_indices, top_weights,
+                      stream ? static_cast<hipStream_t>(stream) : r->stream));
+  });
+}
+
+int llambda_hip_router_run(llambda_hip_router* r, const float* logits, size_t count,
+                           int64_t* top_indices, float* top_weights, size_t batch) {
+  return guarded([&] {
+    if (!r) failf("router_run: null router");
+    if (!logits || !top_indices || !top_weights) failf("router_run: null argument");
+    if (batch == 0 || batch > (1u << 24)) failf("router_run: bad batch %zu", batch);
+    const size_t E = (size_t)r->spec.experts, K = (size_t)r->spec.top_k;
+    if (count != batch * E) failf("router_run: element count %zu does not match %zu x %zu", count, batch, E);
+    std::lock_guard<std::mutex> lock(r->run_mutex);
+    HIPC(hipSetDevice(r->device));
+    if (batch > r->staged_tokens) {
+      r->staged_tokens = 0;
+      r->logits.alloc(batch * E * sizeof(float), "router logits");
+      r->indices.alloc(batch * K * sizeof(int), "expert indices");
+      r->weights.alloc(batch * K * sizeof(float), "expert weights");
+      r->staged_tokens = batch;
+    }
+    HIPC(hipMemcpyAsync(r->logits.ptr, logits, count * sizeof(float), hipMemcpyHostToDevice, r->stream));
+    HIPC(route_launch(r->spec, r->logits.as<float>(), (int)batch, r->indices.as<int>(), r->weights.as<float>(),
+                      r->stream));
+    std::vector<int> idx(batch * K);
+    HIPC(hipMemcpyAsync(idx.data(), r->indices.ptr, idx.size() * sizeof(int), hipMemcpyDeviceToHost, r->stream));
+    HIPC(hipMemcpyAsync(top_weights, r->weights.ptr, idx.size() * sizeof(float), hipMemcpyDeviceToHost, r->stream));
+    HIPC(hipStreamSynchronize(r->stream));
+    for (size_t i = 0; i < idx.size(); ++i) top_indices[i] = idx[i];
+  });
+}
+
+int llambda_hip_moe_session_set_router(llambda_hip_moe_session* s, llambda_hip_router* r) {
+  return guarded([&] {
+    if (!s) failf("moe_session_set_router: null session");
+    std::lock_guard<std::mutex> lock(s->run_mutex);
+    HIPC(hipSetDevice(s->device));
+    if (!r) {
+      s->plan.routed = 0;
+      return;
+    }
+    if (r->spec.experts != s->plan.experts || r->spec.top_k != s->plan.top_k)
+      failf("moe_session_set_router: a router of %d of %d experts on a layer of %d of %d", r->spec.top_k,
+            r->spec.experts, s->plan.top_k, s->plan.experts);
+    RouteSpec spec = r->spec;
+    if (spec.bias) {
+      DevBuf bias;
+      bias.alloc(r->host_bias.size() * sizeof(float), "router bias");
+      HIPC(hipMemcpyAsync(bias.ptr, r->host_bias.data(), bias.bytes, hipMemcpyHostToDevice, s->stream));
+      HIPC(hipStreamSynchronize(s->stream));
+      spec.bias = bias.as<float>();
+      s->route_bias.swap(bias);  // the old one is freed once the device is idle
+    }
+    s->plan.route = spec;
+    s->plan.routed = 1;
   });
 }
 
@@ -1962,6 +2091,151 @@ int llambda_hip_llama_session_sample(llambda_hip_llama_session* session,
       HIPC(hipEventSynchronize(session->done));
     }
     *token = run_sampler(s, session->logits.as<float>(), session->plan.vocab, params);
+  });
+}
+
+}  // extern "C"
+
+// --------------------------------------------------- sampling of a batch
+
+struct llambda_hip_batch_sampler {
+  std::mutex run_mutex;
+  int device = 0;
+  hipStream_t stream = nullptr;
+  size_t vocab = 0, max_rows = 0;
+  DevBuf chunk_max, chunk_mass;
+  DevBuf logits, params, tokens;  // device staging of the host-pointer runs
+  size_t staged = 0;
+  // recorded after every call; the next one, which shares the workspace, waits
+  hipEvent_t done = nullptr;
+  ~llambda_hip_batch_sampler() {
+    if (done) (void)hipEventDestroy(done);
+    if (stream) (void)hipStreamDestroy(stream);
+  }
+};
+
+namespace {
+
+void batch_sample_enqueue(llambda_hip_batch_sampler* s, SampleRows r, hipStream_t st) {
+  r.chunk_max = s->chunk_max.as<float>();
+  r.chunk_mass = s->chunk_mass.as<double>();
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  HIPC(hipStreamIsCapturing(st, &capture));
+  const bool ordered = capture == hipStreamCaptureStatusNone;
+  if (ordered) HIPC(hipStreamWaitEvent(st, s->done, 0));
+  HIPC(sample_rows_launch(r, st));
+  if (ordered) HIPC(hipEventRecord(s->done, st));
+}
+
+void check_batch_sample(const llambda_hip_batch_sampler* s, const char* what, const void* logits,
+                        size_t count, size_t rows, const llambda_hip_batch_sampling* a,
+                        const void* tokens) {
+  if (!s) failf("%s: null sampler", what);
+  if (!logits || !a || !a->random_value || !tokens) failf("%s: null argument", what);
+  if (count == 0 || count > s->vocab)
+    failf("%s: %zu logits do not fit the sampler (vocab %zu)", what, count, s->vocab);
+  if (rows == 0 || rows > s->max_rows) failf("%s: %zu rows are not in 1..%zu", what, rows, s->max_rows);
+}
+
+}  // namespace
+
+extern "C" {
+
+int llambda_hip_batch_sampler_create(size_t vocab, size_t max_rows,
+                                     llambda_hip_batch_sampler** result) {
+  return guarded([&] {
+    if (!result) failf("batch_sampler_create: null result pointer");
+    *result = nullptr;
+    if (vocab == 0 || vocab > (size_t)kBatchMaxVocab)
+      failf("batch_sampler_create: vocab %zu out of range (1..%d)", vocab, kBatchMaxVocab);
+    if (max_rows == 0 || max_rows > 65535)
+      failf("batch_sampler_create: max_rows %zu out of range (1..65535)", max_rows);
+    std::unique_ptr<llambda_hip_batch_sampler> s(new llambda_hip_batch_sampler());
+    s->device = current_device_checked();
+    s->vocab = vocab;
+    s->max_rows = max_rows;
+    HIPC(hipStreamCreateWithFlags(&s->stream, hipStreamNonBlocking));
+    HIPC(hipEventCreateWithFlags(&s->done, hipEventDisableTiming));
+    const size_t chunks = max_rows * (size_t)sample_chunks((int)vocab);
+    s->chunk_max.alloc(chunks * sizeof(float), "chunk maxima");
+    s->chunk_mass.alloc(chunks * sizeof(double), "chunk masses");
+    *result = s.release();
+  });
+}
+
+void llambda_hip_batch_sampler_destroy(llambda_hip_batch_sampler* sampler) { delete sampler; }
+
+int llambda_hip_batch_sampler_sample_device(llambda_hip_batch_sampler* s, const float* logits,
+                                            size_t count, size_t rows,
+                                            const llambda_hip_batch_sampling* a, int32_t* tokens,
+                                            void* stream) {
+  return guarded([&] {
+    check_batch_sample(s, "batch_sampler_sample_device", logits, count, rows, a, tokens);
+    if ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(tokens) |
+         reinterpret_cast<uintptr_t>(a->temperature) | reinterpret_cast<uintptr_t>(a->top_k) |
+         reinterpret_cast<uintptr_t>(a->top_p) | reinterpret_cast<uintptr_t>(a->min_p) |
+         reinterpret_cast<uintptr_t>(a->random_value)) & 3u)
+      failf("batch_sampler_sample_device: pointers must be 4-byte aligned");
+    std::lock_guard<std::mutex> lock(s->run_mutex);
+    HIPC(hipSetDevice(s->device));
+    SampleRows r{logits, (int)count, (int)rows, a->temperature, a->top_k, a->top_p, a->min_p,
+                 a->random_value, tokens, nullptr, nullptr};
+    batch_sample_enqueue(s, r, stream ? static_cast<hipStream_t>(stream) : s->stream);
+  });
+}
+
+int llambda_hip_batch_sampler_sample(llambda_hip_batch_sampler* s, const float* logits, size_t count,
+                                     size_t rows, const llambda_hip_batch_sampling* a,
+                                     int64_t* tokens) {
+  return guarded([&] {
+    check_batch_sample(s, "batch_sampler_sample", logits, count, rows, a, tokens);
+    for (size_t i = 0; i < rows; ++i) {
+      const float r = a->random_value[i], t = a->temperature ? a->temperature[i] : 1.f;
+      const float p = a->top_p ? a->top_p[i] : 1.f, q = a->min_p ? a->min_p[i] : 0.f;
+      const int32_t k = a->top_k ? a->top_k[i] : 0;
+      if (!(r >= 0.f && r < 1.f))
+        failf("Row %zu: RANDOM-VALUE must satisfy 0.0 <= value < 1.0, got %g.", i, (double)r);
+      if (k < 0) failf("Row %zu: TOP-K must be nonnegative, got %d.", i, k);
+      if (!(p > 0.f && p <= 1.f)) failf("Row %zu: TOP-P must satisfy 0.0 < p <= 1.0, got %g.", i, (double)p);
+      if (!(q >= 0.f && q <= 1.f)) failf("Row %zu: MIN-P must satisfy 0.0 <= p <= 1.0, got %g.", i, (double)q);
+      if (!(t >= 0.f && std::isfinite(t)))
+        failf("Row %zu: TEMPERATURE must be finite and not negative, got %g.", i, (double)t);
+    }
+    std::lock_guard<std::mutex> lock(s->run_mutex);
+    HIPC(hipSetDevice(s->device));
+    if (rows > s->staged) {
+      s->staged = 0;
+      s->logits.alloc(rows * s->vocab * sizeof(float), "batch sampling logits");
+      s->params.alloc(rows * 5 * sizeof(float), "batch sampling parameters");
+      s->tokens.alloc(rows * sizeof(int32_t), "batch sampling tokens");
+      s->staged = rows;
+    }
+    HIPC(hipMemcpyAsync(s->logits.ptr, logits, rows * count * sizeof(float), hipMemcpyHostToDevice, s->stream));
+    float* at = s->params.as<float>();
+    auto up = [&](const void* host) -> float* {
+      if (!host) return nullptr;
+      float* p = at;
+      at += rows;
+      HIPC(hipMemcpyAsync(p, host, rows * sizeof(float), hipMemcpyHostToDevice, s->stream));
+      return p;
+    };
+    SampleRows r{};
+    r.logits = s->logits.as<float>();
+    r.n = (int)count;
+    r.rows = (int)rows;
+    r.temperature = up(a->temperature);
+    r.top_k = reinterpret_cast<const int*>(up(a->top_k));
+    r.top_p = up(a->top_p);
+    r.min_p = up(a->min_p);
+    r.random = up(a->random_value);
+    r.tokens = s->tokens.as<int>();
+    batch_sample_enqueue(s, r, s->stream);
+    std::vector<int32_t> got(rows);
+    HIPC(hipMemcpyAsync(got.data(), s->tokens.ptr, rows * sizeof(int32_t), hipMemcpyDeviceToHost, s->stream));
+    HIPC(hipStreamSynchronize(s->stream));
+    for (size_t i = 0; i < rows; ++i)
+      if (got[i] < 0) failf("Row %zu: a NaN logit, or none above minus infinity.", i);
+    for (size_t i = 0; i < rows; ++i) tokens[i] = got[i];
   });
 }
 

@@ -20,6 +20,7 @@
 #pragma once
 
 #include "gemv.h"
+#include "route.h"
 
 namespace llhip {
 
@@ -94,6 +95,10 @@ struct MoePlan {
   float* lsum;         // [capacity][latent_in/16]       and their sums
   float* lat_y;        // [capacity][hidden]             ffn_latent_up output
   int* error;          // [1] nonzero after a run that hit a reference error
+  // a router of the caller's (moe_session_set_router) in place of the
+  // reference's gating
+  int routed;
+  RouteSpec route;
 };
 
 // Grouped expert product over a chunk table (moe_mfma.hip).

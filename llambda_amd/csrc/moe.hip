@@ -3,6 +3,7 @@
 #include "moe.h"
 #include "activations.h"
 #include "moe_gate.h"
+#include "route_token.h"
 
 #include <algorithm>
 #include <cfloat>
@@ -44,6 +45,46 @@ __global__ void __launch_bounds__(256) topk_gate_kernel(MoePlan p, int tokens, i
   const GateRank r = gate_token<JPL>(p, t, tokens, true, sel[threadIdx.x >> 6]);
   if (!single) return;  // the scan kernel counts the experts' pairs
   gate_chunk_table(p, r.valid, r.idx);
+}
+
+// The same with a router of the caller's (route_token.h) in the gating's place:
+// the logits are the router's products alone, the shared expert's gate stays
+// the layer's.
+constexpr int kRouteGateTokens = 2;  // a token's scores take up to 18 KB of LDS
+template <int JPL>
+__global__ void __launch_bounds__(64 * kRouteGateTokens) route_gate_kernel(MoePlan p, int tokens,
+                                                                           int single) {
+  __shared__ RouteScratch<JPL> scratch[kRouteGateTokens];
+  const int t = blockIdx.x * kRouteGateTokens + (threadIdx.x >> 6);
+  if (t >= tokens) return;
+  const int lane = threadIdx.x & 63, E = p.experts, K = p.top_k, ld = E + 1;
+  const bool has_shared_row = p.variant == kQwen3Next && p.shared_ffn > 0;
+  float raw[JPL + 1];
+#pragma unroll
+  for (int j = 0; j <= JPL; ++j) {
+    // slot JPL: the shared expert's gate (rows hold E + 1 entries, the last
+    // one unset without it)
+    const int e = j < JPL ? min(lane + kWave * j, E - 1) : has_shared_row ? E : 0;
+    float v = 0.f;
+    for (int ks = 0; ks < p.router_ks; ++ks) v += p.router_part[((int64_t)ks * tokens + t) * ld + e];
+    raw[j] = v;
+    if (j < JPL && lane + kWave * j < E) p.logits[(int64_t)t * ld + e] = v;
+  }
+  const float shared = raw[JPL];
+  float logits[JPL];
+#pragma unroll
+  for (int j = 0; j < JPL; ++j) logits[j] = raw[j];
+  const RouteRank r = route_token<JPL>(p.route, logits, lane, scratch[threadIdx.x >> 6]);
+  if (lane < K) {
+    p.top_idx[(int64_t)t * K + lane] = r.idx;
+    p.top_w[(int64_t)t * K + lane] = r.w;
+  }
+  if (lane == 0) {
+    if (has_shared_row) p.logits[(int64_t)t * ld + E] = shared;
+    p.shared_w[t] = has_shared_row ? sigmoid_ref(shared) : 1.f;
+    if (r.error) atomicOr(p.error, r.error);
+  }
+  if (single) gate_chunk_table(p, lane < K && r.idx >= 0, r.idx);
 }
 
 // ------------------------------------------------------------ scan/scatter
@@ -344,9 +385,20 @@ hipError_t moe_forward_launch(const MoePlan& p, const float* x, float* y, int to
   const bool joint_up = has_shared && p.sh_up_type == p.up_type && !Li;
   // one token whose up products run in one launch: that launch selects and
   // gates the token itself (one launch fewer)
-  const bool fuse_gate = single && mt == 0 && (!has_shared || joint_up) && K <= kMoeMaxTopK &&
+  const bool fuse_gate = single && !p.routed && mt == 0 && (!has_shared || joint_up) && K <= kMoeMaxTopK &&
                          jpl_for(E) <= 16;
-  if (!fuse_gate) {
+  if (p.routed) {
+    const dim3 tgrid((tokens + kRouteGateTokens - 1) / kRouteGateTokens);
+    switch (jpl_for(E)) {
+      case 1: e = launch(route_gate_kernel<1>, tgrid, dim3(64 * kRouteGateTokens), 0, s, p, tokens, single); break;
+      case 2: e = launch(route_gate_kernel<2>, tgrid, dim3(64 * kRouteGateTokens), 0, s, p, tokens, single); break;
+      case 4: e = launch(route_gate_kernel<4>, tgrid, dim3(64 * kRouteGateTokens), 0, s, p, tokens, single); break;
+      case 8: e = launch(route_gate_kernel<8>, tgrid, dim3(64 * kRouteGateTokens), 0, s, p, tokens, single); break;
+      case 16: e = launch(route_gate_kernel<16>, tgrid, dim3(64 * kRouteGateTokens), 0, s, p, tokens, single); break;
+      default: return hipErrorInvalidValue;
+    }
+    if (e != hipSuccess) return e;
+  } else if (!fuse_gate) {
     const dim3 tgrid((tokens + 3) / 4);
     switch (jpl_for(E)) {
       case 1: e = launch(topk_gate_kernel<1>, tgrid, dim3(256), 0, s, p, tokens, single); break;

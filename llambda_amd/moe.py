@@ -227,9 +227,88 @@ class HipMoeSession:
                                                                stream or None),
                "HIP MoE device run")
 
+    def set_router(self, router: Optional["HipRouter"]) -> None:
+        """Gate later runs with `router` instead of the layer's own gating (None restores it)."""
+        _check(native.lib().llambda_hip_moe_session_set_router(
+            self._live(), None if router is None else router._live()), "HIP MoE router")
+
     def sync(self, stream: int = 0) -> None:
         _check_moe(native.lib().llambda_hip_moe_session_sync(self._live(), stream or None),
                    "HIP MoE sync", self.layer.layer_index)
+
+
+SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+@dataclass
+class Routing:
+    """How a router's logits become experts and weights (llambda_hip_router_desc)."""
+    experts: int
+    top_k: int
+    score: str = "softmax"                    # or "sigmoid"
+    bias: Optional[np.ndarray] = None         # F32 [experts], added to the scores for the choice only
+    groups: int = 1                           # neighbouring experts / groups form one
+    top_groups: int = 1                       # groups whose experts may be chosen
+    group_rank: int = 1                       # a group scores the sum of its 1 or 2 highest
+    weights_norm: bool = True
+    weights_scale: float = 1.0
+
+
+class HipRouter:
+    def __init__(self, routing: Routing):
+        self.pointer = None
+        self.routing = routing
+        if routing.score not in SCORES:
+            raise HipBackendError(f"HIP router score {routing.score!r} is not one of {sorted(SCORES)}.")
+        d = native.RouterDesc()
+        d.score = SCORES[routing.score]
+        d.expert_count, d.top_k = routing.experts, routing.top_k
+        d.groups, d.top_groups, d.group_rank = routing.groups, routing.top_groups, routing.group_rank
+        bias = None
+        if routing.bias is not None:
+            bias = np.ascontiguousarray(routing.bias, dtype=np.float32)
+            if bias.size != routing.experts:
+                raise HipBackendError(f"HIP router bias has {bias.size} elements, not {routing.experts}.")
+            d.bias = bias.ctypes.data
+        d.weights_norm = int(bool(routing.weights_norm))
+        d.weights_scale = routing.weights_scale
+        handle = ctypes.c_void_p()
+        _check(native.lib().llambda_hip_router_create(ctypes.byref(d), ctypes.byref(handle)),
+               "HIP router creation")
+        self.pointer = handle.value
+
+    def close(self) -> None:
+        if self.pointer:
+            native.lib().llambda_hip_router_destroy(self.pointer)
+            self.pointer = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:  # noqa: BLE001 - interpreter shutdown
+            pass
+
+    def _live(self):
+        if not self.pointer:
+            raise HipBackendError("HIP router is closed.")
+        return self.pointer
+
+    def run(self, logits: np.ndarray):
+        """(indices int64, weights) [tokens][top_k] for logits [tokens][experts]."""
+        logits = np.ascontiguousarray(logits, dtype=np.float32).reshape(-1, self.routing.experts)
+        tokens = logits.shape[0]
+        idx = np.empty((tokens, self.routing.top_k), dtype=np.int64)
+        w = np.empty((tokens, self.routing.top_k), dtype=np.float32)
+        _check(native.lib().llambda_hip_router_run(self._live(), logits.ctypes.data, logits.size,
+                                                   idx.ctypes.data, w.ctypes.data, tokens), "HIP router run")
+        return idx, w
+
+    def run_device(self, logits_ptr: int, indices_ptr: int, weights_ptr: int, tokens: int,
+                   stream: int = 0) -> None:
+        """Device pointers; int32 indices."""
+        _check(native.lib().llambda_hip_router_run_device(
+            self._live(), logits_ptr or None, indices_ptr or None, weights_ptr or None, tokens,
+            stream or None), "HIP router device run")
 
 
 def moe_layer_from_model(model, layer_index: int, variant: int, *, expert_used_count: int,

@@ -110,6 +110,21 @@ class SsmDesc(ctypes.Structure):
     ]
 
 
+class RouterDesc(ctypes.Structure):
+    """llambda_hip_router_desc."""
+    _fields_ = [
+        ("score", c_int), ("expert_count", c_i64), ("top_k", c_i64), ("groups", c_i64),
+        ("top_groups", c_i64), ("group_rank", c_i64), ("bias", c_void_p), ("weights_norm", c_int),
+        ("weights_scale", ctypes.c_float),
+    ]
+
+
+class BatchSampling(ctypes.Structure):
+    """llambda_hip_batch_sampling."""
+    _fields_ = [("temperature", c_void_p), ("top_k", c_void_p), ("top_p", c_void_p),
+                ("min_p", c_void_p), ("random_value", c_void_p)]
+
+
 class GgufTensor(ctypes.Structure):
     """llambda_hip_gguf_tensor."""
     _fields_ = [("name", c_void_p), ("name_length", c_size), ("dimension_count", ctypes.c_uint32),
@@ -155,6 +170,12 @@ SIGNATURES = {
     "llambda_hip_moe_session_run_device_noalloc": (c_int, [c_void_p, c_void_p, c_void_p, c_size,
                                                            c_void_p]),
     "llambda_hip_select_top_k": (c_int, [c_void_p, c_size, c_size, c_size, c_void_p, c_void_p]),
+    "llambda_hip_router_create": (c_int, [ctypes.POINTER(RouterDesc), ctypes.POINTER(c_void_p)]),
+    "llambda_hip_router_destroy": (None, [c_void_p]),
+    "llambda_hip_router_run": (c_int, [c_void_p, c_void_p, c_size, c_void_p, c_void_p, c_size]),
+    "llambda_hip_router_run_device": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_size,
+                                              c_void_p]),
+    "llambda_hip_moe_session_set_router": (c_int, [c_void_p, c_void_p]),
     "llambda_hip_stream_read": (c_int, [c_void_p, c_size, c_void_p, c_void_p]),
     "llambda_hip_llama_session_create": (c_int, [ctypes.POINTER(LlamaDesc),
                                                  ctypes.POINTER(c_void_p)]),
@@ -189,6 +210,13 @@ SIGNATURES = {
                                            ctypes.POINTER(Sampling), ctypes.POINTER(c_i64)]),
     "llambda_hip_llama_session_sample": (c_int, [c_void_p, c_void_p, ctypes.POINTER(Sampling),
                                                  ctypes.POINTER(c_i64)]),
+    "llambda_hip_batch_sampler_create": (c_int, [c_size, c_size, ctypes.POINTER(c_void_p)]),
+    "llambda_hip_batch_sampler_destroy": (None, [c_void_p]),
+    "llambda_hip_batch_sampler_sample_device": (c_int, [c_void_p, c_void_p, c_size, c_size,
+                                                        ctypes.POINTER(BatchSampling), c_void_p,
+                                                        c_void_p]),
+    "llambda_hip_batch_sampler_sample": (c_int, [c_void_p, c_void_p, c_size, c_size,
+                                                 ctypes.POINTER(BatchSampling), c_void_p]),
     "llambda_hip_gguf_open": (c_int, [c_char_p, ctypes.POINTER(c_void_p)]),
     "llambda_hip_gguf_close": (None, [c_void_p]),
     "llambda_hip_gguf_header": (c_int, [c_void_p, ctypes.POINTER(ctypes.c_uint32),

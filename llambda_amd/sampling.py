@@ -89,3 +89,65 @@ class HipSampler:
                                                          ctypes.byref(tok)) != 0:
             raise SamplingError(native.last_error())
         return tok.value
+
+
+class HipBatchSampler:
+    """One token per row of a batch of logits (llambda_hip_batch_sampler_*): temperature, top-k,
+    top-p and min-p of each row's own, from given random numbers, in 64 bits."""
+
+    def __init__(self, vocab: int, max_rows: int):
+        self._h = None
+        handle = ctypes.c_void_p()
+        if native.lib().llambda_hip_batch_sampler_create(vocab, max_rows, ctypes.byref(handle)) != 0:
+            raise SamplingError(native.last_error())
+        self._h = handle
+        self.vocab = vocab
+        self.max_rows = max_rows
+
+    def close(self) -> None:
+        if getattr(self, "_h", None):
+            native.lib().llambda_hip_batch_sampler_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:  # noqa: BLE001 - interpreter shutdown
+            pass
+
+    def sample_device(self, logits_ptr: int, rows: int, tokens_ptr: int, random_ptr: int, *,
+                      temperature_ptr: int = 0, top_k_ptr: int = 0, top_p_ptr: int = 0,
+                      min_p_ptr: int = 0, count: Optional[int] = None, stream: int = 0) -> None:
+        """Device pointers: logits [rows][count] (the vocabulary by default), int32 tokens, float32
+        parameters (int32 top-k) of each row, 0 = the default for all.  Not waited for."""
+        p = native.BatchSampling(temperature_ptr or None, top_k_ptr or None, top_p_ptr or None,
+                                 min_p_ptr or None, random_ptr or None)
+        if native.lib().llambda_hip_batch_sampler_sample_device(
+                self._h, logits_ptr or None, self.vocab if count is None else count, rows,
+                ctypes.byref(p), tokens_ptr or None, stream or None) != 0:
+            raise SamplingError(native.last_error())
+
+    def sample(self, logits, *, random_value, temperature=None, top_k=None, top_p=None,
+               min_p=None) -> np.ndarray:
+        """Tokens (int64) of host logits [rows][count]; a parameter is one number or one per row."""
+        a = np.ascontiguousarray(logits, dtype=np.float32)
+        if a.ndim != 2:
+            raise SamplingError(f"logits have {a.ndim} dimensions, not 2")
+        rows = a.shape[0]
+        keep = []
+
+        def each(v, dtype):
+            if v is None:
+                return None
+            v = np.ascontiguousarray(np.broadcast_to(np.asarray(v, dtype=dtype), (rows,)))
+            keep.append(v)
+            return v.ctypes.data
+
+        p = native.BatchSampling(each(temperature, np.float32), each(top_k, np.int32),
+                                 each(top_p, np.float32), each(min_p, np.float32),
+                                 each(random_value, np.float32))
+        out = np.empty(rows, dtype=np.int64)
+        if native.lib().llambda_hip_batch_sampler_sample(self._h, a.ctypes.data, a.shape[1], rows,
+                                                         ctypes.byref(p), out.ctypes.data) != 0:
+            raise SamplingError(native.last_error())
+        return out

@@ -1,0 +1,51 @@
+"""Routers and batch samplers: what their creation refuses before any device work."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from llambda_amd import native
+from llambda_amd.hip_backend import HipBackendError
+from llambda_amd.moe import HipRouter, Routing
+from llambda_amd.sampling import HipBatchSampler, SamplingError
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(experts=0, top_k=1), "expert_count 0"), (dict(experts=1025, top_k=1), "expert_count 1025"),
+    (dict(experts=8, top_k=0), "top_k 0"), (dict(experts=8, top_k=9), "top_k 9 is not in 1..8"),
+    (dict(experts=128, top_k=65), "top_k 65 is not in 1..64"),
+    (dict(experts=8, top_k=1, groups=0), "groups 0"), (dict(experts=8, top_k=1, groups=3), "3 groups do not divide"),
+    (dict(experts=256, top_k=1, groups=128), "groups 128 is not in 1..64"),
+    (dict(experts=8, top_k=1, groups=2, top_groups=3), "top_groups 3"),
+    (dict(experts=8, top_k=5, groups=2, top_groups=1), "top_k 5 is not in 1..4"),
+    (dict(experts=8, top_k=1, group_rank=3), "group_rank 3"), (dict(experts=8, top_k=1, group_rank=0), "group_rank 0"),
+    (dict(experts=8, top_k=1, weights_scale=np.inf), "weights_scale"), (dict(experts=8, top_k=1, score="relu"), "relu"),
+    (dict(experts=8, top_k=1, bias=np.zeros(7, np.float32)), "bias has 7 elements, not 8"),
+])
+def test_routings_that_are_refused(kw, text):
+    with pytest.raises(HipBackendError, match=text):
+        HipRouter(Routing(**kw))
+
+
+def test_null_arguments():
+    L = native.lib()
+    assert L.llambda_hip_router_create(None, None) == -1
+    assert L.llambda_hip_router_create(None, ctypes.byref(ctypes.c_void_p())) == -1
+    d = native.RouterDesc(score=7, expert_count=8, top_k=1, groups=1, top_groups=1, group_rank=1)
+    assert L.llambda_hip_router_create(ctypes.byref(d), ctypes.byref(ctypes.c_void_p())) == -1
+    assert "unknown score 7" in native.last_error()
+    assert L.llambda_hip_router_run(None, None, 0, None, None, 1) == -1
+    assert L.llambda_hip_router_run_device(None, None, None, None, 1, None) == -1
+    assert L.llambda_hip_moe_session_set_router(None, None) == -1
+    L.llambda_hip_router_destroy(None)
+    L.llambda_hip_batch_sampler_destroy(None)
+    assert L.llambda_hip_batch_sampler_create(10, 1, None) == -1
+    assert L.llambda_hip_batch_sampler_sample(None, None, 1, 1, None, None) == -1
+    assert L.llambda_hip_batch_sampler_sample_device(None, None, 1, 1, None, None, None) == -1
+
+
+@pytest.mark.parametrize("vocab,rows,text", [(0, 1, "vocab 0"), (262145, 1, "vocab 262145"), (10, 0, "max_rows 0"),
+                                             (10, 65536, "max_rows 65536")])
+def test_batch_samplers_that_are_refused(vocab, rows, text):
+    with pytest.raises(SamplingError, match=text):
+        HipBatchSampler(vocab, rows)
