@@ -58,7 +58,7 @@ struct SsmLayerPlan {
   int2* segments;          // [max_segments]: sequence, index within it
   int2* chunks;            // [max_chunks]: sequence, index within it
   int* counts;             // segments, chunks
-  float* bc;               // [chunk][G][2][kSsmChunk][N]: B, C after the convolution
+  uint8_t* images;         // [chunk][G][ssm_image_bytes]: B, C after the convolution, C B^T
   float* decay;            // [chunk][H][3][kSsmChunk]: dt, log2 of the decay since the chunk's start (hi, lo)
   // segments of the sequences that have several, max_states in all
   float* seg_states;       // [H][P][N] each: the state that enters it
@@ -81,6 +81,7 @@ inline int ssm_row(const SsmLayerPlan& p) {
 int ssm_segment_tokens(const SsmLayerPlan& p, int64_t tokens);
 int64_t ssm_max_chunks(int64_t tokens, int64_t sequences);
 int64_t ssm_max_segments(const SsmLayerPlan& p, int64_t tokens, int64_t sequences);
+size_t ssm_image_bytes(int state);
 int64_t ssm_max_states(const SsmLayerPlan& p, int64_t tokens);
 
 // Enqueue a call on `stream`: one token of each sequence where offsets is

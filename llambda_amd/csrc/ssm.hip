@@ -47,8 +47,9 @@ __device__ __forceinline__ float exp_f32(float v) {
   return fabsf(t) < 126.f ? fmaf(e, r * 0.69314718056f, e) : e;
 }
 __device__ __forceinline__ float silu_f32(float v) {
-  // large negative v: exp overflows and v / inf = -0, as the limit is
-  return v / (1.f + exp_f32(-v));
+  // (the reciprocal is good to one unit); large negative v: exp overflows, the
+  // reciprocal is 0 and the result -0, as the limit is
+  return v * __builtin_amdgcn_rcpf(1.f + exp_f32(-v));
 }
 // log(1 + e^v) = max(v, 0) + log1p(e^-|v|)
 __device__ __forceinline__ float softplus_f32(float v) {
@@ -182,105 +183,219 @@ __device__ __forceinline__ const float* conv_taps(const SsmLayerPlan& p, int slo
   return slot < 0 ? nullptr : p.conv_states + (int64_t)slot * (p.conv - 1) * channels;
 }
 
-// Block (chunk, y): y < blocks of 256 channels of B | C: their convolution,
-// a thread taking four channels of eight tokens; then blocks of eight heads:
-// dt and the decays, a lane per token.
-constexpr int kPrepChannels = 256;
+// x = hi + mid + lo in bf16, 24 significant bits and single precision's whole
+// range, so products need no scales: |x - hi - mid - lo| <= 2^-25 |x|.  Eight
+// values, packed as a matrix operand's lane holds them.
+struct Split8 {
+  u32x4 hi, mid, lo;
+};
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{a, b}, bf16x2));
+}
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+  hi = bf16_pair(a, b);
+  a -= __builtin_bit_cast(float, hi << 16);
+  b -= __builtin_bit_cast(float, hi & 0xFFFF0000u);
+  mid = bf16_pair(a, b);
+  a -= __builtin_bit_cast(float, mid << 16);
+  b -= __builtin_bit_cast(float, mid & 0xFFFF0000u);
+  lo = bf16_pair(a, b);
+}
+__device__ __forceinline__ Split8 split8(const float* v) {
+  Split8 r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    uint32_t h, m, l;
+    split_pair(v[2 * e], v[2 * e + 1], h, m, l);
+    r.hi[e] = h;
+    r.mid[e] = m;
+    r.lo[e] = l;
+  }
+  return r;
+}
+
+// What a chunk's scan reads of its group, in operand order: fragments of 64
+// lanes x 16 bytes, lane (r, g) = (lane & 15, lane >> 4).
+//   C   [i tile][n block of 32][hi, mid, lo]: token 16 it + r; element e is
+//       n = 32 t + 16 (e / 4) + 4 g + e % 4, the elements of the state's result
+//       tiles that the same lane holds (zeros past n)
+//   B^T [n tile][hi, mid, lo]: row n = 16 nt + r; element e is token
+//       16 (e / 4) + 4 g + e % 4
+//   S^T [(j, i) tiles (0, 0), (0, 1), (1, 1)], fp32: rows j = 16 jt + 4 g ..
+//       + 3, column i = 16 it + r
+constexpr int kFragment = 1024;
+constexpr int n_blocks(int nt) { return (nt + 1) / 2; }
+constexpr int c_fragments(int nt) { return 6 * n_blocks(nt); }
+constexpr int b_fragments(int nt) { return 3 * nt; }
+constexpr int image_fragments(int nt) { return c_fragments(nt) + b_fragments(nt) + 3; }
+
+size_t ssm_image_bytes(int state) { return (size_t)image_fragments(state / 16) * kFragment; }
+
+// Block (chunk, y): y < groups: that group's B and C after the convolution (a
+// thread takes four channels of eight tokens), as the images above; then
+// blocks of eight heads: dt and the decays, a lane per token.
 constexpr int kPrepHeads = 8;
 
-template <int W>
+template <int NT, int W>
 __global__ void __launch_bounds__(256) ssm_prepare_kernel(SsmLayerPlan p, SsmCall c) {
+  constexpr int N = 16 * NT, Q = kSsmChunk, LD = N + 4, NB = n_blocks(NT);
+  __shared__ float sbc[2][Q * LD];
   const int chunk = blockIdx.x;
   if (chunk >= p.counts[1]) return;
   const int2 at = p.chunks[chunk];
   const SsmSequence s = p.sequences[at.x];
   if (!s.run) return;
-  const int inner = p.heads * p.head_dim, gn = p.groups * p.state, channels = inner + 2 * gn;
+  const int inner = p.heads * p.head_dim, gn = p.groups * N, channels = inner + 2 * gn;
   const int64_t stride = inner + channels + p.heads;
   const float* rows = c.x + (int64_t)s.begin * stride + inner;
-  const int tid = threadIdx.x, t0 = at.y * kSsmChunk;
-  const int conv_blocks = (2 * gn + kPrepChannels - 1) / kPrepChannels;
-  if ((int)blockIdx.y < conv_blocks) {
-    const int bc = blockIdx.y * kPrepChannels + 4 * (tid & 63);  // within B | C
-    if (bc >= 2 * gn) return;
-    const int ch = inner + bc, q0 = 8 * (tid >> 6);
+  const int tid = threadIdx.x, t0 = at.y * Q;
+  if ((int)blockIdx.y < p.groups) {
+    const int group = blockIdx.y;
     const float* taps = conv_taps(p, s.from);
-    floatx4 w[W], r[8 + W - 1];
+    for (int item = tid; item < 2 * N; item += 256) {
+      const int quad = item % (N / 2), q0 = 8 * (item / (N / 2));
+      const int which = quad >= N / 4, n = 4 * (quad - which * (N / 4));
+      const int ch = inner + which * gn + group * N + n;
+      floatx4 w[W], r[8 + W - 1];
 #pragma unroll
-    for (int k = 0; k < 8 + W - 1; ++k)
-      r[k] = raw4(rows, stride, taps, channels, W, t0 + q0 - (W - 1) + k, s.length, ch);
+      for (int k = 0; k < 8 + W - 1; ++k)
+        r[k] = raw4(rows, stride, taps, channels, W, t0 + q0 - (W - 1) + k, s.length, ch);
 #pragma unroll
-    for (int k = 0; k < W; ++k)
-      w[k] = *reinterpret_cast<const floatx4*>(p.conv_weight + (int64_t)k * channels + ch);
-    const floatx4 b = *reinterpret_cast<const floatx4*>(p.conv_bias + ch);
-    // [chunk][group][B, C][token][n]
-    const int which = bc >= gn, inside = bc - which * gn;
-    float* out = p.bc + ((((int64_t)chunk * p.groups + inside / p.state) * 2 + which) * kSsmChunk + q0) *
-                            p.state + inside % p.state;
+      for (int k = 0; k < W; ++k)
+        w[k] = *reinterpret_cast<const floatx4*>(p.conv_weight + (int64_t)k * channels + ch);
+      const floatx4 b = *reinterpret_cast<const floatx4*>(p.conv_bias + ch);
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      floatx4 v = b;
+      for (int q = 0; q < 8; ++q) {
+        floatx4 v = b;
 #pragma unroll
-      for (int k = 0; k < W; ++k) v += w[k] * r[q + k];
-      floatx4 u;
+        for (int k = 0; k < W; ++k) v += w[k] * r[q + k];
+        floatx4 u;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) u[e] = t0 + q0 + q < s.length ? silu_f32(v[e]) : 0.f;
-      *reinterpret_cast<floatx4*>(out + (int64_t)q * p.state) = u;
+        for (int e = 0; e < 4; ++e) u[e] = t0 + q0 + q < s.length ? silu_f32(v[e]) : 0.f;
+        *reinterpret_cast<floatx4*>(&sbc[which][(q0 + q) * LD + n]) = u;
+      }
+    }
+    __syncthreads();
+    const int lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
+    uint8_t* image = p.images + ((int64_t)chunk * p.groups + group) * image_fragments(NT) * kFragment;
+    if (wave < 3) {
+      const int jt = wave == 2, it = wave > 0;
+      floatx4 acc{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const floatx4 a = *reinterpret_cast<const floatx4*>(&sbc[0][(16 * jt + col) * LD + 16 * n + 4 * g]);
+        const floatx4 b = *reinterpret_cast<const floatx4*>(&sbc[1][(16 * it + col) * LD + 16 * n + 4 * g]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc = mfma4f32(a[e], b[e], acc);
+      }
+      *reinterpret_cast<floatx4*>(image + (c_fragments(NT) + b_fragments(NT) + wave) * kFragment + 16 * lane) = acc;
+    }
+    for (int f = wave; f < 2 * NB + NT; f += 4) {
+      float v[8];
+      int at3;
+      if (f < 2 * NB) {
+        const int it = f / NB, t = f - it * NB;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          floatx4 q{0.f, 0.f, 0.f, 0.f};
+          if (2 * t + half < NT)
+            q = *reinterpret_cast<const floatx4*>(&sbc[1][(16 * it + col) * LD + 32 * t + 16 * half + 4 * g]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[4 * half + e] = q[e];
+        }
+        at3 = 3 * f;
+      } else {
+        const int nt = f - 2 * NB;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = sbc[0][(16 * (e >> 2) + 4 * g + (e & 3)) * LD + 16 * nt + col];
+        at3 = c_fragments(NT) + 3 * nt;
+      }
+      const Split8 r = split8(v);
+      u32x4* out = reinterpret_cast<u32x4*>(image + at3 * kFragment) + lane;
+      out[0] = r.hi;
+      out[kFragment / 16] = r.mid;
+      out[2 * kFragment / 16] = r.lo;
     }
     return;
   }
-  const int h = ((int)blockIdx.y - conv_blocks) * kPrepHeads + (tid >> 5), q = tid & 31;
+  const int h = ((int)blockIdx.y - p.groups) * kPrepHeads + (tid >> 5), q = tid & 31;
   if (h >= p.heads) return;
   const bool in = t0 + q < s.length;
   const float dt = in ? softplus_f32(rows[(int64_t)(t0 + q) * stride + channels + h] + p.dt_bias[h]) : 0.f;
   double sum = in ? log2_decay(dt, p.a[h]) : 0.0;
-  for (int o = 1; o < kSsmChunk; o <<= 1) {
+  for (int o = 1; o < Q; o <<= 1) {
     const double v = __shfl_up(sum, o, 32);
     if (q >= o) sum += v;
   }
-  float* out = p.decay + ((int64_t)chunk * p.heads + h) * 3 * kSsmChunk + q;
+  float* out = p.decay + ((int64_t)chunk * p.heads + h) * 3 * Q + q;
   const float hi = (float)sum;
   out[0] = dt;
-  out[kSsmChunk] = hi;
-  out[2 * kSsmChunk] = (float)(sum - (double)hi);
+  out[Q] = hi;
+  out[2 * Q] = (float)(sum - (double)hi);
 }
 
 // ------------------------------------------------------------------ the scan
 
-// acc += A B over 32 K elements (16 with N8 = 4): a lane's element e of both
-// operands is the same K element.
-template <int N8>
-__device__ __forceinline__ floatx4 mma(const float* a, const float* b, floatx4 acc) {
-#pragma unroll
-  for (int e = 0; e < N8; ++e) acc = mfma4f32(a[e], b[e], acc);
-  return acc;
+// acc += A B over 32 K elements to single precision: the six products of
+// parts above 2^-24 of the whole.  A lane's element e of both operands is the
+// same K element.
+__device__ __forceinline__ floatx4 mma_one(const u32x4& a, const u32x4& b, const floatx4& c) {
+  return mfma32(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c);
 }
 
-constexpr int kScanWaves = 4;
-constexpr int kScanTiles = 8;  // column tiles of 16 channels per workgroup, two per wave
+constexpr int kScanWaves = 8;
+constexpr int kScanHeads = 4;  // of a workgroup at most (their masked products take 6 KB of LDS each)
+
+// Column tiles of 16 channels per wavefront: the state of one takes N / 4
+// registers.
+constexpr int scan_tiles(int nt) { return nt > 8 ? 1 : 2; }
+// Images in LDS: two, so that a chunk's loads have the chunk before to run;
+// one of N = 256, whose halves are loaded while the other is used.
+constexpr int scan_buffers(int nt) { return nt > 8 ? 1 : 2; }
 
 // Heads per workgroup: as many whole heads of one group as fit its tiles.
 static int scan_heads(const SsmLayerPlan& p) {
   const int share = p.heads / p.groups;
-  int n = std::max(1, kScanTiles * 16 / p.head_dim);
+  int n = std::min(kScanHeads, std::max(1, kScanWaves * scan_tiles(p.state / 16) * 16 / p.head_dim));
   while (share % n) --n;
   return n;
 }
 
+// LDS of a scan workgroup, in bytes.
+template <int NT, bool STATES>
+struct ScanLds {
+  static constexpr int buffers = STATES ? 2 : scan_buffers(NT);
+  static constexpr int image = (STATES ? b_fragments(NT) : image_fragments(NT)) * kFragment;
+  static constexpr int products = STATES ? 0 : 6 * kFragment;  // per head: [i tile][hi, mid, lo]
+  static constexpr int decays = 3 * kSsmChunk * 4;             // per head and buffer
+  static constexpr int tables = 2 * kSsmChunk * 4;             // per head
+  static constexpr int bytes(int hw) { return buffers * (image + hw * decays) + hw * (products + tables); }
+};
+
 // One segment of `hw` heads.  STATES: only the segment's own state, from
 // zeros, to the next segment's place; else outputs and, in a sequence's last
 // segment, the state to its slot.
+//
+// A wavefront owns column tiles (16 channels of a head): their part of the
+// state, x, and outputs.  Per chunk the wavefronts first share the work of the
+// masked products M = S o L (three tiles a head) and of the decay tables, then
+// each forms its tiles' outputs, then its state.  The images of the next chunk
+// come into LDS meanwhile, by loads that need no registers.
 template <int NT, int W, bool STATES>
 __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan p, SsmCall c,
                                                                    int segment_tokens, int hw) {
-  constexpr int N = 16 * NT, Q = kSsmChunk, LD = N + 4;
-  extern __shared__ float lds[];
-  float* sb = lds;                      // [Q][LD]
-  float* sc = sb + Q * LD;              // [Q][LD]
-  float* sm = sc + (STATES ? 0 : Q * LD);  // [hw][3 tiles][64 lanes][4]
-  float* sd = sm + (STATES ? 0 : hw * 3 * 256);  // [hw][3][Q]
+  using Lds = ScanLds<NT, STATES>;
+  constexpr int N = 16 * NT, Q = kSsmChunk, NB = n_blocks(NT), TPW = scan_tiles(NT), BUF = Lds::buffers;
+  constexpr int kC = c_fragments(NT), kB = b_fragments(NT);
+  constexpr int kBAt = STATES ? 0 : kC, kSAt = kC + kB;  // fragments within an image in LDS
+  extern __shared__ __align__(16) uint8_t lds[];
+  uint8_t* products = lds + BUF * (Lds::image + hw * Lds::decays);
+  float* tables = reinterpret_cast<float*>(products + hw * Lds::products);  // [hw][e, w][Q]
+  auto image_at = [&](int buf) { return lds + buf * (Lds::image + hw * Lds::decays); };
+  auto decays_at = [&](int buf) { return reinterpret_cast<float*>(image_at(buf) + Lds::image); };
+
   const int sets = p.heads / hw;
-  // groups vary fastest, so that the workgroups that read one group's B and C
+  // groups vary fastest, so that the workgroups that read one group's images
   // sit on one XCD where there are eight groups
   const int set_in_group = sets / p.groups;
   const int seg = blockIdx.x / sets, rest = blockIdx.x - seg * sets;
@@ -290,21 +405,39 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
   if (!s.run) return;
   if (STATES && at.y == s.segments - 1) return;  // no segment follows
   const int group = rest % p.groups, h0 = (group * set_in_group + rest / p.groups) * hw;
-  const int inner = p.heads * p.head_dim, channels = inner + 2 * p.groups * p.state;
+  const int inner = p.heads * p.head_dim, channels = inner + 2 * p.groups * N;
   const int64_t stride = inner + channels + p.heads;
   const float* rows = c.x + (int64_t)s.begin * stride + inner;
   const float* taps = conv_taps(p, s.from);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int t_begin = at.y * segment_tokens, t_end = min(s.length, t_begin + segment_tokens);
+
+  // the loads of a chunk's image (parts: 1 = C, S and decays, 2 = B)
+  auto request = [&](int t, int buf, int parts) {
+    const int64_t chunk = s.chunk0 + t / Q;
+    const uint8_t* img = uniform_ptr(p.images + (chunk * p.groups + group) * image_fragments(NT) * kFragment);
+    const uint32_t to = lds_address(image_at(buf));
+    for (int f = wave; f < image_fragments(NT); f += kScanWaves) {
+      const bool is_b = f >= kC && f < kC + kB;
+      if (is_b ? !(parts & 2) : (STATES || !(parts & 1))) continue;
+      load_lds16(img, f * kFragment + 16 * lane, __builtin_amdgcn_readfirstlane(to + (f - (STATES ? kC : 0)) * kFragment));
+    }
+    if (parts & 1) {
+      const uint8_t* dec = uniform_ptr(reinterpret_cast<const uint8_t*>(p.decay + (chunk * p.heads + h0) * 3 * Q));
+      const uint32_t dto = __builtin_amdgcn_readfirstlane(lds_address(decays_at(buf)) + 1024 * wave);
+      if (64 * wave + lane < hw * Lds::decays / 16) load_lds16(dec, 1024 * wave + 16 * lane, dto);
+    }
+  };
 
   // this wave's column tiles: channels [p0, p0 + 16) of a head
   const int per_head = p.head_dim / 16, tiles = hw * per_head;
-  bool on[2];
-  int head[2], ch[2];
-  float skip[2], w[2][W], bias[2];
-  floatx4 st[2][NT];
+  bool on[TPW];
+  int head[TPW], ch[TPW];
+  float skip[TPW], w[TPW][W], bias[TPW];
+  floatx4 st[TPW][2 * NB];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < TPW; ++k) {
     const int tile = wave + kScanWaves * k;
     on[k] = tile < tiles;
     head[k] = on[k] ? tile / per_head : 0;
@@ -319,167 +452,236 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
       else if (s.from >= 0) src = p.ssm_states + (int64_t)s.from * inner * N;
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-      st[k][n] = src && on[k] ? *reinterpret_cast<const floatx4*>(src + (int64_t)ch[k] * N + 16 * n + 4 * g)
-                              : floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < 2 * NB; ++n)
+      st[k][n] = src && on[k] && n < NT ? *reinterpret_cast<const floatx4*>(src + (int64_t)ch[k] * N + 16 * n + 4 * g)
+                                        : floatx4{0.f, 0.f, 0.f, 0.f};
   }
-  float total_hi[2] = {0.f, 0.f}, total_lo[2] = {0.f, 0.f};
+  float total_hi[TPW] = {}, total_lo[TPW] = {};
 
-  for (int t0 = t_begin; t0 < t_end; t0 += Q) {
-    const int64_t chunk = s.chunk0 + t0 / Q;
-    __syncthreads();  // the last chunk's operands have been read
-    {
-      const floatx4* src = reinterpret_cast<const floatx4*>(p.bc + (chunk * p.groups + group) * 2 * Q * N);
-      constexpr int kVec = Q * N / 4;
-      for (int i = tid; i < (STATES ? 1 : 2) * kVec; i += 64 * kScanWaves) {
-        const int which = i / kVec, r = (i - which * kVec) / (N / 4), q = i % (N / 4);
-        *reinterpret_cast<floatx4*>((which ? sc : sb) + r * LD + 4 * q) = src[i];
-      }
-      const float* dsrc = p.decay + (chunk * p.heads + h0) * 3 * Q;
-      for (int i = tid; i < hw * 3 * Q; i += 64 * kScanWaves) sd[i] = dsrc[i];
-    }
-    // x of the lane's tokens 4 g .. + 3 and 16 + 4 g .. + 3
-    float x[2][8];
+  // raw x of the lane's tokens 4 g .. + 3 and 16 + 4 g .. + 3, with the rows before each run
+  float raw[TPW][2][4 + W - 1];
+  auto fetch = [&](int t0) {
+    const bool inside = t0 >= W - 1 && t0 + Q <= t_end;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      if (!on[k]) continue;
+    for (int k = 0; k < TPW; ++k)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        float r[4 + W - 1];
-        const int t = t0 + 16 * half + 4 * g;
+        const int t = t0 + 16 * half - (W - 1);
+        if (!on[k]) continue;
+        if (inside) {
+          const uint32_t off = (uint32_t)(4 * g) * (uint32_t)stride + (uint32_t)ch[k];
 #pragma unroll
-        for (int j = 0; j < 4 + W - 1; ++j)
-          r[j] = raw1(rows, stride, taps, channels, W, t - (W - 1) + j, t_end, ch[k]);
+          for (int j = 0; j < 4 + W - 1; ++j) raw[k][half][j] = (rows + (int64_t)(t + j) * stride)[off];
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float v = bias[k];
-#pragma unroll
-          for (int j = 0; j < W; ++j) v = fmaf(w[k][j], r[e + j], v);
-          x[k][4 * half + e] = t + e < t_end ? silu_f32(v) : 0.f;
+          for (int j = 0; j < 4 + W - 1; ++j)
+            raw[k][half][j] = raw1(rows, stride, taps, channels, W, t + 4 * g + j, t_end, ch[k]);
         }
       }
+  };
+
+  if constexpr (!STATES) {
+    // M's upper right quarter is zero throughout
+    for (int i = tid; i < hw * 3 * 64; i += 64 * kScanWaves) {
+      u32x2* z = reinterpret_cast<u32x2*>(products + (i / 192) * Lds::products + (i % 192) * 16 + 8);
+      *z = u32x2{0u, 0u};
     }
-    // A non-finite x_j would reach the tokens before it, as 0 x_j in the masked
-    // part of the product: the products take zero in its place, and the
-    // channel's outputs from token j on are NaN (its state too, by x itself).
-    float xf[2][8];
-    int first_bad[2] = {Q, Q};
+  }
+  if (t_begin < t_end) {
+    request(t_begin, 0, BUF == 2 ? 3 : 1);
+    fetch(t_begin);
+  }
+  int buf = 0;
+  for (int t0 = t_begin; t0 < t_end; t0 += Q) {
+    const int next = t0 + Q;
+    const uint8_t* image = image_at(buf);
+    const float* dec = decays_at(buf);
+    wait_loads<0>();
+    __syncthreads();  // the chunk's image has come; what the last chunk used is free
+    if (BUF == 2) {
+      if (next < t_end) request(next, buf ^ 1, 3);
+    } else {
+      request(t0, 0, 2);
+    }
+    // decays from the chunk's start (e) and to its end, with dt (w)
+    if (tid < hw * Q) {
+      const int h = tid / Q, q = tid % Q;
+      const float* d = dec + h * 3 * Q;
+      tables[h * 2 * Q + q] = __builtin_amdgcn_exp2f(d[Q + q] + d[2 * Q + q]);
+      tables[h * 2 * Q + Q + q] = d[q] * __builtin_amdgcn_exp2f((d[2 * Q - 1] - d[Q + q]) + (d[3 * Q - 1] - d[2 * Q + q]));
+    }
     if constexpr (!STATES) {
+      for (int job = wave; job < 3 * hw; job += kScanWaves) {
+        const int h = job / 3, tile = job - 3 * h, jt = tile == 2, it = tile > 0;
+        const floatx4 sv = *reinterpret_cast<const floatx4*>(image + (kSAt + tile) * kFragment + 16 * lane);
+        const int i = 16 * it + col, j0 = 16 * jt + 4 * g;
+        const float* d = dec + h * 3 * Q;
+        const float ihi = d[Q + i], ilo = d[2 * Q + i];
+        const floatx4 dt = *reinterpret_cast<const floatx4*>(d + j0);
+        const floatx4 jhi = *reinterpret_cast<const floatx4*>(d + Q + j0);
+        const floatx4 jlo = *reinterpret_cast<const floatx4*>(d + 2 * Q + j0);
+        float m[4];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
+        for (int e = 0; e < 4; ++e)
+          m[e] = j0 + e <= i ? sv[e] * (__builtin_amdgcn_exp2f((ihi - jhi[e]) + (ilo - jlo[e])) * dt[e]) : 0.f;
+        u32x2 hi, mid, lo;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          uint32_t a, b, cc;
+          split_pair(m[2 * e], m[2 * e + 1], a, b, cc);
+          hi[e] = a;
+          mid[e] = b;
+          lo[e] = cc;
+        }
+        u32x2* out = reinterpret_cast<u32x2*>(products + h * Lds::products + it * 3 * kFragment + 16 * lane + 8 * jt);
+        out[0] = hi;
+        out[kFragment / 8] = mid;
+        out[2 * kFragment / 8] = lo;
+      }
+    }
+    // x after the convolution
+    float x[TPW][8];
+#pragma unroll
+    for (int k = 0; k < TPW; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float v = bias[k];
+#pragma unroll
+        for (int j = 0; j < W; ++j) v = fmaf(w[k][j], raw[k][e >> 2][(e & 3) + j], v);
+        x[k][e] = on[k] && t0 + 16 * (e >> 2) + 4 * g + (e & 3) < t_end ? silu_f32(v) : 0.f;
+      }
+    if (next < t_end) fetch(next);
+    __syncthreads();
+    if constexpr (!STATES) {
+      floatx4 acc[2][TPW];
+#pragma unroll
+      for (int it = 0; it < 2; ++it)
+#pragma unroll
+        for (int k = 0; k < TPW; ++k) acc[it][k] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int t = 0; t < NB; ++t) {
+        Split8 sp[TPW];
+#pragma unroll
+        for (int k = 0; k < TPW; ++k) {
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = st[k][2 * t + (e >> 2)][e & 3];
+          sp[k] = split8(v);
+        }
+        u32x4 a[2][3];
+#pragma unroll
+        for (int it = 0; it < 2; ++it)
+#pragma unroll
+          for (int part = 0; part < 3; ++part)
+            a[it][part] = *reinterpret_cast<const u32x4*>(image + ((it * NB + t) * 3 + part) * kFragment + 16 * lane);
+        // neighbouring products belong to different accumulators
+#define LLHIP_SSM_PRODUCT(PART, FIELD)                                     \
+  _Pragma("unroll") for (int it = 0; it < 2; ++it)                         \
+      _Pragma("unroll") for (int k = 0; k < TPW; ++k)                      \
+          acc[it][k] = mma_one(a[it][PART], sp[k].FIELD, acc[it][k]);
+        LLHIP_SSM_PRODUCT(2, hi)
+        LLHIP_SSM_PRODUCT(0, lo)
+        LLHIP_SSM_PRODUCT(1, mid)
+        LLHIP_SSM_PRODUCT(1, hi)
+        LLHIP_SSM_PRODUCT(0, mid)
+        LLHIP_SSM_PRODUCT(0, hi)
+      }
+#pragma unroll
+      for (int k = 0; k < TPW; ++k) {
         if (!on[k]) continue;
+        // A non-finite x_j would reach the tokens before it, as 0 x_j in the
+        // masked part of the product: the products take zero in its place,
+        // and the channel's outputs from token j on are NaN (its state too, by
+        // x itself).
+        float xf[8];
+        int first_bad = Q;
         bool bad = false;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          xf[k][e] = x[k][e];
+          xf[e] = x[k][e];
           bad |= !(fabsf(x[k][e]) <= FLT_MAX);
         }
         if (__ballot(bad)) {
-          int f = Q;
 #pragma unroll
           for (int e = 7; e >= 0; --e)
             if (!(fabsf(x[k][e]) <= FLT_MAX)) {
-              f = 16 * (e >> 2) + 4 * g + (e & 3);
-              xf[k][e] = 0.f;
+              first_bad = 16 * (e >> 2) + 4 * g + (e & 3);
+              xf[e] = 0.f;
             }
-          f = min(f, __shfl_xor(f, 16, 64));
-          first_bad[k] = min(f, __shfl_xor(f, 32, 64));
+          first_bad = min(first_bad, __shfl_xor(first_bad, 16, 64));
+          first_bad = min(first_bad, __shfl_xor(first_bad, 32, 64));
         }
-      }
-    }
-    __syncthreads();
-    if constexpr (!STATES) {
-      // S^T tiles (j tile, i tile) = (0, 0), (0, 1), (1, 1), one per wave
-      if (wave < 3) {
-        const int jt = wave == 2, it = wave > 0;
-        floatx4 acc{0.f, 0.f, 0.f, 0.f};
-        const float* pa = sb + (16 * jt + col) * LD + 4 * g;
-        const float* pb = sc + (16 * it + col) * LD + 4 * g;
+        const Split8 xs = split8(xf);
+        const uint8_t* m = products + head[k] * Lds::products;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const floatx4 a = *reinterpret_cast<const floatx4*>(pa + 16 * n);
-          const floatx4 b = *reinterpret_cast<const floatx4*>(pb + 16 * n);
+        for (int it = 0; it < 2; ++it) {
+          const floatx4 e4 = *reinterpret_cast<const floatx4*>(tables + head[k] * 2 * Q + 16 * it + 4 * g);
+          acc[it][k] *= e4;
+          u32x4 a[3];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc = mfma4f32(a[e], b[e], acc);
-        }
-        const int i = 16 * it + col, j0 = 16 * jt + 4 * g;
-        for (int h = 0; h < hw; ++h) {
-          const float* dd = sd + h * 3 * Q;
-          const float ihi = dd[Q + i], ilo = dd[2 * Q + i];
-          floatx4 m;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = j0 + e;
-            const float l = (ihi - dd[Q + j]) + (ilo - dd[2 * Q + j]);
-            m[e] = j <= i ? acc[e] * (__builtin_amdgcn_exp2f(l) * dd[j]) : 0.f;
-          }
-          *reinterpret_cast<floatx4*>(sm + ((h * 3 + wave) * 64 + lane) * 4) = m;
-        }
-      }
-      __syncthreads();
-#pragma unroll
-      for (int it = 0; it < 2; ++it) {
-        floatx4 acc[2] = {floatx4{0.f, 0.f, 0.f, 0.f}, floatx4{0.f, 0.f, 0.f, 0.f}};
-        const float* pa = sc + (16 * it + col) * LD + 4 * g;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const floatx4 a = *reinterpret_cast<const floatx4*>(pa + 16 * n);
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-            if (on[k])
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[k] = mfma4f32(a[e], st[k][n][e], acc[k]);
+          for (int part = 0; part < 3; ++part)
+            a[part] = *reinterpret_cast<const u32x4*>(m + (it * 3 + part) * kFragment + 16 * lane);
+          acc[it][k] = mma_one(a[2], xs.hi, acc[it][k]);
+          acc[it][k] = mma_one(a[0], xs.lo, acc[it][k]);
+          acc[it][k] = mma_one(a[1], xs.mid, acc[it][k]);
+          acc[it][k] = mma_one(a[1], xs.hi, acc[it][k]);
+          acc[it][k] = mma_one(a[0], xs.mid, acc[it][k]);
+          acc[it][k] = mma_one(a[0], xs.hi, acc[it][k]);
         }
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          if (!on[k]) continue;
-          const float* dd = sd + head[k] * 3 * Q;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int i = 16 * it + 4 * g + e;
-            acc[k][e] = acc[k][e] * __builtin_amdgcn_exp2f(dd[Q + i] + dd[2 * Q + i]);
-          }
-          for (int jt = 0; jt <= it; ++jt) {
-            const floatx4 a = *reinterpret_cast<const floatx4*>(sm + ((head[k] * 3 + it + jt) * 64 + lane) * 4);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[k] = mfma4f32(a[e], xf[k][4 * jt + e], acc[k]);
-          }
-          float* out = c.y + (int64_t)(s.begin + t0 + 16 * it + 4 * g) * inner + ch[k];
+        for (int it = 0; it < 2; ++it) {
+          float* out = c.y + (int64_t)(s.begin + t0 + 16 * it) * inner;
+          const uint32_t off = (uint32_t)(4 * g) * (uint32_t)inner + (uint32_t)ch[k];
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (t0 + 16 * it + 4 * g + e < t_end)
-              out[(int64_t)e * inner] = 16 * it + 4 * g + e < first_bad[k]
-                                            ? fmaf(skip[k], xf[k][4 * it + e], acc[k][e])
-                                            : __builtin_nanf("");
+              (out + (int64_t)e * inner)[off] = 16 * it + 4 * g + e < first_bad
+                                                    ? fmaf(skip[k], xf[4 * it + e], acc[it][k][e])
+                                                    : __builtin_nanf("");
         }
+      }
+      if (BUF == 1) {
+        wait_loads<0>();
+        __syncthreads();  // B has come; C, S and the decays are free
+        if (next < t_end) request(next, 0, 1);
       }
     }
     // the state: decayed, plus the tokens' products
+    Split8 xs[TPW];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      if (!on[k]) continue;
-      const float* dd = sd + head[k] * 3 * Q;
-      const float qhi = dd[2 * Q - 1], qlo = dd[3 * Q - 1];
+    for (int k = 0; k < TPW; ++k) {
+      const float* tab = tables + head[k] * 2 * Q;
+      const floatx4 w0 = *reinterpret_cast<const floatx4*>(tab + Q + 4 * g);
+      const floatx4 w1 = *reinterpret_cast<const floatx4*>(tab + Q + 16 + 4 * g);
+      float v[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int j = 16 * (e >> 2) + 4 * g + (e & 3);
-        x[k][e] *= dd[j] * __builtin_amdgcn_exp2f((qhi - dd[Q + j]) + (qlo - dd[2 * Q + j]));
-      }
-      const float e = __builtin_amdgcn_exp2f(qhi + qlo);
+      for (int e = 0; e < 8; ++e) v[e] = x[k][e] * (e < 4 ? w0[e & 3] : w1[e & 3]);
+      xs[k] = split8(v);
+      const float e = tab[Q - 1];
 #pragma unroll
       for (int n = 0; n < NT; ++n) st[k][n] *= e;
-      total_hi[k] += qhi;
-      total_lo[k] += qlo;
+      if (STATES) {
+        total_hi[k] += dec[head[k] * 3 * Q + 2 * Q - 1];
+        total_lo[k] += dec[head[k] * 3 * Q + 3 * Q - 1];
+      }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float b[8];
+      u32x4 a[3];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) b[e] = sb[(16 * (e >> 2) + 4 * g + (e & 3)) * LD + 16 * n + col];
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (on[k]) st[k][n] = mma<8>(b, x[k], st[k][n]);
+      for (int part = 0; part < 3; ++part)
+        a[part] = *reinterpret_cast<const u32x4*>(image + (kBAt + 3 * n + part) * kFragment + 16 * lane);
+#define LLHIP_SSM_UPDATE(PART, FIELD)                                      \
+  _Pragma("unroll") for (int k = 0; k < TPW; ++k)                          \
+      st[k][n] = mma_one(a[PART], xs[k].FIELD, st[k][n]);
+      LLHIP_SSM_UPDATE(2, hi)
+      LLHIP_SSM_UPDATE(0, lo)
+      LLHIP_SSM_UPDATE(1, mid)
+      LLHIP_SSM_UPDATE(1, hi)
+      LLHIP_SSM_UPDATE(0, mid)
+      LLHIP_SSM_UPDATE(0, hi)
     }
+    if (BUF == 2) buf ^= 1;
   }
 
   float* dst = nullptr;
@@ -487,7 +689,7 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
   else if (at.y == s.segments - 1 && s.to >= 0) dst = p.ssm_states + (int64_t)s.to * inner * N;
   if (!dst) return;
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < TPW; ++k) {
     if (!on[k]) continue;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -698,7 +900,7 @@ __global__ void ssm_reset_error_kernel(int* error) {
 int64_t ssm_max_chunks(int64_t tokens, int64_t sequences) { return tokens / kSsmChunk + sequences; }
 
 // Workgroups that a scan should have before a sequence is cut no further.
-constexpr int64_t kScanGroups = 1024;
+constexpr int64_t kScanGroups = 512;
 constexpr int kMinSegment = 128;
 
 int ssm_segment_tokens(const SsmLayerPlan& p, int64_t tokens) {
@@ -766,32 +968,29 @@ hipError_t ssm_step_launch(const SsmLayerPlan& p, const SsmCall& c, hipStream_t 
 template <int NT, int W>
 static hipError_t scan_launch(const SsmLayerPlan& p, const SsmCall& c, int segment_tokens,
                               int64_t max_segments, hipStream_t s) {
-  constexpr int N = 16 * NT, Q = kSsmChunk;
   const int hw = scan_heads(p);
-  const dim3 grid((uint32_t)(max_segments * (p.heads / hw)));
-  const size_t tile = (size_t)Q * (N + 4) * sizeof(float), decays = (size_t)hw * 3 * Q * sizeof(float);
+  const int64_t chunks = ssm_max_chunks(c.tokens, c.sequences);
+  hipError_t e = launch(ssm_prepare_kernel<NT, W>,
+                        dim3((uint32_t)chunks, p.groups + (p.heads + kPrepHeads - 1) / kPrepHeads), dim3(256), 0, s,
+                        p, c);
+  if (e != hipSuccess) return e;
+  const dim3 grid((uint32_t)(max_segments * (p.heads / hw))), block(64 * kScanWaves);
   if (c.tokens > segment_tokens) {
-    hipError_t e = launch(ssm_scan_kernel<NT, W, true>, grid, dim3(64 * kScanWaves), tile + decays, s, p, c,
-                          segment_tokens, hw);
+    e = launch(ssm_scan_kernel<NT, W, true>, grid, block, ScanLds<NT, true>::bytes(hw), s, p, c, segment_tokens, hw);
     if (e != hipSuccess) return e;
-    const int64_t size = (int64_t)p.heads * p.head_dim * N;
+    const int64_t size = (int64_t)p.heads * p.head_dim * 16 * NT;
     e = launch(ssm_join_kernel, dim3(c.sequences, (uint32_t)((size / 4 + 255) / 256)), dim3(256), 0, s, p);
     if (e != hipSuccess) return e;
   }
-  return launch(ssm_scan_kernel<NT, W, false>, grid, dim3(64 * kScanWaves),
-                2 * tile + decays + (size_t)hw * 3 * 256 * sizeof(float), s, p, c, segment_tokens, hw);
+  return launch(ssm_scan_kernel<NT, W, false>, grid, block, ScanLds<NT, false>::bytes(hw), s, p, c, segment_tokens,
+                hw);
 }
 
 template <int W>
 static hipError_t run_launch(const SsmLayerPlan& p, const SsmCall& c, hipStream_t s) {
   const int segment_tokens = ssm_segment_tokens(p, c.tokens);
-  const int64_t chunks = ssm_max_chunks(c.tokens, c.sequences);
   const int64_t segments = c.tokens / segment_tokens + c.sequences;
   hipError_t e = launch(ssm_plan_kernel, dim3(c.sequences), dim3(kPlanThreads), 0, s, p, c, segment_tokens);
-  if (e != hipSuccess) return e;
-  const int blocks = (2 * p.groups * p.state + kPrepChannels - 1) / kPrepChannels +
-                     (p.heads + kPrepHeads - 1) / kPrepHeads;
-  e = launch(ssm_prepare_kernel<W>, dim3((uint32_t)chunks, blocks), dim3(256), 0, s, p, c);
   if (e != hipSuccess) return e;
   switch (p.state) {
     case 16: e = scan_launch<1, W>(p, c, segment_tokens, segments, s); break;
