@@ -51,6 +51,12 @@ __device__ __forceinline__ float silu_f32(float v) {
   // reciprocal is 0 and the result -0, as the limit is
   return v * __builtin_amdgcn_rcpf(1.f + exp_f32(-v));
 }
+// The same without that correction, for the convolution's outputs: the product
+// v log2 e rounds, so the result is off by about (|v| + 5) 2^-24 of it, which is
+// below the rounding of the sum that v is unless v is large, and tiny then.
+__device__ __forceinline__ float silu_conv(float v) {
+  return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -kLog2e));
+}
 // log(1 + e^v) = max(v, 0) + log1p(e^-|v|)
 __device__ __forceinline__ float softplus_f32(float v) {
   return fmaxf(v, 0.f) + log1pf(exp_f32(-fabsf(v)));
@@ -271,7 +277,7 @@ __global__ void __launch_bounds__(256) ssm_prepare_kernel(SsmLayerPlan p, SsmCal
         for (int k = 0; k < W; ++k) v += w[k] * r[q + k];
         floatx4 u;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) u[e] = t0 + q0 + q < s.length ? silu_f32(v[e]) : 0.f;
+        for (int e = 0; e < 4; ++e) u[e] = t0 + q0 + q < s.length ? silu_conv(v[e]) : 0.f;
         *reinterpret_cast<floatx4*>(&sbc[which][(q0 + q) * LD + n]) = u;
       }
     }
@@ -341,6 +347,21 @@ __global__ void __launch_bounds__(256) ssm_prepare_kernel(SsmLayerPlan p, SsmCal
 // same K element.
 __device__ __forceinline__ floatx4 mma_one(const u32x4& a, const u32x4& b, const floatx4& c) {
   return mfma32(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c);
+}
+
+// Wait for every load, in a form that the compiler counts too (it would wait
+// again for the registers, behind the loads that follow).
+__device__ __forceinline__ void wait_all_loads() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  asm volatile("" ::: "memory");
+}
+
+// A buffer of `elements` floats (none if negative; loads past its end give
+// zero, stores there do nothing).
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const float* p, int64_t elements) {
+  const int64_t bytes = elements < 0 ? 0 : elements > (1 << 28) ? (int64_t)1 << 30 : 4 * elements;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(p), 0, (int)bytes, 0x00020000);
 }
 
 constexpr int kScanWaves = 8;
@@ -458,25 +479,43 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
   }
   float total_hi[TPW] = {}, total_lo[TPW] = {};
 
-  // raw x of the lane's tokens 4 g .. + 3 and 16 + 4 g .. + 3, with the rows before each run
-  float raw[TPW][2][4 + W - 1];
-  auto fetch = [&](int t0) {
-    const bool inside = t0 >= W - 1 && t0 + Q <= t_end;
+  // x of the lane's tokens 4 g .. + 3 and 16 + 4 g .. + 3 after the
+  // convolution: raw rows are requested a chunk ahead (zeros past the
+  // segment's end, by the bounds of the buffer that the loads go through) and
+  // convolved while the matrix cores run the chunk before
+  float raw[TPW][2][4 + W - 1], x[TPW][8];
+  uint32_t at_x[TPW], at_y[TPW];
+#pragma unroll
+  for (int k = 0; k < TPW; ++k) {
+    at_x[k] = 4u * ((uint32_t)(4 * g) * (uint32_t)stride + (uint32_t)ch[k]);
+    // a tile that this wave does not have: beyond any buffer's end, without wrapping
+    at_y[k] = on[k] ? 4u * ((uint32_t)(4 * g) * (uint32_t)inner + (uint32_t)ch[k]) : 0x80000000u;
+  }
+  auto fetch = [&](int t) {  // t >= W - 1
+    const __amdgpu_buffer_rsrc_t rows_t = buffer_of(rows + (int64_t)(t - (W - 1)) * stride,
+                                                    (int64_t)(t_end - t + W - 1) * stride);
+#pragma unroll
+    for (int k = 0; k < TPW; ++k) {
+      const uint32_t at0 = opaque(at_x[k]);  // the sums stay in the loop: kept in registers they spill others
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int j = 0; j < 4 + W - 1; ++j)
+          raw[k][half][j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+              rows_t, at0 + (uint32_t)(16 * half + j) * (4u * (uint32_t)stride), 0, 0));
+    }
+  };
+  auto convolve = [&] {
 #pragma unroll
     for (int k = 0; k < TPW; ++k)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int t = t0 + 16 * half - (W - 1);
-        if (!on[k]) continue;
-        if (inside) {
-          const uint32_t off = (uint32_t)(4 * g) * (uint32_t)stride + (uint32_t)ch[k];
+      for (int e = 0; e < 8; ++e) {
+        float v = bias[k];
 #pragma unroll
-          for (int j = 0; j < 4 + W - 1; ++j) raw[k][half][j] = (rows + (int64_t)(t + j) * stride)[off];
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4 + W - 1; ++j)
-            raw[k][half][j] = raw1(rows, stride, taps, channels, W, t + 4 * g + j, t_end, ch[k]);
-        }
+        for (int j = 0; j < W; ++j) v = fmaf(w[k][j], raw[k][e >> 2][(e & 3) + j], v);
+        v = silu_conv(v);  // past the end: what the sequence leaves in the taps, their dt is zero
+        asm("" : "+v"(v));  // one by one: as a vector the taps would be held eight times each
+        x[k][e] = v;
       }
   };
 
@@ -489,20 +528,32 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
   }
   if (t_begin < t_end) {
     request(t_begin, 0, BUF == 2 ? 3 : 1);
-    fetch(t_begin);
+    if (t_begin > 0) {
+      fetch(t_begin);
+    } else {
+#pragma unroll
+      for (int k = 0; k < TPW; ++k)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int j = 0; j < 4 + W - 1; ++j)
+            raw[k][half][j] = raw1(rows, stride, taps, channels, W, 16 * half - (W - 1) + 4 * g + j, t_end, ch[k]);
+    }
+    convolve();
   }
   int buf = 0;
   for (int t0 = t_begin; t0 < t_end; t0 += Q) {
     const int next = t0 + Q;
     const uint8_t* image = image_at(buf);
     const float* dec = decays_at(buf);
-    wait_loads<0>();
+    wait_all_loads();
     __syncthreads();  // the chunk's image has come; what the last chunk used is free
     if (BUF == 2) {
       if (next < t_end) request(next, buf ^ 1, 3);
     } else {
       request(t0, 0, 2);
     }
+    fetch(next);
     // decays from the chunk's start (e) and to its end, with dt (w)
     if (tid < hw * Q) {
       const int h = tid / Q, q = tid % Q;
@@ -539,27 +590,31 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
         out[2 * kFragment / 8] = lo;
       }
     }
-    // x after the convolution
-    float x[TPW][8];
-#pragma unroll
-    for (int k = 0; k < TPW; ++k)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float v = bias[k];
-#pragma unroll
-        for (int j = 0; j < W; ++j) v = fmaf(w[k][j], raw[k][e >> 2][(e & 3) + j], v);
-        x[k][e] = on[k] && t0 + 16 * (e >> 2) + 4 * g + (e & 3) < t_end ? silu_f32(v) : 0.f;
-      }
-    if (next < t_end) fetch(next);
     __syncthreads();
     if constexpr (!STATES) {
+      const __amdgpu_buffer_rsrc_t rows_y = buffer_of(c.y + (int64_t)(s.begin + t0) * inner,
+                                                      (int64_t)(t_end - t0) * inner);
       floatx4 acc[2][TPW];
 #pragma unroll
       for (int it = 0; it < 2; ++it)
 #pragma unroll
         for (int k = 0; k < TPW; ++k) acc[it][k] = floatx4{0.f, 0.f, 0.f, 0.f};
+      // the next block's fragments are read ahead, and no further ahead: read
+      // where the compiler likes they crowd the state out of the registers
+      auto c_at = [&](int t, int it, int part) {
+        return *reinterpret_cast<const u32x4*>(image + ((it * NB + t) * 3 + part) * kFragment + 16 * lane);
+      };
+      u32x4 a[2][3], ahead[2][3];
+#pragma unroll
+      for (int part = 0; part < 6; ++part) ahead[part / 3][part % 3] = c_at(0, part / 3, part % 3);
 #pragma unroll
       for (int t = 0; t < NB; ++t) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int part = 0; part < 6; ++part) {
+          a[part / 3][part % 3] = ahead[part / 3][part % 3];
+          if (t + 1 < NB) ahead[part / 3][part % 3] = c_at(t + 1, part / 3, part % 3);
+        }
         Split8 sp[TPW];
 #pragma unroll
         for (int k = 0; k < TPW; ++k) {
@@ -568,12 +623,6 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
           for (int e = 0; e < 8; ++e) v[e] = st[k][2 * t + (e >> 2)][e & 3];
           sp[k] = split8(v);
         }
-        u32x4 a[2][3];
-#pragma unroll
-        for (int it = 0; it < 2; ++it)
-#pragma unroll
-          for (int part = 0; part < 3; ++part)
-            a[it][part] = *reinterpret_cast<const u32x4*>(image + ((it * NB + t) * 3 + part) * kFragment + 16 * lane);
         // neighbouring products belong to different accumulators
 #define LLHIP_SSM_PRODUCT(PART, FIELD)                                     \
   _Pragma("unroll") for (int it = 0; it < 2; ++it)                         \
@@ -585,23 +634,24 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
         LLHIP_SSM_PRODUCT(1, hi)
         LLHIP_SSM_PRODUCT(0, mid)
         LLHIP_SSM_PRODUCT(0, hi)
+#undef LLHIP_SSM_PRODUCT
       }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int k = 0; k < TPW; ++k) {
-        if (!on[k]) continue;
         // A non-finite x_j would reach the tokens before it, as 0 x_j in the
         // masked part of the product: the products take zero in its place,
         // and the channel's outputs from token j on are NaN (its state too, by
         // x itself).
         float xf[8];
         int first_bad = Q;
-        bool bad = false;
+        float largest = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           xf[e] = x[k][e];
-          bad |= !(fabsf(x[k][e]) <= FLT_MAX);
+          largest = __builtin_elementwise_maximum(largest, fabsf(x[k][e]));  // NaN if one is
         }
-        if (__ballot(bad)) {
+        if (__ballot(!(largest <= FLT_MAX))) {
 #pragma unroll
           for (int e = 7; e >= 0; --e)
             if (!(fabsf(x[k][e]) <= FLT_MAX)) {
@@ -630,18 +680,22 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
         }
 #pragma unroll
         for (int it = 0; it < 2; ++it) {
-          float* out = c.y + (int64_t)(s.begin + t0 + 16 * it) * inner;
-          const uint32_t off = (uint32_t)(4 * g) * (uint32_t)inner + (uint32_t)ch[k];
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float u = fmaf(skip[k], xf[4 * it + e], acc[it][k][e]);
+            v[e] = 16 * it + 4 * g + e < first_bad ? u : __builtin_nanf("");
+          }
+          // rows past the segment's end lie past the buffer's
+          const uint32_t at0 = opaque(at_y[k]);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (t0 + 16 * it + 4 * g + e < t_end)
-              (out + (int64_t)e * inner)[off] = 16 * it + 4 * g + e < first_bad
-                                                    ? fmaf(skip[k], xf[4 * it + e], acc[it][k][e])
-                                                    : __builtin_nanf("");
+            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v[e]), rows_y,
+                                                  at0 + (uint32_t)(16 * it + e) * (4u * (uint32_t)inner), 0, 0);
         }
       }
       if (BUF == 1) {
-        wait_loads<0>();
+        wait_all_loads();
         __syncthreads();  // B has come; C, S and the decays are free
         if (next < t_end) request(next, 0, 1);
       }
@@ -665,22 +719,32 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
         total_lo[k] += dec[head[k] * 3 * Q + 3 * Q - 1];
       }
     }
+    auto b_at = [&](int n, int part) {
+      return *reinterpret_cast<const u32x4*>(image + (kBAt + 3 * n + part) * kFragment + 16 * lane);
+    };
+    u32x4 b[3], ahead[3];
+#pragma unroll
+    for (int part = 0; part < 3; ++part) ahead[part] = b_at(0, part);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      u32x4 a[3];
 #pragma unroll
-      for (int part = 0; part < 3; ++part)
-        a[part] = *reinterpret_cast<const u32x4*>(image + (kBAt + 3 * n + part) * kFragment + 16 * lane);
+      for (int part = 0; part < 3; ++part) {
+        b[part] = ahead[part];
+        if (n + 1 < NT) ahead[part] = b_at(n + 1, part);
+      }
 #define LLHIP_SSM_UPDATE(PART, FIELD)                                      \
   _Pragma("unroll") for (int k = 0; k < TPW; ++k)                          \
-      st[k][n] = mma_one(a[PART], xs[k].FIELD, st[k][n]);
+      st[k][n] = mma_one(b[PART], xs[k].FIELD, st[k][n]);
       LLHIP_SSM_UPDATE(2, hi)
       LLHIP_SSM_UPDATE(0, lo)
       LLHIP_SSM_UPDATE(1, mid)
       LLHIP_SSM_UPDATE(1, hi)
       LLHIP_SSM_UPDATE(0, mid)
       LLHIP_SSM_UPDATE(0, hi)
+#undef LLHIP_SSM_UPDATE
+      if (n % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
+    convolve();
     if (BUF == 2) buf ^= 1;
   }
 
