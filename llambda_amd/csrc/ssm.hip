@@ -357,64 +357,80 @@ __device__ __forceinline__ void wait_all_loads() {
   asm volatile("" ::: "memory");
 }
 
-// A buffer of `elements` floats (none if negative; loads past its end give
-// zero, stores there do nothing).
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const float* p, int64_t elements) {
-  const int64_t bytes = elements < 0 ? 0 : elements > (1 << 28) ? (int64_t)1 << 30 : 4 * elements;
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(p), 0, (int)bytes, 0x00020000);
-}
-
 constexpr int kScanWaves = 8;
-constexpr int kScanHeads = 4;  // of a workgroup at most (their masked products take 6 KB of LDS each)
 
-// Column tiles of 16 channels per wavefront: the state of one takes N / 4
-// registers.
+// Column tiles of 16 channels per wavefront (the state of one takes N / 4
+// registers) and heads per workgroup at most (their masked products take 12 KB
+// of LDS each).
 constexpr int scan_tiles(int nt) { return nt > 8 ? 1 : 2; }
-// Images in LDS: two, so that a chunk's loads have the chunk before to run;
-// one of N = 256, whose halves are loaded while the other is used.
-constexpr int scan_buffers(int nt) { return nt > 8 ? 1 : 2; }
+constexpr int scan_max_heads(int nt) { return nt > 8 ? 2 : 4; }
 
 // Heads per workgroup: as many whole heads of one group as fit its tiles.
 static int scan_heads(const SsmLayerPlan& p) {
-  const int share = p.heads / p.groups;
-  int n = std::min(kScanHeads, std::max(1, kScanWaves * scan_tiles(p.state / 16) * 16 / p.head_dim));
+  const int share = p.heads / p.groups, nt = p.state / 16;
+  int n = std::min(scan_max_heads(nt), std::max(1, kScanWaves * scan_tiles(nt) * 16 / p.head_dim));
   while (share % n) --n;
   return n;
 }
 
-// LDS of a scan workgroup, in bytes.
-template <int NT, bool STATES>
+// LDS of a scan workgroup, in bytes: B and raw rows (two of each in the first
+// pass), C, S, decays, masked products (two), decay tables (two).
+template <int NT, int W, bool STATES>
 struct ScanLds {
-  static constexpr int buffers = STATES ? 2 : scan_buffers(NT);
-  static constexpr int image = (STATES ? b_fragments(NT) : image_fragments(NT)) * kFragment;
+  static constexpr int buffers = STATES ? 2 : 1;  // of B, the rows and the decays
+  static constexpr int b = b_fragments(NT) * kFragment;
+  static constexpr int c = STATES ? 0 : c_fragments(NT) * kFragment;
+  static constexpr int s = STATES ? 0 : 3 * kFragment;
+  static constexpr int decays = 3 * kSsmChunk * 4;             // per head
   static constexpr int products = STATES ? 0 : 6 * kFragment;  // per head: [i tile][hi, mid, lo]
-  static constexpr int decays = 3 * kSsmChunk * 4;             // per head and buffer
-  static constexpr int tables = 2 * kSsmChunk * 4;             // per head
-  static constexpr int bytes(int hw) { return buffers * (image + hw * decays) + hw * (products + tables); }
+  static constexpr int tables = 2 * kSsmChunk * 4;             // per head: [e, w]
+  // raw rows of the workgroup's channels.  The pitch puts the rows 4 apart
+  // that a wavefront reads together 16 banks apart.
+  static constexpr int rows = kSsmChunk + W - 1;
+  __host__ __device__ static constexpr int pitch(int width) { return 4 * (width + 4); }
+  static constexpr int at_c = buffers * b, at_s = at_c + c, at_decays = at_s + s;
+  __host__ __device__ static constexpr int at_products(int hw) { return at_decays + buffers * hw * decays; }
+  __host__ __device__ static constexpr int at_tables(int hw) { return at_products(hw) + 2 * hw * products; }
+  __host__ __device__ static constexpr int at_rows(int hw) { return at_tables(hw) + 2 * hw * tables; }
+  __host__ __device__ static constexpr int bytes(int hw, int width) {
+    return at_rows(hw) + buffers * rows * pitch(width);
+  }
 };
+
+// A 4 x 4 transpose over each four neighbouring lanes: lane q's v[e] becomes
+// lane e's v[q].
+__device__ __forceinline__ void transpose_quads(floatx4& v, bool odd, bool high) {
+  // (every lane takes part in each exchange, so they stand outside the selects)
+  const float x1 = dpp<kDppXor1>(v.x), y1 = dpp<kDppXor1>(v.y), z1 = dpp<kDppXor1>(v.z), w1 = dpp<kDppXor1>(v.w);
+  const float a = odd ? y1 : v.x, b = odd ? v.y : x1, c = odd ? w1 : v.z, d = odd ? v.w : z1;
+  const float a2 = dpp<kDppXor2>(a), b2 = dpp<kDppXor2>(b), c2 = dpp<kDppXor2>(c), d2 = dpp<kDppXor2>(d);
+  v.x = high ? c2 : a;
+  v.z = high ? c : a2;
+  v.y = high ? d2 : b;
+  v.w = high ? d : b2;
+}
 
 // One segment of `hw` heads.  STATES: only the segment's own state, from
 // zeros, to the next segment's place; else outputs and, in a sequence's last
 // segment, the state to its slot.
 //
 // A wavefront owns column tiles (16 channels of a head): their part of the
-// state, x, and outputs.  Per chunk the wavefronts first share the work of the
-// masked products M = S o L (three tiles a head) and of the decay tables, then
-// each forms its tiles' outputs, then its state.  The images of the next chunk
-// come into LDS meanwhile, by loads that need no registers.
+// state, x, and outputs.  Per chunk each forms its tiles' outputs, then their
+// state; beside the state's products, which leave the vector unit idle, the
+// wavefronts convolve x of the next chunk and share the work of its masked
+// products M = S o L (six half tiles a head) and decay tables.  Images and raw
+// rows come into LDS by loads that need no registers, each requested a phase
+// or more ahead: a load of one dword per lane costs the memory pipeline as
+// much as one of sixteen bytes, and reading x that way took it 5000 cycles of
+// a chunk's 17000.
 template <int NT, int W, bool STATES>
 __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan p, SsmCall c,
                                                                    int segment_tokens, int hw) {
-  using Lds = ScanLds<NT, STATES>;
-  constexpr int N = 16 * NT, Q = kSsmChunk, NB = n_blocks(NT), TPW = scan_tiles(NT), BUF = Lds::buffers;
-  constexpr int kC = c_fragments(NT), kB = b_fragments(NT);
-  constexpr int kBAt = STATES ? 0 : kC, kSAt = kC + kB;  // fragments within an image in LDS
+  using Lds = ScanLds<NT, W, STATES>;
+  constexpr int N = 16 * NT, Q = kSsmChunk, NB = n_blocks(NT), TPW = scan_tiles(NT);
+  constexpr int kC = c_fragments(NT), kB = b_fragments(NT), kImage = image_fragments(NT) * kFragment;
   extern __shared__ __align__(16) uint8_t lds[];
-  uint8_t* products = lds + BUF * (Lds::image + hw * Lds::decays);
-  float* tables = reinterpret_cast<float*>(products + hw * Lds::products);  // [hw][e, w][Q]
-  auto image_at = [&](int buf) { return lds + buf * (Lds::image + hw * Lds::decays); };
-  auto decays_at = [&](int buf) { return reinterpret_cast<float*>(image_at(buf) + Lds::image); };
-
+  const int width = hw * p.head_dim, pitch = Lds::pitch(width);
   const int sets = p.heads / hw;
   // groups vary fastest, so that the workgroups that read one group's images
   // sit on one XCD where there are eight groups
@@ -428,33 +444,71 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
   const int group = rest % p.groups, h0 = (group * set_in_group + rest / p.groups) * hw;
   const int inner = p.heads * p.head_dim, channels = inner + 2 * p.groups * N;
   const int64_t stride = inner + channels + p.heads;
-  const float* rows = c.x + (int64_t)s.begin * stride + inner;
+  const float* rows = c.x + (int64_t)s.begin * stride + inner + h0 * p.head_dim;
   const float* taps = conv_taps(p, s.from);
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int t_begin = at.y * segment_tokens, t_end = min(s.length, t_begin + segment_tokens);
 
-  // the loads of a chunk's image (parts: 1 = C, S and decays, 2 = B)
-  auto request = [&](int t, int buf, int parts) {
-    const int64_t chunk = s.chunk0 + t / Q;
-    const uint8_t* img = uniform_ptr(p.images + (chunk * p.groups + group) * image_fragments(NT) * kFragment);
-    const uint32_t to = lds_address(image_at(buf));
-    for (int f = wave; f < image_fragments(NT); f += kScanWaves) {
-      const bool is_b = f >= kC && f < kC + kB;
-      if (is_b ? !(parts & 2) : (STATES || !(parts & 1))) continue;
-      load_lds16(img, f * kFragment + 16 * lane, __builtin_amdgcn_readfirstlane(to + (f - (STATES ? kC : 0)) * kFragment));
-    }
-    if (parts & 1) {
-      const uint8_t* dec = uniform_ptr(reinterpret_cast<const uint8_t*>(p.decay + (chunk * p.heads + h0) * 3 * Q));
-      const uint32_t dto = __builtin_amdgcn_readfirstlane(lds_address(decays_at(buf)) + 1024 * wave);
-      if (64 * wave + lane < hw * Lds::decays / 16) load_lds16(dec, 1024 * wave + 16 * lane, dto);
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_address(lds));
+  // `n` fragments of a chunk's image from `first` on, to LDS at `to`
+  auto request_image = [&](int t, int first, int n, int to) {
+    const uint8_t* img = uniform_ptr(p.images + ((int64_t)(s.chunk0 + t / Q) * p.groups + group) * kImage +
+                                     first * kFragment);
+    const uint32_t off = wave * kFragment + 16 * lane;
+#pragma unroll
+    for (int f = 0; f < n; f += kScanWaves)
+      if (f + wave < n) load_lds16(img, off + f * kFragment, lds0 + to + (f + wave) * kFragment);
+  };
+  auto request_decays = [&](int t, int buf) {
+    const uint8_t* dec = uniform_ptr(reinterpret_cast<const uint8_t*>(
+        p.decay + ((int64_t)(s.chunk0 + t / Q) * p.heads + h0) * 3 * Q));
+    // the last two wavefronts, which have the fewest fragments
+    const int first = (kScanWaves - 1 - wave) * kFragment;
+    if (first + 16 * lane < hw * Lds::decays)
+      load_lds16(dec, first + 16 * lane, lds0 + Lds::at_decays + buf * hw * Lds::decays + first);
+  };
+  // the raw rows that a chunk's convolution reads: before the sequence those
+  // it started with (zeros for a new one), past its end the last row again
+  // (their dt is zero, so any finite row will do)
+  auto request_rows = [&](int t0, int buf) {
+    const uint32_t to = lds0 + Lds::at_rows(hw) + buf * Lds::rows * pitch;
+    if (4 * lane >= width) return;
+    if (t0 >= W - 1 && t0 + Q <= t_end) {
+      const float* src = rows + (int64_t)(t0 - (W - 1) + wave) * stride;
+#pragma unroll
+      for (int r = 0; r < Lds::rows; r += kScanWaves, src += kScanWaves * stride)
+        if (r + wave < Lds::rows)
+          load_lds16(uniform_ptr(reinterpret_cast<const uint8_t*>(src)), 16 * lane, to + (r + wave) * pitch);
+    } else {
+      for (int r = wave; r < Lds::rows; r += kScanWaves) {
+        const int t = t0 - (W - 1) + r;
+        const float* src = t >= 0 ? rows + (int64_t)min(t, t_end - 1) * stride
+                                  : taps ? taps + (int64_t)(W - 1 + t) * channels + h0 * p.head_dim : nullptr;
+        if (src)
+          load_lds16(uniform_ptr(reinterpret_cast<const uint8_t*>(src)), 16 * lane, to + r * pitch);
+        else
+          *reinterpret_cast<floatx4*>(lds + Lds::at_rows(hw) + (buf * Lds::rows + r) * pitch + 16 * lane) =
+              floatx4{0.f, 0.f, 0.f, 0.f};
+      }
     }
   };
+  if (t_begin < t_end) {
+    // all that the first chunk needs, and what its state phase reads of the second
+    request_rows(t_begin, 0);
+    request_decays(t_begin, 0);
+    if (STATES) {
+      request_image(t_begin, kC, kB, 0);
+    } else {
+      request_image(t_begin, kC + kB, 3, Lds::at_s);
+      request_image(t_begin, 0, kC, Lds::at_c);
+    }
+  }
 
   // this wave's column tiles: channels [p0, p0 + 16) of a head
   const int per_head = p.head_dim / 16, tiles = hw * per_head;
   bool on[TPW];
-  int head[TPW], ch[TPW];
+  int head[TPW], ch[TPW];  // ch: within the workgroup's channels
   float skip[TPW], w[TPW][W], bias[TPW];
   floatx4 st[TPW][2 * NB];
 #pragma unroll
@@ -462,11 +516,12 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
     const int tile = wave + kScanWaves * k;
     on[k] = tile < tiles;
     head[k] = on[k] ? tile / per_head : 0;
-    ch[k] = (h0 + head[k]) * p.head_dim + (on[k] ? tile % per_head : 0) * 16 + col;
+    ch[k] = (on[k] ? tile * 16 : 0) + col;
+    const int at_ch = h0 * p.head_dim + ch[k];
     skip[k] = p.d[h0 + head[k]];
-    bias[k] = p.conv_bias[ch[k]];
+    bias[k] = p.conv_bias[at_ch];
 #pragma unroll
-    for (int j = 0; j < W; ++j) w[k][j] = p.conv_weight[(int64_t)j * channels + ch[k]];
+    for (int j = 0; j < W; ++j) w[k][j] = p.conv_weight[(int64_t)j * channels + at_ch];
     const float* src = nullptr;
     if (!STATES) {
       if (s.segments > 1) src = p.seg_states + (int64_t)(s.state0 + at.y) * inner * N;
@@ -474,126 +529,126 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
     }
 #pragma unroll
     for (int n = 0; n < 2 * NB; ++n)
-      st[k][n] = src && on[k] && n < NT ? *reinterpret_cast<const floatx4*>(src + (int64_t)ch[k] * N + 16 * n + 4 * g)
+      st[k][n] = src && on[k] && n < NT ? *reinterpret_cast<const floatx4*>(src + (int64_t)at_ch * N + 16 * n + 4 * g)
                                         : floatx4{0.f, 0.f, 0.f, 0.f};
   }
   float total_hi[TPW] = {}, total_lo[TPW] = {};
 
-  // x of the lane's tokens 4 g .. + 3 and 16 + 4 g .. + 3 after the
-  // convolution: raw rows are requested a chunk ahead (zeros past the
-  // segment's end, by the bounds of the buffer that the loads go through) and
-  // convolved while the matrix cores run the chunk before
-  float raw[TPW][2][4 + W - 1], x[TPW][8];
-  uint32_t at_x[TPW], at_y[TPW];
-#pragma unroll
-  for (int k = 0; k < TPW; ++k) {
-    at_x[k] = 4u * ((uint32_t)(4 * g) * (uint32_t)stride + (uint32_t)ch[k]);
-    // a tile that this wave does not have: beyond any buffer's end, without wrapping
-    at_y[k] = on[k] ? 4u * ((uint32_t)(4 * g) * (uint32_t)inner + (uint32_t)ch[k]) : 0x80000000u;
-  }
-  auto fetch = [&](int t) {  // t >= W - 1
-    const __amdgpu_buffer_rsrc_t rows_t = buffer_of(rows + (int64_t)(t - (W - 1)) * stride,
-                                                    (int64_t)(t_end - t + W - 1) * stride);
+  // x of the lane's tokens 4 g .. + 3 and 16 + 4 g .. + 3 after the convolution
+  float x[TPW][8];
+  auto convolve = [&](int buf) {
 #pragma unroll
     for (int k = 0; k < TPW; ++k) {
-      const uint32_t at0 = opaque(at_x[k]);  // the sums stay in the loop: kept in registers they spill others
+      const uint8_t* from = lds + Lds::at_rows(hw) + buf * Lds::rows * pitch + 4 * g * pitch + 4 * ch[k];
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
+      for (int half = 0; half < 2; ++half) {
+        float raw[4 + W - 1];
 #pragma unroll
-        for (int j = 0; j < 4 + W - 1; ++j)
-          raw[k][half][j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
-              rows_t, at0 + (uint32_t)(16 * half + j) * (4u * (uint32_t)stride), 0, 0));
+        for (int j = 0; j < 4 + W - 1; ++j) raw[j] = *reinterpret_cast<const float*>(from + (16 * half + j) * pitch);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float v = bias[k];
+#pragma unroll
+          for (int j = 0; j < W; ++j) v = fmaf(w[k][j], raw[e + j], v);
+          v = silu_conv(v);
+          asm("" : "+v"(v));  // one by one: as a vector the taps would be held eight times each
+          x[k][4 * half + e] = v;
+        }
+      }
     }
   };
-  auto convolve = [&] {
+  auto decays_at = [&](int buf) { return reinterpret_cast<const float*>(lds + Lds::at_decays + buf * hw * Lds::decays); };
+  auto tables_at = [&](int buf) { return reinterpret_cast<float*>(lds + Lds::at_tables(hw) + buf * hw * Lds::tables); };
+  // decays from the chunk's start (e) and to its end, with dt (w); the same
+  // values from as many threads as there are
+  auto make_tables = [&](int from, int to) {
+    const int h = (tid / Q) % hw, q = tid % Q;
+    const float* d = decays_at(from) + h * 3 * Q;
+    float* t = tables_at(to) + h * 2 * Q + q;
+    t[0] = __builtin_amdgcn_exp2f(d[Q + q] + d[2 * Q + q]);
+    t[Q] = d[q] * __builtin_amdgcn_exp2f((d[2 * Q - 1] - d[Q + q]) + (d[3 * Q - 1] - d[2 * Q + q]));
+  };
+  // M = S o L of the workgroup's heads, as left operands: job (head, tile,
+  // half), a lane's two neighbouring j of column i.  (Past the last job that
+  // one again.)
+  auto make_products = [&](int to) {
+    const float* dec = decays_at(0);
 #pragma unroll
-    for (int k = 0; k < TPW; ++k)
+    for (int n = 0; n < 6 * scan_max_heads(NT); n += kScanWaves) {
+      const int job = min(n + wave, 6 * hw - 1);
+      const int h = job / 6, tile = job % 6 / 2, half = job % 2, jt = tile == 2, it = tile > 0;
+      const floatx2 sv = *reinterpret_cast<const floatx2*>(lds + Lds::at_s + tile * kFragment + 16 * lane + 8 * half);
+      const int i = 16 * it + col, j0 = 16 * jt + 4 * g + 2 * half;
+      const float* d = dec + h * 3 * Q;
+      const float ihi = d[Q + i], ilo = d[2 * Q + i];
+      const floatx2 dt = *reinterpret_cast<const floatx2*>(d + j0);
+      const floatx2 jhi = *reinterpret_cast<const floatx2*>(d + Q + j0);
+      const floatx2 jlo = *reinterpret_cast<const floatx2*>(d + 2 * Q + j0);
+      float m[2];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float v = bias[k];
-#pragma unroll
-        for (int j = 0; j < W; ++j) v = fmaf(w[k][j], raw[k][e >> 2][(e & 3) + j], v);
-        v = silu_conv(v);  // past the end: what the sequence leaves in the taps, their dt is zero
-        asm("" : "+v"(v));  // one by one: as a vector the taps would be held eight times each
-        x[k][e] = v;
+      for (int e = 0; e < 2; ++e) {
+        // (masked exponents may be large: the product is not used)
+        const float v = sv[e] * (__builtin_amdgcn_exp2f((ihi - jhi[e]) + (ilo - jlo[e])) * dt[e]);
+        m[e] = j0 + e <= i ? v : 0.f;
       }
+      uint32_t hi, mid, lo;
+      split_pair(m[0], m[1], hi, mid, lo);
+      uint32_t* out = reinterpret_cast<uint32_t*>(lds + Lds::at_products(hw) + (to * hw + h) * Lds::products +
+                                                  it * 3 * kFragment + 16 * lane + 8 * jt + 4 * half);
+      out[0] = hi;
+      out[kFragment / 4] = mid;
+      out[2 * kFragment / 4] = lo;
+    }
+  };
+
+  // the first pass: log2 of the decay over the chunks so far
+  auto add_total = [&](int from) {
+#pragma unroll
+    for (int k = 0; k < TPW; ++k) {
+      const float* d = decays_at(from) + head[k] * 3 * Q;
+      total_hi[k] += d[2 * Q - 1];
+      total_lo[k] += d[3 * Q - 1];
+    }
   };
 
   if constexpr (!STATES) {
     // M's upper right quarter is zero throughout
-    for (int i = tid; i < hw * 3 * 64; i += 64 * kScanWaves) {
-      u32x2* z = reinterpret_cast<u32x2*>(products + (i / 192) * Lds::products + (i % 192) * 16 + 8);
-      *z = u32x2{0u, 0u};
-    }
+    for (int i = tid; i < 2 * hw * 3 * 64; i += 64 * kScanWaves)
+      *reinterpret_cast<u32x2*>(lds + Lds::at_products(hw) + i / 192 * Lds::products + i % 192 * 16 + 8) = u32x2{0u, 0u};
   }
   if (t_begin < t_end) {
-    request(t_begin, 0, BUF == 2 ? 3 : 1);
-    if (t_begin > 0) {
-      fetch(t_begin);
-    } else {
-#pragma unroll
-      for (int k = 0; k < TPW; ++k)
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int j = 0; j < 4 + W - 1; ++j)
-            raw[k][half][j] = raw1(rows, stride, taps, channels, W, 16 * half - (W - 1) + 4 * g + j, t_end, ch[k]);
-    }
-    convolve();
-  }
-  int buf = 0;
-  for (int t0 = t_begin; t0 < t_end; t0 += Q) {
-    const int next = t0 + Q;
-    const uint8_t* image = image_at(buf);
-    const float* dec = decays_at(buf);
     wait_all_loads();
-    __syncthreads();  // the chunk's image has come; what the last chunk used is free
-    if (BUF == 2) {
-      if (next < t_end) request(next, buf ^ 1, 3);
-    } else {
-      request(t0, 0, 2);
-    }
-    fetch(next);
-    // decays from the chunk's start (e) and to its end, with dt (w)
-    if (tid < hw * Q) {
-      const int h = tid / Q, q = tid % Q;
-      const float* d = dec + h * 3 * Q;
-      tables[h * 2 * Q + q] = __builtin_amdgcn_exp2f(d[Q + q] + d[2 * Q + q]);
-      tables[h * 2 * Q + Q + q] = d[q] * __builtin_amdgcn_exp2f((d[2 * Q - 1] - d[Q + q]) + (d[3 * Q - 1] - d[2 * Q + q]));
-    }
-    if constexpr (!STATES) {
-      for (int job = wave; job < 3 * hw; job += kScanWaves) {
-        const int h = job / 3, tile = job - 3 * h, jt = tile == 2, it = tile > 0;
-        const floatx4 sv = *reinterpret_cast<const floatx4*>(image + (kSAt + tile) * kFragment + 16 * lane);
-        const int i = 16 * it + col, j0 = 16 * jt + 4 * g;
-        const float* d = dec + h * 3 * Q;
-        const float ihi = d[Q + i], ilo = d[2 * Q + i];
-        const floatx4 dt = *reinterpret_cast<const floatx4*>(d + j0);
-        const floatx4 jhi = *reinterpret_cast<const floatx4*>(d + Q + j0);
-        const floatx4 jlo = *reinterpret_cast<const floatx4*>(d + 2 * Q + j0);
-        float m[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          m[e] = j0 + e <= i ? sv[e] * (__builtin_amdgcn_exp2f((ihi - jhi[e]) + (ilo - jlo[e])) * dt[e]) : 0.f;
-        u32x2 hi, mid, lo;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          uint32_t a, b, cc;
-          split_pair(m[2 * e], m[2 * e + 1], a, b, cc);
-          hi[e] = a;
-          mid[e] = b;
-          lo[e] = cc;
-        }
-        u32x2* out = reinterpret_cast<u32x2*>(products + h * Lds::products + it * 3 * kFragment + 16 * lane + 8 * jt);
-        out[0] = hi;
-        out[kFragment / 8] = mid;
-        out[2 * kFragment / 8] = lo;
-      }
-    }
     __syncthreads();
-    if constexpr (!STATES) {
-      const __amdgpu_buffer_rsrc_t rows_y = buffer_of(c.y + (int64_t)(s.begin + t0) * inner,
-                                                      (int64_t)(t_end - t0) * inner);
+    convolve(0);
+    make_tables(0, 0);
+    if constexpr (!STATES) make_products(0);
+    else add_total(0);
+    if (STATES && t_begin + Q < t_end) {
+      request_rows(t_begin + Q, 1);
+      request_decays(t_begin + Q, 1);
+    }
+  }
+  int buf = 0;  // of the chunk's tables and masked products; in the first pass of B, rows and decays too
+  for (int t0 = t_begin; t0 < t_end; t0 += Q, buf ^= 1) {
+    const int next = t0 + Q;
+    wait_all_loads();
+    // the chunk's images, products and tables are there (in the first pass
+    // also the next one's rows and decays); what the last chunk read is free
+    __syncthreads();
+    const float* tables = tables_at(buf);
+    if constexpr (STATES) {
+      if (next < t_end) request_image(next, kC, kB, (buf ^ 1) * Lds::b);
+      if (next + Q < t_end) {
+        request_rows(next + Q, buf);
+        request_decays(next + Q, buf);
+      }
+    } else {
+      request_image(t0, kC, kB, 0);
+      if (next < t_end) {
+        request_rows(next, 0);
+        request_decays(next, 0);
+        request_image(next, kC + kB, 3, Lds::at_s);
+      }
       floatx4 acc[2][TPW];
 #pragma unroll
       for (int it = 0; it < 2; ++it)
@@ -602,7 +657,7 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
       // the next block's fragments are read ahead, and no further ahead: read
       // where the compiler likes they crowd the state out of the registers
       auto c_at = [&](int t, int it, int part) {
-        return *reinterpret_cast<const u32x4*>(image + ((it * NB + t) * 3 + part) * kFragment + 16 * lane);
+        return *reinterpret_cast<const u32x4*>(lds + Lds::at_c + ((it * NB + t) * 3 + part) * kFragment + 16 * lane);
       };
       u32x4 a[2][3], ahead[2][3];
 #pragma unroll
@@ -624,81 +679,93 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
           sp[k] = split8(v);
         }
         // neighbouring products belong to different accumulators
-#define LLHIP_SSM_PRODUCT(PART, FIELD)                                     \
+#define LLHIP_SSM_PRODUCT(A, B)                                            \
   _Pragma("unroll") for (int it = 0; it < 2; ++it)                         \
       _Pragma("unroll") for (int k = 0; k < TPW; ++k)                      \
-          acc[it][k] = mma_one(a[it][PART], sp[k].FIELD, acc[it][k]);
-        LLHIP_SSM_PRODUCT(2, hi)
-        LLHIP_SSM_PRODUCT(0, lo)
-        LLHIP_SSM_PRODUCT(1, mid)
-        LLHIP_SSM_PRODUCT(1, hi)
-        LLHIP_SSM_PRODUCT(0, mid)
-        LLHIP_SSM_PRODUCT(0, hi)
-#undef LLHIP_SSM_PRODUCT
+          acc[it][k] = mma_one(A, B, acc[it][k]);
+        LLHIP_SSM_PRODUCT(a[it][2], sp[k].hi)
+        LLHIP_SSM_PRODUCT(a[it][0], sp[k].lo)
+        LLHIP_SSM_PRODUCT(a[it][1], sp[k].mid)
+        LLHIP_SSM_PRODUCT(a[it][1], sp[k].hi)
+        LLHIP_SSM_PRODUCT(a[it][0], sp[k].mid)
+        LLHIP_SSM_PRODUCT(a[it][0], sp[k].hi)
       }
       __builtin_amdgcn_sched_barrier(0);
+      // A non-finite x_j would reach the tokens before it, as 0 x_j in the
+      // masked part of the product: the products take zero in its place, and
+      // the channel's outputs from token j on are NaN (its state too, by x
+      // itself).
+      float xf[TPW][8], largest = 0.f;
+      int first_bad[TPW];
 #pragma unroll
       for (int k = 0; k < TPW; ++k) {
-        // A non-finite x_j would reach the tokens before it, as 0 x_j in the
-        // masked part of the product: the products take zero in its place,
-        // and the channel's outputs from token j on are NaN (its state too, by
-        // x itself).
-        float xf[8];
-        int first_bad = Q;
-        float largest = 0.f;
+        first_bad[k] = Q;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          xf[e] = x[k][e];
+          xf[k][e] = x[k][e];
           largest = __builtin_elementwise_maximum(largest, fabsf(x[k][e]));  // NaN if one is
         }
-        if (__ballot(!(largest <= FLT_MAX))) {
+      }
+      const bool all_finite = !__ballot(!(largest <= FLT_MAX));
+      if (!all_finite) {
+#pragma unroll
+        for (int k = 0; k < TPW; ++k) {
 #pragma unroll
           for (int e = 7; e >= 0; --e)
             if (!(fabsf(x[k][e]) <= FLT_MAX)) {
-              first_bad = 16 * (e >> 2) + 4 * g + (e & 3);
-              xf[e] = 0.f;
+              first_bad[k] = 16 * (e >> 2) + 4 * g + (e & 3);
+              xf[k][e] = 0.f;
             }
-          first_bad = min(first_bad, __shfl_xor(first_bad, 16, 64));
-          first_bad = min(first_bad, __shfl_xor(first_bad, 32, 64));
+          first_bad[k] = min(first_bad[k], __shfl_xor(first_bad[k], 16, 64));
+          first_bad[k] = min(first_bad[k], __shfl_xor(first_bad[k], 32, 64));
         }
-        const Split8 xs = split8(xf);
-        const uint8_t* m = products + head[k] * Lds::products;
+      }
+      Split8 xs[TPW];
+      u32x4 m[2][TPW][3];
+#pragma unroll
+      for (int k = 0; k < TPW; ++k) {
+        xs[k] = split8(xf[k]);
+        const uint8_t* from = lds + Lds::at_products(hw) + (buf * hw + head[k]) * Lds::products + 16 * lane;
 #pragma unroll
         for (int it = 0; it < 2; ++it) {
-          const floatx4 e4 = *reinterpret_cast<const floatx4*>(tables + head[k] * 2 * Q + 16 * it + 4 * g);
-          acc[it][k] *= e4;
-          u32x4 a[3];
+          acc[it][k] *= *reinterpret_cast<const floatx4*>(tables + head[k] * 2 * Q + 16 * it + 4 * g);
 #pragma unroll
           for (int part = 0; part < 3; ++part)
-            a[part] = *reinterpret_cast<const u32x4*>(m + (it * 3 + part) * kFragment + 16 * lane);
-          acc[it][k] = mma_one(a[2], xs.hi, acc[it][k]);
-          acc[it][k] = mma_one(a[0], xs.lo, acc[it][k]);
-          acc[it][k] = mma_one(a[1], xs.mid, acc[it][k]);
-          acc[it][k] = mma_one(a[1], xs.hi, acc[it][k]);
-          acc[it][k] = mma_one(a[0], xs.mid, acc[it][k]);
-          acc[it][k] = mma_one(a[0], xs.hi, acc[it][k]);
-        }
-#pragma unroll
-        for (int it = 0; it < 2; ++it) {
-          float v[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float u = fmaf(skip[k], xf[4 * it + e], acc[it][k][e]);
-            v[e] = 16 * it + 4 * g + e < first_bad ? u : __builtin_nanf("");
-          }
-          // rows past the segment's end lie past the buffer's
-          const uint32_t at0 = opaque(at_y[k]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v[e]), rows_y,
-                                                  at0 + (uint32_t)(16 * it + e) * (4u * (uint32_t)inner), 0, 0);
+            m[it][k][part] = *reinterpret_cast<const u32x4*>(from + (it * 3 + part) * kFragment);
         }
       }
-      if (BUF == 1) {
-        wait_all_loads();
-        __syncthreads();  // B has come; C, S and the decays are free
-        if (next < t_end) request(next, 0, 1);
+      LLHIP_SSM_PRODUCT(m[it][k][2], xs[k].hi)
+      LLHIP_SSM_PRODUCT(m[it][k][0], xs[k].lo)
+      LLHIP_SSM_PRODUCT(m[it][k][1], xs[k].mid)
+      LLHIP_SSM_PRODUCT(m[it][k][1], xs[k].hi)
+      LLHIP_SSM_PRODUCT(m[it][k][0], xs[k].mid)
+      LLHIP_SSM_PRODUCT(m[it][k][0], xs[k].hi)
+#undef LLHIP_SSM_PRODUCT
+      // the lane's four tokens of a channel become four channels of a token
+      const bool odd = lane & 1, high = lane & 2;
+#pragma unroll
+      for (int it = 0; it < 2; ++it)
+#pragma unroll
+        for (int k = 0; k < TPW; ++k) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[it][k][e] = fmaf(skip[k], xf[k][4 * it + e], acc[it][k][e]);
+          if (!all_finite)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (16 * it + 4 * g + e >= first_bad[k]) acc[it][k][e] = __builtin_nanf("");
+          transpose_quads(acc[it][k], odd, high);
+        }
+      wait_all_loads();  // B, the rows and S, requested a phase ago (and not the stores that follow)
+#pragma unroll
+      for (int it = 0; it < 2; ++it) {
+        const int t = t0 + 16 * it + 4 * g + (lane & 3);
+        float* out = c.y + (int64_t)(s.begin + t) * inner + h0 * p.head_dim + 4 * (col >> 2) - col;
+#pragma unroll
+        for (int k = 0; k < TPW; ++k)
+          if (on[k] && t < t_end) *reinterpret_cast<f32x4a4*>(out + ch[k]) = acc[it][k];
       }
+      __syncthreads();  // B and what the next chunk needs have come; C is free
+      if (next < t_end) request_image(next, 0, kC, Lds::at_c);
     }
     // the state: decayed, plus the tokens' products
     Split8 xs[TPW];
@@ -714,13 +781,9 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
       const float e = tab[Q - 1];
 #pragma unroll
       for (int n = 0; n < NT; ++n) st[k][n] *= e;
-      if (STATES) {
-        total_hi[k] += dec[head[k] * 3 * Q + 2 * Q - 1];
-        total_lo[k] += dec[head[k] * 3 * Q + 3 * Q - 1];
-      }
     }
     auto b_at = [&](int n, int part) {
-      return *reinterpret_cast<const u32x4*>(image + (kBAt + 3 * n + part) * kFragment + 16 * lane);
+      return *reinterpret_cast<const u32x4*>(lds + (STATES ? buf * Lds::b : 0) + (3 * n + part) * kFragment + 16 * lane);
     };
     u32x4 b[3], ahead[3];
 #pragma unroll
@@ -742,10 +805,12 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
       LLHIP_SSM_UPDATE(0, mid)
       LLHIP_SSM_UPDATE(0, hi)
 #undef LLHIP_SSM_UPDATE
-      if (n % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
-    convolve();
-    if (BUF == 2) buf ^= 1;
+    // the next chunk's (past the last one they are not used)
+    convolve(STATES ? buf ^ 1 : 0);
+    make_tables(STATES ? buf ^ 1 : 0, buf ^ 1);
+    if constexpr (!STATES) make_products(buf ^ 1);
+    else if (next < t_end) add_total(buf ^ 1);
   }
 
   float* dst = nullptr;
@@ -755,9 +820,10 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
 #pragma unroll
   for (int k = 0; k < TPW; ++k) {
     if (!on[k]) continue;
+    const int at_ch = h0 * p.head_dim + ch[k];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
-      *reinterpret_cast<floatx4*>(dst + (int64_t)ch[k] * N + 16 * n + 4 * g) = st[k][n];
+      *reinterpret_cast<floatx4*>(dst + (int64_t)at_ch * N + 16 * n + 4 * g) = st[k][n];
     if (STATES && g == 0 && ch[k] % p.head_dim == 0)
       p.seg_decay[(int64_t)(s.state0 + at.y) * p.heads + h0 + head[k]] = total_hi[k] + total_lo[k];
   }
@@ -964,7 +1030,7 @@ __global__ void ssm_reset_error_kernel(int* error) {
 int64_t ssm_max_chunks(int64_t tokens, int64_t sequences) { return tokens / kSsmChunk + sequences; }
 
 // Workgroups that a scan should have before a sequence is cut no further.
-constexpr int64_t kScanGroups = 512;
+constexpr int64_t kScanGroups = 256;
 constexpr int kMinSegment = 128;
 
 int ssm_segment_tokens(const SsmLayerPlan& p, int64_t tokens) {
@@ -1040,13 +1106,13 @@ static hipError_t scan_launch(const SsmLayerPlan& p, const SsmCall& c, int segme
   if (e != hipSuccess) return e;
   const dim3 grid((uint32_t)(max_segments * (p.heads / hw))), block(64 * kScanWaves);
   if (c.tokens > segment_tokens) {
-    e = launch(ssm_scan_kernel<NT, W, true>, grid, block, ScanLds<NT, true>::bytes(hw), s, p, c, segment_tokens, hw);
+    e = launch(ssm_scan_kernel<NT, W, true>, grid, block, ScanLds<NT, W, true>::bytes(hw, hw * p.head_dim), s, p, c, segment_tokens, hw);
     if (e != hipSuccess) return e;
     const int64_t size = (int64_t)p.heads * p.head_dim * 16 * NT;
     e = launch(ssm_join_kernel, dim3(c.sequences, (uint32_t)((size / 4 + 255) / 256)), dim3(256), 0, s, p);
     if (e != hipSuccess) return e;
   }
-  return launch(ssm_scan_kernel<NT, W, false>, grid, block, ScanLds<NT, false>::bytes(hw), s, p, c, segment_tokens,
+  return launch(ssm_scan_kernel<NT, W, false>, grid, block, ScanLds<NT, W, false>::bytes(hw, hw * p.head_dim), s, p, c, segment_tokens,
                 hw);
 }
 
