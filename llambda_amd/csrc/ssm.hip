@@ -536,25 +536,22 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
 
   // x of the lane's tokens 4 g .. + 3 and 16 + 4 g .. + 3 after the convolution
   float x[TPW][8];
-  auto convolve = [&](int buf) {
+  // (half a tile's at a time: its reads, and what is made of them)
+  float raw[4 + W - 1];
+  auto convolve_read = [&](int buf, int k, int half) {
+    const uint8_t* from = lds + Lds::at_rows(hw) + buf * Lds::rows * pitch + (4 * g + 16 * half) * pitch + 4 * ch[k];
 #pragma unroll
-    for (int k = 0; k < TPW; ++k) {
-      const uint8_t* from = lds + Lds::at_rows(hw) + buf * Lds::rows * pitch + 4 * g * pitch + 4 * ch[k];
+    for (int j = 0; j < 4 + W - 1; ++j) raw[j] = *reinterpret_cast<const float*>(from + j * pitch);
+  };
+  auto convolve = [&](int k, int half) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float raw[4 + W - 1];
+    for (int e = 0; e < 4; ++e) {
+      float v = bias[k];
 #pragma unroll
-        for (int j = 0; j < 4 + W - 1; ++j) raw[j] = *reinterpret_cast<const float*>(from + (16 * half + j) * pitch);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float v = bias[k];
-#pragma unroll
-          for (int j = 0; j < W; ++j) v = fmaf(w[k][j], raw[e + j], v);
-          v = silu_conv(v);
-          asm("" : "+v"(v));  // one by one: as a vector the taps would be held eight times each
-          x[k][4 * half + e] = v;
-        }
-      }
+      for (int j = 0; j < W; ++j) v = fmaf(w[k][j], raw[e + j], v);
+      v = silu_conv(v);
+      asm("" : "+v"(v));  // one by one: as a vector the taps would be held eight times each
+      x[k][4 * half + e] = v;
     }
   };
   auto decays_at = [&](int buf) { return reinterpret_cast<const float*>(lds + Lds::at_decays + buf * hw * Lds::decays); };
@@ -571,11 +568,11 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
   // M = S o L of the workgroup's heads, as left operands: job (head, tile,
   // half), a lane's two neighbouring j of column i.  (Past the last job that
   // one again.)
-  auto make_products = [&](int to) {
+  constexpr int kJobs = STATES ? 0 : (6 * scan_max_heads(NT) + kScanWaves - 1) / kScanWaves;
+  auto make_products = [&](int n, int to) {
     const float* dec = decays_at(0);
-#pragma unroll
-    for (int n = 0; n < 6 * scan_max_heads(NT); n += kScanWaves) {
-      const int job = min(n + wave, 6 * hw - 1);
+    {
+      const int job = min(n * kScanWaves + wave, 6 * hw - 1);
       const int h = job / 6, tile = job % 6 / 2, half = job % 2, jt = tile == 2, it = tile > 0;
       const floatx2 sv = *reinterpret_cast<const floatx2*>(lds + Lds::at_s + tile * kFragment + 16 * lane + 8 * half);
       const int i = 16 * it + col, j0 = 16 * jt + 4 * g + 2 * half;
@@ -619,10 +616,15 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
   if (t_begin < t_end) {
     wait_all_loads();
     __syncthreads();
-    convolve(0);
+#pragma unroll
+    for (int k = 0; k < 2 * TPW; ++k) {
+      convolve_read(0, k >> 1, k & 1);
+      convolve(k >> 1, k & 1);
+    }
     make_tables(0, 0);
-    if constexpr (!STATES) make_products(0);
-    else add_total(0);
+#pragma unroll
+    for (int n = 0; n < kJobs; ++n) make_products(n, 0);
+    if (STATES) add_total(0);
     if (STATES && t_begin + Q < t_end) {
       request_rows(t_begin + Q, 1);
       request_decays(t_begin + Q, 1);
@@ -643,12 +645,6 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
         request_decays(next + Q, buf);
       }
     } else {
-      request_image(t0, kC, kB, 0);
-      if (next < t_end) {
-        request_rows(next, 0);
-        request_decays(next, 0);
-        request_image(next, kC + kB, 3, Lds::at_s);
-      }
       floatx4 acc[2][TPW];
 #pragma unroll
       for (int it = 0; it < 2; ++it)
@@ -689,6 +685,14 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
         LLHIP_SSM_PRODUCT(a[it][1], sp[k].hi)
         LLHIP_SSM_PRODUCT(a[it][0], sp[k].mid)
         LLHIP_SSM_PRODUCT(a[it][0], sp[k].hi)
+        // loads for the state phase: in parts, for a wavefront waits where
+        // the memory pipeline is busy with the others'
+        if (t == 0) request_image(t0, kC, kB, 0);
+        if (t == std::min(1, NB - 1) && next < t_end) request_rows(next, 0);
+        if (t == std::min(2, NB - 1) && next < t_end) {
+          request_decays(next, 0);
+          request_image(next, kC + kB, 3, Lds::at_s);
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
       // A non-finite x_j would reach the tokens before it, as 0 x_j in the
@@ -765,7 +769,6 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
           if (on[k] && t < t_end) *reinterpret_cast<f32x4a4*>(out + ch[k]) = acc[it][k];
       }
       __syncthreads();  // B and what the next chunk needs have come; C is free
-      if (next < t_end) request_image(next, 0, kC, Lds::at_c);
     }
     // the state: decayed, plus the tokens' products
     Split8 xs[TPW];
@@ -785,16 +788,31 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
     auto b_at = [&](int n, int part) {
       return *reinterpret_cast<const u32x4*>(lds + (STATES ? buf * Lds::b : 0) + (3 * n + part) * kFragment + 16 * lane);
     };
+    // Between the products of the n tiles, what the next chunk needs (past the
+    // last one it is not used): the wavefronts of a SIMD take turns with the
+    // matrix cores and the vector unit.
+    constexpr int kPieces = 2 * TPW + kJobs + 1;
+    auto piece_read = [&](int i) {
+      if (i < 2 * TPW) convolve_read(STATES ? buf ^ 1 : 0, i >> 1, i & 1);
+    };
+    auto piece = [&](int i) {
+      if (i < 2 * TPW) convolve(i >> 1, i & 1);
+      else if (i < 2 * TPW + kJobs) make_products(i - 2 * TPW, buf ^ 1);
+      else make_tables(STATES ? buf ^ 1 : 0, buf ^ 1);
+    };
     u32x4 b[3], ahead[3];
 #pragma unroll
     for (int part = 0; part < 3; ++part) ahead[part] = b_at(0, part);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int part = 0; part < 3; ++part) {
         b[part] = ahead[part];
         if (n + 1 < NT) ahead[part] = b_at(n + 1, part);
       }
+      const int first = n * kPieces / NT, last = (n + 1) * kPieces / NT;
+      if (first < last) piece_read(first);
 #define LLHIP_SSM_UPDATE(PART, FIELD)                                      \
   _Pragma("unroll") for (int k = 0; k < TPW; ++k)                          \
       st[k][n] = mma_one(b[PART], xs[k].FIELD, st[k][n]);
@@ -805,12 +823,14 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
       LLHIP_SSM_UPDATE(0, mid)
       LLHIP_SSM_UPDATE(0, hi)
 #undef LLHIP_SSM_UPDATE
+#pragma unroll
+      for (int i = first; i < last; ++i) {
+        if (i > first) piece_read(i);
+        piece(i);
+      }
+      if (!STATES && n == 0 && next < t_end) request_image(next, 0, kC, Lds::at_c);
     }
-    // the next chunk's (past the last one they are not used)
-    convolve(STATES ? buf ^ 1 : 0);
-    make_tables(STATES ? buf ^ 1 : 0, buf ^ 1);
-    if constexpr (!STATES) make_products(buf ^ 1);
-    else if (next < t_end) add_total(buf ^ 1);
+    if (STATES && next < t_end) add_total(buf ^ 1);
   }
 
   float* dst = nullptr;
