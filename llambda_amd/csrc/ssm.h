@@ -77,8 +77,7 @@ struct SsmCall {
 inline int ssm_row(const SsmLayerPlan& p) {
   return 2 * p.heads * p.head_dim + 2 * p.groups * p.state + p.heads;
 }
-// Tokens per segment of a call, and the bounds of its tables.
-int ssm_segment_tokens(const SsmLayerPlan& p, int64_t tokens);
+// Bounds of the tables and buffers of a call of at most so many.
 int64_t ssm_max_chunks(int64_t tokens, int64_t sequences);
 int64_t ssm_max_segments(const SsmLayerPlan& p, int64_t tokens, int64_t sequences);
 size_t ssm_image_bytes(int state);

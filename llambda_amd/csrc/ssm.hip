@@ -359,16 +359,16 @@ __device__ __forceinline__ void wait_all_loads() {
 
 constexpr int kScanWaves = 8;
 
-// Column tiles of 16 channels per wavefront (the state of one takes N / 4
-// registers) and heads per workgroup at most (their masked products take 12 KB
-// of LDS each).
-constexpr int scan_tiles(int nt) { return nt > 8 ? 1 : 2; }
+// Column tiles of 16 channels per wavefront at most (the state of one takes
+// N / 4 registers) and heads per workgroup at most (their masked products take
+// 12 KB of LDS each).
+constexpr int scan_max_tiles(int nt) { return nt > 8 ? 1 : 2; }
 constexpr int scan_max_heads(int nt) { return nt > 8 ? 2 : 4; }
 
 // Heads per workgroup: as many whole heads of one group as fit its tiles.
-static int scan_heads(const SsmLayerPlan& p) {
-  const int share = p.heads / p.groups, nt = p.state / 16;
-  int n = std::min(scan_max_heads(nt), std::max(1, kScanWaves * scan_tiles(nt) * 16 / p.head_dim));
+static int scan_heads(const SsmLayerPlan& p, int tiles) {
+  const int share = p.heads / p.groups;
+  int n = std::min(scan_max_heads(p.state / 16), std::max(1, kScanWaves * tiles * 16 / p.head_dim));
   while (share % n) --n;
   return n;
 }
@@ -423,11 +423,11 @@ __device__ __forceinline__ void transpose_quads(floatx4& v, bool odd, bool high)
 // or more ahead: a load of one dword per lane costs the memory pipeline as
 // much as one of sixteen bytes, and reading x that way took it 5000 cycles of
 // a chunk's 17000.
-template <int NT, int W, bool STATES>
+template <int NT, int W, int TPW, bool STATES>
 __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan p, SsmCall c,
                                                                    int segment_tokens, int hw) {
   using Lds = ScanLds<NT, W, STATES>;
-  constexpr int N = 16 * NT, Q = kSsmChunk, NB = n_blocks(NT), TPW = scan_tiles(NT);
+  constexpr int N = 16 * NT, Q = kSsmChunk, NB = n_blocks(NT);
   constexpr int kC = c_fragments(NT), kB = b_fragments(NT), kImage = image_fragments(NT) * kFragment;
   extern __shared__ __align__(16) uint8_t lds[];
   const int width = hw * p.head_dim, pitch = Lds::pitch(width);
@@ -571,7 +571,7 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
   constexpr int kJobs = STATES ? 0 : (6 * scan_max_heads(NT) + kScanWaves - 1) / kScanWaves;
   auto make_products = [&](int n, int to) {
     const float* dec = decays_at(0);
-    {
+    if (n * kScanWaves < 6 * hw) {
       const int job = min(n * kScanWaves + wave, 6 * hw - 1);
       const int h = job / 6, tile = job % 6 / 2, half = job % 2, jt = tile == 2, it = tile > 0;
       const floatx2 sv = *reinterpret_cast<const floatx2*>(lds + Lds::at_s + tile * kFragment + 16 * lane + 8 * half);
@@ -1049,21 +1049,59 @@ __global__ void ssm_reset_error_kernel(int* error) {
 
 int64_t ssm_max_chunks(int64_t tokens, int64_t sequences) { return tokens / kSsmChunk + sequences; }
 
-// Workgroups that a scan should have before a sequence is cut no further.
-constexpr int64_t kScanGroups = 256;
-constexpr int kMinSegment = 128;
+// How a call is cut: column tiles per wavefront and tokens per segment.  A
+// scan workgroup has a CU to itself (its LDS), so a pass takes as many rounds
+// as it has workgroups to the device's 256 CUs.  The times are measured ones of
+// N = 128 (us): two tiles a wavefront share a group's operands between twice
+// the channels; one tile halves a chunk's latency where there are CUs to
+// spare.  Segments add the first pass, the join and the launches of both.
+struct ScanCut {
+  int tiles, segment_tokens;
+};
+constexpr int kScanCus = 256;
+constexpr int kMinSegment = 64;
+static double scan_begin_us(int tiles) { return tiles == 2 ? 6.0 : 5.0; }
+static double scan_chunk_us(int tiles) { return tiles == 2 ? 9.0 : 5.2; }
+constexpr double kFirstPassShare = 0.45, kJoinUs = 12.0;
 
-int ssm_segment_tokens(const SsmLayerPlan& p, int64_t tokens) {
-  const int64_t sets = p.heads / scan_heads(p);
-  const int64_t n = (tokens * sets + kScanGroups - 1) / kScanGroups;
-  return (int)std::max<int64_t>(kMinSegment, (n + kSsmChunk - 1) / kSsmChunk * kSsmChunk);
+// Segments that the whole segments of a call may number.
+static int64_t scan_segment_limit(const SsmLayerPlan& p, int tiles) {
+  return 2 * kScanCus / (p.heads / scan_heads(p, tiles)) + 1;
 }
+
+static ScanCut scan_cut(const SsmLayerPlan& p, int64_t tokens, int64_t sequences) {
+  ScanCut best{1, 0};
+  double least = 1e30;
+  for (int tiles = 1; tiles <= scan_max_tiles(p.state / 16); ++tiles) {
+    const int64_t sets = p.heads / scan_heads(p, tiles);
+    const int64_t most = std::max<int64_t>(1, std::min(tokens / kMinSegment, scan_segment_limit(p, tiles)));
+    for (int64_t m = 1; m <= most; m += std::max<int64_t>(1, m / 8)) {
+      const int64_t part = (tokens + m - 1) / m;
+      const int64_t seg = std::max<int64_t>(kMinSegment, (part + kSsmChunk - 1) / kSsmChunk * kSsmChunk);
+      // the sequences' lengths are on the device: each ends half a segment on
+      // average, and the longest is taken for twice the average
+      const int64_t cut = sequences == 1 ? (tokens + seg - 1) / seg
+                                         : std::max(sequences, tokens / seg + sequences / 2);
+      const int64_t longest = std::min(seg, sequences == 1 ? tokens : 2 * tokens / sequences + kSsmChunk);
+      const double rounds = (double)((cut * sets + kScanCus - 1) / kScanCus);
+      const double chunks = (double)((longest + kSsmChunk - 1) / kSsmChunk);
+      double us = rounds * (scan_begin_us(tiles) + chunks * scan_chunk_us(tiles));
+      if (tokens > seg) us += kJoinUs + rounds * (scan_begin_us(tiles) + kFirstPassShare * chunks * scan_chunk_us(tiles));
+      if (us < least) {
+        least = us;
+        best = ScanCut{tiles, (int)seg};
+      }
+    }
+  }
+  return best;
+}
+
 int64_t ssm_max_segments(const SsmLayerPlan& p, int64_t tokens, int64_t sequences) {
-  // of any call of at most `tokens`: its segments hold kMinSegment tokens at
-  // least, and no more than kScanGroups / sets are full ones
-  return std::min<int64_t>(tokens / kMinSegment, kScanGroups / (p.heads / scan_heads(p))) + sequences;
+  int64_t limit = 0;
+  for (int tiles = 1; tiles <= scan_max_tiles(p.state / 16); ++tiles)
+    limit = std::max(limit, scan_segment_limit(p, tiles));
+  return std::min(tokens / kMinSegment, limit) + sequences;
 }
-
 int64_t ssm_max_states(const SsmLayerPlan& p, int64_t tokens) {
   // a sequence of n > 1 segments fills n - 1 >= n / 2 of them
   return 2 * (ssm_max_segments(p, tokens, 0) + 1);
@@ -1115,50 +1153,56 @@ hipError_t ssm_step_launch(const SsmLayerPlan& p, const SsmCall& c, hipStream_t 
   return finish_launch(p, c, s);
 }
 
-template <int NT, int W>
-static hipError_t scan_launch(const SsmLayerPlan& p, const SsmCall& c, int segment_tokens,
-                              int64_t max_segments, hipStream_t s) {
-  const int hw = scan_heads(p);
-  const int64_t chunks = ssm_max_chunks(c.tokens, c.sequences);
-  hipError_t e = launch(ssm_prepare_kernel<NT, W>,
-                        dim3((uint32_t)chunks, p.groups + (p.heads + kPrepHeads - 1) / kPrepHeads), dim3(256), 0, s,
-                        p, c);
-  if (e != hipSuccess) return e;
-  const dim3 grid((uint32_t)(max_segments * (p.heads / hw))), block(64 * kScanWaves);
+template <int NT, int W, int TPW>
+static hipError_t scan_launch(const SsmLayerPlan& p, const SsmCall& c, int segment_tokens, hipStream_t s) {
+  const int hw = scan_heads(p, TPW), width = hw * p.head_dim;
+  const int64_t segments = c.tokens / segment_tokens + c.sequences;
+  const dim3 grid((uint32_t)(segments * (p.heads / hw))), block(64 * kScanWaves);
   if (c.tokens > segment_tokens) {
-    e = launch(ssm_scan_kernel<NT, W, true>, grid, block, ScanLds<NT, W, true>::bytes(hw, hw * p.head_dim), s, p, c, segment_tokens, hw);
+    hipError_t e = launch(ssm_scan_kernel<NT, W, TPW, true>, grid, block, ScanLds<NT, W, true>::bytes(hw, width), s,
+                          p, c, segment_tokens, hw);
     if (e != hipSuccess) return e;
     const int64_t size = (int64_t)p.heads * p.head_dim * 16 * NT;
     e = launch(ssm_join_kernel, dim3(c.sequences, (uint32_t)((size / 4 + 255) / 256)), dim3(256), 0, s, p);
     if (e != hipSuccess) return e;
   }
-  return launch(ssm_scan_kernel<NT, W, false>, grid, block, ScanLds<NT, W, false>::bytes(hw, hw * p.head_dim), s, p, c, segment_tokens,
-                hw);
+  return launch(ssm_scan_kernel<NT, W, TPW, false>, grid, block, ScanLds<NT, W, false>::bytes(hw, width), s, p, c,
+                segment_tokens, hw);
 }
 
-template <int W>
+template <int NT, int W>
 static hipError_t run_launch(const SsmLayerPlan& p, const SsmCall& c, hipStream_t s) {
-  const int segment_tokens = ssm_segment_tokens(p, c.tokens);
-  const int64_t segments = c.tokens / segment_tokens + c.sequences;
-  hipError_t e = launch(ssm_plan_kernel, dim3(c.sequences), dim3(kPlanThreads), 0, s, p, c, segment_tokens);
+  const ScanCut cut = scan_cut(p, c.tokens, c.sequences);
+  hipError_t e = launch(ssm_plan_kernel, dim3(c.sequences), dim3(kPlanThreads), 0, s, p, c, cut.segment_tokens);
   if (e != hipSuccess) return e;
-  switch (p.state) {
-    case 16: e = scan_launch<1, W>(p, c, segment_tokens, segments, s); break;
-    case 32: e = scan_launch<2, W>(p, c, segment_tokens, segments, s); break;
-    case 64: e = scan_launch<4, W>(p, c, segment_tokens, segments, s); break;
-    case 128: e = scan_launch<8, W>(p, c, segment_tokens, segments, s); break;
-    case 256: e = scan_launch<16, W>(p, c, segment_tokens, segments, s); break;
-    default: return hipErrorInvalidValue;
-  }
+  e = launch(ssm_prepare_kernel<NT, W>,
+             dim3((uint32_t)ssm_max_chunks(c.tokens, c.sequences), p.groups + (p.heads + kPrepHeads - 1) / kPrepHeads),
+             dim3(256), 0, s, p, c);
+  if (e != hipSuccess) return e;
+  if constexpr (scan_max_tiles(NT) == 2)
+    if (cut.tiles == 2) e = scan_launch<NT, W, 2>(p, c, cut.segment_tokens, s);
+  if (cut.tiles == 1) e = scan_launch<NT, W, 1>(p, c, cut.segment_tokens, s);
   if (e != hipSuccess) return e;
   return finish_launch(p, c, s);
 }
 
+template <int W>
+static hipError_t run_state(const SsmLayerPlan& p, const SsmCall& c, hipStream_t s) {
+  switch (p.state) {
+    case 16: return run_launch<1, W>(p, c, s);
+    case 32: return run_launch<2, W>(p, c, s);
+    case 64: return run_launch<4, W>(p, c, s);
+    case 128: return run_launch<8, W>(p, c, s);
+    case 256: return run_launch<16, W>(p, c, s);
+    default: return hipErrorInvalidValue;
+  }
+}
+
 hipError_t ssm_run_launch(const SsmLayerPlan& p, const SsmCall& c, hipStream_t s) {
   switch (p.conv) {
-    case 2: return run_launch<2>(p, c, s);
-    case 3: return run_launch<3>(p, c, s);
-    case 4: return run_launch<4>(p, c, s);
+    case 2: return run_state<2>(p, c, s);
+    case 3: return run_state<3>(p, c, s);
+    case 4: return run_state<4>(p, c, s);
     default: return hipErrorInvalidValue;
   }
 }
