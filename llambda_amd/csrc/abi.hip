@@ -2103,7 +2103,7 @@ struct llambda_hip_batch_sampler {
   int device = 0;
   hipStream_t stream = nullptr;
   size_t vocab = 0, max_rows = 0;
-  DevBuf chunk_max, chunk_mass;
+  DevBuf chunk_max, chunk_mass, bins, list, listed;
   DevBuf logits, params, tokens;  // device staging of the host-pointer runs
   size_t staged = 0;
   // recorded after every call; the next one, which shares the workspace, waits
@@ -2118,7 +2118,10 @@ namespace {
 
 void batch_sample_enqueue(llambda_hip_batch_sampler* s, SampleRows r, hipStream_t st) {
   r.chunk_max = s->chunk_max.as<float>();
-  r.chunk_mass = s->chunk_mass.as<double>();
+  r.chunk_mass = s->chunk_mass.as<uint64_t>();
+  r.bins = s->bins.as<uint64_t>();
+  r.list = s->list.as<uint64_t>();
+  r.listed = s->listed.as<int>();
   hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
   HIPC(hipStreamIsCapturing(st, &capture));
   const bool ordered = capture == hipStreamCaptureStatusNone;
@@ -2158,7 +2161,10 @@ int llambda_hip_batch_sampler_create(size_t vocab, size_t max_rows,
     HIPC(hipEventCreateWithFlags(&s->done, hipEventDisableTiming));
     const size_t chunks = max_rows * (size_t)sample_chunks((int)vocab);
     s->chunk_max.alloc(chunks * sizeof(float), "chunk maxima");
-    s->chunk_mass.alloc(chunks * sizeof(double), "chunk masses");
+    s->chunk_mass.alloc(chunks * sizeof(uint64_t), "chunk masses");
+    s->bins.alloc(max_rows * kBatchBins * sizeof(uint64_t), "sampling bins");
+    s->list.alloc(max_rows * kBatchList * sizeof(uint64_t), "sampling candidates");
+    s->listed.alloc(max_rows * sizeof(int), "sampling candidate counts");
     *result = s.release();
   });
 }
@@ -2179,7 +2185,7 @@ int llambda_hip_batch_sampler_sample_device(llambda_hip_batch_sampler* s, const 
     std::lock_guard<std::mutex> lock(s->run_mutex);
     HIPC(hipSetDevice(s->device));
     SampleRows r{logits, (int)count, (int)rows, a->temperature, a->top_k, a->top_p, a->min_p,
-                 a->random_value, tokens, nullptr, nullptr};
+                 a->random_value, tokens, nullptr, nullptr, nullptr, nullptr, nullptr};
     batch_sample_enqueue(s, r, stream ? static_cast<hipStream_t>(stream) : s->stream);
   });
 }

@@ -15,9 +15,12 @@
 
 namespace llhip {
 
-constexpr int kBatchChunk = 256;  // logits whose maximum and mass the first launch records
+// Workspace: at most 62 KB a row.
+constexpr int kBatchChunk = 256;  // logits whose maximum the first launch records
 constexpr int kBatchMaxVocab = 262144;
 constexpr int kBatchMaxChunks = kBatchMaxVocab / kBatchChunk;
+constexpr int kBatchBins = 2048;  // of (max - l) / T, 64 to one
+constexpr int kBatchList = 4096;  // logits of the bin that a cut falls into, or candidates
 
 struct SampleRows {
   const float* logits;  // [rows][n]
@@ -29,9 +32,12 @@ struct SampleRows {
   const float* min_p;
   const float* random;  // [rows], in [0, 1)
   int* tokens;          // [rows]
-  // workspace: [rows][chunks]
-  float* chunk_max;
-  double* chunk_mass;
+  // workspace, per row
+  float* chunk_max;      // [chunks]
+  uint64_t* chunk_mass;  // [chunks]: weights kept above the cut
+  uint64_t* bins;        // [kBatchBins]
+  uint64_t* list;        // [kBatchList]
+  int* listed;           // [1]
 };
 
 inline int sample_chunks(int n) { return (n + kBatchChunk - 1) / kBatchChunk; }

@@ -1,40 +1,44 @@
 // sample_batch.hip -- the next token of each row (sample_batch.h).
 //
-// sample_chunks_kernel reads the logits once, a wavefront per 256 of them, and
-// records each chunk's maximum (and its mass exp((l - max) / T) where the row
-// needs its total).  sample_finish_kernel, a workgroup per row, then reads only
-// what it has to:
+// sample_chunks_kernel reads the logits once and records the maximum of each
+// 256 of them (a chunk).  What follows reads only what a row has to:
 //   top-k of at most as many ranks as there are chunks: at least k logits are
-//     at or above the k-th highest chunk maximum, and few more; the chunks that
-//     reach it are read again and those logits listed in LDS
-//   min-p: the logits whose weight reaches it, likewise
-//   neither, and no top-p: the draw goes by the chunks' masses and reads one
-//     chunk
-//   else, and where a list outgrows LDS: the whole row, binned by
-//     (max - l) / T in steps of 1/64, the bin that the cut falls into listed or,
-//     if it is too large (equal logits), resolved digit by digit
-// A list is sorted by (logit, index), cut by top-k, top-p and min-p, sorted by
-// index and drawn from.  Masses of whole rows are 64-bit integers in steps of
-// 2^-44, so that sums do not depend on the order of the atomics.
+//     at or above the k-th highest chunk maximum, and few more.  The row's
+//     workgroup (sample_finish_kernel) reads the chunks that reach it and lists
+//     those logits in LDS: up to 64 ranks are settled by one wavefront
+//   no top-k: the row is shared by eight workgroups.  With top-p
+//     (sample_mass_kernel) its weights are summed by bins of (max - l) / T, 64 to
+//     one; then (sample_cut_kernel) every chunk's weight above the bin that the
+//     cut falls into is summed, and that bin's logits are listed; without, every
+//     chunk's weights of at least min-p
+//   more ranks than chunks: the same bins hold counts, and all logits down to
+//     the bin of the k-th are listed
+//   lists that outgrow their 4096 entries (equal logits, more ranks): passes of
+//     the row's workgroup over all of it, resolving the cut digit by digit
+// At the end there is a lowest kept logit and each chunk's kept weight; the
+// draw finds its chunk by their sums and reads that.  Weights of whole rows are
+// integers in steps of 2^-44, so that sums do not depend on the atomics' order;
+// with the bins' powers in a table one takes 5 operations in 64 bits and a
+// short series in 32 (off by 1e-9 of it at most, without a bias), a fourth of
+// an exponential in 64 bits, which bound these passes.
 #include "sample_batch.h"
 
 #include <climits>
+
+#include "moe_gate.h"
 
 namespace llhip {
 
 typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
 
-constexpr int kFinishThreads = 1024;
-constexpr int kListMax = 4096;
-constexpr int kBins = 2048;         // of (max - l) / T, 64 to one; the last takes the rest
+constexpr int kRowThreads = 1024;
 constexpr double kMassOne = 17592186044416.0;  // 2^44
 
-// The parameters of a row, and what follows from them.
+// The parameters of a row.
 struct RowParams {
-  double temperature, top_p, min_p, random;
-  int top_k;      // 0: off
+  double sharpness, top_p, min_p, random;  // sharpness: 1 / temperature
+  int top_k;                               // 0: off
   bool bad;
-  bool mass;      // the row needs its total before it is cut
 };
 
 __device__ __forceinline__ RowParams row_params(const SampleRows& s, int row) {
@@ -45,18 +49,39 @@ __device__ __forceinline__ RowParams row_params(const SampleRows& s, int row) {
   const int k = s.top_k ? s.top_k[row] : 0;
   p.bad = !(t >= 0.f && t <= 3.402823466e38f) || !(tp > 0.f && tp <= 1.f) || !(mp >= 0.f && mp <= 1.f) ||
           !(r >= 0.f && r < 1.f) || k < 0;
-  p.temperature = t > 0.f ? t : 1.0;
+  p.sharpness = t > 0.f ? 1.0 / (double)t : 1.0;
   p.top_k = t > 0.f ? (k >= s.n ? 0 : k) : 1;
   p.top_p = tp;
   p.min_p = mp;
   p.random = r;
-  p.mass = p.top_k == 0 && (tp < 1.f || !(mp > 0.f));
   return p;
 }
 
-// exp(l / T - max / T); 1 for the maximum itself, which may be infinite.
-__device__ __forceinline__ double weight(float l, float top, double t) {
-  return l == top ? 1.0 : exp((double)l / t - (double)top / t);
+// exp(x) for x <= 0 in 64 bits: 2^n e^r with |r| <= ln 2 / 2, e^r by its series
+// to r^12 (what follows is below 2e-16).
+__device__ __forceinline__ double exp_below(double x) {
+  const double n = rint(x * 1.44269504088896340736);
+  double r = fma(n, -6.93147180369123816490e-01, x);  // ln 2 in two parts, the first of 32 bits
+  r = fma(n, -1.90821492927058770002e-10, r);
+  double e = 1.0 / 479001600.0;
+  e = fma(e, r, 1.0 / 39916800.0);
+  e = fma(e, r, 1.0 / 3628800.0);
+  e = fma(e, r, 1.0 / 362880.0);
+  e = fma(e, r, 1.0 / 40320.0);
+  e = fma(e, r, 1.0 / 5040.0);
+  e = fma(e, r, 1.0 / 720.0);
+  e = fma(e, r, 1.0 / 120.0);
+  e = fma(e, r, 1.0 / 24.0);
+  e = fma(e, r, 1.0 / 6.0);
+  e = fma(e, r, 0.5);
+  e = fma(e, r, 1.0);
+  e = fma(e, r, 1.0);
+  return x < -700.0 ? 0.0 : ldexp(e, (int)n);
+}
+
+// exp((l - max) / T), r = 1 / T; 1 for the maximum itself, which may be infinite.
+__device__ __forceinline__ double weight(float l, float top, double r) {
+  return l == top ? 1.0 : exp_below(((double)l - (double)top) * r);
 }
 
 // Order-preserving key of a float that is no NaN; -0 and +0 are equal.
@@ -92,6 +117,9 @@ constexpr int kChunksPerWave = 4;
 __global__ void __launch_bounds__(256) sample_chunks_kernel(SampleRows s) {
   const int row = blockIdx.y, lane = threadIdx.x & 63;
   const int chunks = (s.n + kBatchChunk - 1) / kBatchChunk;
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < kBatchBins; i += gridDim.x * 256)
+    s.bins[(int64_t)row * kBatchBins + i] = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) s.listed[row] = 0;
   const int first = (blockIdx.x * 4 + (threadIdx.x >> 6)) * kChunksPerWave;
   if (first >= chunks) return;
   const float* logits = s.logits + (int64_t)row * s.n;
@@ -99,7 +127,6 @@ __global__ void __launch_bounds__(256) sample_chunks_kernel(SampleRows s) {
 #pragma unroll
   for (int c = 0; c < kChunksPerWave; ++c)
     load_chunk(logits, s.n, min(first + c, chunks - 1), lane, v[c]);
-  const RowParams p = row_params(s, row);
 #pragma unroll
   for (int c = 0; c < kChunksPerWave; ++c) {
     bool nan = false;
@@ -110,39 +137,29 @@ __global__ void __launch_bounds__(256) sample_chunks_kernel(SampleRows s) {
       m = fmaxf(m, v[c][e]);
     }
     m = wave_max(m);
-    double mass = 0.0;
-    if (p.mass) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        mass += v[c][e] > -INFINITY ? weight(v[c][e], m, p.temperature) : 0.0;
-      for (int o = 32; o > 0; o >>= 1) mass += __shfl_xor(mass, o, 64);
-    }
     nan = __ballot(nan) != 0;
-    if (lane == 0 && first + c < chunks) {
-      s.chunk_max[(int64_t)row * chunks + first + c] = nan ? NAN : m;
-      s.chunk_mass[(int64_t)row * chunks + first + c] = mass;
-    }
+    if (lane == 0 && first + c < chunks) s.chunk_max[(int64_t)row * chunks + first + c] = nan ? NAN : m;
   }
 }
 
-// ------------------------------------------------------------------ the row's workgroup
+// ------------------------------------------------------------------ a workgroup on a row
 
-struct FinishLds {
-  uint64_t list[kListMax];
-  double weights[kListMax];       // of the list; the bins' masses
-  uint32_t counts[kBins];
-  double chunk_mass[kBatchMaxChunks];
+struct RowLds {
+  uint64_t list[kBatchList];
+  uint64_t bins[kBatchBins];
+  double powers[kBatchBins];  // e^(-b / 64), times 2^44
+  uint64_t mass[kBatchMaxChunks];
   float chunk_max[kBatchMaxChunks];
-  uint64_t wave[kFinishThreads / 64];
+  uint64_t wave[kRowThreads / 64];
   uint64_t result[4];
   int count;
 };
 
-// Every thread of the block calls the functions below.
+// Every thread of the block calls the functions below, but for draw_by_wave.
 
 // Inclusive prefix sums of T over the block in thread order; *total gets the sum.
 template <typename T>
-__device__ T block_scan(T v, FinishLds& l, T* total) {
+__device__ T block_scan(T v, RowLds& l, T* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   T* part = reinterpret_cast<T*>(l.wave);
   for (int o = 1; o < 64; o <<= 1) {
@@ -152,7 +169,7 @@ __device__ T block_scan(T v, FinishLds& l, T* total) {
   if (lane == 63) part[wave] = v;
   __syncthreads();
   T before = 0, all = 0;
-  for (int w = 0; w < kFinishThreads / 64; ++w) {
+  for (int w = 0; w < kRowThreads / 64; ++w) {
     const T u = part[w];
     before += w < wave ? u : (T)0;
     all += u;
@@ -162,17 +179,69 @@ __device__ T block_scan(T v, FinishLds& l, T* total) {
   return before + v;
 }
 
-// Sort list[0, n) in descending order (n <= kListMax; zeros pad it).
-__device__ void sort_list(FinishLds& l, int n) {
-  int size = 64;
+// The row's highest logit, its chunks' in LDS; false where it has none or a NaN (a chunk with one
+// carries it).
+__device__ bool row_top(RowLds& l, const SampleRows& s, int row, bool bad, float& top) {
+  const int tid = threadIdx.x, chunks = (s.n + kBatchChunk - 1) / kBatchChunk;
+  const float m = tid < chunks ? s.chunk_max[(int64_t)row * chunks + tid] : -INFINITY;
+  const bool nan = m != m;
+  if (tid < chunks) l.chunk_max[tid] = m;
+  top = wave_max(nan ? -INFINITY : m);
+  float* tops = reinterpret_cast<float*>(l.wave);
+  if ((tid & 63) == 0) tops[tid >> 6] = top;
+  const int any = __syncthreads_or(nan || bad);
+  for (int w = 0; w < kRowThreads / 64; ++w) top = fmaxf(top, tops[w]);
+  __syncthreads();
+  return !any && top > -INFINITY;
+}
+
+__device__ void make_powers(RowLds& l) {
+  for (int b = threadIdx.x; b < kBatchBins; b += kRowThreads) l.powers[b] = kMassOne * exp_below(-(double)b / 64);
+  __syncthreads();
+}
+
+// A logit's bin, ascending as the logit falls (the last takes the rest, whose weights round to
+// nothing), and its weight as an integer: the bin's power times e^-f, f < 1 / 64.
+struct Weighed {
+  int bin;
+  uint64_t weight;
+};
+__device__ __forceinline__ Weighed weigh(const RowLds& l, float v, float top, double sharpness) {
+  const double t = v == top ? 0.0 : ((double)top - (double)v) * (64.0 * sharpness);
+  if (!(t < (double)(kBatchBins - 1))) return Weighed{kBatchBins - 1, 0};
+  const int b = (int)t;
+  const float f = (float)(t - (double)b) * (1.f / 64);
+  const float g = f * (1.f - f * (0.5f - f * (1.f / 6 - f * (1.f / 24 - f * (1.f / 120)))));  // 1 - e^-f
+  const double w = l.powers[b];
+  return Weighed{b, (uint64_t)(w - w * (double)g + 0.5)};
+}
+
+// Sort list[0, n) in descending order.  Up to one entry a thread: by counting the larger ones (no two
+// are equal), the threads of an entry sharing the count; else by a bitonic network.
+__device__ void sort_list(RowLds& l, int n) {
+  if (n <= kRowThreads) {
+    int log2g = 0;
+    while (log2g < 4 && n <= (kRowThreads >> (log2g + 1))) ++log2g;
+    const int g = 1 << log2g, item = threadIdx.x >> log2g, part = threadIdx.x & (g - 1);
+    const uint64_t mine = item < n ? l.list[item] : 0;
+    int rank = 0;
+#pragma unroll 8
+    for (int i = part; i < n; i += g) rank += l.list[i] > mine ? 1 : 0;
+    for (int o = 1; o < g; o <<= 1) rank += __shfl_xor(rank, o, 64);
+    __syncthreads();
+    if (item < n && part == 0) l.list[rank] = mine;
+    __syncthreads();
+    return;
+  }
+  int size = 2 * kRowThreads;
   while (size < n) size <<= 1;
-  for (int i = threadIdx.x; i < size; i += kFinishThreads)
+  for (int i = threadIdx.x; i < size; i += kRowThreads)
     if (i >= n) l.list[i] = 0;
   __syncthreads();
   for (int k = 2; k <= size; k <<= 1)
     for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int i = threadIdx.x; i < size / 2; i += kFinishThreads) {
-        const int a = (i / j) * 2 * j + i % j, b = a + j;
+      for (int i = threadIdx.x; i < size / 2; i += kRowThreads) {
+        const int a = ((i & ~(j - 1)) << 1) | (i & (j - 1)), b = a + j;
         const bool descending = (a & k) == 0;
         const uint64_t x = l.list[a], y = l.list[b];
         if (descending ? x < y : x > y) {
@@ -184,113 +253,333 @@ __device__ void sort_list(FinishLds& l, int n) {
     }
 }
 
-// Append where `take`, by every lane of a wavefront; entries past the list's end are counted only.
-__device__ __forceinline__ void append(FinishLds& l, bool take, uint64_t e) {
-  const uint64_t m = __ballot(take);
-  if (!m) return;
+// A chunk's logits where `take` to a list of `count` entries (those past its end are counted only), by
+// every lane of a wavefront.
+template <typename Counter>
+__device__ __forceinline__ void append(uint64_t* list, Counter* count, const bool (&take)[4], const float (&v)[4],
+                                       int chunk) {
   const int lane = threadIdx.x & 63;
+  const uint64_t below = (1ull << lane) - 1ull;
+  int all = 0, ahead = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint64_t m = __ballot(take[e]);
+    all += __popcll(m);
+    ahead += __popcll(m & below);
+  }
+  if (!all) return;
   int at = 0;
-  if (lane == 0) at = atomicAdd(&l.count, __popcll(m));
-  at = __builtin_amdgcn_readfirstlane(at) + __popcll(m & ((1ull << lane) - 1ull));
-  if (take && at < kListMax) l.list[at] = e;
-}
-
-// Weights of list[0, n) and their running sums in list order, kListMax / kFinishThreads entries a
-// thread: before[k] is the sum ahead of entry threadIdx.x * 4 + k.
-constexpr int kOwn = kListMax / kFinishThreads;
-__device__ double list_sums(FinishLds& l, int n, float top, double t, bool by_index, double (&w)[kOwn],
-                            double (&before)[kOwn]) {
-  double sum = 0.0;
+  if (lane == 0) at = atomicAdd(count, all);
+  at = __builtin_amdgcn_readfirstlane(at) + ahead;
 #pragma unroll
-  for (int k = 0; k < kOwn; ++k) {
-    const int i = threadIdx.x * kOwn + k;
-    w[k] = 0.0;
-    if (i < n) {
-      const uint64_t e = l.list[i];
-      w[k] = weight(of_order((uint32_t)(by_index ? e : e >> 32)), top, t);
+  for (int e = 0; e < 4; ++e)
+    if (take[e]) {
+      if (at < kBatchList) list[at] = entry_of(v[e], chunk * kBatchChunk + 4 * lane + e);
+      ++at;
     }
-    before[k] = sum;
-    sum += w[k];
-  }
-  double total;
-  const double mine = block_scan(sum, l, &total) - sum;
-#pragma unroll
-  for (int k = 0; k < kOwn; ++k) before[k] += mine;
-  return total;
 }
 
-// The token of the list of `n` candidates, which holds all that top-k or min-p keep.  `row_mass`:
-// the row's total weight, for rows without top-k.
-__device__ int draw_from_list(FinishLds& l, int n, const RowParams& p, float top, double row_mass) {
-  sort_list(l, n);
-  if (p.top_k) n = min(n, p.top_k);
-  double w[kOwn], before[kOwn];
-  double total = list_sums(l, n, top, p.temperature, false, w, before);
-  const double reach = p.top_p * (p.top_k ? total : row_mass);
-  int kept = 0;
+// The chunks [first, last) of a row by the block's wavefronts, four of each in flight: f(chunk, logits)
+// for those that `wanted` names.
+template <typename Wanted, typename F>
+__device__ __forceinline__ void each_chunk(const float* row, int n, int first, int last, Wanted&& wanted, F&& f) {
+  constexpr int kStep = kRowThreads / 64, kAhead = 4;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // 64 of this wavefront's chunks at a time
+  for (int c0 = first + wave; c0 < last; c0 += kStep * 64) {
+    const int mine = c0 + kStep * lane;
+    uint64_t todo = __ballot(mine < last && wanted(min(mine, last - 1)));
+    while (todo) {
+      float v[kAhead][4];
+      int c[kAhead];
 #pragma unroll
-  for (int k = 0; k < kOwn; ++k) {
-    const int i = threadIdx.x * kOwn + k;
-    // the filters keep a run from the first rank on
-    kept += i < n && (p.top_p >= 1.0 || before[k] < reach || i == 0) && w[k] >= p.min_p ? 1 : 0;
-  }
-  int all;
-  block_scan(kept, l, &all);
-  n = all;
-  for (int i = threadIdx.x; i < n; i += kFinishThreads) l.list[i] = l.list[i] << 32 | l.list[i] >> 32;
-  __syncthreads();
-  sort_list(l, n);
-  total = list_sums(l, n, top, p.temperature, true, w, before);
-  if (threadIdx.x == 0) l.count = INT_MAX;
-  __syncthreads();
-  const double at = p.random * total;
+      for (int k = 0; k < kAhead; ++k) {
+        c[k] = todo ? c0 + kStep * __builtin_ctzll(todo) : -1;
+        todo &= todo - 1;
+        if (c[k] >= 0) load_chunk(row, n, c[k], lane, v[k]);
+      }
 #pragma unroll
-  for (int k = 0; k < kOwn; ++k) {
-    const int i = threadIdx.x * kOwn + k;
-    if (i < n && before[k] + w[k] > at) {
-      atomicMin(&l.count, i);
-      break;
+      for (int k = 0; k < kAhead; ++k)
+        if (c[k] >= 0) f(c[k], v[k]);
     }
   }
+}
+
+__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// A min-p as an integer weight: weights of at least it are kept.
+__device__ __forceinline__ uint64_t least_weight(const RowParams& p) { return (uint64_t)ceil(p.min_p * kMassOne); }
+
+// ------------------------------------------------------------------ rows without top-k
+
+constexpr int kRowShares = 8;  // workgroups on a row
+
+__device__ __forceinline__ void share_of(int chunks, int& first, int& last) {
+  const int per = (chunks + kRowShares - 1) / kRowShares;
+  first = blockIdx.x * per;
+  last = min(chunks, first + per);
+}
+
+__global__ void __launch_bounds__(kRowThreads) sample_mass_kernel(SampleRows s) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  RowLds& l = *reinterpret_cast<RowLds*>(raw);
+  const int row = blockIdx.y;
+  const RowParams p = row_params(s, row);
+  const int chunks = (s.n + kBatchChunk - 1) / kBatchChunk;
+  if (p.bad || (p.top_k ? p.top_k <= chunks : p.top_p >= 1.0)) return;
+  float top;
+  if (!row_top(l, s, row, false, top)) return;
+  for (int b = threadIdx.x; b < kBatchBins; b += kRowThreads) l.bins[b] = 0;
+  make_powers(l);
+  int first, last;
+  share_of(chunks, first, last);
+  each_chunk(s.logits + (int64_t)row * s.n, s.n, first, last, [&](int c) { return l.chunk_max[c] > -INFINITY; },
+             [&](int, const float (&v)[4]) {
+#pragma unroll
+               for (int e = 0; e < 4; ++e) {
+                 const Weighed w = weigh(l, v[e], top, p.sharpness);
+                 const uint64_t count = p.top_k ? (v[e] > -INFINITY ? 1 : 0) : w.weight;
+                 if (count) atomicAdd((unsigned long long*)&l.bins[w.bin], (unsigned long long)count);
+               }
+             });
   __syncthreads();
-  const int i = l.count < n ? l.count : n - 1;
-  return (int)(0xFFFFFFFFu - (uint32_t)(l.list[i] >> 32));
+  for (int b = threadIdx.x; b < kBatchBins; b += kRowThreads)
+    if (l.bins[b])
+      atomicAdd((unsigned long long*)&s.bins[(int64_t)row * kBatchBins + b], (unsigned long long)l.bins[b]);
 }
 
-// 64-bit fixed-point weights of whole rows.
-__device__ __forceinline__ uint64_t fixed_weight(float v, float top, double t) {
-  return (uint64_t)(weight(v, top, t) * kMassOne + 0.5);
+// The bin that the row's cut falls into and how much lies above it, from its bins: counts with top-k,
+// weights without.
+__device__ void cut_bin(RowLds& l, const SampleRows& s, int row, const RowParams& p, int& bin, uint64_t& above,
+                          uint64_t& need) {
+  constexpr int kPer = kBatchBins / kRowThreads;
+  const uint64_t* bins = s.bins + (int64_t)row * kBatchBins + threadIdx.x * kPer;
+  uint64_t own[kPer], sum = 0, total;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    own[k] = bins[k];
+    sum += own[k];
+  }
+  const uint64_t incl = block_scan(sum, l, &total);
+  need = p.top_k ? (uint64_t)p.top_k : (uint64_t)ceil(p.top_p * (double)total);
+  need = need > total ? total : need > 0 ? need : 1;
+  if (incl >= need && incl - sum < need) {
+    uint64_t run = incl - sum;
+    int k = 0;
+    while (run + own[k] < need) run += own[k++];
+    l.result[0] = (uint64_t)(threadIdx.x * kPer + k);
+    l.result[1] = run;
+  }
+  __syncthreads();
+  bin = (int)l.result[0];
+  above = l.result[1];
+  __syncthreads();
 }
 
-// Bin of a logit: ascends as the logit falls.
-__device__ __forceinline__ int bin_of(float v, float top, float scale) {
-  const float b = v == top ? 0.f : (top - v) * scale;
-  return b < (float)(kBins - 1) ? (int)b : kBins - 1;
+__global__ void __launch_bounds__(kRowThreads) sample_cut_kernel(SampleRows s) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  RowLds& l = *reinterpret_cast<RowLds*>(raw);
+  const int row = blockIdx.y, lane = threadIdx.x & 63;
+  const RowParams p = row_params(s, row);
+  const int chunks = (s.n + kBatchChunk - 1) / kBatchChunk;
+  if (p.bad || (p.top_k && p.top_k <= chunks)) return;
+  float top;
+  if (!row_top(l, s, row, false, top)) return;
+  make_powers(l);
+  int bin = kBatchBins;  // without top-p all weights lie above the cut
+  uint64_t above, need;
+  if (p.top_k || p.top_p < 1.0) cut_bin(l, s, row, p, bin, above, need);
+  // (top-k keeps by rank first: all down to the cut's bin are listed, and no weights summed)
+  const uint64_t least = p.top_k ? 0 : least_weight(p);
+  int first, last;
+  share_of(chunks, first, last);
+  uint64_t* mass = s.chunk_mass + (int64_t)row * chunks;
+  // chunks that hold nothing above the cut or in its bin, or nothing that min-p keeps
+  auto wanted = [&](int c) {
+    const Weighed w = weigh(l, l.chunk_max[c], top, p.sharpness);
+    return l.chunk_max[c] > -INFINITY && w.bin <= bin && w.weight >= least;
+  };
+  for (int c = first + threadIdx.x; c < last; c += kRowThreads)
+    if (!p.top_k && !wanted(c)) mass[c] = 0;
+  each_chunk(s.logits + (int64_t)row * s.n, s.n, first, last, wanted, [&](int c, const float (&v)[4]) {
+    uint64_t held = 0;
+    bool take[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const Weighed w = weigh(l, v[e], top, p.sharpness);
+      take[e] = (p.top_k ? w.bin <= bin : w.bin == bin) && v[e] > -INFINITY;
+      if (w.bin < bin && w.weight >= least) held += w.weight;
+    }
+    append(s.list + (int64_t)row * kBatchList, s.listed + row, take, v, c);
+    if (p.top_k) return;
+    held = wave_sum_u64(held);
+    if (lane == 0) mass[c] = held;
+  });
+}
+
+// ------------------------------------------------------------------ the token
+
+// The token of a list of which at most 64 ranks can be kept, by the first wavefront: ranks by
+// counting, then a rank a lane.
+constexpr int kWaveList = 256;
+__device__ void draw_by_wave(RowLds& l, int n, const RowParams& p, float top, int* token) {
+  const int lane = threadIdx.x & 63;
+  const int ranks = min(n, p.top_k);
+  uint64_t mine[kWaveList / 64];
+  int rank[kWaveList / 64];
+#pragma unroll
+  for (int j = 0; j < kWaveList / 64; ++j) {
+    mine[j] = lane + 64 * j < n ? l.list[lane + 64 * j] : 0;
+    rank[j] = 0;
+  }
+  for (int i = 0; i < n; ++i) {
+    const uint64_t e = l.list[i];
+#pragma unroll
+    for (int j = 0; j < kWaveList / 64; ++j)
+      if (64 * j < n) rank[j] += e > mine[j] ? 1 : 0;
+  }
+  uint64_t* sorted = l.bins;
+#pragma unroll
+  for (int j = 0; j < kWaveList / 64; ++j)
+    if (lane + 64 * j < n && rank[j] < ranks) sorted[rank[j]] = mine[j];
+  __builtin_amdgcn_wave_barrier();
+  const uint64_t e = sorted[min(lane, ranks - 1)];
+  __builtin_amdgcn_wave_barrier();
+  double w = lane < ranks ? weight(entry_logit(e), top, p.sharpness) : 0.0;
+  double upto = w;
+  for (int o = 1; o < 64; o <<= 1) {
+    const double u = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += u;
+  }
+  const double all = __shfl(upto, 63, 64);
+  // the filters keep a run from the first rank on
+  const bool keep = lane < ranks && (lane == 0 || p.top_p >= 1.0 || upto - w < p.top_p * all) && w >= p.min_p;
+  const int kept = __popcll(__ballot(keep));
+  if (lane >= kept) w = 0.0;
+  const int index = lane < kept ? entry_index(e) : INT_MAX;
+  // the sum up to each one's index
+  double run = 0.0, total = 0.0;
+  for (int i = 0; i < kept; ++i) {
+    const double wi = __shfl(w, i, 64);
+    total += wi;
+    run += __shfl(index, i, 64) <= index ? wi : 0.0;
+  }
+  const bool past = lane < kept && run > p.random * total;
+  const int found = wave_min(past ? index : INT_MAX), last = wave_max_i(lane < kept ? index : -1);
+  if (lane == 0) *token = found < INT_MAX ? found : last;
+}
+
+// The token by the chunks' kept weights and the lowest entry kept.
+__device__ int draw_from_chunks(RowLds& l, const float* row, int n, const RowParams& p, float top, uint64_t cut) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int chunks = (n + kBatchChunk - 1) / kBatchChunk;
+  const uint64_t least = least_weight(p);
+  uint64_t total;
+  const uint64_t mine = tid < chunks ? l.mass[tid] : 0;
+  const uint64_t upto = block_scan(mine, l, &total);
+  const double at = p.random * (double)total;
+  if (tid == 0) {
+    l.result[0] = ~0ull;
+    l.count = INT_MAX;
+  }
+  __syncthreads();
+  // the chunk at which the sum passes the mark, then the logit
+  if (tid < chunks && (double)upto > at && !((double)(upto - mine) > at)) {
+    l.result[0] = (uint64_t)tid;
+    l.result[1] = upto - mine;
+  }
+  __syncthreads();
+  const int chunk = (int)l.result[0];
+  if (chunk < 0) return -1;
+  if (wave == 0) {
+    float v[4];
+    load_chunk(row, n, chunk, lane, v);
+    uint64_t own[4], sum = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      own[e] = 0;
+      if (v[e] > -INFINITY && entry_of(v[e], chunk * kBatchChunk + 4 * lane + e) >= cut) {
+        const uint64_t w = weigh(l, v[e], top, p.sharpness).weight;
+        own[e] = w >= least ? w : 0;
+      }
+      sum += own[e];
+    }
+    uint64_t incl = sum;
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint64_t u = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += u;
+    }
+    uint64_t run = l.result[1] + incl - sum;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      run += own[e];
+      if (own[e] && (double)run > at) atomicMin(&l.count, chunk * kBatchChunk + 4 * lane + e);
+    }
+  }
+  __syncthreads();
+  return l.count;
+}
+
+// What of a sorted list is kept, into the chunks' weights: the first `ranks` whose weights ahead of
+// them do not reach `need`, of at least min-p.  Returns the lowest entry kept by rank and need.
+constexpr int kOwn = kBatchList / kRowThreads;
+__device__ uint64_t keep_from_list(RowLds& l, int n, const RowParams& p, float top, uint64_t above, uint64_t need) {
+  const int tid = threadIdx.x;
+  const uint64_t least = least_weight(p);
+  uint64_t own = 0, values[kOwn], total;
+#pragma unroll
+  for (int k = 0; k < kOwn; ++k) {
+    const int i = tid * kOwn + k;
+    values[k] = i < n ? weigh(l, entry_logit(l.list[i]), top, p.sharpness).weight : 0;
+    own += values[k];
+  }
+  uint64_t run = above + block_scan(own, l, &total) - own;
+  if (tid == 0) l.result[2] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kOwn; ++k) {
+    const int i = tid * kOwn + k;
+    if (i < n && run < need) {
+      if (values[k] >= least)
+        atomicAdd((unsigned long long*)&l.mass[entry_index(l.list[i]) / kBatchChunk], (unsigned long long)values[k]);
+      // the last of them
+      if (run + values[k] >= need || i == n - 1) l.result[2] = l.list[i];
+    }
+    run += values[k];
+  }
+  __syncthreads();
+  const uint64_t cut = l.result[2];
+  __syncthreads();
+  return cut;
 }
 
 // The highest entry e such that the entries >= e reach `need` (their number, or their mass where
 // `by_mass`), among the entries <= limit of the row.  0 where all of them do not.  `reached`: what the
 // entries above e hold.
-__device__ uint64_t row_cut(FinishLds& l, const float* row, int n, float top, double t, bool by_mass,
+__device__ uint64_t row_cut(RowLds& l, const float* row, int n, float top, double t, bool by_mass,
                             uint64_t need, uint64_t floor_entry) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int chunks = (n + kBatchChunk - 1) / kBatchChunk;
-  const float scale = (float)(64.0 / t);
-  uint64_t* bins = reinterpret_cast<uint64_t*>(l.weights);
-  for (int i = tid; i < kBins; i += kFinishThreads) bins[i] = 0;
+  uint64_t* bins = l.bins;
+  for (int i = tid; i < kBatchBins; i += kRowThreads) bins[i] = 0;
   __syncthreads();
-  auto value = [&](float v) { return by_mass ? fixed_weight(v, top, t) : 1ull; };
-  for (int c = wave; c < chunks; c += kFinishThreads / 64) {
+  auto value = [&](const Weighed& w) -> uint64_t { return by_mass ? w.weight : 1; };
+  for (int c = wave; c < chunks; c += kRowThreads / 64) {
     float v[4];
     load_chunk(row, n, c, lane, v);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (v[e] > -INFINITY && entry_of(v[e], c * kBatchChunk + 4 * lane + e) >= floor_entry)
-        atomicAdd((unsigned long long*)&bins[bin_of(v[e], top, scale)], (unsigned long long)value(v[e]));
+      if (v[e] > -INFINITY && entry_of(v[e], c * kBatchChunk + 4 * lane + e) >= floor_entry) {
+        const Weighed w = weigh(l, v[e], top, t);
+        atomicAdd((unsigned long long*)&bins[w.bin], (unsigned long long)value(w));
+      }
   }
   __syncthreads();
   // the bin that reaches it
-  constexpr int kPer = kBins / kFinishThreads;
+  constexpr int kPer = kBatchBins / kRowThreads;
   uint64_t sum = 0;
   for (int k = 0; k < kPer; ++k) sum += bins[tid * kPer + k];
   uint64_t total;
@@ -308,25 +597,26 @@ __device__ uint64_t row_cut(FinishLds& l, const float* row, int n, float top, do
   const int bin = (int)l.result[0];
   uint64_t above = l.result[1];
   __syncthreads();
-  for (int c = wave; c < chunks; c += kFinishThreads / 64) {
+  for (int c = wave; c < chunks; c += kRowThreads / 64) {
     float v[4];
     load_chunk(row, n, c, lane, v);
+    bool take[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint64_t x = entry_of(v[e], c * kBatchChunk + 4 * lane + e);
-      append(l, v[e] > -INFINITY && x >= floor_entry && bin_of(v[e], top, scale) == bin, x);
-    }
+    for (int e = 0; e < 4; ++e)
+      take[e] = v[e] > -INFINITY && entry_of(v[e], c * kBatchChunk + 4 * lane + e) >= floor_entry &&
+                weigh(l, v[e], top, t).bin == bin;
+    append(l.list, &l.count, take, v, c);
   }
   __syncthreads();
   const int listed = l.count;
   __syncthreads();
-  if (listed <= kListMax) {
+  if (listed <= kBatchList) {
     sort_list(l, listed);
     uint64_t own = 0, values[kOwn];
 #pragma unroll
     for (int k = 0; k < kOwn; ++k) {
       const int i = tid * kOwn + k;
-      values[k] = i < listed ? value(entry_logit(l.list[i])) : 0;
+      values[k] = i < listed ? value(weigh(l, entry_logit(l.list[i]), top, t)) : 0;
       own += values[k];
     }
     uint64_t run = above + block_scan(own, l, &total) - own;
@@ -345,17 +635,17 @@ __device__ uint64_t row_cut(FinishLds& l, const float* row, int n, float top, do
   // too many for the list: eight bits of the entries at a time
   uint64_t prefix = 0;
   for (int shift = 56; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kFinishThreads) bins[i] = 0;
+    for (int i = tid; i < 256; i += kRowThreads) bins[i] = 0;
     __syncthreads();
-    for (int c = wave; c < chunks; c += kFinishThreads / 64) {
+    for (int c = wave; c < chunks; c += kRowThreads / 64) {
       float v[4];
       load_chunk(row, n, c, lane, v);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint64_t x = entry_of(v[e], c * kBatchChunk + 4 * lane + e);
-        if (v[e] > -INFINITY && x >= floor_entry && bin_of(v[e], top, scale) == bin &&
-            (shift == 56 || x >> (shift + 8) == prefix))
-          atomicAdd((unsigned long long*)&bins[(x >> shift) & 255], (unsigned long long)value(v[e]));
+        const Weighed w = weigh(l, v[e], top, t);
+        if (v[e] > -INFINITY && x >= floor_entry && w.bin == bin && (shift == 56 || x >> (shift + 8) == prefix))
+          atomicAdd((unsigned long long*)&bins[(x >> shift) & 255], (unsigned long long)value(w));
       }
     }
     __syncthreads();
@@ -374,203 +664,181 @@ __device__ uint64_t row_cut(FinishLds& l, const float* row, int n, float top, do
 }
 
 // The token of a row by passes over all of it.
-__device__ int draw_from_row(FinishLds& l, const float* row, int n, const RowParams& p, float top) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int chunks = (n + kBatchChunk - 1) / kBatchChunk;
-  const double t = p.temperature;
-  uint64_t cut = 0;
-  if (p.top_k) cut = row_cut(l, row, n, top, t, false, (uint64_t)p.top_k, 0);
-  uint64_t* mass = reinterpret_cast<uint64_t*>(l.chunk_mass);
-  uint64_t total;
-  auto chunk_masses = [&] {
-    for (int c = wave; c < chunks; c += kFinishThreads / 64) {
-      float v[4];
-      load_chunk(row, n, c, lane, v);
-      uint64_t sum = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (v[e] > -INFINITY && entry_of(v[e], c * kBatchChunk + 4 * lane + e) >= cut) {
-          const double w = weight(v[e], top, t);
-          sum += w >= p.min_p ? (uint64_t)(w * kMassOne + 0.5) : 0;
-        }
-      for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-      if (lane == 0) mass[c] = sum;
-    }
-    __syncthreads();
-  };
-  if (p.top_p < 1.0) {
-    // what top-k kept, without min-p
+__device__ int draw_from_row(RowLds& l, const float* row, int n, const RowParams& p, float top) {
+  const int lane = threadIdx.x & 63, chunks = (n + kBatchChunk - 1) / kBatchChunk;
+  const double t = p.sharpness;
+  uint64_t cut = 0, total;
+  auto kept_of = [&](const float (&v)[4], int c, uint64_t least) {
     uint64_t sum = 0;
-    for (int c = wave; c < chunks; c += kFinishThreads / 64) {
-      float v[4];
-      load_chunk(row, n, c, lane, v);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (v[e] > -INFINITY && entry_of(v[e], c * kBatchChunk + 4 * lane + e) >= cut)
-          sum += fixed_weight(v[e], top, t);
-    }
+    for (int e = 0; e < 4; ++e)
+      if (v[e] > -INFINITY && entry_of(v[e], c * kBatchChunk + 4 * lane + e) >= cut) {
+        const uint64_t w = weigh(l, v[e], top, t).weight;
+        sum += w >= least ? w : 0;
+      }
+    return sum;
+  };
+  auto all = [](int) { return true; };
+  if (p.top_k) cut = row_cut(l, row, n, top, t, false, (uint64_t)p.top_k, 0);
+  if (p.top_p < 1.0) {
+    // of what top-k kept
+    uint64_t sum = 0;
+    each_chunk(row, n, 0, chunks, all, [&](int c, const float (&v)[4]) { sum += kept_of(v, c, 0); });
     block_scan(sum, l, &total);
-    const double reach = p.top_p * (double)total;
-    uint64_t need = (uint64_t)reach;
-    need += (double)need < reach ? 1 : 0;
+    const uint64_t need = (uint64_t)ceil(p.top_p * (double)total);
     cut = row_cut(l, row, n, top, t, true, need > 0 ? need : 1, cut);
   }
-  chunk_masses();
-  const uint64_t mine = tid < chunks ? mass[tid] : 0;
-  const uint64_t upto = block_scan(mine, l, &total);
-  const double at = p.random * (double)total;
-  if (tid == 0) l.result[0] = ~0ull;
+  const uint64_t least = least_weight(p);
+  each_chunk(row, n, 0, chunks, all, [&](int c, const float (&v)[4]) {
+    const uint64_t sum = wave_sum_u64(kept_of(v, c, least));
+    if (lane == 0) l.mass[c] = sum;
+  });
   __syncthreads();
-  // the chunk at which the sum passes the mark, then the logit
-  if (tid < chunks && (double)upto > at && !((double)(upto - mine) > at)) {
-    l.result[0] = (uint64_t)tid;
-    l.result[1] = upto - mine;
-  }
-  __syncthreads();
-  const int chunk = (int)l.result[0];
-  if (chunk < 0) return -1;
-  uint64_t run = l.result[1];
-  if (tid == 0) l.count = INT_MAX;
-  __syncthreads();
-  if (wave == 0) {
-    float v[4];
-    load_chunk(row, n, chunk, lane, v);
-    uint64_t own[4], sum = 0;
+  return draw_from_chunks(l, row, n, p, top, cut);
+}
+
+// Rows with top-k: the candidates to the list; their number (beyond the list's end: too many).
+__device__ int list_candidates(RowLds& l, const float* row, int n, const RowParams& p, float top) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int chunks = (n + kBatchChunk - 1) / kBatchChunk;
+  float bound = -INFINITY;
+  if (p.top_k <= kMoeMaxTopK) {
+    if (wave == 0) {
+      constexpr int kPer = kBatchMaxChunks / 64;
+      float v[kPer];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      own[e] = 0;
-      if (v[e] > -INFINITY && entry_of(v[e], chunk * kBatchChunk + 4 * lane + e) >= cut) {
-        const double w = weight(v[e], top, t);
-        own[e] = w >= p.min_p ? (uint64_t)(w * kMassOne + 0.5) : 0;
+      for (int j = 0; j < kPer; ++j) v[j] = lane + 64 * j < chunks ? l.chunk_max[lane + 64 * j] : -INFINITY;
+      int at;
+      float kth;
+      wave_select<kPer>(v, p.top_k, lane, reinterpret_cast<int64_t*>(l.bins), at, kth);
+      // (fewer chunks with a logit: every logit is a candidate)
+      if (lane == p.top_k - 1) l.result[0] = __builtin_bit_cast(uint32_t, at >= 0 ? kth : -INFINITY);
+    }
+    __syncthreads();
+    bound = __builtin_bit_cast(float, (uint32_t)l.result[0]);
+  } else {
+    // the highest chunk maxima by their keys' upper bits, eight at a time: the bound is at most the
+    // k-th's, and close to it
+    uint32_t prefix = 0;
+    int above = 0;
+    uint32_t* hist = reinterpret_cast<uint32_t*>(l.bins);
+    const uint32_t key = tid < chunks ? order_of(l.chunk_max[tid]) : 0;
+    for (int shift = 24; shift >= 8; shift -= 8) {
+      for (int i = tid; i < 256; i += kRowThreads) hist[i] = 0;
+      __syncthreads();
+      if (tid < chunks && (shift == 24 || key >> (shift + 8) == prefix)) atomicAdd(&hist[(key >> shift) & 255], 1u);
+      __syncthreads();
+      if (tid < 64) {
+        // four bins a lane, from the top
+        int c[4], sum = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum += c[j] = (int)hist[255 - 4 * lane - j];
+        int incl = sum;
+        for (int o = 1; o < 64; o <<= 1) {
+          const int u = __shfl_up(incl, o, 64);
+          if (lane >= o) incl += u;
+        }
+        int run = above + incl - sum;
+        if (run < p.top_k && run + sum >= p.top_k) {
+          int j = 0;
+          while (run + c[j] < p.top_k) run += c[j++];
+          l.result[0] = (uint64_t)(255 - 4 * lane - j);
+          l.result[1] = (uint64_t)run;
+        }
       }
-      sum += own[e];
+      __syncthreads();
+      prefix = prefix << 8 | (uint32_t)l.result[0];
+      above = (int)l.result[1];
+      __syncthreads();
     }
-    uint64_t incl = sum;
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint64_t u = __shfl_up(incl, o, 64);
-      if (lane >= o) incl += u;
-    }
-    run += incl - sum;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      run += own[e];
-      if (own[e] && (double)run > at) atomicMin(&l.count, chunk * kBatchChunk + 4 * lane + e);
-    }
+    bound = of_order(prefix << 8);
+    if (!(bound == bound)) bound = -INFINITY;  // the keys below -inf's
   }
+  if (tid == 0) l.count = 0;
+  __syncthreads();
+  each_chunk(row, n, 0, chunks, [&](int c) { return l.chunk_max[c] >= bound && l.chunk_max[c] > -INFINITY; },
+             [&](int c, const float (&v)[4]) {
+               bool take[4];
+#pragma unroll
+               for (int e = 0; e < 4; ++e) take[e] = v[e] >= bound && v[e] > -INFINITY;
+               append(l.list, &l.count, take, v, c);
+             });
   __syncthreads();
   return l.count;
 }
 
-__global__ void __launch_bounds__(kFinishThreads) sample_finish_kernel(SampleRows s) {
+__global__ void __launch_bounds__(kRowThreads) sample_finish_kernel(SampleRows s) {
   extern __shared__ __align__(16) uint8_t raw[];
-  FinishLds& l = *reinterpret_cast<FinishLds*>(raw);
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  RowLds& l = *reinterpret_cast<RowLds*>(raw);
+  const int row = blockIdx.x, tid = threadIdx.x;
   const int chunks = (s.n + kBatchChunk - 1) / kBatchChunk;
   const float* logits = s.logits + (int64_t)row * s.n;
   const RowParams p = row_params(s, row);
-  const float* cmax = s.chunk_max + (int64_t)row * chunks;
-  // the row's maximum; a chunk with a NaN carries it
-  float m = tid < chunks ? cmax[tid] : -INFINITY;
-  const bool nan = m != m;
-  if (tid < chunks) l.chunk_max[tid] = m;
-  if (tid == 0) l.count = 0;
-  float top = wave_max(nan ? -INFINITY : m);
-  float* tops = reinterpret_cast<float*>(l.wave);
-  if (lane == 0) tops[wave] = top;
-  const int bad = __syncthreads_or(nan || p.bad);
-  for (int w = 0; w < kFinishThreads / 64; ++w) top = fmaxf(top, tops[w]);
-  __syncthreads();
-  if (bad || !(top > -INFINITY)) {
+  float top;
+  if (!row_top(l, s, row, p.bad, top)) {
     if (tid == 0) s.tokens[row] = -1;
     return;
   }
-  const double t = p.temperature;
-  double row_mass = 0.0;
-  if (p.mass) {
-    const double mine = tid < chunks && m > -INFINITY
-                            ? s.chunk_mass[(int64_t)row * chunks + tid] * weight(m, top, t) : 0.0;
-    const double upto = block_scan(mine, l, &row_mass);
-    if (p.top_p >= 1.0) {
-      // no filter: the chunk at which the sum passes the mark, then the logit
-      const double at = p.random * row_mass;
-      if (tid == 0) l.count = INT_MAX;
+  int token;
+  if (p.top_k) {
+    int n;
+    if (p.top_k <= chunks) {
+      n = list_candidates(l, logits, s.n, p, top);
+    } else {
+      n = s.listed[row];
+      for (int i = tid; i < min(n, kBatchList); i += kRowThreads) l.list[i] = s.list[(int64_t)row * kBatchList + i];
       __syncthreads();
-      if (mine > 0.0 && upto > at) atomicMin(&l.count, tid);
-      __syncthreads();
-      int chunk = l.count;
-      __syncthreads();
-      if (chunk == INT_MAX) {  // the mark lies past the last sum's rounding: the last chunk with mass
-        if (tid == 0) l.count = -1;
-        __syncthreads();
-        if (mine > 0.0) atomicMax(&l.count, tid);
-        __syncthreads();
-        chunk = l.count;
-        __syncthreads();
-      }
-      if (tid == chunk) l.weights[0] = upto - mine;
-      __syncthreads();
-      if (wave == 0) {
-        float v[4];
-        load_chunk(logits, s.n, chunk, lane, v);
-        double w[4], sum = 0.0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          w[e] = v[e] > -INFINITY ? weight(v[e], top, t) : 0.0;
-          sum += w[e];
-        }
-        double incl = sum;
-        for (int o = 1; o < 64; o <<= 1) {
-          const double u = __shfl_up(incl, o, 64);
-          if (lane >= o) incl += u;
-        }
-        double run = l.weights[0] + (incl - sum);
-        int found = INT_MAX, last = -1;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          run += w[e];
-          const int i = chunk * kBatchChunk + 4 * lane + e;
-          if (w[e] > 0.0) {
-            if (run > at) found = min(found, i);
-            last = i;
-          }
-        }
-        for (int o = 32; o > 0; o >>= 1) {
-          found = min(found, __shfl_xor(found, o, 64));
-          last = max(last, __shfl_xor(last, o, 64));
-        }
-        if (lane == 0) s.tokens[row] = found == INT_MAX ? last : found;
-      }
+    }
+    if (p.top_k <= kMoeMaxTopK && n <= kWaveList) {
+      if (tid < 64) draw_by_wave(l, n, p, top, s.tokens + row);
       return;
     }
-  }
-  bool list = p.top_k ? p.top_k <= chunks : p.min_p > 0.0;
-  if (list) {
-    // the chunks that hold candidates, and the candidates
-    uint32_t bound = 0;
-    if (p.top_k) {
-      if (tid < chunks) l.list[tid] = (uint64_t)order_of(m) << 32 | (uint32_t)tid;
-      __syncthreads();
-      sort_list(l, chunks);
-      bound = (uint32_t)(l.list[p.top_k - 1] >> 32);
-      __syncthreads();
-    }
-    for (int c = wave; c < chunks; c += kFinishThreads / 64) {
-      const float cm = l.chunk_max[c];
-      if (!(cm > -INFINITY) || (p.top_k ? order_of(cm) < bound : weight(cm, top, t) < p.min_p)) continue;
-      float v[4];
-      load_chunk(logits, s.n, c, lane, v);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        append(l, v[e] > -INFINITY && (p.top_k ? order_of(v[e]) >= bound : weight(v[e], top, t) >= p.min_p),
-               entry_of(v[e], c * kBatchChunk + 4 * lane + e));
-    }
     __syncthreads();
-    list = l.count <= kListMax;
+    make_powers(l);
+    if (n <= kBatchList) {
+      sort_list(l, n);
+      const int ranks = min(n, p.top_k);
+      uint64_t total, sum = 0;
+      for (int i = tid; i < ranks; i += kRowThreads) sum += weigh(l, entry_logit(l.list[i]), top, p.sharpness).weight;
+      block_scan(sum, l, &total);
+      for (int c = tid; c < chunks; c += kRowThreads) l.mass[c] = 0;
+      __syncthreads();
+      const uint64_t need = p.top_p < 1.0 ? (uint64_t)ceil(p.top_p * (double)total) : ~0ull;
+      const uint64_t cut = keep_from_list(l, ranks, p, top, 0, need > 0 ? need : 1);
+      token = draw_from_chunks(l, logits, s.n, p, top, cut);
+    } else {
+      token = draw_from_row(l, logits, s.n, p, top);
+    }
+  } else {
+    make_powers(l);
+    int bin;
+    uint64_t above = 0, need = 0;
+    if (p.top_p < 1.0) cut_bin(l, s, row, p, bin, above, need);
+    const int n = p.top_p < 1.0 ? s.listed[row] : 0;
+    if (n > kBatchList) {
+      token = draw_from_row(l, logits, s.n, p, top);
+    } else {
+      for (int c = tid; c < chunks; c += kRowThreads) l.mass[c] = s.chunk_mass[(int64_t)row * chunks + c];
+      for (int i = tid; i < n; i += kRowThreads) l.list[i] = s.list[(int64_t)row * kBatchList + i];
+      __syncthreads();
+      uint64_t cut = 0;
+      if (n) {
+        sort_list(l, n);
+        cut = keep_from_list(l, n, p, top, above, need);
+      }
+      token = draw_from_chunks(l, logits, s.n, p, top, cut);
+    }
   }
-  const int n = l.count;
-  __syncthreads();
-  const int token = list ? draw_from_list(l, n, p, top, row_mass) : draw_from_row(l, logits, s.n, p, top);
   if (tid == 0) s.tokens[row] = token;
+}
+
+template <typename Kernel>
+static hipError_t launch_rows(Kernel k, dim3 grid, const SampleRows& s, hipStream_t stream) {
+  hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)sizeof(RowLds));
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(k, grid, dim3(kRowThreads), sizeof(RowLds), stream, s);
+  return hipGetLastError();
 }
 
 hipError_t sample_rows_launch(const SampleRows& s, hipStream_t stream) {
@@ -579,11 +847,12 @@ hipError_t sample_rows_launch(const SampleRows& s, hipStream_t stream) {
                      dim3(256), 0, stream, s);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  e = hipFuncSetAttribute(reinterpret_cast<const void*>(sample_finish_kernel),
-                          hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(FinishLds));
+  // (which rows have a top-k or top-p is known on the device only; no array: none has)
+  if (s.top_p || s.top_k) e = launch_rows(sample_mass_kernel, dim3(kRowShares, s.rows), s, stream);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(sample_finish_kernel, dim3(s.rows), dim3(kFinishThreads), sizeof(FinishLds), stream, s);
-  return hipGetLastError();
+  e = launch_rows(sample_cut_kernel, dim3(kRowShares, s.rows), s, stream);
+  if (e != hipSuccess) return e;
+  return launch_rows(sample_finish_kernel, dim3(s.rows), s, stream);
 }
 
 }  // namespace llhip
