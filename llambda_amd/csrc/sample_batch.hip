@@ -6,7 +6,7 @@
 //     at or above the k-th highest chunk maximum, and few more.  The row's
 //     workgroup (sample_finish_kernel) reads the chunks that reach it and lists
 //     those logits in LDS: up to 64 ranks are settled by one wavefront
-//   no top-k: the row is shared by eight workgroups.  With top-p
+//   no top-k: the row is shared by as many workgroups as fit.  With top-p
 //     (sample_mass_kernel) its weights are summed by bins of (max - l) / T, 64 to
 //     one; then (sample_cut_kernel) every chunk's weight above the bin that the
 //     cut falls into is summed, and that bin's logits are listed; without, every
@@ -213,7 +213,9 @@ __device__ __forceinline__ Weighed weigh(const RowLds& l, float v, float top, do
   const float f = (float)(t - (double)b) * (1.f / 64);
   const float g = f * (1.f - f * (0.5f - f * (1.f / 6 - f * (1.f / 24 - f * (1.f / 120)))));  // 1 - e^-f
   const double w = l.powers[b];
-  return Weighed{b, (uint64_t)(w - w * (double)g + 0.5)};
+  // (the integer is the low bits of the sum with 2^52)
+  const uint64_t bits = __builtin_bit_cast(uint64_t, fma(w, -(double)g, w) + 4503599627370496.0);
+  return Weighed{b, bits & 0xFFFFFFFFFFFFFull};
 }
 
 // Sort list[0, n) in descending order.  Up to one entry a thread: by counting the larger ones (no two
@@ -305,9 +307,20 @@ __device__ __forceinline__ void each_chunk(const float* row, int n, int first, i
   }
 }
 
+template <int CTRL>
+__device__ __forceinline__ uint64_t dpp_u64(uint64_t v) {
+  return (uint64_t)(uint32_t)dpp_i<CTRL>((int)(v >> 32)) << 32 | (uint32_t)dpp_i<CTRL>((int)v);
+}
+__device__ __forceinline__ uint64_t readlane_u64(uint64_t v, int lane) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
 __device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+  v += dpp_u64<kDppXor1>(v);
+  v += dpp_u64<kDppXor2>(v);
+  v += dpp_u64<kDppHalfMirror>(v);
+  v += dpp_u64<kDppMirror>(v);
+  return readlane_u64(v, 0) + readlane_u64(v, 16) + readlane_u64(v, 32) + readlane_u64(v, 48);
 }
 
 // A min-p as an integer weight: weights of at least it are kept.
@@ -315,10 +328,9 @@ __device__ __forceinline__ uint64_t least_weight(const RowParams& p) { return (u
 
 // ------------------------------------------------------------------ rows without top-k
 
-constexpr int kRowShares = 8;  // workgroups on a row
-
+// The row's chunks to this workgroup of those on it.
 __device__ __forceinline__ void share_of(int chunks, int& first, int& last) {
-  const int per = (chunks + kRowShares - 1) / kRowShares;
+  const int shares = gridDim.x, per = (chunks + shares - 1) / shares;
   first = blockIdx.x * per;
   last = min(chunks, first + per);
 }
@@ -463,9 +475,9 @@ __device__ void draw_by_wave(RowLds& l, int n, const RowParams& p, float top, in
   // the sum up to each one's index
   double run = 0.0, total = 0.0;
   for (int i = 0; i < kept; ++i) {
-    const double wi = __shfl(w, i, 64);
+    const double wi = __builtin_bit_cast(double, readlane_u64(__builtin_bit_cast(uint64_t, w), i));
     total += wi;
-    run += __shfl(index, i, 64) <= index ? wi : 0.0;
+    run += __builtin_amdgcn_readlane(index, i) <= index ? wi : 0.0;
   }
   const bool past = lane < kept && run > p.random * total;
   const int found = wave_min(past ? index : INT_MAX), last = wave_max_i(lane < kept ? index : -1);
@@ -847,10 +859,12 @@ hipError_t sample_rows_launch(const SampleRows& s, hipStream_t stream) {
                      dim3(256), 0, stream, s);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
+  // Workgroups to a row: a CU holds two, and each may find its row to have.
+  const int shares = max(1, min(1024 / s.rows, (chunks + 15) / 16));
   // (which rows have a top-k or top-p is known on the device only; no array: none has)
-  if (s.top_p || s.top_k) e = launch_rows(sample_mass_kernel, dim3(kRowShares, s.rows), s, stream);
+  if (s.top_p || s.top_k) e = launch_rows(sample_mass_kernel, dim3(shares, s.rows), s, stream);
   if (e != hipSuccess) return e;
-  e = launch_rows(sample_cut_kernel, dim3(kRowShares, s.rows), s, stream);
+  e = launch_rows(sample_cut_kernel, dim3(shares, s.rows), s, stream);
   if (e != hipSuccess) return e;
   return launch_rows(sample_finish_kernel, dim3(s.rows), s, stream);
 }

@@ -78,9 +78,12 @@ __device__ __forceinline__ int slot_of(const int* list, int i) { return list ? l
 // Whether sequence i may run, by the block's threads together (uniform): its
 // slots lie in the pool, and no other sequence reads or writes the slot that
 // it writes.  `flag`: one int of LDS.
+__device__ __forceinline__ bool slots_in_pool(const SsmLayerPlan& p, int from, int to) {
+  return !(from < -1 || from >= p.slots || to < -1 || to >= p.slots);
+}
 __device__ bool slots_allowed(const SsmLayerPlan& p, const SsmCall& c, int i, int* flag) {
   const int from = slot_of(c.from, i), to = slot_of(c.to, i);
-  int bad = (from < -1 || from >= p.slots || to < -1 || to >= p.slots) ? kSsmErrSlot : 0;
+  int bad = slots_in_pool(p, from, to) ? 0 : kSsmErrSlot;
   if (threadIdx.x == 0) *flag = bad;
   __syncthreads();
   if (!bad && to >= 0 && (c.from || c.to)) {
@@ -896,14 +899,15 @@ __global__ void __launch_bounds__(256) ssm_step_kernel(SsmLayerPlan p, SsmCall c
   __shared__ float sx[kSsmMaxHeadDim], sb[N], sc[N];
   __shared__ int flag;
   const int i = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
-  if (!slots_allowed(p, c, i, &flag)) return;
-  const int from = slot_of(c.from, i), to = slot_of(c.to, i);
+  const int to = slot_of(c.to, i);
+  int from = slot_of(c.from, i);
+  if (!slots_in_pool(p, from, to)) from = -1;  // (refused below)
   const int P = p.head_dim, inner = p.heads * P, gn = p.groups * N, channels = inner + 2 * gn, W = p.conv;
   const int group = h / (p.heads / p.groups);
   const float* row = c.x + (int64_t)i * (inner + channels + p.heads);
   const float* taps = conv_taps(p, from);
   const int p0 = blockIdx.z * (kStepElements / N), np = min(P - p0, kStepElements / N);
-  // the state first: its loads run while the convolution is formed
+  // the state first: its loads run while the slots are checked and the convolution is formed
   const int q = tid % LANES, r0 = tid / LANES;
   const int64_t at = ((int64_t)h * P + p0) * N + 4 * q;
   floatx4 st[kRounds];
@@ -914,6 +918,7 @@ __global__ void __launch_bounds__(256) ssm_step_kernel(SsmLayerPlan p, SsmCall c
                 ? *reinterpret_cast<const floatx4*>(p.ssm_states + (int64_t)from * inner * N + at + (int64_t)r * N)
                 : floatx4{0.f, 0.f, 0.f, 0.f};
   }
+  if (!slots_allowed(p, c, i, &flag)) return;
   const float dt = softplus_f32(row[inner + channels + h] + p.dt_bias[h]);
   const float a = __builtin_amdgcn_exp2f((float)log2_decay(dt, p.a[h]));
   for (int k = tid; k < np + 2 * N; k += 256) {
