@@ -888,14 +888,13 @@ __global__ void __launch_bounds__(256) ssm_join_kernel(SsmLayerPlan p) {
 
 // ------------------------------------------------------------------ one token
 
-// Block (sequence, head, part): kStepElements state elements of a head.  N / 4
-// lanes share a channel's state row.
-constexpr int kStepElements = 8192;
-
-template <int N>
+// Block (sequence, head, part): ELEMENTS state elements of a head.  N / 4 lanes share a channel's
+// state row.  The states are read and written past the caches' ordinary policy (48 states of 2 MiB in
+// rotation: 44 us, 55 with plain accesses): a layer's are not met again before all others'.
+template <int N, int ELEMENTS>
 __global__ void __launch_bounds__(256) ssm_step_kernel(SsmLayerPlan p, SsmCall c) {
   constexpr int LANES = N / 4, ROWS = 256 / LANES;  // channels per round of the block
-  constexpr int kRounds = kStepElements / (ROWS * N);
+  constexpr int kRounds = ELEMENTS / (ROWS * N);
   __shared__ float sx[kSsmMaxHeadDim], sb[N], sc[N];
   __shared__ int flag;
   const int i = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
@@ -906,7 +905,7 @@ __global__ void __launch_bounds__(256) ssm_step_kernel(SsmLayerPlan p, SsmCall c
   const int group = h / (p.heads / p.groups);
   const float* row = c.x + (int64_t)i * (inner + channels + p.heads);
   const float* taps = conv_taps(p, from);
-  const int p0 = blockIdx.z * (kStepElements / N), np = min(P - p0, kStepElements / N);
+  const int p0 = blockIdx.z * (ELEMENTS / N), np = min(P - p0, ELEMENTS / N);
   // the state first: its loads run while the slots are checked and the convolution is formed
   const int q = tid % LANES, r0 = tid / LANES;
   const int64_t at = ((int64_t)h * P + p0) * N + 4 * q;
@@ -915,7 +914,8 @@ __global__ void __launch_bounds__(256) ssm_step_kernel(SsmLayerPlan p, SsmCall c
   for (int k = 0; k < kRounds; ++k) {
     const int r = r0 + ROWS * k;
     st[k] = from >= 0 && r < np
-                ? *reinterpret_cast<const floatx4*>(p.ssm_states + (int64_t)from * inner * N + at + (int64_t)r * N)
+                ? __builtin_nontemporal_load(reinterpret_cast<const floatx4*>(
+                      p.ssm_states + (int64_t)from * inner * N + at + (int64_t)r * N))
                 : floatx4{0.f, 0.f, 0.f, 0.f};
   }
   if (!slots_allowed(p, c, i, &flag)) return;
@@ -944,7 +944,8 @@ __global__ void __launch_bounds__(256) ssm_step_kernel(SsmLayerPlan p, SsmCall c
     y = segment_sum<LANES>(y);
     if (r >= np) continue;
     if (to >= 0)
-      *reinterpret_cast<floatx4*>(p.ssm_states + (int64_t)to * inner * N + at + (int64_t)r * N) = st[k];
+      __builtin_nontemporal_store(st[k], reinterpret_cast<floatx4*>(p.ssm_states + (int64_t)to * inner * N + at +
+                                                                    (int64_t)r * N));
     if (q == 0) c.y[(int64_t)i * inner + h * P + p0 + r] = fmaf(d, x, y);
   }
 }
@@ -1143,17 +1144,25 @@ static hipError_t finish_launch(const SsmLayerPlan& p, const SsmCall& c, hipStre
   return launch(ssm_finish_kernel<1024>, b.second, dim3(1024), 0, s, p, c, b.first);
 }
 
-hipError_t ssm_step_launch(const SsmLayerPlan& p, const SsmCall& c, hipStream_t s) {
-  const dim3 grid(c.sequences, p.heads, (p.head_dim * p.state + kStepElements - 1) / kStepElements);
-  hipError_t e;
+template <int ELEMENTS>
+static hipError_t step_launch(const SsmLayerPlan& p, const SsmCall& c, hipStream_t s) {
+  const dim3 grid(c.sequences, p.heads, (p.head_dim * p.state + ELEMENTS - 1) / ELEMENTS);
   switch (p.state) {
-    case 16: e = launch(ssm_step_kernel<16>, grid, dim3(256), 0, s, p, c); break;
-    case 32: e = launch(ssm_step_kernel<32>, grid, dim3(256), 0, s, p, c); break;
-    case 64: e = launch(ssm_step_kernel<64>, grid, dim3(256), 0, s, p, c); break;
-    case 128: e = launch(ssm_step_kernel<128>, grid, dim3(256), 0, s, p, c); break;
-    case 256: e = launch(ssm_step_kernel<256>, grid, dim3(256), 0, s, p, c); break;
+    case 16: return launch(ssm_step_kernel<16, ELEMENTS>, grid, dim3(256), 0, s, p, c);
+    case 32: return launch(ssm_step_kernel<32, ELEMENTS>, grid, dim3(256), 0, s, p, c);
+    case 64: return launch(ssm_step_kernel<64, ELEMENTS>, grid, dim3(256), 0, s, p, c);
+    case 128: return launch(ssm_step_kernel<128, ELEMENTS>, grid, dim3(256), 0, s, p, c);
+    case 256: return launch(ssm_step_kernel<256, ELEMENTS>, grid, dim3(256), 0, s, p, c);
     default: return hipErrorInvalidValue;
   }
+}
+
+hipError_t ssm_step_launch(const SsmLayerPlan& p, const SsmCall& c, hipStream_t s) {
+  // Parts of 2048 elements put a short call on more CUs, each of whose workgroups forms B and C again:
+  // 64 heads of 64 x 128, one sequence 6.0 us (8.3 in parts of 8192), 8 sequences 12.1 (13.0), 10 16.1
+  // (13.7), 48 57 (44).
+  const int64_t parts = (int64_t)c.sequences * p.heads * ((p.head_dim * p.state + 8191) / 8192);
+  const hipError_t e = parts <= 512 ? step_launch<2048>(p, c, s) : step_launch<8192>(p, c, s);
   if (e != hipSuccess) return e;
   return finish_launch(p, c, s);
 }
