@@ -303,7 +303,8 @@ int llambda_hip_router_run_device(llambda_hip_router* router, const float* logit
  * the router tensor's products alone, the shared expert's gate stays as it is,
  * and the run's input errors are raised as before (unfilled places; with
  * weights_norm a sum that is not positive).  Graphs captured before the change
- * keep the gating they hold and have to be captured anew. */
+ * keep the gating that they were captured with (the session keeps each bias it
+ * was given until it is destroyed). */
 int llambda_hip_moe_session_set_router(llambda_hip_moe_session* session,
                                        llambda_hip_router* router);
 
@@ -564,7 +565,8 @@ typedef struct llambda_hip_batch_sampling {
   const float* random_value;  /* [0, 1); required */
 } llambda_hip_batch_sampling;
 
-/* Workspace for up to max_rows rows of up to `vocab` logits (at most 262144).
+/* Workspace for up to max_rows rows of up to `vocab` logits (at most 262144),
+ * 49 to 61 KB a row.
  * No counterpart in the reference, which samples one row at a time. */
 int llambda_hip_batch_sampler_create(size_t vocab, size_t max_rows,
                                      llambda_hip_batch_sampler** result);
@@ -572,7 +574,8 @@ void llambda_hip_batch_sampler_destroy(llambda_hip_batch_sampler* sampler);
 
 /* One token per row of logits[rows][count], all device memory, on `stream`
  * (null = the sampler's), not waited for, with no allocation.  Per row, in 64
- * bits, with x = logit / temperature: weights are exp(x - max x); ranks go by
+ * bits, with x = logit / temperature: weights are exp(x - max x), to 2e-9 of
+ * themselves and 2^-45, and their sums of these are exact; ranks go by
  * logit, the lower index first among equals.  Kept are the top_k first ranks;
  * of those the shortest run from the first whose weights reach top_p of their
  * total; of those the weights of at least min_p (the largest weight is 1).

@@ -527,7 +527,12 @@ struct llambda_hip_moe_session {
   MoePlan plan{};
   DevBuf router, bias, gate, up, down, sh_gate, sh_up, sh_down, lat_down, lat_up;
   DevBuf up_g, down_g, sh_up_g, sh_down_g;  // stage-major copies (group pipeline)
-  DevBuf route_bias;
+  // of the routers set so far: captured graphs may hold any of them
+  struct RouteBias {
+    std::vector<float> host;
+    DevBuf device;
+  };
+  std::vector<std::unique_ptr<RouteBias>> route_biases;
   DevBuf logits, router_part, top_idx, top_w, shared_w, perm, chunks, chunk_counts,
       down_out, error, xq, xsum, aq, asum, lat, lq, lsum, lat_y;
   DevBuf x, y;     // device staging for the host-pointer runs
@@ -1173,12 +1178,19 @@ int llambda_hip_moe_session_set_router(llambda_hip_moe_session* s, llambda_hip_r
             r->spec.experts, s->plan.top_k, s->plan.experts);
     RouteSpec spec = r->spec;
     if (spec.bias) {
-      DevBuf bias;
-      bias.alloc(r->host_bias.size() * sizeof(float), "router bias");
-      HIPC(hipMemcpyAsync(bias.ptr, r->host_bias.data(), bias.bytes, hipMemcpyHostToDevice, s->stream));
-      HIPC(hipStreamSynchronize(s->stream));
-      spec.bias = bias.as<float>();
-      s->route_bias.swap(bias);  // the old one is freed once the device is idle
+      const llambda_hip_moe_session::RouteBias* bias = nullptr;
+      for (const auto& b : s->route_biases)
+        if (!memcmp(b->host.data(), r->host_bias.data(), b->host.size() * sizeof(float))) bias = b.get();
+      if (!bias) {
+        auto b = std::make_unique<llambda_hip_moe_session::RouteBias>();
+        b->host = r->host_bias;
+        b->device.alloc(b->host.size() * sizeof(float), "router bias");
+        HIPC(hipMemcpyAsync(b->device.ptr, b->host.data(), b->device.bytes, hipMemcpyHostToDevice, s->stream));
+        HIPC(hipStreamSynchronize(s->stream));
+        bias = b.get();
+        s->route_biases.push_back(std::move(b));
+      }
+      spec.bias = bias->device.as<float>();
     }
     s->plan.route = spec;
     s->plan.routed = 1;

@@ -15,7 +15,7 @@
 
 namespace llhip {
 
-// Workspace: at most 62 KB a row.
+// Workspace: at most 61 KB a row.
 constexpr int kBatchChunk = 256;  // logits whose maximum the first launch records
 constexpr int kBatchMaxVocab = 262144;
 constexpr int kBatchMaxChunks = kBatchMaxVocab / kBatchChunk;

@@ -1,6 +1,6 @@
 """Sampling of a batch (llambda_hip_batch_sampler_*) against its definition in
-64 bits.  Both sides sum the same weights in 64 bits or in steps of 2^-44, so
-the tokens are equal unless a random number lies within about 1e-11 of a
+64 bits.  The weights are good to 2e-9 and summed exactly in steps of 2^-44, so
+the tokens are equal unless a random number lies within about 2e-9 of a
 boundary."""
 import numpy as np
 import pytest

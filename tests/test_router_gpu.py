@@ -240,6 +240,37 @@ def test_moe_layer_with_the_reference_gating_as_a_router(hip):
         assert np.abs(y - y2).max() <= 16 * 2.0 ** -24 * np.abs(y).max() * 4
 
 
+def test_captured_gating_outlives_a_change_of_router(hip):
+    """A graph keeps the router that it was captured with."""
+    import torch
+    rng = np.random.default_rng(12)
+    layer = synthetic_qwen3next(rng, hidden=512, experts=16, top_k=4, ffn=256, shared_ffn=256)
+    session = HipMoeSession(layer)
+    biases = [(rng.normal(size=16) * 2).astype(np.float32) for _ in range(4)]
+    x = torch.from_numpy(synthetic.activations(rng, 3, 512)).cuda()
+    y = torch.zeros(3, 512, device="cuda")
+    want = []
+    for b in biases:
+        session.set_router(HipRouter(Routing(16, 4, bias=b)))
+        want.append(session.run(x.cpu().numpy()))
+    assert len({w.tobytes() for w in want}) == len(want)
+    stream = torch.cuda.Stream()
+    graphs = []
+    for b in biases[:2]:
+        session.set_router(HipRouter(Routing(16, 4, bias=b)))
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream, capture_error_mode="relaxed"):
+            session.run_device(x.data_ptr(), y.data_ptr(), 3, stream.cuda_stream)
+        graphs.append(graph)
+    for b in biases[2:] + [None]:
+        session.set_router(None if b is None else HipRouter(Routing(16, 4, bias=b)))
+        for graph, w in zip(graphs, want):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert np.array_equal(y.cpu().numpy(), w)
+
+
 def test_moe_layer_errors_with_a_router(hip):
     from llambda_amd.moe import MoeLayerInputError
     rng = np.random.default_rng(10)
