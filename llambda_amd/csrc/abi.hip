@@ -1624,7 +1624,7 @@ struct llambda_hip_ssm_session {
   hipStream_t stream = nullptr;
   SsmLayerPlan plan{};
   DevBuf weights, pool_conv, pool_ssm, error;
-  DevBuf sequences, segments, chunks, counts, images, decay, seg_states, seg_decay;
+  DevBuf sequences, segments, chunks, counts, images, scales, decay, seg_states, seg_decay;
   DevBuf x, y, lists;  // device staging of the host-pointer runs; lists: offsets, slot
   size_t staged_tokens = 0;
   // recorded after every call that uses the workspace; the next one waits
@@ -1786,6 +1786,7 @@ int llambda_hip_ssm_session_create(const llambda_hip_ssm_desc* d,
     s->segments.alloc(segments * sizeof(int2), "segment table");
     s->chunks.alloc(chunks * sizeof(int2), "chunk table");
     s->images.alloc(chunks * p.groups * ssm_image_bytes(p.state), "convolved B and C");
+    s->scales.alloc(chunks * p.groups * 2 * kSsmChunk * sizeof(float), "scales of B and C");
     s->decay.alloc(chunks * 3 * H * kSsmChunk * sizeof(float), "decays");
     const size_t states = (size_t)ssm_max_states(p, p.max_tokens);
     s->seg_states.alloc(states * s->ssm_elements() * sizeof(float), "segment states");
@@ -1796,6 +1797,7 @@ int llambda_hip_ssm_session_create(const llambda_hip_ssm_desc* d,
     p.segments = s->segments.as<int2>();
     p.chunks = s->chunks.as<int2>();
     p.images = s->images.as<uint8_t>();
+    p.scales = s->scales.as<float>();
     p.decay = s->decay.as<float>();
     p.seg_states = s->seg_states.as<float>();
     p.seg_decay = s->seg_decay.as<float>();

@@ -59,6 +59,7 @@ struct SsmLayerPlan {
   int2* chunks;            // [max_chunks]: sequence, index within it
   int* counts;             // segments, chunks
   uint8_t* images;         // [chunk][G][ssm_image_bytes]: B, C after the convolution, C B^T
+  float* scales;           // [chunk][G][2][kSsmChunk]: 2^14 over the scales of B's and C's images
   float* decay;            // [chunk][H][3][kSsmChunk]: dt, log2 of the decay since the chunk's start (hi, lo)
   // segments of the sequences that have several, max_states in all
   float* seg_states;       // [H][P][N] each: the state that enters it

@@ -223,19 +223,50 @@ __device__ __forceinline__ Split8 split8(const float* v) {
   return r;
 }
 
+// v s = hi + lo in f16 for values whose largest is brought to [2^14, 2^15) by
+// the power of two s: 22 significant bits, or 2^-40 of the largest, whichever is
+// more.  Three products (of 2^-22 of the whole the fourth) where the three bf16
+// parts take six: the operands that are scaled in common by a row or column of
+// a product, whose result takes the scale back, are held so.
+struct Split2 {
+  u32x4 hi, lo;
+};
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ Split2 split_f16(const float* v) {
+  Split2 r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const f16x2 h = __builtin_convertvector(floatx2{v[2 * e], v[2 * e + 1]}, f16x2);
+    const f16x2 l = __builtin_convertvector(floatx2{v[2 * e] - (float)h.x, v[2 * e + 1] - (float)h.y}, f16x2);
+    r.hi[e] = __builtin_bit_cast(uint32_t, h);
+    r.lo[e] = __builtin_bit_cast(uint32_t, l);
+  }
+  return r;
+}
+// The scale as a float's bits, at most 2^100, for values of at most |m| (its sign
+// bit clear), and a power of two's reciprocal.
+__device__ __forceinline__ int scale_bits(float m) {
+  return (227 << 23) - max((__builtin_bit_cast(int, m) & 0x7F800000) - (41 << 23), 0);
+}
+__device__ __forceinline__ float power(int bits) { return __builtin_bit_cast(float, bits); }
+constexpr int k2p14 = 14 << 23;  // to add to or take from such bits
+__device__ __forceinline__ int reciprocal_bits(int bits) { return (254 << 23) - bits; }
+
 // What a chunk's scan reads of its group, in operand order: fragments of 64
 // lanes x 16 bytes, lane (r, g) = (lane & 15, lane >> 4).
-//   C   [i tile][n block of 32][hi, mid, lo]: token 16 it + r; element e is
+//   C   [i tile][n block of 32][hi, lo]: token 16 it + r; element e is
 //       n = 32 t + 16 (e / 4) + 4 g + e % 4, the elements of the state's result
 //       tiles that the same lane holds (zeros past n)
-//   B^T [n tile][hi, mid, lo]: row n = 16 nt + r; element e is token
+//   B^T [n tile][hi, lo]: row n = 16 nt + r; element e is token
 //       16 (e / 4) + 4 g + e % 4
+//   (both f16, scaled per token: 2^14 over the scales lies in p.scales)
 //   S^T [(j, i) tiles (0, 0), (0, 1), (1, 1)], fp32: rows j = 16 jt + 4 g ..
 //       + 3, column i = 16 it + r
 constexpr int kFragment = 1024;
 constexpr int n_blocks(int nt) { return (nt + 1) / 2; }
-constexpr int c_fragments(int nt) { return 6 * n_blocks(nt); }
-constexpr int b_fragments(int nt) { return 3 * nt; }
+constexpr int c_fragments(int nt) { return 4 * n_blocks(nt); }
+constexpr int b_fragments(int nt) { return 2 * nt; }
 constexpr int image_fragments(int nt) { return c_fragments(nt) + b_fragments(nt) + 3; }
 
 size_t ssm_image_bytes(int state) { return (size_t)image_fragments(state / 16) * kFragment; }
@@ -248,7 +279,7 @@ constexpr int kPrepHeads = 8;
 template <int NT, int W>
 __global__ void __launch_bounds__(256) ssm_prepare_kernel(SsmLayerPlan p, SsmCall c) {
   constexpr int N = 16 * NT, Q = kSsmChunk, LD = N + 4, NB = n_blocks(NT);
-  __shared__ float sbc[2][Q * LD];
+  __shared__ float sbc[2][Q * LD], scale[2][Q];
   const int chunk = blockIdx.x;
   if (chunk >= p.counts[1]) return;
   const int2 at = p.chunks[chunk];
@@ -285,6 +316,24 @@ __global__ void __launch_bounds__(256) ssm_prepare_kernel(SsmLayerPlan p, SsmCal
       }
     }
     __syncthreads();
+    {
+      // a token's scale: four threads take its B and C (what is not finite has none to give)
+      const int which = tid >> 7, q = (tid >> 2) & 31, part = tid & 3;
+      float m = 0.f;
+      for (int n = 4 * part; n < N; n += 16) {
+        const floatx4 v = *reinterpret_cast<const floatx4*>(&sbc[which][q * LD + n]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(v[e]) <= FLT_MAX ? fabsf(v[e]) : 0.f);
+      }
+      m = fmaxf(m, dpp<kDppXor1>(m));
+      m = fmaxf(m, dpp<kDppXor2>(m));
+      if (part == 0) {
+        const int bits = scale_bits(m);
+        scale[which][q] = power(bits);
+        p.scales[((int64_t)chunk * p.groups + group) * 2 * Q + which * Q + q] = power(reciprocal_bits(bits) + k2p14);
+      }
+    }
+    __syncthreads();
     const int lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
     uint8_t* image = p.images + ((int64_t)chunk * p.groups + group) * image_fragments(NT) * kFragment;
     if (wave < 3) {
@@ -301,7 +350,7 @@ __global__ void __launch_bounds__(256) ssm_prepare_kernel(SsmLayerPlan p, SsmCal
     }
     for (int f = wave; f < 2 * NB + NT; f += 4) {
       float v[8];
-      int at3;
+      int first;
       if (f < 2 * NB) {
         const int it = f / NB, t = f - it * NB;
 #pragma unroll
@@ -309,21 +358,24 @@ __global__ void __launch_bounds__(256) ssm_prepare_kernel(SsmLayerPlan p, SsmCal
           floatx4 q{0.f, 0.f, 0.f, 0.f};
           if (2 * t + half < NT)
             q = *reinterpret_cast<const floatx4*>(&sbc[1][(16 * it + col) * LD + 32 * t + 16 * half + 4 * g]);
+          const float by = scale[1][16 * it + col];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[4 * half + e] = q[e];
+          for (int e = 0; e < 4; ++e) v[4 * half + e] = q[e] * by;
         }
-        at3 = 3 * f;
+        first = 2 * f;
       } else {
         const int nt = f - 2 * NB;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = sbc[0][(16 * (e >> 2) + 4 * g + (e & 3)) * LD + 16 * nt + col];
-        at3 = c_fragments(NT) + 3 * nt;
+        for (int e = 0; e < 8; ++e) {
+          const int q = 16 * (e >> 2) + 4 * g + (e & 3);
+          v[e] = sbc[0][q * LD + 16 * nt + col] * scale[0][q];
+        }
+        first = c_fragments(NT) + 2 * nt;
       }
-      const Split8 r = split8(v);
-      u32x4* out = reinterpret_cast<u32x4*>(image + at3 * kFragment) + lane;
+      const Split2 r = split_f16(v);
+      u32x4* out = reinterpret_cast<u32x4*>(image + first * kFragment) + lane;
       out[0] = r.hi;
-      out[kFragment / 16] = r.mid;
-      out[2 * kFragment / 16] = r.lo;
+      out[kFragment / 16] = r.lo;
     }
     return;
   }
@@ -350,6 +402,19 @@ __global__ void __launch_bounds__(256) ssm_prepare_kernel(SsmLayerPlan p, SsmCal
 // same K element.
 __device__ __forceinline__ floatx4 mma_one(const u32x4& a, const u32x4& b, const floatx4& c) {
   return mfma32(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c);
+}
+
+__device__ __forceinline__ floatx4 mma_f16(const u32x4& a, const u32x4& b, const floatx4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// The maximum over the four lanes that hold one column (row swaps as in
+// row_pair_sum).
+__device__ __forceinline__ float column_max(float v) {
+  float a = v, b = v;
+  asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+  a = b = fmaxf(a, b);
+  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+  return fmaxf(a, b);
 }
 
 // Wait for every load, in a form that the compiler counts too (it would wait
@@ -386,13 +451,15 @@ struct ScanLds {
   static constexpr int s = STATES ? 0 : 3 * kFragment;
   static constexpr int decays = 3 * kSsmChunk * 4;             // per head
   static constexpr int products = STATES ? 0 : 6 * kFragment;  // per head: [i tile][hi, mid, lo]
-  static constexpr int tables = 2 * kSsmChunk * 4;             // per head: [e, w]
+  static constexpr int tables = (2 * kSsmChunk + 4) * 4;       // per head: [e, w], the chunk's whole decay
+  static constexpr int scales = 2 * kSsmChunk * 4;             // B's, C's
   // raw rows of the workgroup's channels.  The pitch puts the rows 4 apart
   // that a wavefront reads together 16 banks apart.
   static constexpr int rows = kSsmChunk + W - 1;
   __host__ __device__ static constexpr int pitch(int width) { return 4 * (width + 4); }
   static constexpr int at_c = buffers * b, at_s = at_c + c, at_decays = at_s + s;
-  __host__ __device__ static constexpr int at_products(int hw) { return at_decays + buffers * hw * decays; }
+  __host__ __device__ static constexpr int at_scales(int hw) { return at_decays + buffers * hw * decays; }
+  __host__ __device__ static constexpr int at_products(int hw) { return at_scales(hw) + buffers * scales; }
   __host__ __device__ static constexpr int at_tables(int hw) { return at_products(hw) + 2 * hw * products; }
   __host__ __device__ static constexpr int at_rows(int hw) { return at_tables(hw) + 2 * hw * tables; }
   __host__ __device__ static constexpr int bytes(int hw, int width) {
@@ -470,6 +537,11 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
     const int first = (kScanWaves - 1 - wave) * kFragment;
     if (first + 16 * lane < hw * Lds::decays)
       load_lds16(dec, first + 16 * lane, lds0 + Lds::at_decays + buf * hw * Lds::decays + first);
+    // and the group's scales
+    if (wave == kScanWaves - 3 && 16 * lane < Lds::scales)
+      load_lds16(uniform_ptr(reinterpret_cast<const uint8_t*>(
+                     p.scales + ((int64_t)(s.chunk0 + t / Q) * p.groups + group) * 2 * Q)),
+                 16 * lane, lds0 + Lds::at_scales(hw) + buf * Lds::scales);
   };
   // the raw rows that a chunk's convolution reads: before the sequence those
   // it started with (zeros for a new one), past its end the last row again
@@ -536,6 +608,28 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
                                         : floatx4{0.f, 0.f, 0.f, 0.f};
   }
   float total_hi[TPW] = {}, total_lo[TPW] = {};
+  // The state is held times a power of two per column, which changes with the
+  // inputs (below); `most` bounds it there.
+  int held[TPW];
+  float most[TPW];
+  auto state_max = [&](int k) {
+    float m = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(st[k][n][e]));
+    return column_max(m);
+  };
+#pragma unroll
+  for (int k = 0; k < TPW; ++k) {
+    held[k] = 127 << 23;
+    most[k] = 0.f;
+    if (!STATES) {
+      held[k] = max(scale_bits(state_max(k)), (1 << 23) + k2p14);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) st[k][n] *= power(held[k]);
+    }
+  }
 
   // x of the lane's tokens 4 g .. + 3 and 16 + 4 g .. + 3 after the convolution
   float x[TPW][8];
@@ -559,14 +653,18 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
   };
   auto decays_at = [&](int buf) { return reinterpret_cast<const float*>(lds + Lds::at_decays + buf * hw * Lds::decays); };
   auto tables_at = [&](int buf) { return reinterpret_cast<float*>(lds + Lds::at_tables(hw) + buf * hw * Lds::tables); };
-  // decays from the chunk's start (e) and to its end, with dt (w); the same
+  // decays from the chunk's start (e) and to its end, with dt (w), and C's and
+  // B's scales taken back; the same
   // values from as many threads as there are
   auto make_tables = [&](int from, int to) {
     const int h = (tid / Q) % hw, q = tid % Q;
     const float* d = decays_at(from) + h * 3 * Q;
-    float* t = tables_at(to) + h * 2 * Q + q;
-    t[0] = __builtin_amdgcn_exp2f(d[Q + q] + d[2 * Q + q]);
-    t[Q] = d[q] * __builtin_amdgcn_exp2f((d[2 * Q - 1] - d[Q + q]) + (d[3 * Q - 1] - d[2 * Q + q]));
+    const float* scale = reinterpret_cast<const float*>(lds + Lds::at_scales(hw) + from * Lds::scales);
+    float* t = tables_at(to) + h * (Lds::tables / 4) + q;
+    const float e = __builtin_amdgcn_exp2f(d[Q + q] + d[2 * Q + q]);
+    t[0] = e * scale[Q + q];
+    t[Q] = d[q] * __builtin_amdgcn_exp2f((d[2 * Q - 1] - d[Q + q]) + (d[3 * Q - 1] - d[2 * Q + q])) * scale[q];
+    if (q == Q - 1) t[Q + 1] = e;
   };
   // M = S o L of the workgroup's heads, as left operands: job (head, tile,
   // half), a lane's two neighbouring j of column i.  (Past the last job that
@@ -653,41 +751,44 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
       for (int it = 0; it < 2; ++it)
 #pragma unroll
         for (int k = 0; k < TPW; ++k) acc[it][k] = floatx4{0.f, 0.f, 0.f, 0.f};
+      int by[TPW];  // the state's scale as an operand, beyond the held one
+#pragma unroll
+      for (int k = 0; k < TPW; ++k) {
+        most[k] = state_max(k);
+        by[k] = scale_bits(most[k]);
+      }
       // the next block's fragments are read ahead, and no further ahead: read
       // where the compiler likes they crowd the state out of the registers
       auto c_at = [&](int t, int it, int part) {
-        return *reinterpret_cast<const u32x4*>(lds + Lds::at_c + ((it * NB + t) * 3 + part) * kFragment + 16 * lane);
+        return *reinterpret_cast<const u32x4*>(lds + Lds::at_c + ((it * NB + t) * 2 + part) * kFragment + 16 * lane);
       };
-      u32x4 a[2][3], ahead[2][3];
+      u32x4 a[2][2], ahead[2][2];
 #pragma unroll
-      for (int part = 0; part < 6; ++part) ahead[part / 3][part % 3] = c_at(0, part / 3, part % 3);
+      for (int part = 0; part < 4; ++part) ahead[part / 2][part % 2] = c_at(0, part / 2, part % 2);
 #pragma unroll
       for (int t = 0; t < NB; ++t) {
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int part = 0; part < 6; ++part) {
-          a[part / 3][part % 3] = ahead[part / 3][part % 3];
-          if (t + 1 < NB) ahead[part / 3][part % 3] = c_at(t + 1, part / 3, part % 3);
+        for (int part = 0; part < 4; ++part) {
+          a[part / 2][part % 2] = ahead[part / 2][part % 2];
+          if (t + 1 < NB) ahead[part / 2][part % 2] = c_at(t + 1, part / 2, part % 2);
         }
-        Split8 sp[TPW];
+        Split2 sp[TPW];
 #pragma unroll
         for (int k = 0; k < TPW; ++k) {
           float v[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = st[k][2 * t + (e >> 2)][e & 3];
-          sp[k] = split8(v);
+          for (int e = 0; e < 8; ++e) v[e] = st[k][2 * t + (e >> 2)][e & 3] * power(by[k]);
+          sp[k] = split_f16(v);
         }
         // neighbouring products belong to different accumulators
-#define LLHIP_SSM_PRODUCT(A, B)                                            \
+#define LLHIP_SSM_PRODUCT(MMA, A, B)                                       \
   _Pragma("unroll") for (int it = 0; it < 2; ++it)                         \
       _Pragma("unroll") for (int k = 0; k < TPW; ++k)                      \
-          acc[it][k] = mma_one(A, B, acc[it][k]);
-        LLHIP_SSM_PRODUCT(a[it][2], sp[k].hi)
-        LLHIP_SSM_PRODUCT(a[it][0], sp[k].lo)
-        LLHIP_SSM_PRODUCT(a[it][1], sp[k].mid)
-        LLHIP_SSM_PRODUCT(a[it][1], sp[k].hi)
-        LLHIP_SSM_PRODUCT(a[it][0], sp[k].mid)
-        LLHIP_SSM_PRODUCT(a[it][0], sp[k].hi)
+          acc[it][k] = MMA(A, B, acc[it][k]);
+        LLHIP_SSM_PRODUCT(mma_f16, a[it][0], sp[k].lo)
+        LLHIP_SSM_PRODUCT(mma_f16, a[it][1], sp[k].hi)
+        LLHIP_SSM_PRODUCT(mma_f16, a[it][0], sp[k].hi)
         // loads for the state phase: in parts, for a wavefront waits where
         // the memory pipeline is busy with the others'
         if (t == 0) request_image(t0, kC, kB, 0);
@@ -732,21 +833,24 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
 #pragma unroll
       for (int k = 0; k < TPW; ++k) {
         xs[k] = split8(xf[k]);
+        // (one by one, so that none of them leaves single precision's range)
+        const float back = power(reciprocal_bits(by[k]) - k2p14), own = power(reciprocal_bits(held[k]));
         const uint8_t* from = lds + Lds::at_products(hw) + (buf * hw + head[k]) * Lds::products + 16 * lane;
 #pragma unroll
         for (int it = 0; it < 2; ++it) {
-          acc[it][k] *= *reinterpret_cast<const floatx4*>(tables + head[k] * 2 * Q + 16 * it + 4 * g);
+          acc[it][k] = acc[it][k] * back * own *
+                       *reinterpret_cast<const floatx4*>(tables + head[k] * (Lds::tables / 4) + 16 * it + 4 * g);
 #pragma unroll
           for (int part = 0; part < 3; ++part)
             m[it][k][part] = *reinterpret_cast<const u32x4*>(from + (it * 3 + part) * kFragment);
         }
       }
-      LLHIP_SSM_PRODUCT(m[it][k][2], xs[k].hi)
-      LLHIP_SSM_PRODUCT(m[it][k][0], xs[k].lo)
-      LLHIP_SSM_PRODUCT(m[it][k][1], xs[k].mid)
-      LLHIP_SSM_PRODUCT(m[it][k][1], xs[k].hi)
-      LLHIP_SSM_PRODUCT(m[it][k][0], xs[k].mid)
-      LLHIP_SSM_PRODUCT(m[it][k][0], xs[k].hi)
+      LLHIP_SSM_PRODUCT(mma_one, m[it][k][2], xs[k].hi)
+      LLHIP_SSM_PRODUCT(mma_one, m[it][k][0], xs[k].lo)
+      LLHIP_SSM_PRODUCT(mma_one, m[it][k][1], xs[k].mid)
+      LLHIP_SSM_PRODUCT(mma_one, m[it][k][1], xs[k].hi)
+      LLHIP_SSM_PRODUCT(mma_one, m[it][k][0], xs[k].mid)
+      LLHIP_SSM_PRODUCT(mma_one, m[it][k][0], xs[k].hi)
 #undef LLHIP_SSM_PRODUCT
       // the lane's four tokens of a channel become four channels of a token
       const bool odd = lane & 1, high = lane & 2;
@@ -773,23 +877,36 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
       }
       __syncthreads();  // B and what the next chunk needs have come; C is free
     }
-    // the state: decayed, plus the tokens' products
-    Split8 xs[TPW];
+    // The state: decayed, plus the tokens' products.  These inputs' scale
+    // becomes the one that the state is held times, unless that brought it
+    // near the end of single precision (inputs of next to nothing: they keep
+    // the digits that matter beside it).
+    Split2 xs[TPW];
 #pragma unroll
     for (int k = 0; k < TPW; ++k) {
-      const float* tab = tables + head[k] * 2 * Q;
+      const float* tab = tables + head[k] * (Lds::tables / 4);
       const floatx4 w0 = *reinterpret_cast<const floatx4*>(tab + Q + 4 * g);
       const floatx4 w1 = *reinterpret_cast<const floatx4*>(tab + Q + 16 + 4 * g);
-      float v[8];
+      float v[8], m = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = x[k][e] * (e < 4 ? w0[e & 3] : w1[e & 3]);
-      xs[k] = split8(v);
-      const float e = tab[Q - 1];
+      for (int e = 0; e < 8; ++e) {
+        v[e] = x[k][e] * (e < 4 ? w0[e & 3] : w1[e & 3]);
+        m = fmaxf(m, fabsf(v[e]));
+      }
+      const int room = (100 << 23) - max((__builtin_bit_cast(int, most[k]) & 0x7F800000) - (127 << 23), 0);
+      const int now = max(held[k] + min(scale_bits(column_max(m)) + k2p14 - held[k], room), (1 << 23) + k2p14);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= power(now - k2p14);
+      xs[k] = split_f16(v);
+      const float e = tab[2 * Q] * (power(now) * power(reciprocal_bits(held[k])));
+      held[k] = now;
+      // (32 products of two operands below 2^15)
+      if (STATES) most[k] = fmaf(most[k], e, 0x1p35f);
 #pragma unroll
       for (int n = 0; n < NT; ++n) st[k][n] *= e;
     }
     auto b_at = [&](int n, int part) {
-      return *reinterpret_cast<const u32x4*>(lds + (STATES ? buf * Lds::b : 0) + (3 * n + part) * kFragment + 16 * lane);
+      return *reinterpret_cast<const u32x4*>(lds + (STATES ? buf * Lds::b : 0) + (2 * n + part) * kFragment + 16 * lane);
     };
     // Between the products of the n tiles, what the next chunk needs (past the
     // last one it is not used): the wavefronts of a SIMD take turns with the
@@ -803,14 +920,14 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
       else if (i < 2 * TPW + kJobs) make_products(i - 2 * TPW, buf ^ 1);
       else make_tables(STATES ? buf ^ 1 : 0, buf ^ 1);
     };
-    u32x4 b[3], ahead[3];
+    u32x4 b[2], ahead[2];
 #pragma unroll
-    for (int part = 0; part < 3; ++part) ahead[part] = b_at(0, part);
+    for (int part = 0; part < 2; ++part) ahead[part] = b_at(0, part);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int part = 0; part < 3; ++part) {
+      for (int part = 0; part < 2; ++part) {
         b[part] = ahead[part];
         if (n + 1 < NT) ahead[part] = b_at(n + 1, part);
       }
@@ -818,12 +935,9 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
       if (first < last) piece_read(first);
 #define LLHIP_SSM_UPDATE(PART, FIELD)                                      \
   _Pragma("unroll") for (int k = 0; k < TPW; ++k)                          \
-      st[k][n] = mma_one(b[PART], xs[k].FIELD, st[k][n]);
-      LLHIP_SSM_UPDATE(2, hi)
+      st[k][n] = mma_f16(b[PART], xs[k].FIELD, st[k][n]);
       LLHIP_SSM_UPDATE(0, lo)
-      LLHIP_SSM_UPDATE(1, mid)
       LLHIP_SSM_UPDATE(1, hi)
-      LLHIP_SSM_UPDATE(0, mid)
       LLHIP_SSM_UPDATE(0, hi)
 #undef LLHIP_SSM_UPDATE
 #pragma unroll
@@ -846,7 +960,7 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
     const int at_ch = h0 * p.head_dim + ch[k];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
-      *reinterpret_cast<floatx4*>(dst + (int64_t)at_ch * N + 16 * n + 4 * g) = st[k][n];
+      *reinterpret_cast<floatx4*>(dst + (int64_t)at_ch * N + 16 * n + 4 * g) = st[k][n] * power(reciprocal_bits(held[k]));
     if (STATES && g == 0 && ch[k] % p.head_dim == 0)
       p.seg_decay[(int64_t)(s.state0 + at.y) * p.heads + h0 + head[k]] = total_hi[k] + total_lo[k];
   }
@@ -952,6 +1066,24 @@ __global__ void __launch_bounds__(256) ssm_step_kernel(SsmLayerPlan p, SsmCall c
 
 // ------------------------------------------------------------------ gate, norm, convolution state
 
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, (uint64_t)(uint32_t)dpp_i<CTRL>((int)(u >> 32)) << 32 | (uint32_t)dpp_i<CTRL>((int)u));
+}
+__device__ __forceinline__ double readlane_f64(double v, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(u >> 32), lane) << 32 |
+                                        (uint32_t)__builtin_amdgcn_readlane((int)u, lane));
+}
+__device__ __forceinline__ double wave_sum_f64(double v) {
+  v += dpp_f64<kDppXor1>(v);
+  v += dpp_f64<kDppXor2>(v);
+  v += dpp_f64<kDppHalfMirror>(v);
+  v += dpp_f64<kDppMirror>(v);
+  return (readlane_f64(v, 0) + readlane_f64(v, 16)) + (readlane_f64(v, 32) + readlane_f64(v, 48));
+}
+
 // Blocks [0, norm_blocks): rows y of (token, group), THREADS threads each:
 // v = y silu(z), out = v / sqrt(mean v^2 + eps) * norm, in place.  The others:
 // the convolution state of a sequence, 256 channels a block (a thread reads
@@ -961,7 +1093,7 @@ __global__ void __launch_bounds__(256 > THREADS ? 256 : THREADS)
 ssm_finish_kernel(SsmLayerPlan p, SsmCall c, int norm_blocks) {
   constexpr int BLOCK = 256 > THREADS ? 256 : THREADS;
   constexpr int kPer = 4;  // vectors of four channels per thread, THREADS * 16 channels at most
-  __shared__ float red[BLOCK / 64];
+  __shared__ double red[BLOCK / 64];
   __shared__ int flag;
   const int tid = threadIdx.x, P = p.head_dim, inner = p.heads * P, gn = p.groups * p.state;
   const int channels = inner + 2 * gn;
@@ -1015,7 +1147,7 @@ ssm_finish_kernel(SsmLayerPlan p, SsmCall c, int norm_blocks) {
   float* y = c.y + (live ? t : 0) * inner + group * width;
   const float* z = c.x + (live ? t : 0) * stride + group * width;
   floatx4 v[kPer];
-  float sum = 0.f;
+  double sum = 0.0;  // (squares leave single precision's range before what is normed does)
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
     const int i = 4 * (l + THREADS * k);
@@ -1026,17 +1158,18 @@ ssm_finish_kernel(SsmLayerPlan p, SsmCall c, int norm_blocks) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[k][e] = yv[e] * silu_f32(zv[e]);
     }
-    sum += (v[k].x * v[k].x + v[k].y * v[k].y) + (v[k].z * v[k].z + v[k].w * v[k].w);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum = fma((double)v[k][e], (double)v[k][e], sum);
   }
-  sum = segment_sum<64>(sum);
+  sum = wave_sum_f64(sum);
   if constexpr (THREADS > 64) {
     if ((tid & 63) == 0) red[tid >> 6] = sum;
     __syncthreads();
-    sum = 0.f;
+    sum = 0.0;
     for (int k = 0; k < THREADS / 64; ++k) sum += red[k];
   }
   if (!live) return;
-  const float scale = 1.f / sqrtf(sum / (float)width + p.epsilon);
+  const float scale = (float)(1.0 / sqrt(sum / (double)width + (double)p.epsilon));
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
     const int i = 4 * (l + THREADS * k);
@@ -1067,7 +1200,7 @@ struct ScanCut {
 constexpr int kScanCus = 256;
 constexpr int kMinSegment = 64;
 static double scan_begin_us(int tiles) { return tiles == 2 ? 6.0 : 5.0; }
-static double scan_chunk_us(int tiles) { return tiles == 2 ? 9.0 : 5.2; }
+static double scan_chunk_us(int tiles) { return tiles == 2 ? 7.6 : 4.4; }
 constexpr double kFirstPassShare = 0.45, kJoinUs = 12.0;
 
 // Segments that the whole segments of a call may number.

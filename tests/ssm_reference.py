@@ -9,6 +9,12 @@ moves a decay e^-c by 8 u c e^-c < 3 u), the sum over the state (N, or N / 2
 with fewer), the sum over a chunk of 32 tokens, one product with a decay per
 chunk and segment, and the skip.  K roundings move it by at most K u of the
 absolute expression (to first order, K u < 1e-3 here).
+
+Near the end of single precision's range a product of the state is off by more
+than u of itself: its operands are at best 2^100 x 2^14 times x dt B / |B|, whose
+f16 parts are multiples of 2^-24, so off by 2^-25, and 2^14 B / |B|, below 2^15.
+The product is off by 2^(-25 + 15 - 114) = 2^-124 (the smallest normal number is
+2^-126): each token adds that to its state.
 """
 import numpy as np
 
@@ -33,6 +39,8 @@ def sequence(layer, x, conv, ssm):
     w = L.conv_weight.astype(np.float64)
     s = ssm.astype(np.float64)
     s_abs = np.abs(s)
+    K = 3 * (W + 8) + N + 32 + T // 16 + 32
+    lost = 2.0 ** -124 / (K * U)
     y, y_abs = np.empty((T, inner)), np.empty((T, inner))
     share = H // G
     a, d = L.a.astype(np.float64), L.d.astype(np.float64)
@@ -50,10 +58,9 @@ def sequence(layer, x, conv, ssm):
         ba = np.repeat(u_abs[inner:inner + G * N].reshape(G, N), share, 0)
         ca = np.repeat(u_abs[inner + G * N:].reshape(G, N), share, 0)
         s = e[:, None, None] * s + (dt[:, None] * xs)[:, :, None] * bs[:, None, :]
-        s_abs = e[:, None, None] * s_abs + (dt[:, None] * xa)[:, :, None] * ba[:, None, :]
+        s_abs = e[:, None, None] * s_abs + (dt[:, None] * xa)[:, :, None] * ba[:, None, :] + lost
         y[t] = ((s * cs[:, None, :]).sum(-1) + d[:, None] * xs).reshape(-1)
         y_abs[t] = ((s_abs * ca[:, None, :]).sum(-1) + np.abs(d)[:, None] * xa).reshape(-1)
-    K = 3 * (W + 8) + N + 32 + T // 16 + 32
     z = _silu(x[:, :inner])
     v, dv = y * z, K * U * y_abs * np.abs(z) + 8 * U * np.abs(y * z)
     vg, dg = v.reshape(T, G, inner // G), dv.reshape(T, G, inner // G)

@@ -356,3 +356,27 @@ def test_refused_on_the_host(hip):
     assert L.llambda_hip_ssm_session_read_state(s.pointer, 0, None, None) == -1
     assert L.llambda_hip_ssm_session_sync(None, None) == -1
     assert L.llambda_hip_ssm_session_create(None, ctypes.byref(ctypes.c_void_p())) == -1
+
+
+@pytest.mark.parametrize("layout", ["hybrid", "wide", "narrow"])
+@pytest.mark.parametrize("x,b,c,state", [(1e-12, 1, 1, 1), (1e6, 1e-6, 1e3, 1e-9), (1e-18, 1e-10, 1e25, 1e-15),
+                                         (1e8, 1e4, 1e-10, 1e15), (1, 1e-30, 1e20, 1)], ids=str)
+def test_magnitudes(hip, layout, x, b, c, state):
+    """Operands are held at powers of two that follow their largest values: of x from chunk to chunk (here by
+    up to 10^12 either way), of B and C from token to token, of the state with its inputs."""
+    rng = np.random.default_rng(21)
+    layer = synthetic_ssm(rng, **LAYOUTS[layout])
+    part = np.repeat([x, b, c], [layer.inner, layer.groups * layer.state, layer.groups * layer.state])
+    layer.conv_weight = (layer.conv_weight * part[:, None]).astype(np.float32)
+    if layer.conv_bias is not None:
+        layer.conv_bias = (layer.conv_bias * part).astype(np.float32)
+    case = Case(layout, [150, 300], 22, layer=layer)
+    case.ssm *= np.float32(state)
+    row = 0
+    while row < case.tokens:
+        case.x[row:row + 40, layer.inner:2 * layer.inner] *= np.float32(10.0 ** rng.integers(-6, 7))
+        row += 40
+    case.device()
+    case.run()
+    case.session.sync()
+    case.check()
