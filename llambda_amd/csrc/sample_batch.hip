@@ -159,7 +159,7 @@ struct RowLds {
 
 // Inclusive prefix sums of T over the block in thread order; *total gets the sum.
 template <typename T>
-__device__ T block_scan(T v, RowLds& l, T* total) {
+__device__ __forceinline__ T block_scan(T v, RowLds& l, T* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   T* part = reinterpret_cast<T*>(l.wave);
   for (int o = 1; o < 64; o <<= 1) {
@@ -181,7 +181,7 @@ __device__ T block_scan(T v, RowLds& l, T* total) {
 
 // The row's highest logit, its chunks' in LDS; false where it has none or a NaN (a chunk with one
 // carries it).
-__device__ bool row_top(RowLds& l, const SampleRows& s, int row, bool bad, float& top) {
+__device__ __forceinline__ bool row_top(RowLds& l, const SampleRows& s, int row, bool bad, float& top) {
   const int tid = threadIdx.x, chunks = (s.n + kBatchChunk - 1) / kBatchChunk;
   const float m = tid < chunks ? s.chunk_max[(int64_t)row * chunks + tid] : -INFINITY;
   const bool nan = m != m;
@@ -195,7 +195,7 @@ __device__ bool row_top(RowLds& l, const SampleRows& s, int row, bool bad, float
   return !any && top > -INFINITY;
 }
 
-__device__ void make_powers(RowLds& l) {
+__device__ __forceinline__ void make_powers(RowLds& l) {
   for (int b = threadIdx.x; b < kBatchBins; b += kRowThreads) l.powers[b] = kMassOne * exp_below(-(double)b / 64);
   __syncthreads();
 }
@@ -220,7 +220,7 @@ __device__ __forceinline__ Weighed weigh(const RowLds& l, float v, float top, do
 
 // Sort list[0, n) in descending order.  Up to one entry a thread: by counting the larger ones (no two
 // are equal), the threads of an entry sharing the count; else by a bitonic network.
-__device__ void sort_list(RowLds& l, int n) {
+__device__ __forceinline__ void sort_list(RowLds& l, int n) {
   if (n <= kRowThreads) {
     int log2g = 0;
     while (log2g < 4 && n <= (kRowThreads >> (log2g + 1))) ++log2g;
@@ -324,7 +324,7 @@ __device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
 }
 
 // A min-p as an integer weight: weights of at least it are kept.
-__device__ __forceinline__ uint64_t least_weight(const RowParams& p) { return (uint64_t)ceil(p.min_p * kMassOne); }
+__device__ __forceinline__ uint64_t least_weight(RowParams p) { return (uint64_t)ceil(p.min_p * kMassOne); }
 
 // ------------------------------------------------------------------ rows without top-k
 
@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_mass_kernel(SampleRows s) 
 
 // The bin that the row's cut falls into and how much lies above it, from its bins: counts with top-k,
 // weights without.
-__device__ void cut_bin(RowLds& l, const SampleRows& s, int row, const RowParams& p, int& bin, uint64_t& above,
+__device__ __forceinline__ void cut_bin(RowLds& l, const SampleRows& s, int row, RowParams p, int& bin, uint64_t& above,
                           uint64_t& need) {
   constexpr int kPer = kBatchBins / kRowThreads;
   const uint64_t* bins = s.bins + (int64_t)row * kBatchBins + threadIdx.x * kPer;
@@ -380,9 +380,14 @@ __device__ void cut_bin(RowLds& l, const SampleRows& s, int row, const RowParams
   need = need > total ? total : need > 0 ? need : 1;
   if (incl >= need && incl - sum < need) {
     uint64_t run = incl - sum;
-    int k = 0;
-    while (run + own[k] < need) run += own[k++];
-    l.result[0] = (uint64_t)(threadIdx.x * kPer + k);
+    int at = 0;
+#pragma unroll
+    for (int k = 0; k + 1 < kPer; ++k)
+      if (at == k && run + own[k] < need) {
+        run += own[k];
+        ++at;
+      }
+    l.result[0] = (uint64_t)(threadIdx.x * kPer + at);
     l.result[1] = run;
   }
   __syncthreads();
@@ -437,7 +442,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_cut_kernel(SampleRows s) {
 // The token of a list of which at most 64 ranks can be kept, by the first wavefront: ranks by
 // counting, then a rank a lane.
 constexpr int kWaveList = 256;
-__device__ void draw_by_wave(RowLds& l, int n, const RowParams& p, float top, int* token) {
+__device__ __forceinline__ void draw_by_wave(RowLds& l, int n, RowParams p, float top, int* token) {
   const int lane = threadIdx.x & 63;
   const int ranks = min(n, p.top_k);
   uint64_t mine[kWaveList / 64];
@@ -485,7 +490,8 @@ __device__ void draw_by_wave(RowLds& l, int n, const RowParams& p, float top, in
 }
 
 // The token by the chunks' kept weights and the lowest entry kept.
-__device__ int draw_from_chunks(RowLds& l, const float* row, int n, const RowParams& p, float top, uint64_t cut) {
+__device__ __forceinline__ int draw_from_chunks(RowLds& l, const float* row, int n, RowParams p, float top,
+                                                uint64_t cut) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int chunks = (n + kBatchChunk - 1) / kBatchChunk;
   const uint64_t least = least_weight(p);
@@ -538,7 +544,8 @@ __device__ int draw_from_chunks(RowLds& l, const float* row, int n, const RowPar
 // What of a sorted list is kept, into the chunks' weights: the first `ranks` whose weights ahead of
 // them do not reach `need`, of at least min-p.  Returns the lowest entry kept by rank and need.
 constexpr int kOwn = kBatchList / kRowThreads;
-__device__ uint64_t keep_from_list(RowLds& l, int n, const RowParams& p, float top, uint64_t above, uint64_t need) {
+__device__ __forceinline__ uint64_t keep_from_list(RowLds& l, int n, RowParams p, float top, uint64_t above,
+                                                   uint64_t need) {
   const int tid = threadIdx.x;
   const uint64_t least = least_weight(p);
   uint64_t own = 0, values[kOwn], total;
@@ -571,7 +578,7 @@ __device__ uint64_t keep_from_list(RowLds& l, int n, const RowParams& p, float t
 // The highest entry e such that the entries >= e reach `need` (their number, or their mass where
 // `by_mass`), among the entries <= limit of the row.  0 where all of them do not.  `reached`: what the
 // entries above e hold.
-__device__ uint64_t row_cut(RowLds& l, const float* row, int n, float top, double t, bool by_mass,
+__device__ __forceinline__ uint64_t row_cut(RowLds& l, const float* row, int n, float top, double t, bool by_mass,
                             uint64_t need, uint64_t floor_entry) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int chunks = (n + kBatchChunk - 1) / kBatchChunk;
@@ -676,7 +683,7 @@ __device__ uint64_t row_cut(RowLds& l, const float* row, int n, float top, doubl
 }
 
 // The token of a row by passes over all of it.
-__device__ int draw_from_row(RowLds& l, const float* row, int n, const RowParams& p, float top) {
+__device__ __forceinline__ int draw_from_row(RowLds& l, const float* row, int n, RowParams p, float top) {
   const int lane = threadIdx.x & 63, chunks = (n + kBatchChunk - 1) / kBatchChunk;
   const double t = p.sharpness;
   uint64_t cut = 0, total;
@@ -710,7 +717,7 @@ __device__ int draw_from_row(RowLds& l, const float* row, int n, const RowParams
 }
 
 // Rows with top-k: the candidates to the list; their number (beyond the list's end: too many).
-__device__ int list_candidates(RowLds& l, const float* row, int n, const RowParams& p, float top) {
+__device__ __forceinline__ int list_candidates(RowLds& l, const float* row, int n, RowParams p, float top) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int chunks = (n + kBatchChunk - 1) / kBatchChunk;
   float bound = -INFINITY;
@@ -752,9 +759,14 @@ __device__ int list_candidates(RowLds& l, const float* row, int n, const RowPara
         }
         int run = above + incl - sum;
         if (run < p.top_k && run + sum >= p.top_k) {
-          int j = 0;
-          while (run + c[j] < p.top_k) run += c[j++];
-          l.result[0] = (uint64_t)(255 - 4 * lane - j);
+          int at = 0;
+#pragma unroll
+          for (int j = 0; j < 3; ++j)
+            if (at == j && run + c[j] < p.top_k) {
+              run += c[j];
+              ++at;
+            }
+          l.result[0] = (uint64_t)(255 - 4 * lane - at);
           l.result[1] = (uint64_t)run;
         }
       }

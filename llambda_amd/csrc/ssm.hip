@@ -1,9 +1,10 @@
 // ssm.hip -- the Mamba-2 mixer's kernels (ssm.h).
 //
 // One token per sequence (ssm_step_kernel): a workgroup per sequence, head and
-// 8192 state elements reads them, applies the recurrence and writes them;
-// bound by the state's traffic.  ssm_finish_kernel then gates and norms the
-// rows and shifts the convolution's state.
+// 8192 or 2048 state elements reads them, applies the recurrence and writes
+// them; bound by the state's traffic (48 sequences of 2 MiB: 44 us, 4.6 TB/s).
+// ssm_finish_kernel then gates and norms the rows and shifts the convolution's
+// state (8192 rows of 4096: 68 us, 5.9 TB/s).
 //
 // Sequences of any lengths: the plan kernel checks the call and cuts the
 // sequences into segments and chunks of Q = 32 tokens; ssm_prepare_kernel
@@ -20,6 +21,17 @@
 // is M's left operand.  Exponents are sums in 64 bits, kept as two floats,
 // and subtracted before exp2 is taken, so a strong decay early in the chunk
 // costs the later tokens no precision.
+// The products are of single precision on the matrix cores' 16-bit operands:
+// C s and the state's, which need only scales that run along a row or column
+// of the product, as two f16 parts and three products; (S o L) X, whose S o L
+// has no such scale at hand, as three bf16 parts and six.  (All in bf16 parts
+// 8192 tokens of 64 heads took 170 us for the scan and 77 for its first pass;
+// so 142 and 67.  fp32 matrix instructions have an eighth of the rate.)
+// Bound by latency: a chunk of 256 channels takes a workgroup 8.5 us, of which
+// the matrix cores work 1.6, the vector units about 2 and the LDS about 1.2;
+// its LDS (124 KB) and registers (232 of 256) leave no room for a second
+// workgroup.  Half as many channels leave it, but two of those take as long
+// (187 us where 128 registers had to do, 171 without).
 // Long sequences of few heads are cut into segments so that the grid fills the
 // device: a first pass forms each segment's own state, a small kernel joins
 // them in order, and the scan proper starts each segment from its state.
@@ -1200,7 +1212,7 @@ struct ScanCut {
 constexpr int kScanCus = 256;
 constexpr int kMinSegment = 64;
 static double scan_begin_us(int tiles) { return tiles == 2 ? 6.0 : 5.0; }
-static double scan_chunk_us(int tiles) { return tiles == 2 ? 7.6 : 4.4; }
+static double scan_chunk_us(int tiles) { return tiles == 2 ? 8.8 : 4.75; }
 constexpr double kFirstPassShare = 0.45, kJoinUs = 12.0;
 
 // Segments that the whole segments of a call may number.
