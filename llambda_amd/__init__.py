@@ -6,7 +6,9 @@ protocol.
 Modules:
   native       ctypes bindings of libllambda_hip.so (the C ABI)
   hip_backend  projection sessions and the :hip backend descriptor
-  moe          routed-MoE layer sessions
+  moe          routed-MoE layer sessions and routers
+  ssm          Mamba-2 mixer sessions
+  sampling     a token from logits, of one row or of a batch
   accelerator  the backend descriptor protocol
   projection   the tensor-indexed binding store with runtime fallback
   ggml         type tags and block geometry

@@ -5,7 +5,7 @@
 //   top-k of at most as many ranks as there are chunks: at least k logits are
 //     at or above the k-th highest chunk maximum, and few more.  The row's
 //     workgroup (sample_finish_kernel) reads the chunks that reach it and lists
-//     those logits in LDS: up to 64 ranks are settled by one wavefront
+//     those logits in LDS: up to 32 ranks are settled by one wavefront
 //   no top-k: the row is shared by as many workgroups as fit.  With top-p
 //     (sample_mass_kernel) its weights are summed by bins of (max - l) / T, 64 to
 //     one; then (sample_cut_kernel) every chunk's weight above the bin that the
@@ -21,6 +21,10 @@
 // with the bins' powers in a table one takes 5 operations in 64 bits and a
 // short series in 32 (off by 1e-9 of it at most, without a bias), a fourth of
 // an exponential in 64 bits, which bound these passes.
+// Rows of 128256 logits (us), launch by launch: maxima 13 for 160 rows (6.3 TB/s),
+// 4 for one; bins 33 and 5, weights above the cut 59 and 10 where all rows have
+// top-p, 25 where all have min-p alone; the finish 28 and 24 with 200 ranks (some
+// 15 barriers of the row's workgroup), 18 and 16 with top-p, 7 with min-p.
 #include "sample_batch.h"
 
 #include <climits>
@@ -439,9 +443,12 @@ __global__ void __launch_bounds__(kRowThreads) sample_cut_kernel(SampleRows s) {
 
 // ------------------------------------------------------------------ the token
 
-// The token of a list of which at most 64 ranks can be kept, by the first wavefront: ranks by
-// counting, then a rank a lane.
-constexpr int kWaveList = 256;
+// Rows of at most so many ranks have their bound found by one wavefront, which draws the token too if no
+// more logits than kWaveList reach it.  160 rows, 16 ranks 10.6 us for the last launch (15.8 by the whole
+// workgroup), 32 13.1 (16.8), 40 23.2 (17.7: the bound's selection leaves its fast path).
+constexpr int kWaveRanks = 32, kWaveList = 256;
+
+// The token of a list by the first wavefront: ranks by counting, then a rank a lane.
 __device__ __forceinline__ void draw_by_wave(RowLds& l, int n, RowParams p, float top, int* token) {
   const int lane = threadIdx.x & 63;
   const int ranks = min(n, p.top_k);
@@ -721,7 +728,7 @@ __device__ __forceinline__ int list_candidates(RowLds& l, const float* row, int 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int chunks = (n + kBatchChunk - 1) / kBatchChunk;
   float bound = -INFINITY;
-  if (p.top_k <= kMoeMaxTopK) {
+  if (p.top_k <= kWaveRanks) {
     if (wave == 0) {
       constexpr int kPer = kBatchMaxChunks / 64;
       float v[kPer];
@@ -813,7 +820,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_finish_kernel(SampleRows s
       for (int i = tid; i < min(n, kBatchList); i += kRowThreads) l.list[i] = s.list[(int64_t)row * kBatchList + i];
       __syncthreads();
     }
-    if (p.top_k <= kMoeMaxTopK && n <= kWaveList) {
+    if (p.top_k <= kWaveRanks && n <= kWaveList) {
       if (tid < 64) draw_by_wave(l, n, p, top, s.tokens + row);
       return;
     }
@@ -871,7 +878,9 @@ hipError_t sample_rows_launch(const SampleRows& s, hipStream_t stream) {
                      dim3(256), 0, stream, s);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  // Workgroups to a row: a CU holds two, and each may find its row to have.
+  // Workgroups to a row: twice what fills the device, for rows with top-k leave theirs idle.  160 rows,
+  // a third of them without top-k, 25 us for the last of these passes, with half as many 32; but where
+  // all have top-p 59 and 43 (each workgroup reads the maxima and makes the powers anew).
   const int shares = max(1, min(1024 / s.rows, (chunks + 15) / 16));
   // (which rows have a top-k or top-p is known on the device only; no array: none has)
   if (s.top_p || s.top_k) e = launch_rows(sample_mass_kernel, dim3(shares, s.rows), s, stream);
