@@ -34,6 +34,7 @@
 namespace llhip {
 
 typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kRowThreads = 1024;
 constexpr double kMassOne = 17592186044416.0;  // 2^44
@@ -229,10 +230,17 @@ __device__ __forceinline__ void sort_list(RowLds& l, int n) {
     int log2g = 0;
     while (log2g < 4 && n <= (kRowThreads >> (log2g + 1))) ++log2g;
     const int g = 1 << log2g, item = threadIdx.x >> log2g, part = threadIdx.x & (g - 1);
+    if (threadIdx.x == 0) l.list[n] = 0;  // entries are read in pairs
+    __syncthreads();
     const uint64_t mine = item < n ? l.list[item] : 0;
     int rank = 0;
-#pragma unroll 8
-    for (int i = part; i < n; i += g) rank += l.list[i] > mine ? 1 : 0;
+    if (item < n) {
+#pragma unroll 4
+      for (int i = 2 * part; i < n; i += 2 * g) {
+        const u64x2 pair = *reinterpret_cast<const u64x2*>(&l.list[i]);
+        rank += (pair.x > mine ? 1 : 0) + (pair.y > mine ? 1 : 0);
+      }
+    }
     for (int o = 1; o < g; o <<= 1) rank += __shfl_xor(rank, o, 64);
     __syncthreads();
     if (item < n && part == 0) l.list[rank] = mine;
