@@ -2117,7 +2117,7 @@ struct llambda_hip_batch_sampler {
   int device = 0;
   hipStream_t stream = nullptr;
   size_t vocab = 0, max_rows = 0;
-  DevBuf chunk_max, chunk_mass, bins, list, listed;
+  DevBuf chunk_max, chunk_mass, bins, list, listed, filled;
   DevBuf logits, params, tokens;  // device staging of the host-pointer runs
   size_t staged = 0;
   // recorded after every call; the next one, which shares the workspace, waits
@@ -2136,6 +2136,7 @@ void batch_sample_enqueue(llambda_hip_batch_sampler* s, SampleRows r, hipStream_
   r.bins = s->bins.as<uint64_t>();
   r.list = s->list.as<uint64_t>();
   r.listed = s->listed.as<int>();
+  r.filled = s->filled.as<float>();
   hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
   HIPC(hipStreamIsCapturing(st, &capture));
   const bool ordered = capture == hipStreamCaptureStatusNone;
@@ -2179,6 +2180,7 @@ int llambda_hip_batch_sampler_create(size_t vocab, size_t max_rows,
     s->bins.alloc(max_rows * kBatchBins * sizeof(uint64_t), "sampling bins");
     s->list.alloc(max_rows * kBatchList * sizeof(uint64_t), "sampling candidates");
     s->listed.alloc(max_rows * sizeof(int), "sampling candidate counts");
+    s->filled.alloc(max_rows * 4 * sizeof(float), "rows of fewer than four logits");
     *result = s.release();
   });
 }
@@ -2199,7 +2201,7 @@ int llambda_hip_batch_sampler_sample_device(llambda_hip_batch_sampler* s, const 
     std::lock_guard<std::mutex> lock(s->run_mutex);
     HIPC(hipSetDevice(s->device));
     SampleRows r{logits, (int)count, (int)rows, a->temperature, a->top_k, a->top_p, a->min_p,
-                 a->random_value, tokens, nullptr, nullptr, nullptr, nullptr, nullptr};
+                 a->random_value, tokens, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
     batch_sample_enqueue(s, r, stream ? static_cast<hipStream_t>(stream) : s->stream);
   });
 }

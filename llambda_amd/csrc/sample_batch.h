@@ -38,9 +38,10 @@ struct SampleRows {
   uint64_t* bins;        // [kBatchBins]
   uint64_t* list;        // [kBatchList]
   int* listed;           // [1]
+  float* filled;         // [4]: a row of fewer logits
 };
 
 inline int sample_chunks(int n) { return (n + kBatchChunk - 1) / kBatchChunk; }
-hipError_t sample_rows_launch(const SampleRows& s, hipStream_t stream);
+hipError_t sample_rows_launch(SampleRows s, hipStream_t stream);
 
 }  // namespace llhip

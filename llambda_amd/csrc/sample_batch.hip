@@ -104,17 +104,35 @@ __device__ __forceinline__ uint64_t entry_of(float l, int i) {
 __device__ __forceinline__ float entry_logit(uint64_t e) { return of_order((uint32_t)(e >> 32)); }
 __device__ __forceinline__ int entry_index(uint64_t e) { return (int)(0xFFFFFFFFu - (uint32_t)e); }
 
-// The chunk's four logits of this lane, -inf past the row.
-__device__ __forceinline__ void load_chunk(const float* row, int n, int chunk, int lane, float (&v)[4]) {
-  const int i = chunk * kBatchChunk + 4 * lane;
-  if (i + 4 <= n) {
-    const f32x4a4 q = *reinterpret_cast<const f32x4a4*>(row + i);
+// The chunk's four logits of this lane.  Rows have four at least; a lane whose
+// four pass the row's end reads its last four, and takes its own from them, with
+// -inf past the row, when they are used: a branch at the load would have it wait
+// for the one before.
+__device__ __forceinline__ f32x4a4 request_chunk(const float* row, int n, int chunk, int lane) {
+  return *reinterpret_cast<const f32x4a4*>(row + min(chunk * kBatchChunk + 4 * lane, n - 4));
+}
+__device__ __forceinline__ void take_chunk(const f32x4a4& q, int n, int chunk, int lane, float (&v)[4]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = q[e];
-  } else {
+  for (int e = 0; e < 4; ++e) v[e] = q[e];
+  if ((chunk + 1) * kBatchChunk <= n) return;
+  const int i = chunk * kBatchChunk + 4 * lane, past = i - min(i, n - 4);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = i + e < n ? row[i + e] : -INFINITY;
+  for (int e = 0; e < 4; ++e) {
+    float own = -INFINITY;
+#pragma unroll
+    for (int f = e; f < 4; ++f) own = f - e == past ? q[f] : own;
+    v[e] = own;
   }
+}
+__device__ __forceinline__ void load_chunk(const float* row, int n, int chunk, int lane, float (&v)[4]) {
+  take_chunk(request_chunk(row, n, chunk, lane), n, chunk, lane, v);
+}
+
+// Rows of fewer than four logits, filled up with -inf.
+__global__ void __launch_bounds__(256) sample_fill_kernel(SampleRows s) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= 4 * s.rows) return;
+  s.filled[i] = (i & 3) < s.n ? s.logits[(int64_t)(i >> 2) * s.n + (i & 3)] : -INFINITY;
 }
 
 constexpr int kChunksPerWave = 4;
@@ -128,18 +146,19 @@ __global__ void __launch_bounds__(256) sample_chunks_kernel(SampleRows s) {
   const int first = (blockIdx.x * 4 + (threadIdx.x >> 6)) * kChunksPerWave;
   if (first >= chunks) return;
   const float* logits = s.logits + (int64_t)row * s.n;
-  float v[kChunksPerWave][4];
+  f32x4a4 q[kChunksPerWave];
 #pragma unroll
-  for (int c = 0; c < kChunksPerWave; ++c)
-    load_chunk(logits, s.n, min(first + c, chunks - 1), lane, v[c]);
+  for (int c = 0; c < kChunksPerWave; ++c) q[c] = request_chunk(logits, s.n, min(first + c, chunks - 1), lane);
 #pragma unroll
   for (int c = 0; c < kChunksPerWave; ++c) {
+    float v[4];
+    take_chunk(q[c], s.n, min(first + c, chunks - 1), lane, v);
     bool nan = false;
     float m = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      nan |= v[c][e] != v[c][e];
-      m = fmaxf(m, v[c][e]);
+      nan |= v[e] != v[e];
+      m = fmaxf(m, v[e]);
     }
     m = wave_max(m);
     nan = __ballot(nan) != 0;
@@ -304,17 +323,21 @@ __device__ __forceinline__ void each_chunk(const float* row, int n, int first, i
     const int mine = c0 + kStep * lane;
     uint64_t todo = __ballot(mine < last && wanted(min(mine, last - 1)));
     while (todo) {
-      float v[kAhead][4];
+      f32x4a4 q[kAhead];
       int c[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
         c[k] = todo ? c0 + kStep * __builtin_ctzll(todo) : -1;
         todo &= todo - 1;
-        if (c[k] >= 0) load_chunk(row, n, c[k], lane, v[k]);
+        q[k] = request_chunk(row, n, c[k] >= 0 ? c[k] : c[0], lane);
       }
 #pragma unroll
       for (int k = 0; k < kAhead; ++k)
-        if (c[k] >= 0) f(c[k], v[k]);
+        if (c[k] >= 0) {
+          float v[4];
+          take_chunk(q[k], n, c[k], lane, v);
+          f(c[k], v);
+        }
     }
   }
 }
@@ -880,7 +903,14 @@ static hipError_t launch_rows(Kernel k, dim3 grid, const SampleRows& s, hipStrea
   return hipGetLastError();
 }
 
-hipError_t sample_rows_launch(const SampleRows& s, hipStream_t stream) {
+hipError_t sample_rows_launch(SampleRows s, hipStream_t stream) {
+  if (s.n < 4) {
+    hipLaunchKernelGGL(sample_fill_kernel, dim3((4 * s.rows + 255) / 256), dim3(256), 0, stream, s);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    s.logits = s.filled;
+    s.n = 4;
+  }
   const int chunks = sample_chunks(s.n);
   hipLaunchKernelGGL(sample_chunks_kernel, dim3((chunks + 4 * kChunksPerWave - 1) / (4 * kChunksPerWave), s.rows),
                      dim3(256), 0, stream, s);
