@@ -23,8 +23,9 @@
 // an exponential in 64 bits, which bound these passes.
 // Rows of 128256 logits (us), launch by launch: maxima 13 for 160 rows (6.3 TB/s),
 // 4 for one; bins 33 and 5, weights above the cut 59 and 10 where all rows have
-// top-p, 25 where all have min-p alone; the finish 28 and 24 with 200 ranks (some
-// 15 barriers of the row's workgroup), 18 and 16 with top-p, 7 with min-p.
+// top-p, 25 where all have min-p alone; the finish 25 and 22 with 200 ranks (of one
+// row's 9 are the reading of 200 chunks: a CU alone gets 20 GB/s from beyond its
+// L2; the bound 2.6, the sort 2.5, the draw 2.6), 17 and 15 with top-p, 7 with min-p.
 #include "sample_batch.h"
 
 #include <climits>
@@ -579,8 +580,8 @@ __device__ __forceinline__ int draw_from_chunks(RowLds& l, const float* row, int
   return l.count;
 }
 
-// What of a sorted list is kept, into the chunks' weights: the first `ranks` whose weights ahead of
-// them do not reach `need`, of at least min-p.  Returns the lowest entry kept by rank and need.
+// What of a sorted list is kept, into the chunks' weights: the first whose weights ahead of them do not
+// reach `need` (0: top-p of the list's total), of at least min-p.  Returns the lowest entry kept by need.
 constexpr int kOwn = kBatchList / kRowThreads;
 __device__ __forceinline__ uint64_t keep_from_list(RowLds& l, int n, RowParams p, float top, uint64_t above,
                                                    uint64_t need) {
@@ -594,6 +595,7 @@ __device__ __forceinline__ uint64_t keep_from_list(RowLds& l, int n, RowParams p
     own += values[k];
   }
   uint64_t run = above + block_scan(own, l, &total) - own;
+  if (need == 0) need = p.top_p < 1.0 ? max((uint64_t)ceil(p.top_p * (double)total), (uint64_t)1) : ~0ull;
   if (tid == 0) l.result[2] = 0;
   __syncthreads();
 #pragma unroll
@@ -860,13 +862,9 @@ __global__ void __launch_bounds__(kRowThreads) sample_finish_kernel(SampleRows s
     if (n <= kBatchList) {
       sort_list(l, n);
       const int ranks = min(n, p.top_k);
-      uint64_t total, sum = 0;
-      for (int i = tid; i < ranks; i += kRowThreads) sum += weigh(l, entry_logit(l.list[i]), top, p.sharpness).weight;
-      block_scan(sum, l, &total);
       for (int c = tid; c < chunks; c += kRowThreads) l.mass[c] = 0;
       __syncthreads();
-      const uint64_t need = p.top_p < 1.0 ? (uint64_t)ceil(p.top_p * (double)total) : ~0ull;
-      const uint64_t cut = keep_from_list(l, ranks, p, top, 0, need > 0 ? need : 1);
+      const uint64_t cut = keep_from_list(l, ranks, p, top, 0, 0);
       token = draw_from_chunks(l, logits, s.n, p, top, cut);
     } else {
       token = draw_from_row(l, logits, s.n, p, top);
