@@ -634,7 +634,7 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
   };
 #pragma unroll
   for (int k = 0; k < TPW; ++k) {
-    held[k] = 127 << 23;
+    held[k] = 227 << 23;  // (of zeros)
     most[k] = 0.f;
     if (!STATES) {
       held[k] = max(scale_bits(state_max(k)), (1 << 23) + k2p14);
