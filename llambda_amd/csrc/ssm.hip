@@ -453,7 +453,7 @@ static int scan_heads(const SsmLayerPlan& p, int tiles) {
   return n;
 }
 
-// LDS of a scan workgroup, in bytes: B and raw rows (two of each in the first
+// LDS of a scan workgroup, in bytes: B, raw rows, decays and scales (two of each in the first
 // pass), C, S, decays, masked products (two), decay tables (two).
 template <int NT, int W, bool STATES>
 struct ScanLds {

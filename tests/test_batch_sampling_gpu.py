@@ -189,6 +189,56 @@ def test_defaults_shorter_rows_streams_and_a_graph(hip):
         assert b.tolist() == [reference(logits[i], r[i], p=0.9) for i in range(rows)]
 
 
+@pytest.mark.parametrize("n", [3, 700])
+def test_many_rows(hip, n):
+    rng = np.random.default_rng(n)
+    rows = 2500
+    s = HipBatchSampler(n, rows)
+    check(s, head_like(rng, rows, n), rng.random(rows).astype(np.float32) * np.float32(0.999999),
+          t=rng.choice([0.0, 0.7, 1.0, 2.0], size=rows).astype(np.float32),
+          k=rng.choice([0, 1, 2, 3, 40], size=rows), p=rng.choice([1.0, 0.9, 0.3], size=rows).astype(np.float32),
+          m=rng.choice([0.0, 0.1], size=rows).astype(np.float32))
+
+
+@pytest.mark.parametrize("n", [2, 20000])
+def test_replays_between_eager_calls_with_every_filter(hip, n):
+    """A captured call and eager ones of the same sampler, in turn."""
+    import torch
+    rng = np.random.default_rng(14)
+    rows = 8
+    s = HipBatchSampler(32768, rows)
+    filters = dict(t=rng.choice([0.5, 1.0, 1.5], size=rows).astype(np.float32),
+                   k=np.array([0, 0, 1, 5, 40, 300, 3000, 0], np.int32),
+                   p=np.array([1, 0.9, 1, 0.9, 0.95, 0.8, 0.9, 0.05], np.float32),
+                   m=np.array([0, 0, 0, 0.1, 0, 0.01, 0, 0], np.float32))
+    d = {k: torch.from_numpy(v).cuda() for k, v in filters.items()}
+    x, u = torch.zeros(rows, n, device="cuda"), torch.zeros(rows, device="cuda")
+    a, b = (torch.zeros(rows, dtype=torch.int32, device="cuda") for _ in range(2))
+    stream = torch.cuda.Stream()
+
+    def call(out, at):
+        s.sample_device(x.data_ptr(), rows, out.data_ptr(), u.data_ptr(), temperature_ptr=d["t"].data_ptr(),
+                        top_k_ptr=d["k"].data_ptr(), top_p_ptr=d["p"].data_ptr(), min_p_ptr=d["m"].data_ptr(),
+                        count=n, stream=at)
+
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream, capture_error_mode="relaxed"):
+        call(a, stream.cuda_stream)
+    for _ in range(4):
+        logits = head_like(rng, rows, n)
+        r = rng.random(rows).astype(np.float32) * np.float32(0.999999)
+        x.copy_(torch.from_numpy(logits))
+        u.copy_(torch.from_numpy(r))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        call(b, 0)
+        torch.cuda.synchronize()
+        want = [reference(logits[i], r[i], *(filters[k][i] for k in "tkpm")) for i in range(rows)]
+        assert a.tolist() == want and b.tolist() == want
+
+
 def test_refusals(sampler):
     x = np.zeros((2, 100), np.float32)
     for kw, text in [(dict(random_value=1.0), "RANDOM-VALUE"), (dict(random_value=[0.5, -0.1]), "Row 1: RANDOM-VALUE"),

@@ -122,6 +122,19 @@ def test_steps(hip, layout, n):
     c.check()
 
 
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+def test_steps_of_many_sequences(hip, layout):
+    """Enough for the larger parts of a state (more than 512 of 8192 elements)."""
+    n = {"hybrid": 11, "one_group": 100, "wide": 37, "narrow": 71, "thin": 180, "odd": 109, "broad_norm": 13}[layout]
+    rng = np.random.default_rng(n)
+    old = rng.permutation(n)
+    old[::5] = -1
+    c = Case(layout, [1] * n, 12, old, n + rng.permutation(n), slots=2 * n).device()
+    c.step()
+    c.session.sync()
+    c.check()
+
+
 def test_steps_in_place_new_and_dropped(hip):
     c = Case("hybrid", [1] * 5, 13, [3, -1, 2, 6, -1], [3, 0, 2, -1, -1], slots=7).device()
     c.step()
@@ -378,5 +391,19 @@ def test_magnitudes(hip, layout, x, b, c, state):
         row += 40
     case.device()
     case.run()
+    case.session.sync()
+    case.check()
+
+
+@pytest.mark.parametrize("run", [True, False])
+def test_outputs_whose_squares_leave_single_precision(hip, run):
+    rng = np.random.default_rng(23)
+    layer = synthetic_ssm(rng, **LAYOUTS["one_group"])
+    layer.d = (layer.d * 1e25).astype(np.float32)
+    case = Case("one_group", [1, 1, 1], 24, layer=layer).device()
+    if run:
+        case.run()
+    else:
+        case.step()
     case.session.sync()
     case.check()
