@@ -2179,7 +2179,7 @@ int llambda_hip_batch_sampler_create(size_t vocab, size_t max_rows,
     s->chunk_mass.alloc(chunks * sizeof(uint64_t), "chunk masses");
     s->bins.alloc(max_rows * kBatchBins * sizeof(uint64_t), "sampling bins");
     s->list.alloc(max_rows * kBatchList * sizeof(uint64_t), "sampling candidates");
-    s->listed.alloc(max_rows * sizeof(int), "sampling candidate counts");
+    s->listed.alloc(max_rows * kBatchCounter * sizeof(int), "sampling candidate counts");
     s->filled.alloc(max_rows * 4 * sizeof(float), "rows of fewer than four logits");
     *result = s.release();
   });
@@ -2201,7 +2201,7 @@ int llambda_hip_batch_sampler_sample_device(llambda_hip_batch_sampler* s, const 
     std::lock_guard<std::mutex> lock(s->run_mutex);
     HIPC(hipSetDevice(s->device));
     SampleRows r{logits, (int)count, (int)rows, a->temperature, a->top_k, a->top_p, a->min_p,
-                 a->random_value, tokens, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
+                 a->random_value, tokens, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 0};
     batch_sample_enqueue(s, r, stream ? static_cast<hipStream_t>(stream) : s->stream);
   });
 }

@@ -19,6 +19,7 @@ namespace llhip {
 constexpr int kBatchChunk = 256;  // logits whose maximum the first launch records
 constexpr int kBatchMaxVocab = 262144;
 constexpr int kBatchMaxChunks = kBatchMaxVocab / kBatchChunk;
+constexpr int kBatchCounter = 64;  // ints from a row's counter to the next: additions to one line wait for each other
 constexpr int kBatchBins = 2048;  // of (max - l) / T, 64 to one
 constexpr int kBatchList = 4096;  // logits of the bin that a cut falls into, or candidates
 
@@ -37,8 +38,9 @@ struct SampleRows {
   uint64_t* chunk_mass;  // [chunks]: weights kept above the cut
   uint64_t* bins;        // [kBatchBins]
   uint64_t* list;        // [kBatchList]
-  int* listed;           // [1]
+  int* listed;           // [kBatchCounter], the first counts
   float* filled;         // [4]: a row of fewer logits
+  int spread;            // set by the launch: few rows, each with many workgroups
 };
 
 inline int sample_chunks(int n) { return (n + kBatchChunk - 1) / kBatchChunk; }

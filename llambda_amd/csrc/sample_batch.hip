@@ -5,7 +5,8 @@
 //   top-k of at most as many ranks as there are chunks: at least k logits are
 //     at or above the k-th highest chunk maximum, and few more.  The row's
 //     workgroup (sample_finish_kernel) reads the chunks that reach it and lists
-//     those logits in LDS: up to 32 ranks are settled by one wavefront
+//     those logits in LDS: up to 32 ranks are settled by one wavefront.  Of few
+//     rows with more ranks several workgroups list them, in the launch before
 //   no top-k: the row is shared by as many workgroups as fit.  With top-p
 //     (sample_mass_kernel) its weights are summed by bins of (max - l) / T, 64 to
 //     one; then (sample_cut_kernel) every chunk's weight above the bin that the
@@ -22,10 +23,10 @@
 // short series in 32 (off by 1e-9 of it at most, without a bias), a fourth of
 // an exponential in 64 bits, which bound these passes.
 // Rows of 128256 logits (us), launch by launch: maxima 13 for 160 rows (6.3 TB/s),
-// 4 for one; bins 33 and 5, weights above the cut 59 and 10 where all rows have
-// top-p, 25 where all have min-p alone; the finish 25 and 22 with 200 ranks (of one
-// row's 9 are the reading of 200 chunks: a CU alone gets 20 GB/s from beyond its
-// L2; the bound 2.6, the sort 2.5, the draw 2.6), 17 and 15 with top-p, 7 with min-p.
+// 3 for one; bins 33 and 6, weights above the cut 44 and 10 where all rows have
+// top-p, 25 where all have min-p alone; the finish 25 with 200 ranks (of one row's
+// then 22, 9 were the reading of 200 chunks, the bound 2.6, the sort 2.5, the draw
+// 2.6; now 8.5 in the launch before and 11), 18 and 15 with top-p, 7 with min-p.
 #include "sample_batch.h"
 
 #include <climits>
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(256) sample_chunks_kernel(SampleRows s) {
   const int chunks = (s.n + kBatchChunk - 1) / kBatchChunk;
   for (int i = blockIdx.x * 256 + threadIdx.x; i < kBatchBins; i += gridDim.x * 256)
     s.bins[(int64_t)row * kBatchBins + i] = 0;
-  if (blockIdx.x == 0 && threadIdx.x == 0) s.listed[row] = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) s.listed[row * kBatchCounter] = 0;
   const int first = (blockIdx.x * 4 + (threadIdx.x >> 6)) * kChunksPerWave;
   if (first >= chunks) return;
   const float* logits = s.logits + (int64_t)row * s.n;
@@ -432,15 +433,89 @@ __device__ __forceinline__ void cut_bin(RowLds& l, const SampleRows& s, int row,
   __syncthreads();
 }
 
+// Rows of at most so many ranks have their bound found by one wavefront, which draws the token too if no
+// more logits than kWaveList reach it.  160 rows, 16 ranks 10.6 us for the last launch (15.8 by the whole
+// workgroup), 32 13.1 (16.8), 40 23.2 (17.7: the bound's selection leaves its fast path).
+constexpr int kWaveRanks = 32, kWaveList = 256;
+
+// Whether the candidates of a row with more ranks are listed by the row's workgroups before the last launch.
+__device__ __forceinline__ bool listed_ahead(const SampleRows& s, RowParams p) { return s.spread && p.top_k > kWaveRanks; }
+
+// A bound that at least `ranks` chunks reach, and few more: the highest chunk maxima by their keys' upper
+// bits, eight at a time.
+__device__ __forceinline__ float ranks_bound(RowLds& l, int chunks, int ranks) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  uint32_t prefix = 0;
+  int above = 0;
+  uint32_t* hist = reinterpret_cast<uint32_t*>(l.bins);
+  const uint32_t key = tid < chunks ? order_of(l.chunk_max[tid]) : 0;
+  for (int shift = 24; shift >= 8; shift -= 8) {
+    for (int i = tid; i < 256; i += kRowThreads) hist[i] = 0;
+    __syncthreads();
+    if (tid < chunks && (shift == 24 || key >> (shift + 8) == prefix)) atomicAdd(&hist[(key >> shift) & 255], 1u);
+    __syncthreads();
+    if (tid < 64) {
+      // four bins a lane, from the top
+      int c[4], sum = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum += c[j] = (int)hist[255 - 4 * lane - j];
+      int incl = sum;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(incl, o, 64);
+        if (lane >= o) incl += u;
+      }
+      int run = above + incl - sum;
+      if (run < ranks && run + sum >= ranks) {
+        int at = 0;
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+          if (at == j && run + c[j] < ranks) {
+            run += c[j];
+            ++at;
+          }
+        l.result[0] = (uint64_t)(255 - 4 * lane - at);
+        l.result[1] = (uint64_t)run;
+      }
+    }
+    __syncthreads();
+    prefix = prefix << 8 | (uint32_t)l.result[0];
+    above = (int)l.result[1];
+    __syncthreads();
+  }
+  const float bound = of_order(prefix << 8);
+  return bound == bound ? bound : -INFINITY;  // (the keys below -inf's)
+}
+
+// The row's logits of at least `bound` in the chunks [first, last) to a list.
+template <typename Counter>
+__device__ __forceinline__ void list_from(const RowLds& l, const float* row, int n, int first, int last, float bound,
+                                          uint64_t* list, Counter* count) {
+  each_chunk(row, n, first, last, [&](int c) { return l.chunk_max[c] >= bound && l.chunk_max[c] > -INFINITY; },
+             [&](int c, const float (&v)[4]) {
+               bool take[4];
+#pragma unroll
+               for (int e = 0; e < 4; ++e) take[e] = v[e] >= bound && v[e] > -INFINITY;
+               append(list, count, take, v, c);
+             });
+}
+
 __global__ void __launch_bounds__(kRowThreads) sample_cut_kernel(SampleRows s) {
   extern __shared__ __align__(16) uint8_t raw[];
   RowLds& l = *reinterpret_cast<RowLds*>(raw);
   const int row = blockIdx.y, lane = threadIdx.x & 63;
   const RowParams p = row_params(s, row);
   const int chunks = (s.n + kBatchChunk - 1) / kBatchChunk;
-  if (p.bad || (p.top_k && p.top_k <= chunks)) return;
+  if (p.bad || (p.top_k && p.top_k <= chunks && !listed_ahead(s, p))) return;
   float top;
   if (!row_top(l, s, row, false, top)) return;
+  if (p.top_k && p.top_k <= chunks) {
+    const float bound = ranks_bound(l, chunks, p.top_k);
+    int first, last;
+    share_of(chunks, first, last);
+    list_from(l, s.logits + (int64_t)row * s.n, s.n, first, last, bound, s.list + (int64_t)row * kBatchList,
+              s.listed + row * kBatchCounter);
+    return;
+  }
   make_powers(l);
   int bin = kBatchBins;  // without top-p all weights lie above the cut
   uint64_t above, need;
@@ -466,7 +541,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_cut_kernel(SampleRows s) {
       take[e] = (p.top_k ? w.bin <= bin : w.bin == bin) && v[e] > -INFINITY;
       if (w.bin < bin && w.weight >= least) held += w.weight;
     }
-    append(s.list + (int64_t)row * kBatchList, s.listed + row, take, v, c);
+    append(s.list + (int64_t)row * kBatchList, s.listed + row * kBatchCounter, take, v, c);
     if (p.top_k) return;
     held = wave_sum_u64(held);
     if (lane == 0) mass[c] = held;
@@ -474,11 +549,6 @@ __global__ void __launch_bounds__(kRowThreads) sample_cut_kernel(SampleRows s) {
 }
 
 // ------------------------------------------------------------------ the token
-
-// Rows of at most so many ranks have their bound found by one wavefront, which draws the token too if no
-// more logits than kWaveList reach it.  160 rows, 16 ranks 10.6 us for the last launch (15.8 by the whole
-// workgroup), 32 13.1 (16.8), 40 23.2 (17.7: the bound's selection leaves its fast path).
-constexpr int kWaveRanks = 32, kWaveList = 256;
 
 // The token of a list by the first wavefront: ranks by counting, then a rank a lane.
 __device__ __forceinline__ void draw_by_wave(RowLds& l, int n, RowParams p, float top, int* token) {
@@ -776,57 +846,11 @@ __device__ __forceinline__ int list_candidates(RowLds& l, const float* row, int 
     __syncthreads();
     bound = __builtin_bit_cast(float, (uint32_t)l.result[0]);
   } else {
-    // the highest chunk maxima by their keys' upper bits, eight at a time: the bound is at most the
-    // k-th's, and close to it
-    uint32_t prefix = 0;
-    int above = 0;
-    uint32_t* hist = reinterpret_cast<uint32_t*>(l.bins);
-    const uint32_t key = tid < chunks ? order_of(l.chunk_max[tid]) : 0;
-    for (int shift = 24; shift >= 8; shift -= 8) {
-      for (int i = tid; i < 256; i += kRowThreads) hist[i] = 0;
-      __syncthreads();
-      if (tid < chunks && (shift == 24 || key >> (shift + 8) == prefix)) atomicAdd(&hist[(key >> shift) & 255], 1u);
-      __syncthreads();
-      if (tid < 64) {
-        // four bins a lane, from the top
-        int c[4], sum = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sum += c[j] = (int)hist[255 - 4 * lane - j];
-        int incl = sum;
-        for (int o = 1; o < 64; o <<= 1) {
-          const int u = __shfl_up(incl, o, 64);
-          if (lane >= o) incl += u;
-        }
-        int run = above + incl - sum;
-        if (run < p.top_k && run + sum >= p.top_k) {
-          int at = 0;
-#pragma unroll
-          for (int j = 0; j < 3; ++j)
-            if (at == j && run + c[j] < p.top_k) {
-              run += c[j];
-              ++at;
-            }
-          l.result[0] = (uint64_t)(255 - 4 * lane - at);
-          l.result[1] = (uint64_t)run;
-        }
-      }
-      __syncthreads();
-      prefix = prefix << 8 | (uint32_t)l.result[0];
-      above = (int)l.result[1];
-      __syncthreads();
-    }
-    bound = of_order(prefix << 8);
-    if (!(bound == bound)) bound = -INFINITY;  // the keys below -inf's
+    bound = ranks_bound(l, chunks, p.top_k);
   }
   if (tid == 0) l.count = 0;
   __syncthreads();
-  each_chunk(row, n, 0, chunks, [&](int c) { return l.chunk_max[c] >= bound && l.chunk_max[c] > -INFINITY; },
-             [&](int c, const float (&v)[4]) {
-               bool take[4];
-#pragma unroll
-               for (int e = 0; e < 4; ++e) take[e] = v[e] >= bound && v[e] > -INFINITY;
-               append(l.list, &l.count, take, v, c);
-             });
+  list_from(l, row, n, 0, chunks, bound, l.list, &l.count);
   __syncthreads();
   return l.count;
 }
@@ -846,10 +870,10 @@ __global__ void __launch_bounds__(kRowThreads) sample_finish_kernel(SampleRows s
   int token;
   if (p.top_k) {
     int n;
-    if (p.top_k <= chunks) {
+    if (p.top_k <= chunks && !listed_ahead(s, p)) {
       n = list_candidates(l, logits, s.n, p, top);
     } else {
-      n = s.listed[row];
+      n = s.listed[row * kBatchCounter];
       for (int i = tid; i < min(n, kBatchList); i += kRowThreads) l.list[i] = s.list[(int64_t)row * kBatchList + i];
       __syncthreads();
     }
@@ -874,7 +898,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_finish_kernel(SampleRows s
     int bin;
     uint64_t above = 0, need = 0;
     if (p.top_p < 1.0) cut_bin(l, s, row, p, bin, above, need);
-    const int n = p.top_p < 1.0 ? s.listed[row] : 0;
+    const int n = p.top_p < 1.0 ? s.listed[row * kBatchCounter] : 0;
     if (n > kBatchList) {
       token = draw_from_row(l, logits, s.n, p, top);
     } else {
@@ -901,6 +925,11 @@ static hipError_t launch_rows(Kernel k, dim3 grid, const SampleRows& s, hipStrea
   return hipGetLastError();
 }
 
+// Rows up to which their workgroups list the candidates of a top-k above kWaveRanks: a CU alone gets 20 GB/s
+// from beyond its L2.  A call with 200 ranks of 128256: one row 23.4 us (29.0 by the row's workgroup), 16
+// rows 27.3 (30.9), 32 36.6 (34.0), 160 52.6 (46.2).
+constexpr int kSpreadRows = 16;
+
 hipError_t sample_rows_launch(SampleRows s, hipStream_t stream) {
   if (s.n < 4) {
     hipLaunchKernelGGL(sample_fill_kernel, dim3((4 * s.rows + 255) / 256), dim3(256), 0, stream, s);
@@ -915,9 +944,10 @@ hipError_t sample_rows_launch(SampleRows s, hipStream_t stream) {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   // Workgroups to a row: twice what fills the device, for rows with top-k leave theirs idle.  160 rows,
-  // a third of them without top-k, 25 us for the last of these passes, with half as many 32; but where
-  // all have top-p 59 and 43 (each workgroup reads the maxima and makes the powers anew).
+  // a third of them without top-k, 16 + 25 us for these passes, with half as many 23 + 32; but where all
+  // have top-p 33 + 44 and 27 + 39 (each workgroup reads the maxima and makes the powers anew).
   const int shares = max(1, min(1024 / s.rows, (chunks + 15) / 16));
+  s.spread = s.rows <= kSpreadRows;
   // (which rows have a top-k or top-p is known on the device only; no array: none has)
   if (s.top_p || s.top_k) e = launch_rows(sample_mass_kernel, dim3(shares, s.rows), s, stream);
   if (e != hipSuccess) return e;
