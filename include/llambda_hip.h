@@ -467,7 +467,9 @@ size_t llambda_hip_ssm_session_input_element_count(const llambda_hip_ssm_session
 size_t llambda_hip_ssm_session_output_element_count(const llambda_hip_ssm_session* session);
 
 /* `tokens` rows of one sequence, host memory, synchronous: continues from the
- * state in `slot` and leaves the new state there. */
+ * state in `slot` and leaves the new state there.  Waits for the session's
+ * earlier run_device calls, whatever stream they ran on; steps on other streams
+ * and replays of graphs that use the slot have to have ended. */
 int llambda_hip_ssm_session_run(llambda_hip_ssm_session* session, int64_t slot,
                                 const float* input, size_t input_element_count, float* output,
                                 size_t output_element_count, size_t tokens);
@@ -487,8 +489,9 @@ int llambda_hip_ssm_session_run(llambda_hip_ssm_session* session, int64_t slot,
  * Enqueued on `stream` (null = the session's stream), not waited for, with no
  * allocation.  The calls of a session share its workspace: each waits on the
  * device for the one before, whatever stream it ran on.  Under stream capture
- * no wait or record is made: the graph orders its own calls, and replays of
- * graphs that hold calls of one session must not overlap. */
+ * no wait or record is made: the graph orders its own calls, and a replay of a
+ * graph that holds calls of a session must not overlap another's, nor the
+ * session's calls outside of graphs. */
 int llambda_hip_ssm_session_run_device(llambda_hip_ssm_session* session, const float* input,
                                        float* output, size_t tokens, const int32_t* offsets,
                                        size_t sequences, const int32_t* from_slots,

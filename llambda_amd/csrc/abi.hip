@@ -1684,7 +1684,7 @@ void ssm_enqueue(llambda_hip_ssm_session* s, const SsmCall& c, hipStream_t st) {
   HIPC(hipStreamIsCapturing(st, &capture));
   const bool ordered = capture == hipStreamCaptureStatusNone;
   if (ordered) HIPC(hipStreamWaitEvent(st, s->done, 0));
-  HIPC(ssm_run_launch(s->plan, c, st));
+  HIPC(c.offsets ? ssm_run_launch(s->plan, c, st) : ssm_step_launch(s->plan, c, st));
   if (ordered) HIPC(hipEventRecord(s->done, st));
 }
 
@@ -1842,11 +1842,7 @@ int llambda_hip_ssm_session_run(llambda_hip_ssm_session* s, int64_t slot, const 
     HIPC(hipMemcpyAsync(s->x.ptr, input, n_in * sizeof(float), hipMemcpyHostToDevice, s->stream));
     const int* dl = s->lists.as<int>();
     SsmCall c{s->x.as<float>(), s->y.as<float>(), (int)tokens, 1, tokens == 1 ? nullptr : dl, dl + 2, dl + 2};
-    if (tokens == 1) {
-      HIPC(ssm_step_launch(s->plan, c, s->stream));
-    } else {
-      ssm_enqueue(s, c, s->stream);
-    }
+    ssm_enqueue(s, c, s->stream);  // behind the session's calls in flight, which may use the slot
     HIPC(hipMemcpyAsync(output, s->y.ptr, n_out * sizeof(float), hipMemcpyDeviceToHost, s->stream));
     HIPC(hipStreamSynchronize(s->stream));
   });

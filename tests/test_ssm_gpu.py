@@ -321,6 +321,31 @@ def test_calls_on_several_streams_share_the_workspace(hip):
         assert torch.equal(out, outs[0])
 
 
+@pytest.mark.parametrize("rows", [1, 2])
+def test_host_runs_wait_for_device_calls_in_flight(hip, rows):
+    """Prompts of a slot on a stream of the caller's, at once followed by a host run of the same slot."""
+    import torch
+    c = Case("hybrid", [2000], 34).device()
+    more = np.random.default_rng(35).normal(size=(rows, c.layer.row)).astype(np.float32)
+    stream = torch.cuda.Stream()
+
+    def outcome(wait):
+        c.dconv.copy_(torch.from_numpy(c.conv))
+        c.dssm.copy_(torch.from_numpy(c.ssm))
+        torch.cuda.synchronize()
+        for _ in range(8):
+            c.run(stream.cuda_stream)
+        if wait:
+            torch.cuda.synchronize()
+        y = c.session.run(more)
+        torch.cuda.synchronize()
+        c.session.sync()
+        return [y, *c.session.read_state(0)]
+
+    for a, b in zip(outcome(True), outcome(False)):
+        assert np.array_equal(a, b)
+
+
 def test_host_runs_and_states(hip):
     rng = np.random.default_rng(31)
     layer = synthetic_ssm(rng, **LAYOUTS["one_group"])
