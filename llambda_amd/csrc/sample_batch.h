@@ -12,6 +12,7 @@
 #pragma once
 
 #include "common.h"
+#include "sample_weight.h"
 
 namespace llhip {
 
@@ -20,7 +21,6 @@ constexpr int kBatchChunk = 256;  // logits whose maximum the first launch recor
 constexpr int kBatchMaxVocab = 262144;
 constexpr int kBatchMaxChunks = kBatchMaxVocab / kBatchChunk;
 constexpr int kBatchCounter = 64;  // ints from a row's counter to the next: additions to one line wait for each other
-constexpr int kBatchBins = 2048;  // of (max - l) / T, 64 to one
 constexpr int kBatchList = 4096;  // logits of the bin that a cut falls into, or candidates
 
 struct SampleRows {

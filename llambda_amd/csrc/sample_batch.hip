@@ -39,7 +39,6 @@ typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kRowThreads = 1024;
-constexpr double kMassOne = 17592186044416.0;  // 2^44
 
 // The parameters of a row.
 struct RowParams {
@@ -226,24 +225,6 @@ __device__ __forceinline__ void make_powers(RowLds& l) {
   __syncthreads();
 }
 
-// A logit's bin, ascending as the logit falls (the last takes the rest, whose weights round to
-// nothing), and its weight as an integer: the bin's power times e^-f, f < 1 / 64.
-struct Weighed {
-  int bin;
-  uint64_t weight;
-};
-__device__ __forceinline__ Weighed weigh(const RowLds& l, float v, float top, double sharpness) {
-  const double t = v == top ? 0.0 : ((double)top - (double)v) * (64.0 * sharpness);
-  if (!(t < (double)(kBatchBins - 1))) return Weighed{kBatchBins - 1, 0};
-  const int b = (int)t;
-  const float f = (float)(t - (double)b) * (1.f / 64);
-  const float g = f * (1.f - f * (0.5f - f * (1.f / 6 - f * (1.f / 24 - f * (1.f / 120)))));  // 1 - e^-f
-  const double w = l.powers[b];
-  // (the integer is the low bits of the sum with 2^52)
-  const uint64_t bits = __builtin_bit_cast(uint64_t, fma(w, -(double)g, w) + 4503599627370496.0);
-  return Weighed{b, bits & 0xFFFFFFFFFFFFFull};
-}
-
 // Sort list[0, n) in descending order.  Up to one entry a thread: by counting the larger ones (no two
 // are equal), the threads of an entry sharing the count; else by a bitonic network.
 __device__ __forceinline__ void sort_list(RowLds& l, int n) {
@@ -389,7 +370,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_mass_kernel(SampleRows s) 
              [&](int, const float (&v)[4]) {
 #pragma unroll
                for (int e = 0; e < 4; ++e) {
-                 const Weighed w = weigh(l, v[e], top, p.sharpness);
+                 const Weighed w = weigh(l.powers, v[e], top, p.sharpness);
                  const uint64_t count = p.top_k ? (v[e] > -INFINITY ? 1 : 0) : w.weight;
                  if (count) atomicAdd((unsigned long long*)&l.bins[w.bin], (unsigned long long)count);
                }
@@ -527,7 +508,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_cut_kernel(SampleRows s) {
   uint64_t* mass = s.chunk_mass + (int64_t)row * chunks;
   // chunks that hold nothing above the cut or in its bin, or nothing that min-p keeps
   auto wanted = [&](int c) {
-    const Weighed w = weigh(l, l.chunk_max[c], top, p.sharpness);
+    const Weighed w = weigh(l.powers, l.chunk_max[c], top, p.sharpness);
     return l.chunk_max[c] > -INFINITY && w.bin <= bin && w.weight >= least;
   };
   for (int c = first + threadIdx.x; c < last; c += kRowThreads)
@@ -537,7 +518,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_cut_kernel(SampleRows s) {
     bool take[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const Weighed w = weigh(l, v[e], top, p.sharpness);
+      const Weighed w = weigh(l.powers, v[e], top, p.sharpness);
       take[e] = (p.top_k ? w.bin <= bin : w.bin == bin) && v[e] > -INFINITY;
       if (w.bin < bin && w.weight >= least) held += w.weight;
     }
@@ -629,7 +610,7 @@ __device__ __forceinline__ int draw_from_chunks(RowLds& l, const float* row, int
     for (int e = 0; e < 4; ++e) {
       own[e] = 0;
       if (v[e] > -INFINITY && entry_of(v[e], chunk * kBatchChunk + 4 * lane + e) >= cut) {
-        const uint64_t w = weigh(l, v[e], top, p.sharpness).weight;
+        const uint64_t w = weigh(l.powers, v[e], top, p.sharpness).weight;
         own[e] = w >= least ? w : 0;
       }
       sum += own[e];
@@ -661,7 +642,7 @@ __device__ __forceinline__ uint64_t keep_from_list(RowLds& l, int n, RowParams p
 #pragma unroll
   for (int k = 0; k < kOwn; ++k) {
     const int i = tid * kOwn + k;
-    values[k] = i < n ? weigh(l, entry_logit(l.list[i]), top, p.sharpness).weight : 0;
+    values[k] = i < n ? weigh(l.powers, entry_logit(l.list[i]), top, p.sharpness).weight : 0;
     own += values[k];
   }
   uint64_t run = above + block_scan(own, l, &total) - own;
@@ -702,7 +683,7 @@ __device__ __forceinline__ uint64_t row_cut(RowLds& l, const float* row, int n, 
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (v[e] > -INFINITY && entry_of(v[e], c * kBatchChunk + 4 * lane + e) >= floor_entry) {
-        const Weighed w = weigh(l, v[e], top, t);
+        const Weighed w = weigh(l.powers, v[e], top, t);
         atomicAdd((unsigned long long*)&bins[w.bin], (unsigned long long)value(w));
       }
   }
@@ -733,7 +714,7 @@ __device__ __forceinline__ uint64_t row_cut(RowLds& l, const float* row, int n, 
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       take[e] = v[e] > -INFINITY && entry_of(v[e], c * kBatchChunk + 4 * lane + e) >= floor_entry &&
-                weigh(l, v[e], top, t).bin == bin;
+                weigh(l.powers, v[e], top, t).bin == bin;
     append(l.list, &l.count, take, v, c);
   }
   __syncthreads();
@@ -745,7 +726,7 @@ __device__ __forceinline__ uint64_t row_cut(RowLds& l, const float* row, int n, 
 #pragma unroll
     for (int k = 0; k < kOwn; ++k) {
       const int i = tid * kOwn + k;
-      values[k] = i < listed ? value(weigh(l, entry_logit(l.list[i]), top, t)) : 0;
+      values[k] = i < listed ? value(weigh(l.powers, entry_logit(l.list[i]), top, t)) : 0;
       own += values[k];
     }
     uint64_t run = above + block_scan(own, l, &total) - own;
@@ -772,7 +753,7 @@ __device__ __forceinline__ uint64_t row_cut(RowLds& l, const float* row, int n, 
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint64_t x = entry_of(v[e], c * kBatchChunk + 4 * lane + e);
-        const Weighed w = weigh(l, v[e], top, t);
+        const Weighed w = weigh(l.powers, v[e], top, t);
         if (v[e] > -INFINITY && x >= floor_entry && w.bin == bin && (shift == 56 || x >> (shift + 8) == prefix))
           atomicAdd((unsigned long long*)&bins[(x >> shift) & 255], (unsigned long long)value(w));
       }
@@ -802,7 +783,7 @@ __device__ __forceinline__ int draw_from_row(RowLds& l, const float* row, int n,
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (v[e] > -INFINITY && entry_of(v[e], c * kBatchChunk + 4 * lane + e) >= cut) {
-        const uint64_t w = weigh(l, v[e], top, t).weight;
+        const uint64_t w = weigh(l.powers, v[e], top, t).weight;
         sum += w >= least ? w : 0;
       }
     return sum;
