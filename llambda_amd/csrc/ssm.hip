@@ -619,7 +619,7 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
       st[k][n] = src && on[k] && n < NT ? *reinterpret_cast<const floatx4*>(src + (int64_t)at_ch * N + 16 * n + 4 * g)
                                         : floatx4{0.f, 0.f, 0.f, 0.f};
   }
-  float total_hi[TPW] = {}, total_lo[TPW] = {};
+  double total[TPW] = {};
   // The state is held times a power of two per column, which changes with the
   // inputs (below); `most` bounds it there.
   int held[TPW];
@@ -711,13 +711,13 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
     }
   };
 
-  // the first pass: log2 of the decay over the chunks so far
+  // the first pass: log2 of the decay over the chunks so far (in 64 bits: a segment may have hundreds,
+  // and sums of single precision would round at each)
   auto add_total = [&](int from) {
 #pragma unroll
     for (int k = 0; k < TPW; ++k) {
       const float* d = decays_at(from) + head[k] * 3 * Q;
-      total_hi[k] += d[2 * Q - 1];
-      total_lo[k] += d[3 * Q - 1];
+      total[k] += (double)d[2 * Q - 1] + (double)d[3 * Q - 1];
     }
   };
 
@@ -974,7 +974,7 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
     for (int n = 0; n < NT; ++n)
       *reinterpret_cast<floatx4*>(dst + (int64_t)at_ch * N + 16 * n + 4 * g) = st[k][n] * power(reciprocal_bits(held[k]));
     if (STATES && g == 0 && ch[k] % p.head_dim == 0)
-      p.seg_decay[(int64_t)(s.state0 + at.y) * p.heads + h0 + head[k]] = total_hi[k] + total_lo[k];
+      p.seg_decay[(int64_t)(s.state0 + at.y) * p.heads + h0 + head[k]] = (float)total[k];
   }
 }
 

@@ -9,6 +9,7 @@ import ssm_reference
 from llambda_amd import native
 from llambda_amd.hip_backend import HipBackendError
 from llambda_amd.ssm import HipSsmSession, synthetic_ssm
+from ssm_reference import U
 
 pytestmark = pytest.mark.gpu
 
@@ -173,6 +174,33 @@ def test_long_sequence_of_many_segments(hip):
     c.run()
     c.session.sync()
     c.check()
+
+
+def test_decays_of_long_segments(hip):
+    """A state that only decays, by about 2^-100 over each of two segments of 64 chunks (512 narrow heads are
+    128 workgroups to a segment).  Steps of 32 have a softplus that is exact, so the decay is 2^(32 a log2 e)
+    a token.  Over the second segment each chunk multiplies by an exponential (off by 2^-23 of itself, and by
+    2^-25 ln 2 for its argument of less than 2) and rounds: 3.4 2^-24 a chunk.  Over the first there is one,
+    of a sum that is rounded once: 2^-25 of 128, times ln 2, and 3 2^-24."""
+    import torch
+    heads, tokens = 512, 4096
+    rng = np.random.default_rng(36)
+    layer = synthetic_ssm(rng, heads=heads, head_dim=16, groups=1, state=16, conv_bias=False)
+    layer.dt_bias[:] = 32
+    layer.a = (-rng.uniform(80, 100, size=heads) * np.log(2) / (32 * 2048)).astype(np.float32)
+    conv = torch.zeros(1, 3, layer.channels, device="cuda")
+    start = (rng.uniform(1, 2, size=(1, heads, 16, 16)) * 2.0 ** 120).astype(np.float32)
+    ssm = torch.from_numpy(start).cuda()
+    x, y = torch.zeros(tokens, layer.row, device="cuda"), torch.empty(tokens, layer.inner, device="cuda")
+    offsets = torch.tensor([0, tokens], dtype=torch.int32, device="cuda")
+    session = HipSsmSession(layer, max_tokens=tokens, conv_states_ptr=conv.data_ptr(), ssm_states_ptr=ssm.data_ptr())
+    torch.cuda.synchronize()
+    session.run_device(x.data_ptr(), y.data_ptr(), tokens, offsets.data_ptr(), 1)
+    session.sync()
+    want = start.astype(np.float64) * np.exp(tokens * 32 * layer.a.astype(np.float64))[None, :, None, None]
+    off = np.abs(ssm.cpu().numpy() / want - 1).max()
+    assert off <= 64 * 3.4 * U + 128 * U / 2 * np.log(2) + 3 * U
+    assert not y.cpu().numpy().any() and not conv.cpu().numpy().any()
 
 
 def test_misaligned_rows_and_buffers(hip):
