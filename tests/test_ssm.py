@@ -6,6 +6,7 @@ import dataclasses
 import numpy as np
 import pytest
 
+import ssm_reference
 from llambda_amd import ggml, native, projection
 from llambda_amd.hip_backend import HipBackendError
 from llambda_amd.ssm import HipSsmSession, ssm_layer_from_model, synthetic_ssm
@@ -89,3 +90,30 @@ def test_layer_from_model():
         ssm_layer_from_model(projection.ProjectionModel(tensors, layer_count=4), 3, heads=5, groups=2)
     with pytest.raises(KeyError, match="ssm_conv1d.weight"):
         ssm_layer_from_model(projection.ProjectionModel(tensors[1:], layer_count=4), 3, heads=4, groups=2)
+
+
+@pytest.mark.parametrize("names", ["xBCs", "x", "B", "C", "s"])
+@pytest.mark.parametrize("kw", [dict(heads=4, head_dim=64, groups=2, state=128), dict(heads=4, head_dim=32, state=16),
+                                dict(heads=2, head_dim=128, groups=1, state=256)], ids=str)
+def test_operands_of_half_the_digits_are_seen(kw, names):
+    """An operand of 16 bits leaves what a call's outputs may differ by together."""
+    rng = np.random.default_rng(7)
+    layer = _layer(**kw)
+    x = rng.normal(size=(129, layer.row)).astype(np.float32)
+    conv = rng.normal(size=(layer.conv_width - 1, layer.channels)).astype(np.float32)
+    ssm = rng.normal(size=(layer.heads, layer.head_dim, layer.state)).astype(np.float32)
+
+    def rounded(bits):
+        def operand(name, v):
+            if name not in names:
+                return v
+            m, e = np.frexp(v)
+            return np.ldexp(np.round(m * 2.0 ** bits), e - bits)
+        return operand
+
+    want = ssm_reference.sequence(layer, x, conv, ssm)
+    few, all_ = (ssm_reference.sequence(layer, x, conv, ssm, rounded(bits)) for bits in (16, 24))
+    assert ssm_reference.together(few[0], want[0]) > ssm_reference.TOGETHER
+    assert ssm_reference.together(all_[0], want[0]) < ssm_reference.TOGETHER / 4
+    if "x" in names or "B" in names:
+        assert ssm_reference.together(few[2], want[2]) > ssm_reference.TOGETHER

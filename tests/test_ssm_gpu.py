@@ -114,6 +114,26 @@ def test_prompts(hip, layout, lengths):
 
 
 @pytest.mark.parametrize("layout", list(LAYOUTS))
+@pytest.mark.parametrize("lengths", [[1] * 9, [40, 260]], ids=str)
+@pytest.mark.parametrize("fresh", [False, True])
+def test_errors_together(hip, layout, lengths, fresh):
+    """All outputs and all states together differ by single precision's roundings, not by a product's of fewer bits."""
+    n = len(lengths)
+    c = Case(layout, lengths, 37, np.full(n, -1) if fresh else np.arange(n), n + np.arange(n), slots=2 * n).device()
+    if max(lengths) > 1:
+        c.run()
+    else:
+        c.step()
+    c.session.sync()
+    want = c.reference()
+    y, ssm = c.dy.cpu().numpy().astype(np.float64), c.dssm.cpu().numpy().astype(np.float64)
+    off = ssm_reference.together(y, np.concatenate([w[0] for w in want]))
+    state_off = ssm_reference.together(ssm[n:], np.stack([w[2] for w in want]))
+    print(f"{layout} {lengths}: outputs {off:.2e}, states {state_off:.2e}")
+    assert off <= ssm_reference.TOGETHER and state_off <= ssm_reference.TOGETHER
+
+
+@pytest.mark.parametrize("layout", list(LAYOUTS))
 @pytest.mark.parametrize("n", [1, 7])
 def test_steps(hip, layout, n):
     rng = np.random.default_rng(n)
