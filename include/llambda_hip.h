@@ -268,6 +268,10 @@ enum {
  *   the top_k highest c among them, lower index first among equals
  *   weights: s of those, over their sum when weights_norm (and the sum is
  *   positive), times weights_scale
+ * Scores may round to the same number in 64 bits (sigmoids of logits from about
+ * 37 on are 1, softmax scores some 745 below the highest are 0): without a bias
+ * and groups such experts rank by their logits, as the unrounded scores do; with
+ * a bias, be it of zeros, or groups they are equals, lower index first.
  * NaN logits and logits <= -FLT_MAX are never chosen and add nothing to a
  * softmax; places left unfilled hold (-1, 0). */
 typedef struct llambda_hip_router_desc {

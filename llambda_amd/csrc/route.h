@@ -15,6 +15,8 @@ constexpr int kRouteMaxGroups = 64;
 //   highest c; the top_groups highest groups stay (all where groups is 1)
 //   the top_k highest c of those are taken, lower index first among equals
 //   w = s of the taken, divided by their sum where `norm`, times scale
+// (without a bias and with one group the order is the logits', which also
+// tells apart scores that round to the same number)
 // NaN and l <= -FLT_MAX are never taken and add nothing to a softmax; places
 // that stay unfilled hold (-1, 0).
 struct RouteSpec {

@@ -112,6 +112,25 @@ def test_masked_equal_and_infinite_logits(hip, groups, bias, score):
     check(Routing(E, 6, score=score, bias=b, groups=groups, top_groups=max(1, groups // 2), group_rank=2), logits)
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_scores_that_round_to_the_same_number(hip, score):
+    """Without a bias and groups they rank by their logits, else they are equals."""
+    rng = np.random.default_rng(13)
+    logits = rng.normal(size=(3, 64)).astype(np.float32)
+    logits[0, [5, 9, 40, 41]] = [40, 50, 60, 45]     # sigmoids of 1
+    logits[1] = -2000 - rng.permutation(64)          # softmax scores of 0 beside the highest's 1
+    logits[1, 33] = 0
+    logits[2] = rng.permutation(64) - 900            # sigmoids of 0
+    plain, zeros = Routing(64, 4, score=score), Routing(64, 4, score=score, bias=np.zeros(64, np.float32))
+    for r in (plain, zeros, Routing(64, 4, score=score, groups=4, top_groups=4)):
+        check(r, logits)
+    row = 0 if score == "sigmoid" else 1
+    by_logit = np.argsort(-logits[row], kind="stable")[:4]
+    assert HipRouter(plain).run(logits)[0][row].tolist() == by_logit.tolist()
+    first = [5, 9, 40, 41] if score == "sigmoid" else [33, 0, 1, 2]
+    assert HipRouter(zeros).run(logits)[0][row].tolist() == first
+
+
 def test_biases_that_are_not_finite(hip):
     rng = np.random.default_rng(6)
     logits = rng.normal(size=(4, 96)).astype(np.float32)
