@@ -264,7 +264,7 @@ enum {
  * the sums, llambda.lisp:5892-5913).  Per token, in 64 bits, with logits l:
  *   s = softmax(l) or sigmoid(l);  c = s + bias
  *   a group, expert_count / groups neighbours, scores the sum of its
- *   group_rank highest c; the experts of the top_groups highest groups stay
+ *   group_rank highest c (+inf if one is +inf); the experts of the top_groups highest groups stay
  *   the top_k highest c among them, lower index first among equals
  *   weights: s of those, over their sum when weights_norm (and the sum is
  *   positive), times weights_scale
@@ -281,7 +281,8 @@ typedef struct llambda_hip_router_desc {
   int64_t groups;             /* 1..64, divides expert_count; 1 = no groups */
   int64_t top_groups;
   int64_t group_rank;         /* 1 or 2 */
-  const float* bias;          /* host, [expert_count], NULL = none; copied */
+  const float* bias;          /* host, [expert_count], NULL = none; copied.  +inf: before all
+                                 others, -inf: behind them, NaN: never chosen */
   int weights_norm;
   float weights_scale;
 } llambda_hip_router_desc;

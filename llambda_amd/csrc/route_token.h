@@ -204,7 +204,9 @@ __device__ __forceinline__ RouteRank route_token(const RouteSpec& p, const float
         b = low > high ? low : high;
       }
       double score = -INFINITY;
-      if (a != kNoKey) score = of_key(a) + (p.group_rank > 1 && b != kNoKey ? of_key(b) : 0.0);
+      if (a != kNoKey) score = of_key(a);
+      // (beside -inf, +inf stays: their sum would be NaN, which ranks nowhere)
+      if (p.group_rank > 1 && a != kNoKey && b != kNoKey && score < INFINITY) score += of_key(b);
       const bool leader = g < p.groups && lane == g * lanes;
       if (leader) s.group[g] = score;
       __builtin_amdgcn_wave_barrier();

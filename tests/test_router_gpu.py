@@ -141,6 +141,28 @@ def test_biases_that_are_not_finite(hip):
     check(Routing(96, 5, score="sigmoid", bias=bias), logits)
 
 
+@pytest.mark.parametrize("experts,groups", [(96, 8), (1024, 16)])
+def test_infinite_biases_in_groups(hip, experts, groups):
+    """A group that holds +inf and -inf is as one that holds +inf; no more groups open than top_groups."""
+    rng = np.random.default_rng(15)
+    size = experts // groups
+    logits = rng.normal(size=(5, experts)).astype(np.float32)
+    bias = np.full(experts, -np.inf, np.float32)
+    bias[2 * size:] = 0
+    bias[size + 3] = np.inf  # the second group: one of +inf, the others of -inf
+    r = Routing(experts, 6, score="sigmoid", bias=bias, groups=groups, top_groups=2, group_rank=2)
+    idx, w = HipRouter(r).run(logits)
+    s = 1 / (1 + np.exp(-logits.astype(np.float64)))
+    for t in range(len(logits)):
+        rank = np.sort(s[t].reshape(groups, size), axis=1)[:, -2:].sum(1)
+        g = 2 + int(rank[2:].argmax())
+        best = g * size + np.argsort(-s[t, g * size:(g + 1) * size], kind="stable")[:5]
+        want = [size + 3, *best]
+        assert idx[t].tolist() == want
+        share = s[t, want] / s[t, want].sum()
+        assert np.all(np.abs(w[t] - share) <= 2.0 ** -23 * share)
+
+
 def test_scores_that_underflow(hip):
     """Weights whose sum is zero stay as they are (zeros)."""
     logits = np.full((2, 64), -1e30, np.float32)
