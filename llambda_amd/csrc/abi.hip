@@ -1679,7 +1679,15 @@ void check_ssm_call(const llambda_hip_ssm_session* s, const char* what, const fl
     failf("%s: input and output overlap", what);
 }
 
+// Before anything of a call is enqueued: a launch that failed behind others would leave half of it done.
+void check_ssm_grids(const llambda_hip_ssm_session* s, const SsmCall& c) {
+  if (!ssm_call_fits(s->plan, c))
+    failf("ssm: %d tokens of %d sequences are too many for one call of a layer of %d heads in %d groups", c.tokens,
+          c.sequences, s->plan.heads, s->plan.groups);
+}
+
 void ssm_enqueue(llambda_hip_ssm_session* s, const SsmCall& c, hipStream_t st) {
+  check_ssm_grids(s, c);
   hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
   HIPC(hipStreamIsCapturing(st, &capture));
   const bool ordered = capture == hipStreamCaptureStatusNone;
@@ -1873,6 +1881,7 @@ int llambda_hip_ssm_session_step_device(llambda_hip_ssm_session* s, const float*
     std::lock_guard<std::mutex> lock(s->run_mutex);
     HIPC(hipSetDevice(s->device));
     SsmCall c{input, output, (int)sequences, (int)sequences, nullptr, from_slots, to_slots};
+    check_ssm_grids(s, c);
     HIPC(ssm_step_launch(s->plan, c, stream ? static_cast<hipStream_t>(stream) : s->stream));
   });
 }

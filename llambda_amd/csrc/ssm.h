@@ -84,7 +84,9 @@ int64_t ssm_max_segments(const SsmLayerPlan& p, int64_t tokens, int64_t sequence
 size_t ssm_image_bytes(int state);
 int64_t ssm_max_states(const SsmLayerPlan& p, int64_t tokens);
 
-// Enqueue a call on `stream`: one token of each sequence where offsets is
+// Whether a call's launches have grids that exist.
+bool ssm_call_fits(const SsmLayerPlan& p, const SsmCall& c);
+// Enqueue a call (one that fits) on `stream`: one token of each sequence where offsets is
 // null, else sequences of any lengths.
 hipError_t ssm_step_launch(const SsmLayerPlan& p, const SsmCall& c, hipStream_t stream);
 hipError_t ssm_run_launch(const SsmLayerPlan& p, const SsmCall& c, hipStream_t stream);

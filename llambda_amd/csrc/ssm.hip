@@ -1269,24 +1269,33 @@ static hipError_t launch(Kernel k, dim3 grid, dim3 block, size_t lds, hipStream_
   return hipGetLastError();
 }
 
-static hipError_t finish_launch(const SsmLayerPlan& p, const SsmCall& c, hipStream_t s) {
+// The last launch: threads to a row, and to a block; blocks that norm rows, and all.
+struct FinishGrid {
+  int threads, block;
+  int64_t norm, all;
+};
+static FinishGrid finish_grid(const SsmLayerPlan& p, const SsmCall& c) {
   const int inner = p.heads * p.head_dim, channels = inner + 2 * p.groups * p.state;
   const int width = inner / p.groups;
-  const int64_t items = (int64_t)c.tokens * p.groups;
-  auto blocks = [&](int block, int per_block) {
-    const int64_t norm = (items + per_block - 1) / per_block;
-    return std::pair<int, dim3>((int)norm, dim3((uint32_t)(norm + (int64_t)c.sequences * ((channels + block - 1) / block))));
-  };
+  FinishGrid g{256, 256, (int64_t)c.tokens * p.groups, 0};
   if (width <= 1024 && c.offsets) {  // a row's refusal is the block's where a row is a sequence
-    const auto b = blocks(256, 4);
-    return launch(ssm_finish_kernel<64>, b.second, dim3(256), 0, s, p, c, b.first);
+    g.threads = 64;
+    g.norm = (g.norm + 3) / 4;
+  } else if (width > 4096) {
+    g.threads = g.block = 1024;
   }
-  if (width <= 4096) {
-    const auto b = blocks(256, 1);
-    return launch(ssm_finish_kernel<256>, b.second, dim3(256), 0, s, p, c, b.first);
+  g.all = g.norm + (int64_t)c.sequences * ((channels + g.block - 1) / g.block);
+  return g;
+}
+
+static hipError_t finish_launch(const SsmLayerPlan& p, const SsmCall& c, hipStream_t s) {
+  const FinishGrid g = finish_grid(p, c);
+  const dim3 grid((uint32_t)g.all), block(g.block);
+  switch (g.threads) {
+    case 64: return launch(ssm_finish_kernel<64>, grid, block, 0, s, p, c, (int)g.norm);
+    case 256: return launch(ssm_finish_kernel<256>, grid, block, 0, s, p, c, (int)g.norm);
+    default: return launch(ssm_finish_kernel<1024>, grid, block, 0, s, p, c, (int)g.norm);
   }
-  const auto b = blocks(1024, 1);
-  return launch(ssm_finish_kernel<1024>, b.second, dim3(1024), 0, s, p, c, b.first);
 }
 
 template <int ELEMENTS>
@@ -1312,11 +1321,23 @@ hipError_t ssm_step_launch(const SsmLayerPlan& p, const SsmCall& c, hipStream_t 
   return finish_launch(p, c, s);
 }
 
+static int64_t scan_blocks(const SsmLayerPlan& p, const SsmCall& c, ScanCut cut) {
+  return (int64_t)(c.tokens / cut.segment_tokens + c.sequences) * (p.heads / scan_heads(p, cut.tiles));
+}
+
+// A launch has fewer than 2^32 threads.  (The most blocks of any cut come from the shortest segments and one tile
+// a wavefront: a call that fits so needs no cut made for it here.)
+bool ssm_call_fits(const SsmLayerPlan& p, const SsmCall& c) {
+  const FinishGrid g = finish_grid(p, c);
+  if (g.all * g.block > UINT32_MAX) return false;
+  if (!c.offsets || scan_blocks(p, c, ScanCut{1, kMinSegment}) * 64 * kScanWaves <= UINT32_MAX) return true;
+  return scan_blocks(p, c, scan_cut(p, c.tokens, c.sequences)) * 64 * kScanWaves <= UINT32_MAX;
+}
+
 template <int NT, int W, int TPW>
 static hipError_t scan_launch(const SsmLayerPlan& p, const SsmCall& c, int segment_tokens, hipStream_t s) {
   const int hw = scan_heads(p, TPW), width = hw * p.head_dim;
-  const int64_t segments = c.tokens / segment_tokens + c.sequences;
-  const dim3 grid((uint32_t)(segments * (p.heads / hw))), block(64 * kScanWaves);
+  const dim3 grid((uint32_t)scan_blocks(p, c, ScanCut{TPW, segment_tokens})), block(64 * kScanWaves);
   if (c.tokens > segment_tokens) {
     hipError_t e = launch(ssm_scan_kernel<NT, W, TPW, true>, grid, block, ScanLds<NT, W, true>::bytes(hw, width), s,
                           p, c, segment_tokens, hw);

@@ -444,6 +444,27 @@ def test_refused_on_the_host(hip):
     assert L.llambda_hip_ssm_session_create(None, ctypes.byref(ctypes.c_void_p())) == -1
 
 
+def test_more_workgroups_than_a_launch_has(hip):
+    """Refused before anything is enqueued: 65535 sequences of 131 heads, one head to a workgroup of 512 threads,
+    are more than 2^32 threads.  The slots take part of them."""
+    import torch
+    layer = synthetic_ssm(np.random.default_rng(38), heads=131, head_dim=16, groups=1, state=16)
+    session = HipSsmSession(layer, slots=8, max_tokens=65535, max_sequences=65535)
+    x = torch.zeros(65535, layer.row, device="cuda")
+    y = torch.full((65535, layer.inner), 7.25, device="cuda")
+    few = torch.arange(9, dtype=torch.int32, device="cuda")
+    many = torch.full((65536,), -1, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    with pytest.raises(HipBackendError, match="65535 tokens of 65535 sequences are too many"):
+        # (nothing is read: the rows and the offsets are not those of such a call)
+        session.run_device(x.data_ptr(), y.data_ptr(), 65535, many.data_ptr(), 65535, many.data_ptr(), many.data_ptr())
+    session.sync()
+    assert bool((y == 7.25).all())
+    session.run_device(x.data_ptr(), y.data_ptr(), 8, few.data_ptr(), 8)  # the session goes on
+    session.sync()
+    assert bool((y[8:] == 7.25).all()) and bool((y[:8] != 7.25).all())
+
+
 @pytest.mark.parametrize("layout", ["hybrid", "wide", "narrow"])
 @pytest.mark.parametrize("x,b,c,state", [(1e-12, 1, 1, 1), (1e6, 1e-6, 1e3, 1e-9), (1e-18, 1e-10, 1e25, 1e-15),
                                          (1e8, 1e4, 1e-10, 1e15), (1, 1e-30, 1e20, 1)], ids=str)
