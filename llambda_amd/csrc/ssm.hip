@@ -557,7 +557,7 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
   };
   // the raw rows that a chunk's convolution reads: before the sequence those
   // it started with (zeros for a new one), past its end the last row again
-  // (their dt is zero, so any finite row will do)
+  // (their outputs are not stored, and the state takes zeros for them)
   auto request_rows = [&](int t0, int buf) {
     const uint32_t to = lds0 + Lds::at_rows(hw) + buf * Lds::rows * pitch;
     if (4 * lane >= width) return;
@@ -888,6 +888,14 @@ __global__ void __launch_bounds__(64 * kScanWaves) ssm_scan_kernel(SsmLayerPlan 
           if (on[k] && t < t_end) *reinterpret_cast<f32x4a4*>(out + ch[k]) = acc[it][k];
       }
       __syncthreads();  // B and what the next chunk needs have come; C is free
+    }
+    // Past the sequence's end x is of repeated rows, whose sum of taps may be
+    // infinite where no token's is: times a step of zero it would be NaN.
+    if (!STATES && next > t_end) {  // (segments that another follows end with a chunk)
+#pragma unroll
+      for (int k = 0; k < TPW; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[k][e] = t0 + 16 * (e >> 2) + 4 * g + (e & 3) < t_end ? x[k][e] : 0.f;
     }
     // The state: decayed, plus the tokens' products.  These inputs' scale
     // becomes the one that the state is held times, unless that brought it

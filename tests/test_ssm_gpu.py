@@ -489,6 +489,22 @@ def test_magnitudes(hip, layout, x, b, c, state):
     case.check()
 
 
+@pytest.mark.parametrize("layout", ["narrow", "odd", "wide"])
+def test_last_rows_near_the_end_of_single_precision(hip, layout):
+    """Taps of 0.5 of a last row of 2.5e38 are finite; those of the row repeated, as the chunk is filled up, are not."""
+    rng = np.random.default_rng(39)
+    layer = synthetic_ssm(rng, **LAYOUTS[layout])
+    layer.conv_weight[:layer.inner] = 0.9 if layer.conv_width == 2 else 0.5
+    layer.d[:] = 0.5
+    case = Case(layout, [33, 64, 150, 1], 40, layer=layer)
+    for end in case.offsets[1:]:
+        case.x[end - 1, layer.inner:layer.inner + 40] = 2.5e38
+        case.x[end - 1, :layer.inner] = 1e-30  # (the gate, so that the row's norm is of ordinary numbers)
+    case.device().run()
+    case.session.sync()
+    case.check()
+
+
 @pytest.mark.parametrize("run", [True, False])
 def test_outputs_whose_squares_leave_single_precision(hip, run):
     rng = np.random.default_rng(23)
