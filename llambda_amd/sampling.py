@@ -91,6 +91,23 @@ class HipSampler:
         return tok.value
 
 
+def _per_row(value, rows: int, dtype) -> np.ndarray:
+    """One number or one per row as `rows` of `dtype` (int32: whole numbers only; those beyond it are its ends)."""
+    v = np.asarray(value)
+    if np.dtype(dtype) == np.int32:
+        if v.dtype.kind not in "iu":
+            raise SamplingError(f"TOP-K must be whole numbers, got {v.dtype}.")
+        ends = np.iinfo(np.int32)
+        v = np.minimum(v if v.dtype.kind == "u" else np.maximum(v, ends.min), ends.max)
+    return np.ascontiguousarray(np.broadcast_to(v.astype(dtype), (rows,)))
+
+
+def _random_per_row(value, rows: int) -> np.ndarray:
+    """Numbers in [0, 1) in float32: those of more digits that would round to 1 become the largest below it."""
+    v = np.asarray(value, dtype=np.float64)
+    return _per_row(np.where(v < 1, np.minimum(v, 1 - 2.0 ** -24), v), rows, np.float32)
+
+
 class HipBatchSampler:
     """One token per row of a batch of logits (llambda_hip_batch_sampler_*): temperature, top-k,
     top-p and min-p of each row's own, from given random numbers, in 64 bits."""
@@ -136,16 +153,17 @@ class HipBatchSampler:
         rows = a.shape[0]
         keep = []
 
-        def each(v, dtype):
+        def each(v):
             if v is None:
                 return None
-            v = np.ascontiguousarray(np.broadcast_to(np.asarray(v, dtype=dtype), (rows,)))
             keep.append(v)
             return v.ctypes.data
 
-        p = native.BatchSampling(each(temperature, np.float32), each(top_k, np.int32),
-                                 each(top_p, np.float32), each(min_p, np.float32),
-                                 each(random_value, np.float32))
+        def optional(v, dtype=np.float32):
+            return each(None if v is None else _per_row(v, rows, dtype))
+
+        p = native.BatchSampling(optional(temperature), optional(top_k, np.int32), optional(top_p), optional(min_p),
+                                 each(_random_per_row(random_value, rows)))
         out = np.empty(rows, dtype=np.int64)
         if native.lib().llambda_hip_batch_sampler_sample(self._h, a.ctypes.data, a.shape[1], rows,
                                                          ctypes.byref(p), out.ctypes.data) != 0:

@@ -239,6 +239,13 @@ def test_replays_between_eager_calls_with_every_filter(hip, n):
         assert a.tolist() == want and b.tolist() == want
 
 
+def test_random_numbers_of_more_digits(sampler):
+    """Numbers just below 1 are no error on the host, and a top-k beyond 32 bits keeps all."""
+    x = head_like(np.random.default_rng(16), 2, 700)
+    got = sampler.sample(x, random_value=1 - 2.0 ** -50, top_k=2 ** 33 + 1)
+    assert got.tolist() == [reference(r, 1 - 2.0 ** -24) for r in x]
+
+
 def test_refusals(sampler):
     x = np.zeros((2, 100), np.float32)
     for kw, text in [(dict(random_value=1.0), "RANDOM-VALUE"), (dict(random_value=[0.5, -0.1]), "Row 1: RANDOM-VALUE"),

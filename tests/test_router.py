@@ -7,7 +7,7 @@ import pytest
 from llambda_amd import native
 from llambda_amd.hip_backend import HipBackendError
 from llambda_amd.moe import HipRouter, Routing
-from llambda_amd.sampling import HipBatchSampler, SamplingError
+from llambda_amd.sampling import HipBatchSampler, SamplingError, _per_row, _random_per_row
 
 
 @pytest.mark.parametrize("kw,text", [
@@ -49,3 +49,19 @@ def test_null_arguments():
 def test_batch_samplers_that_are_refused(vocab, rows, text):
     with pytest.raises(SamplingError, match=text):
         HipBatchSampler(vocab, rows)
+
+
+def test_parameters_of_rows():
+    """Random numbers of more digits than float32 stay below 1; counts are whole and do not wrap around."""
+    last = np.float32(1 - 2.0 ** -24)
+    assert _random_per_row(1 - 2.0 ** -40, 2).tolist() == [last, last]
+    assert _random_per_row([0.25, 0.99999999], 2).tolist() == [0.25, last]
+    assert _random_per_row([1.0, -1e-9], 2).tolist() == [1.0, np.float32(-1e-9)]  # (refused by the call)
+    assert np.isnan(_random_per_row(np.nan, 1)[0])
+    assert _per_row(np.array([2 ** 40, -2 ** 40, 7]), 3, np.int32).tolist() == [2 ** 31 - 1, -2 ** 31, 7]
+    assert _per_row(2 ** 40, 2, np.int32).tolist() == [2 ** 31 - 1] * 2
+    assert _per_row(np.uint64(2 ** 63), 1, np.int32).tolist() == [2 ** 31 - 1]
+    for v in (2.5, [1, 2.0], True, "3", None):
+        with pytest.raises(SamplingError, match="TOP-K must be whole numbers"):
+            _per_row(v, 2, np.int32)
+    assert _per_row([0.5], 2, np.float32).tolist() == [0.5, 0.5]
