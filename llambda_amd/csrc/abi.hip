@@ -1645,7 +1645,8 @@ struct llambda_hip_ssm_session {
     HIPC(hipMemcpyAsync(&flag, plan.error, sizeof flag, hipMemcpyDeviceToHost, s));
     HIPC(hipStreamSynchronize(s));
     if (!flag) return;
-    HIPC(ssm_reset_error_launch(plan, s));
+    HIPC(ssm_take_error_launch(plan, s));
+    HIPC(hipMemcpyAsync(&flag, plan.error + 1, sizeof flag, hipMemcpyDeviceToHost, s));
     HIPC(hipStreamSynchronize(s));
     failf("ssm: a call was refused on the device:%s%s%s",
           flag & kSsmErrOffsets ? " offsets do not ascend within its tokens;" : "",
@@ -1788,7 +1789,7 @@ int llambda_hip_ssm_session_create(const llambda_hip_ssm_desc* d,
     }
     const size_t chunks = (size_t)ssm_max_chunks(p.max_tokens, p.max_sequences);
     const size_t segments = (size_t)ssm_max_segments(p, p.max_tokens, p.max_sequences);
-    s->error.alloc(sizeof(int), "error flag");
+    s->error.alloc(2 * sizeof(int), "error flags");
     s->counts.alloc(2 * sizeof(int), "segment and chunk counts");
     s->sequences.alloc((size_t)p.max_sequences * sizeof(SsmSequence), "sequence table");
     s->segments.alloc(segments * sizeof(int2), "segment table");
@@ -1809,7 +1810,7 @@ int llambda_hip_ssm_session_create(const llambda_hip_ssm_desc* d,
     p.decay = s->decay.as<float>();
     p.seg_states = s->seg_states.as<float>();
     p.seg_decay = s->seg_decay.as<float>();
-    HIPC(ssm_reset_error_launch(p, s->stream));
+    HIPC(ssm_take_error_launch(p, s->stream));
     HIPC(hipStreamSynchronize(s->stream));
     *result = s.release();
   });

@@ -52,7 +52,7 @@ struct SsmLayerPlan {
   const float* norm;         // [HP]
   float* conv_states;
   float* ssm_states;
-  int* error;
+  int* error;  // [2]: SsmErrors of the calls since they were last taken, those taken
   // workspace of calls with offsets, for max_tokens and max_sequences
   SsmSequence* sequences;  // [max_sequences]
   int2* segments;          // [max_segments]: sequence, index within it
@@ -90,6 +90,6 @@ bool ssm_call_fits(const SsmLayerPlan& p, const SsmCall& c);
 // null, else sequences of any lengths.
 hipError_t ssm_step_launch(const SsmLayerPlan& p, const SsmCall& c, hipStream_t stream);
 hipError_t ssm_run_launch(const SsmLayerPlan& p, const SsmCall& c, hipStream_t stream);
-hipError_t ssm_reset_error_launch(const SsmLayerPlan& p, hipStream_t stream);
+hipError_t ssm_take_error_launch(const SsmLayerPlan& p, hipStream_t stream);
 
 }  // namespace llhip

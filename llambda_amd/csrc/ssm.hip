@@ -1200,8 +1200,9 @@ ssm_finish_kernel(SsmLayerPlan p, SsmCall c, int norm_blocks) {
   }
 }
 
-__global__ void ssm_reset_error_kernel(int* error) {
-  if (threadIdx.x == 0) *error = 0;
+// error[1] = what error[0] gathered, which starts anew: in one step, for calls on other streams may add to it.
+__global__ void ssm_take_error_kernel(int* error) {
+  if (threadIdx.x == 0) error[1] = atomicExch(error, 0);
 }
 
 // ------------------------------------------------------------------ host
@@ -1395,8 +1396,8 @@ hipError_t ssm_run_launch(const SsmLayerPlan& p, const SsmCall& c, hipStream_t s
   }
 }
 
-hipError_t ssm_reset_error_launch(const SsmLayerPlan& p, hipStream_t s) {
-  return launch(ssm_reset_error_kernel, dim3(1), dim3(64), 0, s, p.error);
+hipError_t ssm_take_error_launch(const SsmLayerPlan& p, hipStream_t s) {
+  return launch(ssm_take_error_kernel, dim3(1), dim3(64), 0, s, p.error);
 }
 
 }  // namespace llhip

@@ -303,6 +303,25 @@ def test_refused_on_the_device(hip):
     c.check(refused=(0, 2, 3, 5))
 
 
+def test_refusals_of_several_calls_are_reported_together(hip):
+    """Of calls on several streams since the last report; then none is left."""
+    import torch
+    c = Case("thin", [5, 3, 4], 41, slots=3).device()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    bad = torch.tensor([0, 5, 3, 12], dtype=torch.int32, device="cuda")
+    c.dold[1] = 9
+    torch.cuda.synchronize()
+    for _ in range(2):
+        c.session.run_device(c.dx.data_ptr(), c.dy.data_ptr(), c.tokens, bad.data_ptr(), 3, c.dnew.data_ptr(),
+                             c.dnew.data_ptr(), streams[0].cuda_stream)
+        c.run(streams[1].cuda_stream)
+        torch.cuda.synchronize()
+        with pytest.raises(HipBackendError, match="offsets do not ascend.*outside the pool"):
+            c.session.sync(streams[0].cuda_stream)
+        for s in streams:
+            c.session.sync(s.cuda_stream)
+
+
 @pytest.mark.parametrize("offsets", [[0, 5, 3, 12], [0, 5, 12, 13], [-1, 5, 6, 12], [0, 12, 0, 12]])
 def test_offsets_that_do_not_ascend(hip, offsets):
     import torch
