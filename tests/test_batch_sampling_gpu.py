@@ -265,3 +265,16 @@ def test_refusals(sampler):
         sampler.sample_device(0, 1, 0, 0)
     with pytest.raises(SamplingError, match="dimensions"):
         sampler.sample(np.zeros(100, np.float32), random_value=0.5)
+
+
+@pytest.mark.parametrize("n", [3, 5])
+def test_the_most_rows(hip, n):
+    rng = np.random.default_rng(17)
+    rows = 65535
+    s = HipBatchSampler(n, rows)
+    x = (rng.normal(size=(rows, n)) * 2).astype(np.float32)
+    u = rng.random(rows).astype(np.float32) * np.float32(0.999999)
+    got = s.sample(x, random_value=u, top_k=2, top_p=0.9)
+    at = rng.integers(0, rows, size=300).tolist() + [0, rows - 1]
+    assert [int(got[i]) for i in at] == [reference(x[i], u[i], k=2, p=0.9) for i in at]
+    assert got.min() >= 0 and got.max() < n

@@ -263,6 +263,31 @@ def test_moe_layer_with_a_router(hip, variant, tokens):
         assert np.array_equal(a, b)
 
 
+@pytest.mark.parametrize("experts,top_k", [(64, 8), (128, 6), (200, 16), (512, 10), (1000, 64)])
+@pytest.mark.parametrize("kind", ["qwen3next", "no shared", "nemotron", "latent"])
+def test_moe_layers_of_many_experts_with_a_router(hip, kind, experts, top_k):
+    rng = np.random.default_rng(18)
+    if kind in ("qwen3next", "no shared"):
+        layer = synthetic_qwen3next(rng, hidden=256, experts=experts, top_k=top_k, ffn=256,
+                                    shared_ffn=0 if kind == "no shared" else 256)
+    else:
+        layer = synthetic_nemotron_h(rng, hidden=256, experts=experts, top_k=top_k, ffn=32, shared_ffn=64,
+                                     **(dict(latent_in=64, latent_out=64) if kind == "latent" else {}))
+    session = HipMoeSession(layer)
+    for routing in (Routing(experts, top_k, weights_norm=False, weights_scale=3),
+                    Routing(experts, top_k, score="sigmoid", bias=(rng.normal(size=experts) * 0.3).astype(np.float32),
+                            groups=8, top_groups=5, group_rank=2)):
+        router = HipRouter(routing)
+        session.set_router(router)
+        for tokens in (1, 3, 70):
+            x = synthetic.activations(rng, tokens, layer.hidden)
+            y, idx, w, logits = session.run(x, with_routing=True)
+            check(routing, logits, (idx, w))
+            assert np.isfinite(y).all()
+            alone = router.run(logits)
+            assert np.array_equal(alone[0], idx) and np.array_equal(alone[1], w)
+
+
 def test_moe_layer_with_the_reference_gating_as_a_router(hip):
     """Qwen3Next's gating is a sigmoid router without bias and groups."""
     rng = np.random.default_rng(9)

@@ -536,3 +536,58 @@ def test_outputs_whose_squares_leave_single_precision(hip, run):
         case.step()
     case.session.sync()
     case.check()
+
+
+@pytest.mark.parametrize("state", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("conv_width", [2, 3, 4])
+def test_every_state_and_number_of_taps(hip, state, conv_width):
+    layer = synthetic_ssm(np.random.default_rng(42), heads=6, head_dim=48, groups=2, state=state, conv_width=conv_width)
+    for lengths, old in (([1, 33, 130], [0, -1, 2]), ([1, 1, 1], [2, -1, 0])):
+        c = Case(None, lengths, 43, old, [3, 4, 5], slots=6, layer=layer).device()
+        c.run()
+        c.session.sync()
+        c.check()
+    c.dconv.copy_(c.torch.from_numpy(c.conv))
+    c.dssm.copy_(c.torch.from_numpy(c.ssm))
+    c.dy.fill_(7.25)
+    c.step()
+    c.session.sync()
+    c.check()
+
+
+@pytest.mark.parametrize("heads,head_dim,groups", [(20, 128, 1), (96, 128, 3), (128, 128, 1), (512, 16, 256), (4, 16, 4)])
+def test_norm_widths(hip, heads, head_dim, groups):
+    """Groups of 2560, 4096, 16384 (the most), 32 and 16 channels."""
+    layer = synthetic_ssm(np.random.default_rng(44), heads=heads, head_dim=head_dim, groups=groups, state=16)
+    c = Case(None, [1, 3, 40], 45, [0, -1, 2], [3, 4, 5], slots=6, extra_rows=2, layer=layer).device()
+    c.run()
+    c.session.sync()
+    c.check()
+    c = Case(None, [1, 1, 1], 46, [0, -1, 2], [3, 4, 5], slots=6, layer=layer).device()
+    c.step()
+    c.session.sync()
+    c.check()
+
+
+def test_rows_before_the_first_sequence(hip):
+    c = Case("narrow", [50, 0, 7], 47, slots=3, extra_rows=5)
+    c.offsets += 5
+    c.device().run()
+    c.session.sync()
+    assert bool((c.dy[:5] == 7.25).all())
+    c.check()
+
+
+@pytest.mark.parametrize("given", ["old", "new"])
+def test_one_slot_list(hip, given):
+    """The list that is not given is slot i."""
+    old, new = ([3, -1, 4], None) if given == "old" else (None, [3, -1, 4])
+    for lengths in ([40, 2, 1], [1, 1, 1]):
+        c = Case("narrow", lengths, 48, old, new, slots=5).device()
+        lists = (c.dold.data_ptr(), 0) if given == "old" else (0, c.dnew.data_ptr())
+        if max(lengths) > 1:
+            c.session.run_device(c.dx.data_ptr(), c.dy.data_ptr(), c.tokens, c.doff.data_ptr(), 3, *lists)
+        else:
+            c.session.step_device(c.dx.data_ptr(), c.dy.data_ptr(), 3, *lists)
+        c.session.sync()
+        c.check()
