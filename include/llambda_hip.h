@@ -434,7 +434,8 @@ int llambda_hip_llama_session_sync(llambda_hip_llama_session* session, void* str
  * with u = silu(conv(x | B | C)), dt = softplus(dt + ssm_dt), per head
  *   s = exp(dt ssm_a) s + dt u_x u_B^T,   y = s u_C + ssm_d u_x,
  * then v = y silu(z) and, per group of heads, v / sqrt(mean(v^2) + epsilon)
- * times ssm_norm.  All fp32; logarithms of decays are summed in 64 bits. */
+ * times ssm_norm.  All fp32; logarithms of decays are summed in 64 bits.  dt is
+ * not clamped: a layer with limits of its own on the step is not expressed. */
 typedef struct llambda_hip_ssm_desc {
   int64_t heads;
   int64_t head_dim;           /* a multiple of 16, 16 to 128 */

@@ -20,13 +20,12 @@
 // draw finds its chunk by their sums and reads that.  Weights of whole rows are
 // integers in steps of 2^-44, so that sums do not depend on the atomics' order;
 // with the bins' powers in a table one takes 5 operations in 64 bits and a
-// short series in 32 (off by 1e-9 of it at most, without a bias), a fourth of
-// an exponential in 64 bits, which bound these passes.
-// Rows of 128256 logits (us), launch by launch: maxima 13 for 160 rows (6.3 TB/s),
-// 3 for one; bins 33 and 6, weights above the cut 44 and 10 where all rows have
-// top-p, 25 where all have min-p alone; the finish 25 with 200 ranks (of one row's
-// then 22, 9 were the reading of 200 chunks, the bound 2.6, the sort 2.5, the draw
-// 2.6; now 8.5 in the launch before and 11), 18 and 15 with top-p, 7 with min-p.
+// short series in 32 (off by 1.4e-9 of it at most), a fourth of an exponential in
+// 64 bits, which bound these passes.
+// Rows of 128256 logits (us), launch by launch: maxima 14 for 160 rows (5.9 TB/s),
+// 3.5 for one; bins 32 and 6, weights above the cut 44 and 10 where all rows have
+// top-p, 25 where all have min-p alone; the finish 25 with 200 ranks (of one row 8.5
+// in the launch before and 11), 18 and 15 with top-p, 7 with min-p.
 #include "sample_batch.h"
 
 #include <climits>
@@ -63,11 +62,12 @@ __device__ __forceinline__ RowParams row_params(const SampleRows& s, int row) {
   return p;
 }
 
-// exp(x) for x <= 0 in 64 bits: 2^n e^r with |r| <= ln 2 / 2, e^r by its series
-// to r^12 (what follows is below 2e-16).
+// exp(x) for x <= 0 in 64 bits: 2^n e^r with |r| <= ln 2 / 2, e^r by its Taylor
+// series to r^12 (what follows is below 2e-16).  r by Cody and Waite's reduction: ln 2
+// as the sum of its first 32 bits, whose products with n are exact, and the rest.
 __device__ __forceinline__ double exp_below(double x) {
   const double n = rint(x * 1.44269504088896340736);
-  double r = fma(n, -6.93147180369123816490e-01, x);  // ln 2 in two parts, the first of 32 bits
+  double r = fma(n, -6.93147180369123816490e-01, x);
   r = fma(n, -1.90821492927058770002e-10, r);
   double e = 1.0 / 479001600.0;
   e = fma(e, r, 1.0 / 39916800.0);
@@ -666,9 +666,8 @@ __device__ __forceinline__ uint64_t keep_from_list(RowLds& l, int n, RowParams p
   return cut;
 }
 
-// The highest entry e such that the entries >= e reach `need` (their number, or their mass where
-// `by_mass`), among the entries <= limit of the row.  0 where all of them do not.  `reached`: what the
-// entries above e hold.
+// The highest entry e such that the entries >= e reach `need` (their number, or their weight where
+// `by_mass`), of the row's entries >= floor_entry; floor_entry where all of those do not.
 __device__ __forceinline__ uint64_t row_cut(RowLds& l, const float* row, int n, float top, double t, bool by_mass,
                             uint64_t need, uint64_t floor_entry) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;

@@ -29,9 +29,10 @@
 // so 142 and 67.  fp32 matrix instructions have an eighth of the rate.)
 // Bound by latency: a chunk of 256 channels takes a workgroup 8.5 us, of which
 // the matrix cores work 1.6, the vector units about 2 and the LDS about 1.2;
-// its LDS (124 KB) and registers (232 of 256) leave no room for a second
-// workgroup.  Half as many channels leave it, but two of those take as long
-// (187 us where 128 registers had to do, 171 without).
+// its LDS (124 KB) and registers (238 of 256) leave no room for a second
+// workgroup.  Half as many channels leave it, but two of those took longer:
+// when the scan was at 154 us, 187 in the 128 registers of two workgroups (with
+// 80 bytes of scratch) and 171 without that limit.
 // Long sequences of few heads are cut into segments so that the grid fills the
 // device: a first pass forms each segment's own state, a small kernel joins
 // them in order, and the scan proper starts each segment from its state.
@@ -1212,9 +1213,11 @@ int64_t ssm_max_chunks(int64_t tokens, int64_t sequences) { return tokens / kSsm
 // How a call is cut: column tiles per wavefront and tokens per segment.  A
 // scan workgroup has a CU to itself (its LDS), so a pass takes as many rounds
 // as it has workgroups to the device's 256 CUs.  The times are measured ones of
-// N = 128 (us): two tiles a wavefront share a group's operands between twice
-// the channels; one tile halves a chunk's latency where there are CUs to
-// spare.  Segments add the first pass, the join and the launches of both.
+// N = 128 (us) and stand for all: a chunk of N = 256 takes one tile 6.6 instead of
+// 4.75, those of smaller states were not timed alone.  Two tiles a wavefront share
+// a group's operands between twice the channels; one tile halves a chunk's latency
+// where there are CUs to spare.  Segments add the first pass, the join and the
+// launches of both.
 struct ScanCut {
   int tiles, segment_tokens;
 };
