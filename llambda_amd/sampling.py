@@ -95,9 +95,10 @@ def _per_row(value, rows: int, dtype) -> np.ndarray:
     """One number or one per row as `rows` of `dtype` (int32: whole numbers only; those beyond it are its ends)."""
     v = np.asarray(value)
     if np.dtype(dtype) == np.int32:
-        if v.dtype.kind not in "iu":
-            raise SamplingError(f"TOP-K must be whole numbers, got {v.dtype}.")
+        if v.dtype.kind not in "iubf" or (v.dtype.kind == "f" and not np.all(np.floor(v) == v)):
+            raise SamplingError(f"TOP-K must be whole numbers, got {value}.")
         ends = np.iinfo(np.int32)
+        v = v.astype(np.float64 if v.dtype.kind == "f" else np.uint64 if v.dtype.kind == "u" else np.int64)
         v = np.minimum(v if v.dtype.kind == "u" else np.maximum(v, ends.min), ends.max)
     return np.ascontiguousarray(np.broadcast_to(v.astype(dtype), (rows,)))
 

@@ -61,7 +61,9 @@ def test_parameters_of_rows():
     assert _per_row(np.array([2 ** 40, -2 ** 40, 7]), 3, np.int32).tolist() == [2 ** 31 - 1, -2 ** 31, 7]
     assert _per_row(2 ** 40, 2, np.int32).tolist() == [2 ** 31 - 1] * 2
     assert _per_row(np.uint64(2 ** 63), 1, np.int32).tolist() == [2 ** 31 - 1]
-    for v in (2.5, [1, 2.0], True, "3", None):
+    assert _per_row(np.array([40.0, 1e30, -1e30]), 3, np.int32).tolist() == [40, 2 ** 31 - 1, -2 ** 31]
+    assert _per_row(np.float32(7), 1, np.int32).tolist() == [7] and _per_row(True, 1, np.int32).tolist() == [1]
+    for v in (2.5, [1, 2.25], np.nan, "3", None):
         with pytest.raises(SamplingError, match="TOP-K must be whole numbers"):
             _per_row(v, 2, np.int32)
     assert _per_row([0.5], 2, np.float32).tolist() == [0.5, 0.5]
