@@ -494,7 +494,7 @@ int llambda_hip_ssm_session_run(llambda_hip_ssm_session* session, int64_t slot,
  * they are).  llambda_hip_ssm_session_sync reports them.
  * A call is refused, with nothing of it enqueued, where a launch of it would
  * have 2^32 threads: from about 2^23 pairs of a sequence and a workgroup of one
- * to four heads, or 2^24 to 2^26 pairs of a row and a group, on.
+ * to four heads, or 2^22 to 2^26 pairs of a row and a group, on.
  * Enqueued on `stream` (null = the session's stream), not waited for, with no
  * allocation.  The calls of a session share its workspace: each waits on the
  * device for the one before, whatever stream it ran on.  Under stream capture
