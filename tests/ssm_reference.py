@@ -29,10 +29,8 @@ def _softplus(v):
     return np.maximum(v, 0) + np.log1p(np.exp(-np.abs(v)))
 
 
-def sequence(layer, x, conv, ssm, operand=lambda name, v: v):
-    """One sequence: (y, conv, ssm, y's bound, ssm's bound) for rows x [T][row] from a state.
-    operand(name, v): what a product takes of x dt ("x"), B, C or the state ("s"), for the emulation of
-    operands of fewer bits."""
+def sequence(layer, x, conv, ssm):
+    """One sequence: (y, conv, ssm, y's bound, ssm's bound) for rows x [T][row] from a state."""
     L, H, P, G, N, W = layer, layer.heads, layer.head_dim, layer.groups, layer.state, layer.conv_width
     x = x.astype(np.float64)
     T, inner, channels = x.shape[0], L.inner, L.channels
@@ -59,9 +57,9 @@ def sequence(layer, x, conv, ssm, operand=lambda name, v: v):
         xa = u_abs[:inner].reshape(H, P)
         ba = np.repeat(u_abs[inner:inner + G * N].reshape(G, N), share, 0)
         ca = np.repeat(u_abs[inner + G * N:].reshape(G, N), share, 0)
-        s = e[:, None, None] * s + operand("x", dt[:, None] * xs)[:, :, None] * operand("B", bs)[:, None, :]
+        s = e[:, None, None] * s + (dt[:, None] * xs)[:, :, None] * bs[:, None, :]
         s_abs = e[:, None, None] * s_abs + (dt[:, None] * xa)[:, :, None] * ba[:, None, :] + lost
-        y[t] = ((operand("s", s) * operand("C", cs)[:, None, :]).sum(-1) + d[:, None] * xs).reshape(-1)
+        y[t] = ((s * cs[:, None, :]).sum(-1) + d[:, None] * xs).reshape(-1)
         y_abs[t] = ((s_abs * ca[:, None, :]).sum(-1) + np.abs(d)[:, None] * xa).reshape(-1)
     z = _silu(x[:, :inner])
     v, dv = y * z, K * U * y_abs * np.abs(z) + 8 * U * np.abs(y * z)
@@ -82,6 +80,27 @@ def sequence(layer, x, conv, ssm, operand=lambda name, v: v):
 # them follow one another on a full value (the convolution and silu of x, B and C, the step and its decay, a product,
 # a sum in a tree, the skip, the gate and the norm), so 0.4 U sqrt(45) = 2.7 U = 1.6e-7; three times that is allowed.
 TOGETHER = 8 * U
+
+
+def with_operands(layer, x, conv, ssm, operand):
+    """(y, ssm) of a sequence whose products take operand(name, v) of x dt ("x"), B, C and the state ("s")."""
+    H, P, G, N, W, inner = layer.heads, layer.head_dim, layer.groups, layer.state, layer.conv_width, layer.inner
+    x, s = x.astype(np.float64), ssm.astype(np.float64)
+    T, channels = len(x), layer.channels
+    raw = np.concatenate([conv, x[:, inner:inner + channels]])
+    u = np.zeros(channels) if layer.conv_bias is None else layer.conv_bias
+    u = _silu(u + sum(layer.conv_weight[:, k].astype(np.float64) * raw[k:k + T] for k in range(W)))
+    dt = _softplus(x[:, inner + channels:] + layer.dt_bias)
+    heads = u[:, :inner].reshape(T, H, P)
+    b, c = (np.repeat(v.reshape(T, G, N), H // G, 1) for v in (u[:, inner:inner + G * N], u[:, inner + G * N:]))
+    left, b, c = operand("x", dt[:, :, None] * heads), operand("B", b), operand("C", c)
+    y = np.empty((T, H, P))
+    for t in range(T):
+        s = np.exp(dt[t] * layer.a)[:, None, None] * s + left[t][:, :, None] * b[t][:, None, :]
+        y[t] = (operand("s", s) * c[t][:, None, :]).sum(-1) + layer.d[:, None] * heads[t]
+    v = (y.reshape(T, inner) * _silu(x[:, :inner])).reshape(T, G, -1)
+    v = v / np.sqrt((v * v).mean(-1, keepdims=True) + layer.norm_epsilon)
+    return v.reshape(T, inner) * layer.norm, s
 
 
 def together(got, want):

@@ -112,8 +112,11 @@ def test_operands_of_half_the_digits_are_seen(kw, names):
         return operand
 
     want = ssm_reference.sequence(layer, x, conv, ssm)
-    few, all_ = (ssm_reference.sequence(layer, x, conv, ssm, rounded(bits)) for bits in (16, 24))
+    few, all_ = (ssm_reference.with_operands(layer, x, conv, ssm, rounded(bits)) for bits in (16, 24))
     assert ssm_reference.together(few[0], want[0]) > ssm_reference.TOGETHER
     assert ssm_reference.together(all_[0], want[0]) < ssm_reference.TOGETHER / 4
     if "x" in names or "B" in names:
-        assert ssm_reference.together(few[2], want[2]) > ssm_reference.TOGETHER
+        assert ssm_reference.together(few[1], want[2]) > ssm_reference.TOGETHER
+    exact = ssm_reference.with_operands(layer, x, conv, ssm, lambda name, v: v)
+    for got, of in ((exact[0], want[0]), (exact[1], want[2])):
+        assert ssm_reference.together(got, of) < 1e-8  # (the epsilon of one is rounded to float32)
