@@ -45,6 +45,7 @@ typedef struct llambda_hip_llama_session llambda_hip_llama_session;
 typedef struct llambda_hip_sampler llambda_hip_sampler;
 typedef struct llambda_hip_gguf llambda_hip_gguf;
 typedef struct llambda_hip_ssm_session llambda_hip_ssm_session;
+typedef struct llambda_hip_attention_session llambda_hip_attention_session;
 typedef struct llambda_hip_router llambda_hip_router;
 typedef struct llambda_hip_batch_sampler llambda_hip_batch_sampler;
 
@@ -527,6 +528,128 @@ int llambda_hip_ssm_session_write_state(llambda_hip_ssm_session* session, int64_
                                         const float* conv, const float* ssm, int on_device);
 int llambda_hip_ssm_session_read_state(llambda_hip_ssm_session* session, int64_t slot,
                                        float* conv, float* ssm);
+
+/* ---- attention over a paged cache ------------------------------------------ */
+
+enum {                          /* GGML's tags */
+  LLAMBDA_HIP_TYPE_F32 = 0,
+  LLAMBDA_HIP_TYPE_F16 = 1,
+  LLAMBDA_HIP_TYPE_BF16 = 30
+};
+
+/* Causal attention with grouped heads of the new rows of many sequences, between
+ * the projections of a layer: prompts of several lengths, one row of each sequence,
+ * or trees of drafted tokens.  Sequence i has context[i] = c tokens cached; its new
+ * row r gets position c + r.  Its keys and values, rounded to the cache's type
+ * (beyond its range: infinities), are put into the cache there, and with group =
+ * heads / kv_heads, per head h,
+ *   s_j = scale q_h . K_j,  p = softmax(s),  y_h = sum_j p_j V_j,  K, V of kv head h / group
+ * over the positions j that the row sees: j <= c + r.  Rows are taken as they are:
+ * a model that rotates queries and keys does so before.  fp32 rows keep single precision
+ * throughout; rows in 16 bits have their probabilities rounded to that type.  Values
+ * that are infinite or NaN reach only the rows that see them (as either).
+ *
+ * The cache is a pool of pages, key_pages and value_pages [layers][pages][kv_heads]
+ * [page_tokens][head_dim]; position j of sequence i is row j % page_tokens of page
+ * table[i][j / page_tokens].  Pages may be in any order and shared by sequences, but
+ * one that a call writes to belongs to one sequence of the call. */
+typedef struct llambda_hip_attention_desc {
+  int64_t heads;              /* at most 1024 */
+  int64_t kv_heads;           /* divides heads */
+  int64_t head_dim;           /* a multiple of 16, 16 to 256 */
+  float scale;                /* 0: 1 / sqrt(head_dim) */
+  int row_type;               /* LLAMBDA_HIP_TYPE_*, of q, k, v and output */
+  int cache_type;             /* any below fp32 rows, else the rows' */
+  int64_t layers;             /* layers that share the tables and the workspace */
+  int64_t page_tokens;        /* a power of two, 16 to 2^20 */
+  int64_t pages;              /* of a layer */
+  int64_t max_context;        /* most tokens of a sequence, cached and new */
+  int64_t max_tokens;         /* most rows of one call */
+  int64_t max_sequences;      /* most sequences of one call */
+  /* Device memory, 16-byte aligned.  Both NULL: the session allocates it, zeroed. */
+  void* key_pages;
+  void* value_pages;
+} llambda_hip_attention_desc;
+
+/* New rows, device memory: q, output [tokens][heads][head_dim], k, v [tokens][kv_heads]
+ * [head_dim], strides in elements from row to row (0: dense).  Rows start at 16-byte
+ * aligned addresses.  output shares no memory with the others, but all may be columns of
+ * one buffer. */
+typedef struct llambda_hip_attention_rows {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* output;
+  int64_t q_stride;
+  int64_t k_stride;
+  int64_t v_stride;
+  int64_t output_stride;
+} llambda_hip_attention_rows;
+
+/* Whose rows they are; lists in device memory. */
+typedef struct llambda_hip_attention_batch {
+  size_t tokens;              /* rows in all */
+  size_t sequences;
+  const int32_t* offsets;     /* [sequences + 1], ascending: sequence i's rows are [offsets[i],
+                                 offsets[i + 1]), none if equal; rows of no sequence are left as
+                                 they are in output.  NULL: row i is sequence i's */
+  const int32_t* context;     /* [sequences] */
+  const int32_t* table;       /* [sequences][table_stride] */
+  size_t table_stride;        /* at least, and with 0, max_context / page_tokens, rounded up */
+  const int32_t* parents;     /* [tokens], NULL: causal.  Else each sequence's rows are a tree of
+                                 at most 256 nodes: parents[row] is the number within the sequence
+                                 of the row's parent, an earlier row, or -1.  A row then sees the
+                                 cached tokens, its ancestors and itself */
+} llambda_hip_attention_batch;
+
+/* No counterpart in the reference's bridge: it is the per-layer hook for the attention of its
+ * step functions (llambda.lisp:5122-5167, 5951-6018), which take one token at a time. */
+int llambda_hip_attention_session_create(const llambda_hip_attention_desc* desc,
+                                         llambda_hip_attention_session** result);
+void llambda_hip_attention_session_destroy(llambda_hip_attention_session* session);
+
+/* Enqueued on `stream` (null = the session's stream), not waited for, with no allocation.
+ * What only the device can see is checked there, before anything of a sequence is read or
+ * written: offsets (nothing of the call is run); a sequence's tokens beyond max_context, its
+ * pages outside the pool, its parents (the sequence is not run: its rows and pages stay as they
+ * are).  llambda_hip_attention_session_sync reports them.  Counts of cached tokens are the
+ * caller's: they are not changed.  The calls of a session are ordered as
+ * llambda_hip_ssm_session_run_device's, under capture too. */
+int llambda_hip_attention_session_run_device(llambda_hip_attention_session* session, int64_t layer,
+                                             const llambda_hip_attention_rows* rows,
+                                             const llambda_hip_attention_batch* batch, void* stream);
+
+/* Dense rows of one sequence in host memory, synchronous; table: its row. */
+int llambda_hip_attention_session_run(llambda_hip_attention_session* session, int64_t layer,
+                                      const void* q, const void* k, const void* v, void* output,
+                                      size_t tokens, int64_t context, const int32_t* table,
+                                      const int32_t* parents);
+
+/* Of sequence i's tree, whose rows are at positions context[i] and on, counts[i] nodes are
+ * accepted: paths[i][0] < paths[i][1] < ..., numbers within the tree.  Their keys and values move,
+ * in all layers, to positions context[i], context[i] + 1, ...  (the caller then adds counts[i] to
+ * context[i]).  counts of 0 move nothing.  Lists in device memory, paths [sequences][path_stride];
+ * a sequence whose path does not ascend below 256, or whose places or pages are out of range, is
+ * left as it is and reported by _sync.  Stream and order as run_device. */
+int llambda_hip_attention_session_accept_device(llambda_hip_attention_session* session,
+                                                const int32_t* context, const int32_t* table,
+                                                size_t table_stride, const int32_t* paths,
+                                                size_t path_stride, const int32_t* counts,
+                                                size_t sequences, void* stream);
+
+/* Wait for `stream` (null = the session's stream) and report, once, any sequence that was
+ * refused on the device since the last report. */
+int llambda_hip_attention_session_sync(llambda_hip_attention_session* session, void* stream);
+
+/* Copy positions [first, first + count) of a sequence whose table row is `table` (host memory)
+ * into or out of the pages: keys and values [count][kv_heads][head_dim] of the cache's type, host
+ * memory.  Synchronous; waits for the session's calls, whatever stream they ran on. */
+int llambda_hip_attention_session_write(llambda_hip_attention_session* session, int64_t layer,
+                                        const int32_t* table, int64_t first, int64_t count,
+                                        const void* keys, const void* values);
+int llambda_hip_attention_session_read(llambda_hip_attention_session* session, int64_t layer,
+                                       const int32_t* table, int64_t first, int64_t count,
+                                       void* keys, void* values);
 
 /* ---- sampling ------------------------------------------------------------ */
 

@@ -8,6 +8,7 @@ Modules:
   hip_backend  projection sessions and the :hip backend descriptor
   moe          routed-MoE layer sessions and routers
   ssm          Mamba-2 mixer sessions
+  attention    attention sessions over a paged cache
   sampling     a token from logits, of one row or of a batch
   accelerator  the backend descriptor protocol
   projection   the tensor-indexed binding store with runtime fallback

@@ -22,6 +22,7 @@
 #include <string>
 #include <vector>
 
+#include "attention.h"
 #include "decoder.h"
 #include "gemv.h"
 #include "gguf.h"
@@ -1941,6 +1942,381 @@ int llambda_hip_ssm_session_read_state(llambda_hip_ssm_session* s, int64_t slot,
     HIPC(hipMemcpyAsync(conv, s->plan.conv_states + slot * nc, nc * sizeof(float), hipMemcpyDeviceToHost, s->stream));
     HIPC(hipMemcpyAsync(ssm, s->plan.ssm_states + slot * ns, ns * sizeof(float), hipMemcpyDeviceToHost, s->stream));
     HIPC(hipStreamSynchronize(s->stream));
+  });
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------- attention
+
+struct llambda_hip_attention_session {
+  std::mutex run_mutex;
+  int device = 0;
+  hipStream_t stream = nullptr;
+  AttnPlan plan{};
+  DevBuf pool_keys, pool_values, error, run, items, joins, counts, tree, part_y, part_ml;
+  DevBuf q, k, v, y, lists;  // device staging of the host-pointer runs; lists: offsets, context, parents, table
+  int64_t staged_tokens = 0;
+  // recorded after every call that uses the workspace; the next one waits
+  hipEvent_t done = nullptr;
+  ~llambda_hip_attention_session() {
+    if (done) (void)hipEventDestroy(done);
+    if (stream) (void)hipStreamDestroy(stream);
+  }
+  size_t row_bytes() const { return plan.row_type == kAttnF32 ? 4 : 2; }
+  size_t cell_bytes() const { return plan.cache_type == kAttnF32 ? 4 : 2; }
+  size_t q_elements() const { return (size_t)plan.heads * plan.head_dim; }
+  size_t kv_elements() const { return (size_t)plan.kv_heads * plan.head_dim; }
+  int page_tokens() const { return 1 << plan.page_shift; }
+  void raise_error(hipStream_t s) {
+    int flag = 0;
+    HIPC(hipMemcpyAsync(&flag, plan.error, sizeof flag, hipMemcpyDeviceToHost, s));
+    HIPC(hipStreamSynchronize(s));
+    if (!flag) return;
+    HIPC(attn_take_error_launch(plan, s));
+    HIPC(hipMemcpyAsync(&flag, plan.error + 1, sizeof flag, hipMemcpyDeviceToHost, s));
+    HIPC(hipStreamSynchronize(s));
+    failf("attention: a call was refused on the device:%s%s%s%s%s",
+          flag & kAttnErrOffsets ? " offsets do not ascend within its tokens;" : "",
+          flag & kAttnErrContext ? " a sequence's tokens do not fit the session's context;" : "",
+          flag & kAttnErrPage ? " a page lies outside the pool;" : "",
+          flag & kAttnErrTree ? " a tree has too many nodes or a parent that is no earlier node;" : "",
+          flag & kAttnErrPath ? " an accepted path does not ascend within a tree's nodes;" : "");
+  }
+};
+
+namespace {
+
+// The session's device is the current one within a scope.
+struct DeviceScope {
+  int before = 0;
+  explicit DeviceScope(int device) {
+    HIPC(hipGetDevice(&before));
+    if (before != device) HIPC(hipSetDevice(device));
+  }
+  ~DeviceScope() { (void)hipSetDevice(before); }
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+};
+
+// Rows of a call: `width` elements, `stride` from row to row.
+struct RowSpan {
+  const char* name;
+  const void* ptr;
+  int64_t stride, width;
+};
+
+// Whether rows of `a` and `b` share memory: rows of one stride may be columns of the same buffer.
+bool rows_overlap(const RowSpan& a, const RowSpan& b, size_t rows, size_t size) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.ptr), y = reinterpret_cast<uintptr_t>(b.ptr);
+  const size_t ax = ((rows - 1) * a.stride + a.width) * size, bx = ((rows - 1) * b.stride + b.width) * size;
+  if (!(x < y + bx && y < x + ax)) return false;
+  if (a.stride != b.stride) return true;
+  const size_t stride = a.stride * size;
+  const size_t delta = x < y ? (y - x) % stride : (stride - (x - y) % stride) % stride;  // of b's row behind a's
+  return delta < a.width * size || delta + b.width * size > stride;
+}
+
+AttnCall attention_call(const llambda_hip_attention_session* s, int64_t layer, const llambda_hip_attention_rows* r,
+                        const llambda_hip_attention_batch* b) {
+  const char* what = "attention_session_run_device";
+  const AttnPlan& p = s->plan;
+  if (!r || !b) failf("%s: null argument", what);
+  if (layer < 0 || layer >= p.layers) failf("%s: layer %lld is not in 0..%d", what, (long long)layer, p.layers - 1);
+  if (!b->context || !b->table) failf("%s: null context or table", what);
+  if (b->tokens == 0 || b->tokens > (size_t)p.max_tokens)
+    failf("%s: %zu tokens are not in 1..%d", what, b->tokens, p.max_tokens);
+  if (b->sequences == 0 || b->sequences > (size_t)p.max_sequences)
+    failf("%s: %zu sequences are not in 1..%d", what, b->sequences, p.max_sequences);
+  if (!b->offsets && b->tokens != b->sequences)
+    failf("%s: %zu tokens of %zu sequences without offsets", what, b->tokens, b->sequences);
+  if ((reinterpret_cast<uintptr_t>(b->offsets) | reinterpret_cast<uintptr_t>(b->context) |
+       reinterpret_cast<uintptr_t>(b->table) | reinterpret_cast<uintptr_t>(b->parents)) & 3u)
+    failf("%s: lists must be 4-byte aligned", what);
+  const int64_t width = attn_table_width(p), size = (int64_t)s->row_bytes();
+  const int64_t table_stride = b->table_stride ? b->table_stride : width;
+  if (table_stride < width || table_stride > INT32_MAX)
+    failf("%s: table rows of %lld entries, %lld are needed", what, (long long)table_stride, (long long)width);
+  RowSpan spans[4] = {{"q", r->q, r->q_stride, (int64_t)s->q_elements()},
+                      {"k", r->k, r->k_stride, (int64_t)s->kv_elements()},
+                      {"v", r->v, r->v_stride, (int64_t)s->kv_elements()},
+                      {"output", r->output, r->output_stride, (int64_t)s->q_elements()}};
+  for (RowSpan& x : spans) {
+    if (!x.ptr) failf("%s: null %s", what, x.name);
+    if (!x.stride) x.stride = x.width;
+    if (x.stride < x.width || x.stride > INT32_MAX)
+      failf("%s: stride %lld of %s is not in %lld..%d", what, (long long)x.stride, x.name, (long long)x.width, INT32_MAX);
+    if ((reinterpret_cast<uintptr_t>(x.ptr) | (uintptr_t)(x.stride * size)) & 15u)
+      failf("%s: rows of %s must be 16-byte aligned", what, x.name);
+  }
+  for (int i = 0; i < 3; ++i)
+    if (rows_overlap(spans[i], spans[3], b->tokens, size)) failf("%s: %s and output overlap", what, spans[i].name);
+  return AttnCall{r->q, r->k, r->v, r->output, spans[0].stride, spans[1].stride, spans[2].stride, spans[3].stride,
+                  (int)layer, (int)b->tokens, (int)b->sequences, b->offsets, b->context, b->table, table_stride,
+                  b->parents};
+}
+
+template <typename Launch>
+void attention_ordered(llambda_hip_attention_session* s, hipStream_t st, Launch&& launch) {
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  HIPC(hipStreamIsCapturing(st, &capture));
+  const bool ordered = capture == hipStreamCaptureStatusNone;
+  if (ordered) HIPC(hipStreamWaitEvent(st, s->done, 0));
+  HIPC(launch());
+  if (ordered) HIPC(hipEventRecord(s->done, st));
+}
+
+void attention_enqueue(llambda_hip_attention_session* s, const AttnCall& c, hipStream_t st) {
+  if (!attn_call_fits(s->plan, c))
+    failf("attention: %d tokens of %d sequences are too many for one call", c.tokens, c.sequences);
+  attention_ordered(s, st, [&] { return attn_run_launch(s->plan, c, st); });
+}
+
+// Copies positions [first, first + count) of a sequence between its pages and host rows [count][kv_heads][head_dim].
+void attention_copy(llambda_hip_attention_session* s, const char* what, int64_t layer, const int32_t* table,
+                    int64_t first, int64_t count, void* keys, void* values, bool write) {
+  if (!s || !table || !keys || !values) failf("%s: null argument", what);
+  const AttnPlan& p = s->plan;
+  if (layer < 0 || layer >= p.layers) failf("%s: layer %lld is not in 0..%d", what, (long long)layer, p.layers - 1);
+  if (first < 0 || count < 0 || first > p.max_context || count > p.max_context - first)
+    failf("%s: positions [%lld, %lld) are not in the context %d", what, (long long)first, (long long)(first + count),
+          p.max_context);
+  const int64_t page = s->page_tokens();
+  for (int64_t e = first / page; count > 0 && e <= (first + count - 1) / page; ++e)
+    if (table[e] < 0 || table[e] >= p.pages)
+      failf("%s: page %d of entry %lld is not in 0..%d", what, table[e], (long long)e, p.pages - 1);
+  if (count == 0) return;
+  std::lock_guard<std::mutex> lock(s->run_mutex);
+  DeviceScope scope(s->device);
+  HIPC(hipStreamWaitEvent(s->stream, s->done, 0));
+  const size_t w = (size_t)p.head_dim * s->cell_bytes(), row = w * p.kv_heads;
+  for (int64_t at = first; at < first + count;) {
+    const int64_t n = std::min(first + count, (at / page + 1) * page) - at;
+    for (int h = 0; h < p.kv_heads; ++h) {
+      const size_t in = ((((size_t)layer * p.pages + table[at / page]) * p.kv_heads + h) * page + at % page) * w;
+      const size_t out = (size_t)(at - first) * row + h * w;
+      for (auto [pool, host] : {std::pair(p.keys, keys), std::pair(p.values, values)}) {
+        uint8_t* d = static_cast<uint8_t*>(pool) + in;
+        uint8_t* x = static_cast<uint8_t*>(host) + out;
+        HIPC(write ? hipMemcpy2DAsync(d, w, x, row, w, n, hipMemcpyHostToDevice, s->stream)
+                   : hipMemcpy2DAsync(x, row, d, w, w, n, hipMemcpyDeviceToHost, s->stream));
+      }
+    }
+    at += n;
+  }
+  HIPC(hipStreamSynchronize(s->stream));
+}
+
+}  // namespace
+
+extern "C" {
+
+int llambda_hip_attention_session_create(const llambda_hip_attention_desc* d,
+                                         llambda_hip_attention_session** result) {
+  return guarded([&] {
+    const char* what = "attention_session_create";
+    if (!result) failf("%s: null result pointer", what);
+    *result = nullptr;
+    if (!d) failf("%s: null description", what);
+    auto in = [&](int64_t v, int64_t lo, int64_t hi, const char* name) {
+      if (v < lo || v > hi)
+        failf("%s: %s %lld is not in %lld..%lld", what, name, (long long)v, (long long)lo, (long long)hi);
+    };
+    in(d->heads, 1, 1024, "heads");
+    in(d->kv_heads, 1, d->heads, "kv_heads");
+    if (d->heads % d->kv_heads)
+      failf("%s: %lld kv_heads do not divide %lld heads", what, (long long)d->kv_heads, (long long)d->heads);
+    in(d->head_dim, 16, kAttnMaxHeadDim, "head_dim");
+    if (d->head_dim % 16) failf("%s: head_dim %lld is not a multiple of 16", what, (long long)d->head_dim);
+    if (!(d->scale >= 0.f && std::isfinite(d->scale))) failf("%s: scale %g", what, (double)d->scale);
+    const bool types = d->row_type == kAttnF32
+                           ? d->cache_type == kAttnF32 || d->cache_type == kAttnF16 || d->cache_type == kAttnBF16
+                           : d->row_type == d->cache_type && (d->row_type == kAttnF16 || d->row_type == kAttnBF16);
+    if (!types) failf("%s: no rows of type %d over a cache of type %d", what, d->row_type, d->cache_type);
+    in(d->page_tokens, 16, 1 << 20, "page_tokens");
+    if (d->page_tokens & (d->page_tokens - 1))
+      failf("%s: page_tokens %lld is not a power of two", what, (long long)d->page_tokens);
+    in(d->layers, 1, 4096, "layers");
+    in(d->pages, 1, INT32_MAX, "pages");
+    in(d->max_context, 1, 1 << 30, "max_context");
+    in(d->max_tokens, 1, 1 << 20, "max_tokens");
+    in(d->max_sequences, 1, 65535, "max_sequences");
+    if (!d->key_pages != !d->value_pages) failf("%s: one pool without the other", what);
+    if ((reinterpret_cast<uintptr_t>(d->key_pages) | reinterpret_cast<uintptr_t>(d->value_pages)) & 15u)
+      failf("%s: pools must be 16-byte aligned", what);
+    std::unique_ptr<llambda_hip_attention_session> s(new llambda_hip_attention_session());
+    AttnPlan& p = s->plan;
+    p.heads = (int)d->heads;
+    p.kv_heads = (int)d->kv_heads;
+    p.group = (int)(d->heads / d->kv_heads);
+    p.head_dim = (int)d->head_dim;
+    p.row_type = d->row_type;
+    p.cache_type = d->cache_type;
+    p.scale = d->scale > 0.f ? d->scale : (float)(1.0 / std::sqrt((double)d->head_dim));
+    p.layers = (int)d->layers;
+    p.pages = (int)d->pages;
+    while (s->page_tokens() < d->page_tokens) ++p.page_shift;
+    p.max_context = (int)d->max_context;
+    p.max_tokens = (int)d->max_tokens;
+    p.max_sequences = (int)d->max_sequences;
+    // a whole pool's bytes in 64 bits
+    const double pool = (double)p.layers * p.pages * s->page_tokens() * s->kv_elements() * s->cell_bytes();
+    if (pool > 1e15) failf("%s: a pool of %.3g bytes", what, pool);
+    s->device = current_device_checked();
+    HIPC(hipStreamCreateWithFlags(&s->stream, hipStreamNonBlocking));
+    HIPC(hipEventCreateWithFlags(&s->done, hipEventDisableTiming));
+    if (d->key_pages) {
+      p.keys = d->key_pages;
+      p.values = d->value_pages;
+    } else {
+      const size_t n = (size_t)p.layers * p.pages * s->page_tokens() * s->kv_elements() * s->cell_bytes();
+      s->pool_keys.alloc(n, "key pages");
+      s->pool_values.alloc(n, "value pages");
+      HIPC(hipMemsetAsync(s->pool_keys.ptr, 0, n, s->stream));
+      HIPC(hipMemsetAsync(s->pool_values.ptr, 0, n, s->stream));
+      p.keys = s->pool_keys.ptr;
+      p.values = s->pool_values.ptr;
+    }
+    const AttnSizes sizes = attn_sizes(p);
+    s->error.alloc(2 * sizeof(int), "error flags");
+    s->run.alloc((size_t)p.max_sequences * sizeof(int), "sequences to run");
+    s->items.alloc((size_t)sizes.items * sizeof(AttnItem), "attention items");
+    s->joins.alloc((size_t)sizes.joins * sizeof(AttnJoin), "attention joins");
+    s->counts.alloc(2 * sizeof(int), "item counts");
+    s->tree.alloc((size_t)p.max_tokens * kAttnTreeWords * sizeof(uint32_t), "ancestors");
+    s->part_y.alloc((size_t)sizes.part_rows * attn_padded(p.head_dim) * sizeof(float), "partial results");
+    s->part_ml.alloc((size_t)sizes.part_rows * sizeof(float2), "partial sums");
+    p.error = s->error.as<int>();
+    p.run = s->run.as<int>();
+    p.items = s->items.as<AttnItem>();
+    p.joins = s->joins.as<AttnJoin>();
+    p.counts = s->counts.as<int>();
+    p.tree = s->tree.as<uint32_t>();
+    p.part_y = s->part_y.as<float>();
+    p.part_ml = s->part_ml.as<float2>();
+    HIPC(hipMemsetAsync(p.error, 0, 2 * sizeof(int), s->stream));
+    HIPC(hipStreamSynchronize(s->stream));
+    *result = s.release();
+  });
+}
+
+void llambda_hip_attention_session_destroy(llambda_hip_attention_session* session) { delete session; }
+
+int llambda_hip_attention_session_run_device(llambda_hip_attention_session* s, int64_t layer,
+                                             const llambda_hip_attention_rows* rows,
+                                             const llambda_hip_attention_batch* batch, void* stream) {
+  return guarded([&] {
+    if (!s) failf("attention_session_run_device: null session");
+    const AttnCall c = attention_call(s, layer, rows, batch);
+    std::lock_guard<std::mutex> lock(s->run_mutex);
+    DeviceScope scope(s->device);
+    attention_enqueue(s, c, stream ? static_cast<hipStream_t>(stream) : s->stream);
+  });
+}
+
+int llambda_hip_attention_session_run(llambda_hip_attention_session* s, int64_t layer, const void* q, const void* k,
+                                      const void* v, void* output, size_t tokens, int64_t context,
+                                      const int32_t* table, const int32_t* parents) {
+  return guarded([&] {
+    const char* what = "attention_session_run";
+    if (!s) failf("%s: null session", what);
+    if (!q || !k || !v || !output || !table) failf("%s: null argument", what);
+    const AttnPlan& p = s->plan;
+    if (layer < 0 || layer >= p.layers) failf("%s: layer %lld is not in 0..%d", what, (long long)layer, p.layers - 1);
+    if (tokens == 0 || tokens > (size_t)p.max_tokens)
+      failf("%s: %zu tokens are not in 1..%d", what, tokens, p.max_tokens);
+    if (context < 0 || context > p.max_context - (int64_t)tokens)
+      failf("%s: %zu tokens behind %lld do not fit the context %d", what, tokens, (long long)context, p.max_context);
+    const int64_t n = (int64_t)tokens, width = attn_table_width(p);
+    const int64_t entries = (context + n + s->page_tokens() - 1) >> p.page_shift;
+    for (int64_t e = 0; e < entries; ++e)
+      if (table[e] < 0 || table[e] >= p.pages)
+        failf("%s: page %d of entry %lld is not in 0..%d", what, table[e], (long long)e, p.pages - 1);
+    if (parents) {
+      if (n > kAttnTreeNodes) failf("%s: a tree of %lld nodes, at most %d", what, (long long)n, kAttnTreeNodes);
+      for (int64_t j = 0; j < n; ++j)
+        if (parents[j] < -1 || parents[j] >= j)
+          failf("%s: parent %d of node %lld is no earlier node", what, parents[j], (long long)j);
+    }
+    std::lock_guard<std::mutex> lock(s->run_mutex);
+    DeviceScope scope(s->device);
+    const size_t qb = s->q_elements() * s->row_bytes(), kb = s->kv_elements() * s->row_bytes();
+    if (n > s->staged_tokens) {
+      s->staged_tokens = 0;
+      s->q.alloc(n * qb, "attention q");
+      s->k.alloc(n * kb, "attention k");
+      s->v.alloc(n * kb, "attention v");
+      s->y.alloc(n * qb, "attention output");
+      s->staged_tokens = n;
+    }
+    const int64_t lists = 3 + kAttnTreeNodes + width;
+    if (!s->lists.ptr) s->lists.alloc(lists * sizeof(int32_t), "attention lists");
+    std::vector<int32_t> list(3 + kAttnTreeNodes + entries);
+    list[1] = (int32_t)n;
+    list[2] = (int32_t)context;
+    if (parents) std::copy_n(parents, n, list.data() + 3);
+    std::copy_n(table, entries, list.data() + 3 + kAttnTreeNodes);
+    HIPC(hipMemcpyAsync(s->lists.ptr, list.data(), list.size() * sizeof(int32_t), hipMemcpyHostToDevice, s->stream));
+    HIPC(hipMemcpyAsync(s->q.ptr, q, n * qb, hipMemcpyHostToDevice, s->stream));
+    HIPC(hipMemcpyAsync(s->k.ptr, k, n * kb, hipMemcpyHostToDevice, s->stream));
+    HIPC(hipMemcpyAsync(s->v.ptr, v, n * kb, hipMemcpyHostToDevice, s->stream));
+    const int* dl = s->lists.as<int>();
+    const AttnCall c{s->q.ptr, s->k.ptr, s->v.ptr, s->y.ptr, (int64_t)s->q_elements(), (int64_t)s->kv_elements(),
+                     (int64_t)s->kv_elements(), (int64_t)s->q_elements(), (int)layer, (int)n, 1, dl, dl + 2,
+                     dl + 3 + kAttnTreeNodes, width, parents ? dl + 3 : nullptr};
+    attention_enqueue(s, c, s->stream);
+    HIPC(hipMemcpyAsync(output, s->y.ptr, n * qb, hipMemcpyDeviceToHost, s->stream));
+    HIPC(hipStreamSynchronize(s->stream));
+  });
+}
+
+int llambda_hip_attention_session_accept_device(llambda_hip_attention_session* s, const int32_t* context,
+                                                const int32_t* table, size_t table_stride, const int32_t* paths,
+                                                size_t path_stride, const int32_t* counts, size_t sequences,
+                                                void* stream) {
+  return guarded([&] {
+    const char* what = "attention_session_accept_device";
+    if (!s) failf("%s: null session", what);
+    if (!context || !table || !paths || !counts) failf("%s: null argument", what);
+    if ((reinterpret_cast<uintptr_t>(context) | reinterpret_cast<uintptr_t>(table) |
+         reinterpret_cast<uintptr_t>(paths) | reinterpret_cast<uintptr_t>(counts)) & 3u)
+      failf("%s: lists must be 4-byte aligned", what);
+    if (sequences == 0 || sequences > (size_t)s->plan.max_sequences)
+      failf("%s: %zu sequences are not in 1..%d", what, sequences, s->plan.max_sequences);
+    const size_t width = (size_t)attn_table_width(s->plan);
+    if (!table_stride) table_stride = width;
+    if (table_stride < width || table_stride > INT32_MAX)
+      failf("%s: table rows of %zu entries, %zu are needed", what, table_stride, width);
+    if (path_stride == 0 || path_stride > INT32_MAX) failf("%s: paths of %zu entries", what, path_stride);
+    const AttnAccept a{context, table, (int64_t)table_stride, paths, (int64_t)path_stride, counts, (int)sequences};
+    std::lock_guard<std::mutex> lock(s->run_mutex);
+    DeviceScope scope(s->device);
+    const hipStream_t st = stream ? static_cast<hipStream_t>(stream) : s->stream;
+    attention_ordered(s, st, [&] { return attn_accept_launch(s->plan, a, st); });
+  });
+}
+
+int llambda_hip_attention_session_sync(llambda_hip_attention_session* s, void* stream) {
+  return guarded([&] {
+    if (!s) failf("attention_session_sync: null session");
+    std::lock_guard<std::mutex> lock(s->run_mutex);
+    DeviceScope scope(s->device);
+    s->raise_error(stream ? static_cast<hipStream_t>(stream) : s->stream);
+  });
+}
+
+int llambda_hip_attention_session_write(llambda_hip_attention_session* s, int64_t layer, const int32_t* table,
+                                        int64_t first, int64_t count, const void* keys, const void* values) {
+  return guarded([&] {
+    attention_copy(s, "attention_session_write", layer, table, first, count, const_cast<void*>(keys),
+                   const_cast<void*>(values), true);
+  });
+}
+
+int llambda_hip_attention_session_read(llambda_hip_attention_session* s, int64_t layer, const int32_t* table,
+                                       int64_t first, int64_t count, void* keys, void* values) {
+  return guarded([&] {
+    attention_copy(s, "attention_session_read", layer, table, first, count, keys, values, false);
   });
 }
 

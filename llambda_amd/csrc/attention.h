@@ -1,0 +1,112 @@
+// attention.h -- attention of new rows of several sequences over a paged cache
+// (attention.hip, attention_tile.h).
+//
+// Sequence i has c cached tokens and n new rows.  The rows' keys and values are
+// rounded to the cache's type and put at positions c .. c + n - 1; then, per row
+// r and head h (of kv head h / group), over the positions j that the row sees,
+//   s_j = scale q . K_j,   p = softmax(s),   y = sum_j p_j V_j
+// A row sees j <= c + r, or, as a node of a tree, j < c, itself and its ancestors.
+// Position j of a sequence is row j % page of page table[i][j / page] of the pool
+// [layers][pages][kv_heads][page][head_dim].
+#pragma once
+
+#include "common.h"
+
+namespace llhip {
+
+constexpr int kAttnMaxHeadDim = 256;
+constexpr int kAttnTreeNodes = 256;                    // nodes of a tree, at most
+constexpr int kAttnTreeWords = kAttnTreeNodes / 32;
+
+enum AttnType : int { kAttnF32 = 0, kAttnF16 = 1, kAttnBF16 = 30 };  // GGML's tags
+
+enum AttnError : int {
+  kAttnErrOffsets = 1,  // offsets not ascending within the call's tokens
+  kAttnErrContext = 2,  // more tokens than the session's context, or fewer than none
+  kAttnErrPage = 4,     // a page outside the pool
+  kAttnErrTree = 8,     // a parent that is no earlier node, or too many nodes
+  kAttnErrPath = 16,    // an accepted path that does not ascend
+};
+
+// Rows of one sequence and a range of its positions: a workgroup's work for one kv head.
+// Row m of a sequence's kv head is token m / group, head m % group of the group.
+struct AttnItem {
+  int sequence, begin, length, context;  // the sequence's first row in the call, its rows, cached tokens
+  int m0, key0, key1;
+  int part;                              // -1: all it sees; else where in the partial results it goes
+};
+// Rows whose range of positions several items share.
+struct AttnJoin {
+  int begin, length, m0, parts, part0, sequence;
+};
+
+struct AttnPlan {
+  int heads, kv_heads, group, head_dim;
+  int row_type, cache_type;
+  float scale;
+  int layers, pages, page_shift;
+  int max_context, max_tokens, max_sequences;
+  void* keys;
+  void* values;
+  int* error;  // [2]: AttnErrors of the calls since they were last taken, those taken
+  // workspace of a call
+  int* run;             // [max_sequences]: 0: refused, nothing of it is read or written
+  AttnItem* items;      // [attn_max_items]
+  AttnJoin* joins;      // [attn_max_joins]
+  int* counts;          // items, joins
+  uint32_t* tree;       // [max_tokens][kAttnTreeWords]: a row's ancestors and itself
+  float* part_y;        // [part][kv_heads][tile rows][padded head_dim]
+  float2* part_ml;      // [part][kv_heads][tile rows]: reference exponent and sum
+};
+
+struct AttnCall {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* y;
+  int64_t q_stride, k_stride, v_stride, y_stride;  // elements from row to row
+  int layer, tokens, sequences;
+  const int* offsets;   // [sequences + 1], null: one row each
+  const int* context;   // [sequences]
+  const int* table;     // [sequences][table_stride]
+  int64_t table_stride;
+  const int* parents;   // [tokens], null: causal
+};
+
+struct AttnAccept {
+  const int* context;
+  const int* table;
+  int64_t table_stride;
+  const int* paths;     // [sequences][path_stride]
+  int64_t path_stride;
+  const int* counts;    // [sequences]
+  int sequences;
+};
+
+// Workspace for calls of at most max_tokens and max_sequences.
+struct AttnSizes {
+  int64_t items, joins, part_rows;  // part_rows: rows of part_ml; part_y has attn_padded(head_dim) floats for each
+};
+AttnSizes attn_sizes(const AttnPlan& p);
+inline int attn_padded(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+inline int attn_table_width(const AttnPlan& p) { return (p.max_context + (1 << p.page_shift) - 1) >> p.page_shift; }
+
+// Whether a call's launches have grids that exist.
+bool attn_call_fits(const AttnPlan& p, const AttnCall& c);
+hipError_t attn_run_launch(const AttnPlan& p, const AttnCall& c, hipStream_t stream);
+hipError_t attn_accept_launch(const AttnPlan& p, const AttnAccept& a, hipStream_t stream);
+hipError_t attn_take_error_launch(const AttnPlan& p, hipStream_t stream);
+
+// How a call is cut: rows of an item, keys of a part at least, workgroups the device holds.
+struct AttnCut {
+  bool shared;      // the waves of a workgroup share a tile of keys (and have rows of their own), or the reverse
+  int rows;         // of an item
+  int min_keys;     // of a part
+  int slots;        // parts over all kv heads come to about this many workgroups
+};
+// The kernels of one cache type (attention_f16.hip, attention_bf16.hip, attention_f32.hip).
+hipError_t attn_attend_f16(const AttnPlan& p, const AttnCall& c, const AttnCut& cut, uint32_t grid, hipStream_t s);
+hipError_t attn_attend_bf16(const AttnPlan& p, const AttnCall& c, const AttnCut& cut, uint32_t grid, hipStream_t s);
+hipError_t attn_attend_f32(const AttnPlan& p, const AttnCall& c, const AttnCut& cut, uint32_t grid, hipStream_t s);
+
+}  // namespace llhip

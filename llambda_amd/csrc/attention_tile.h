@@ -1,0 +1,753 @@
+// attention_tile.h -- the attention kernels over one range of positions (attention.h).
+//
+// A wavefront takes 32 rows and forms both products transposed, S^T = K Q^T and
+// Y^T = V^T P^T, on 32 x 32 tiles: a lane then holds one row of the softmax, half
+// of its keys, so maximum, sum and every factor of a row are that lane's own (one
+// exchange with lane ^ 32), and the results of S^T are the operand P^T of the
+// second product without a move: which key an operand's K element stands for is
+// free as long as both operands agree, and the lane's keys 8 i + 4 (lane / 32) +
+// 0..3 are what two transposing LDS reads bring of V.
+//
+// Softmax runs over the keys once, with the running maximum and sum in fp32.
+//
+// Operands.  A cache in 16 bits is an operand as it is.  fp32 rows, and the fp32
+// probabilities of such rows, are split into parts of the cache's type whose
+// products are added: two of f16 (22 bits; q times a power of two for each row, p
+// times 2^15, so that the parts stay normal), three of bf16 (24 bits).  Rows in 16
+// bits are one part, and so are their probabilities: rounding those to 8 or 11 bits
+// costs what rounding the output costs.  An fp32 cache uses the fp32 products.
+//
+// Keys and values pass through LDS, loaded there directly, a tile ahead, 16-byte
+// pieces permuted so that neither read meets a bank twice.
+#pragma once
+
+#include "attention.h"
+#include "mfma.h"
+
+namespace llhip {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+typedef _Float16 halfx4 __attribute__((ext_vector_type(4)));
+typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) const uint8_t* lds_bytes;
+__device__ __forceinline__ lds_bytes lds_at(uint32_t address) { return reinterpret_cast<lds_bytes>(address); }
+
+__device__ __forceinline__ float half_pair_max(float v) {
+  float a = v, b = v;
+  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+  return fmaxf(a, b);
+}
+
+// ---------------------------------------------------------------- operands
+template <int TYPE>
+struct Cell;
+template <>
+struct Cell<kAttnF16> {
+  typedef _Float16 T;
+  typedef halfx8 Frag;
+  static constexpr float kLift = 15.f;  // p times 2^15: down to 2^-29 its first part is a normal number
+  static __device__ __forceinline__ floatx16 mfma(Frag a, Frag b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{a, b}, halfx2));
+  }
+  static __device__ __forceinline__ floatx2 unpack(uint32_t v) {
+    return __builtin_convertvector(__builtin_bit_cast(halfx2, v), floatx2);
+  }
+};
+template <>
+struct Cell<kAttnBF16> {
+  typedef __bf16 T;
+  typedef bf16x8 Frag;
+  static constexpr float kLift = 0.f;
+  static __device__ __forceinline__ floatx16 mfma(Frag a, Frag b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{a, b}, bf16x2));
+  }
+  static __device__ __forceinline__ floatx2 unpack(uint32_t v) {
+    return floatx2{__builtin_bit_cast(float, v << 16), __builtin_bit_cast(float, v & 0xFFFF0000u)};
+  }
+};
+
+// Parts of the cache's type that a number of the rows' type takes.
+template <int TYPE, typename Row>
+constexpr int attn_parts() {
+  return sizeof(Row) == 2 ? 1 : TYPE == kAttnF16 ? 2 : 3;
+}
+
+// (a, b) as N packed pairs whose sums they are.
+template <int TYPE, int N>
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t (&out)[N]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    out[n] = Cell<TYPE>::pack(a, b);
+    if (n + 1 < N) {
+      const floatx2 u = Cell<TYPE>::unpack(out[n]);
+      a -= u.x;
+      b -= u.y;
+    }
+  }
+}
+
+template <typename Row>
+__device__ __forceinline__ void load8(const Row* p, float (&v)[8]) {
+  if constexpr (sizeof(Row) == 4) {
+    const floatx4 a = *reinterpret_cast<const floatx4*>(p), b = *reinterpret_cast<const floatx4*>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+  } else {
+    typedef Row Row8 __attribute__((ext_vector_type(8)));
+    const Row8 a = *reinterpret_cast<const Row8*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
+  }
+}
+template <typename Row>
+__device__ __forceinline__ void store4(Row* p, floatx4 v) {
+  if constexpr (sizeof(Row) == 4) {
+    *reinterpret_cast<floatx4*>(p) = v;
+  } else {
+    typedef Row Row4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<Row4*>(p) = __builtin_convertvector(v, Row4);
+  }
+}
+
+// ------------------------------------------------------------------- layout
+// A tile of keys (or values) in LDS: rows of kRow bytes, their 16-byte pieces permuted.
+template <int SIZE, int DP>
+struct TileLayout {
+  static constexpr int kRow = DP * SIZE;
+  static constexpr int kPieces = kRow / 16;
+  static constexpr int kRowsPerLoad = 64 / kPieces;  // 64 lanes load 16 bytes each
+  // Where a piece of keys goes: 16-byte reads of 16 rows (rows n and n + 8 among them) fill the banks once.
+  static __device__ __forceinline__ int key_swizzle(int row) { return kPieces == 8 ? (row >> 1) & 7 : row & 15; }
+  // Of values in 16 bits: transposing reads of 64 bytes of 4 neighbouring rows do.  fp32 reads need none.
+  static __device__ __forceinline__ int value_swizzle(int row) {
+    return SIZE == 4 ? 0 : kPieces == 8 ? 4 * ((row >> 1) & 1) : 4 * (row & 3);
+  }
+};
+
+// The pages of one kv head of one sequence, for loads of tiles into LDS.
+template <int SIZE, int DP, int KT>
+struct TileLoader {
+  typedef TileLayout<SIZE, DP> L;
+  static constexpr int kLoads = KT / L::kRowsPerLoad;  // of keys, and of values, by one wavefront
+  const uint8_t* keys;
+  const uint8_t* values;
+  int kv_heads, head, page_shift, head_dim;
+  int last;  // the sequence's last position; tiles past it hold rows near it again
+
+  // Lane l's page: the one of position base + l.
+  __device__ __forceinline__ int entry(int base, int lane) const {
+    return min(base + lane, last) >> page_shift;
+  }
+  // Loads [from, kLoads) in steps of `step`, of tile `base`; pages: entry()'s, by lane.
+  __device__ __forceinline__ void load(int base, int pages, uint32_t lds_k, uint32_t lds_v, int from, int step,
+                                       int lane) const {
+    constexpr int R = L::kRowsPerLoad;
+    const int row = lane / L::kPieces, piece = lane % L::kPieces;
+    const int bytes = head_dim * SIZE;
+    for (int i = from; i < kLoads; i += step) {
+      const int r0 = i * R;
+      const int pos = min(base + r0, last & ~(R - 1));
+      const int page = __builtin_amdgcn_readlane(pages, r0);
+      const int64_t at =
+          ((((int64_t)page * kv_heads + head) << page_shift) + (pos & ((1 << page_shift) - 1))) * bytes;
+      int pk = piece ^ L::key_swizzle(r0 + row), pv = piece ^ L::value_swizzle(r0 + row);
+      // a row shorter than the tile's: its first piece again (the row's q has zeros there, its y is not stored)
+      if (16 * pk >= bytes) pk = 0;
+      if (16 * pv >= bytes) pv = 0;
+      load_lds16(keys + at, (uint32_t)(row * bytes + 16 * pk), lds_k + 1024u * i);
+      load_lds16(values + at, (uint32_t)(row * bytes + 16 * pv), lds_v + 1024u * i);
+    }
+  }
+};
+
+// ---------------------------------------------------------- a wavefront's rows
+// Bits of the keys base .. base + 31 that a lane's row sees.
+struct Sight {
+  int limit;             // causal: positions below it; a tree's: the cached ones
+  const uint32_t* tree;  // null: causal
+  __device__ __forceinline__ uint32_t bits(int base) const {
+    const int n = limit - base;
+    if (!tree) return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1;
+    if (n >= 32) return ~0u;
+    if (n > 0) return ((1u << n) - 1) | (tree[0] << n);
+    const int w = -n >> 5, s = -n & 31;
+    if (w >= kAttnTreeWords) return 0;
+    const uint32_t lo = tree[w], hi = w + 1 < kAttnTreeWords ? tree[w + 1] : 0;
+    return (uint32_t)((((uint64_t)hi << 32) | lo) >> s);
+  }
+};
+
+// Sums of 32 rows over the keys so far: y holds rows 32 b + 8 (i / 4) + 4 (lane / 32) + i % 4 of Y^T, column lane % 32.
+template <int DP>
+struct RowSums {
+  floatx16 y[DP / 32];
+  float reference;  // the exponent that p is taken against; -inf: no key yet
+  float sum;        // of this lane's keys
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b) y[b] = floatx16{};
+    reference = -__builtin_inff();
+    sum = 0.f;
+  }
+  template <int KB>
+  __device__ __forceinline__ void spoil(const uint32_t* bits, const uint32_t (&sight)[KB], int half) {
+    uint32_t bad[DP / 32] = {};
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+      for (int k = 0; k < 32; ++k)
+        if (sight[b] >> k & 1)
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d) bad[d] |= bits[(32 * b + k) * (DP / 32) + d];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        y[d][i] = bad[d] >> (8 * (i / 4) + 4 * half + i % 4) & 1 ? __builtin_nanf("") : y[d][i];
+  }
+  // The scores s of KB blocks of 32 keys become probabilities.
+  template <int KB>
+  __device__ __forceinline__ void softmax(floatx16 (&s)[KB], float factor, float lift) {
+    float top = s[0][0];
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+    top = half_pair_max(top) * factor;
+    if (__ballot(top > reference)) {
+      const float next = fmaxf(reference, top);
+      // a row that has seen nothing has nothing to scale (and no reference)
+      const float scale = next == reference ? 1.f : __builtin_amdgcn_exp2f(reference - next);
+      reference = next;
+      sum *= scale;
+#pragma unroll
+      for (int b = 0; b < DP / 32; ++b) y[b] *= scale;
+    }
+    const float shift = lift - (reference == -__builtin_inff() ? 0.f : reference);
+    float part[4] = {};
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], factor, shift));
+        part[i & 3] += s[b][i];
+      }
+    sum += (part[0] + part[1]) + (part[2] + part[3]);
+  }
+};
+
+template <int KB>
+__device__ __forceinline__ void mask_scores(floatx16 (&s)[KB], const uint32_t (&sight)[KB], int half) {
+#pragma unroll
+  for (int b = 0; b < KB; ++b) {
+    const uint32_t v = sight[b] >> (4 * half);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[b][i] = v >> (8 * (i / 4) + i % 4) & 1 ? s[b][i] : -__builtin_inff();
+  }
+}
+
+// Values that are infinite or NaN, where a row may see only part of a tile: a masked probability of 0 would make NaN
+// of them.  They become zeros in LDS, noted by key and element, and rows that see one get NaN there afterwards.
+template <int SIZE, int DP, int KT>
+struct Spoiled {
+  static constexpr int kWords = DP / 32;
+  static constexpr int kBytes = (KT * kWords + 1) * 4;
+  uint32_t* bits;  // LDS: [KT][kWords], then whether there are any
+  __device__ __forceinline__ void clear(int thread, int threads) const {
+    for (int i = thread; i <= KT * kWords; i += threads) bits[i] = 0;
+  }
+  // The tile at `tile`, by `threads` threads; the words are clear.
+  __device__ __forceinline__ void scan(uint8_t* tile, int thread, int threads) const {
+    typedef TileLayout<SIZE, DP> L;
+    for (int i = thread; i < KT * L::kPieces; i += threads) {
+      u32x4 v = *reinterpret_cast<const u32x4*>(tile + 16 * i);
+      const int key = i / L::kPieces;
+      const int d = ((i % L::kPieces) ^ L::value_swizzle(key)) * (16 / SIZE);
+      uint32_t bad = 0;
+      if constexpr (SIZE == 4) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if ((v[k] & 0x7F800000u) == 0x7F800000u) bad |= 1u << k, v[k] = 0;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if ((v[k / 2] >> (16 * (k & 1)) & exponent) == exponent)
+            bad |= 1u << k, v[k / 2] &= k & 1 ? 0xFFFFu : 0xFFFF0000u;
+      }
+      if (bad) {
+        *reinterpret_cast<u32x4*>(tile + 16 * i) = v;
+        atomicOr(bits + key * kWords + d / 32, bad << (d % 32));
+        bits[KT * kWords] = 1;
+      }
+    }
+  }
+  __device__ __forceinline__ bool any() const { return __builtin_amdgcn_readfirstlane(bits[KT * kWords]) != 0; }
+  uint32_t exponent;  // of 16 bits
+};
+
+template <int TYPE, typename Row, int DP>
+struct RowTile {
+  typedef Cell<TYPE> C;
+  typedef typename C::Frag Frag;
+  typedef TileLayout<2, DP> L;
+  static constexpr int N = attn_parts<TYPE, Row>(), kSteps = DP / 16, kBlocks = DP / 32;
+  Frag q[N][kSteps];
+  RowSums<DP> sums;
+  float factor;  // of the products, into exponents of two
+  uint32_t key_at, value_at;
+  int half;
+
+  // row: null for rows behind the last.  Lane l holds elements 16 s + 8 (l / 32) + 0..7 of row l % 32.
+  __device__ __forceinline__ void start(const Row* row, int head_dim, float scale_log2, int lane) {
+    half = lane >> 5;
+    sums.clear();
+    const int r = lane & 31, j = lane & 15;
+    key_at = r * L::kRow + 16 * (half ^ L::key_swizzle(r));
+    value_at = (4 * half + (j >> 2)) * L::kRow + 16 * L::value_swizzle(j >> 2) + ((lane >> 4) & 1) * 32 + (j & 3) * 8;
+    float v[kSteps][8], top = 0.f;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[s][i] = 0.f;
+      if (row && 16 * s < head_dim) load8(row + 16 * s + 8 * half, v[s]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[s][i]));
+    }
+    float lift = 1.f;
+    if (N == 2) {
+      // the row's largest between 2^13 and 2^14 (rows next to zero, infinities and NaN as they are)
+      top = half_pair_max(top);
+      const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23);
+      if (e > 20 && e < 255) {
+        lift = __builtin_bit_cast(float, (uint32_t)(127 + 13 + 127 - e) << 23);
+        factor = scale_log2 * __builtin_bit_cast(float, (uint32_t)(e - 13) << 23);
+      } else {
+        factor = scale_log2;
+      }
+    } else {
+      factor = scale_log2;
+    }
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      u32x4 packed[N];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t p[N];
+        split_pair<TYPE, N>(v[s][2 * i] * lift, v[s][2 * i + 1] * lift, p);
+#pragma unroll
+        for (int n = 0; n < N; ++n) packed[n][i] = p[n];
+      }
+#pragma unroll
+      for (int n = 0; n < N; ++n) q[n][s] = __builtin_bit_cast(Frag, packed[n]);
+    }
+  }
+
+  // KB blocks of 32 keys at LDS addresses lds_k, lds_v; sight: what each lane's row sees of them, if masked.
+  template <int KB>
+  __device__ __forceinline__ void tile(uint32_t lds_k, uint32_t lds_v, bool masked, const uint32_t (&sight)[KB]) {
+    floatx16 s[KB];
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+      s[b] = floatx16{};
+#pragma unroll
+      for (int t = 0; t < kSteps; ++t) {
+        const Frag k = *reinterpret_cast<const __attribute__((address_space(3))) Frag*>(
+            lds_at(lds_k + (key_at ^ (32u * t))) + 32 * b * L::kRow);
+#pragma unroll
+        for (int n = 0; n < N; ++n) s[b] = C::mfma(k, q[n][t], s[b]);
+      }
+    }
+    if (masked) mask_scores(s, sight, half);
+    sums.softmax(s, factor, C::kLift);
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        u32x4 packed[N];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t p[N];
+          split_pair<TYPE, N>(s[b][8 * t + 2 * i], s[b][8 * t + 2 * i + 1], p);
+#pragma unroll
+          for (int n = 0; n < N; ++n) packed[n][i] = p[n];
+        }
+#pragma unroll
+        for (int d = 0; d < kBlocks; ++d) {
+          const Frag v = __builtin_bit_cast(Frag, value(lds_v, 32 * b + 16 * t, d));
+#pragma unroll
+          for (int n = 0; n < N; ++n)
+            sums.y[d] = C::mfma(v, __builtin_bit_cast(Frag, packed[n]), sums.y[d]);
+        }
+      }
+  }
+
+  // Keys key .. key + 15, elements 32 d .. 32 d + 31: lane l holds element l % 32 of keys 4 (l / 32) + 0..3 and
+  // 8 more on.
+  __device__ __forceinline__ u32x4 value(uint32_t lds_v, int key, int d) const {
+    const lds_bytes at = lds_at(lds_v + (value_at ^ (64u * d)));
+    typedef short shortx4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) shortx4* ptr;
+    const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(at + key * L::kRow)));
+    const u32x2 c = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(at + (key + 8) * L::kRow)));
+    return u32x4{a.x, a.y, c.x, c.y};
+  }
+};
+
+// fp32 rows over an fp32 cache: the 32x32x2 products, lane l's K element is the one of its half.
+template <typename Row, int DP>
+struct RowTile<kAttnF32, Row, DP> {
+  typedef TileLayout<4, DP> L;
+  static constexpr int kSteps = DP / 8, kBlocks = DP / 32;
+  floatx4 q[kSteps];  // elements 8 s + 4 (lane / 32) + 0..3
+  RowSums<DP> sums;
+  float factor;
+  uint32_t key_at, value_at;
+  int half;
+
+  static __device__ __forceinline__ floatx16 mfma(float a, float b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
+  }
+  __device__ __forceinline__ void start(const Row* row, int head_dim, float scale_log2, int lane) {
+    half = lane >> 5;
+    sums.clear();
+    const int r = lane & 31;
+    key_at = r * L::kRow + 16 * (half ^ L::key_swizzle(r));
+    value_at = 4 * half * L::kRow + 4 * r;
+    factor = scale_log2;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+      q[s] = row && 8 * s < head_dim ? *reinterpret_cast<const floatx4*>(row + 8 * s + 4 * half) : floatx4{};
+  }
+  template <int KB>
+  __device__ __forceinline__ void tile(uint32_t lds_k, uint32_t lds_v, bool masked, const uint32_t (&sight)[KB]) {
+    floatx16 s[KB];
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+      s[b] = floatx16{};
+#pragma unroll
+      for (int t = 0; t < kSteps; ++t) {
+        const floatx4 k = *reinterpret_cast<const __attribute__((address_space(3))) floatx4*>(
+            lds_at(lds_k + (key_at ^ (32u * t))) + 32 * b * L::kRow);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[b] = mfma(k[i], q[t][i], s[b]);
+      }
+    }
+    if (masked) mask_scores(s, sight, half);
+    sums.softmax(s, factor, 0.f);
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int d = 0; d < kBlocks; ++d)
+          sums.y[d] = mfma(value(lds_v, 32 * b + 8 * (i / 4) + i % 4, d), s[b][i], sums.y[d]);
+  }
+  __device__ __forceinline__ float value(uint32_t lds_v, int key, int d) const {
+    return *reinterpret_cast<const __attribute__((address_space(3))) float*>(lds_at(lds_v + value_at) +
+                                                                             key * L::kRow + 128 * d);
+  }
+};
+
+// -------------------------------------------------------------------- kernels
+constexpr float kAttnLog2e = 1.44269504088896340736f;
+constexpr int kAttnPageList = 1024;  // entries of a table's row in LDS
+
+template <int TYPE>
+constexpr int attn_cell_bytes() {
+  return TYPE == kAttnF32 ? 4 : 2;
+}
+
+template <int TYPE>
+constexpr uint32_t attn_exponent() {
+  return TYPE == kAttnF16 ? 0x7C00u : 0x7F80u;
+}
+// LDS accesses of this wavefront so far are done before those that follow.
+__device__ __forceinline__ void wave_lds_order() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// What an item's rows are, for one of its wavefronts (32 rows from m on).
+template <typename Row>
+struct ItemRows {
+  int rows;    // of the sequence's kv head
+  int m;       // this lane's
+  int token;   // its token, the last one's for rows behind it
+  bool real;
+  __device__ __forceinline__ ItemRows(const AttnPlan& p, const AttnItem& it, int m0, int lane) {
+    rows = it.length * p.group;
+    m = m0 + (lane & 31);
+    real = m < rows;
+    token = min(m, rows - 1) / p.group;
+  }
+  __device__ __forceinline__ int head(const AttnPlan& p, int kv_head) const {
+    return kv_head * p.group + min(m, rows - 1) % p.group;
+  }
+  __device__ __forceinline__ const Row* q(const AttnPlan& p, const AttnCall& c, const AttnItem& it, int kv_head) const {
+    return real ? static_cast<const Row*>(c.q) + (it.begin + token) * c.q_stride + head(p, kv_head) * p.head_dim
+                : nullptr;
+  }
+  __device__ __forceinline__ Row* y(const AttnPlan& p, const AttnCall& c, const AttnItem& it, int kv_head) const {
+    return static_cast<Row*>(c.y) + (it.begin + token) * c.y_stride + head(p, kv_head) * p.head_dim;
+  }
+  __device__ __forceinline__ Sight sight(const AttnPlan& p, const AttnCall& c, const AttnItem& it) const {
+    if (c.parents) return Sight{it.context, p.tree + (size_t)(it.begin + token) * kAttnTreeWords};
+    return Sight{it.context + token + 1, nullptr};
+  }
+};
+
+// Waves share tiles of KT keys, two of which are in LDS; each has 32 rows of its own.
+template <int TYPE, typename Row, int DP, int WAVES, int KT>
+__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_shared_kernel(AttnPlan p, AttnCall c) {
+  constexpr int SIZE = attn_cell_bytes<TYPE>(), KB = KT / 32;
+  typedef TileLoader<SIZE, DP, KT> Loader;
+  constexpr uint32_t kTile = KT * DP * SIZE;
+  extern __shared__ __align__(16) uint8_t lds[];
+  const int index = blockIdx.x / p.kv_heads, kv_head = blockIdx.x % p.kv_heads;
+  if (index >= p.counts[0]) return;
+  const AttnItem it = p.items[index];
+  if (!p.run[it.sequence]) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m0 = it.m0 + 32 * wave;
+  const ItemRows<Row> rows(p, it, m0, lane);
+  const bool any = m0 < rows.rows;
+  const Sight sight = rows.sight(p, c, it);
+  // below all_sure every row of the item sees everything, from end on none of this wavefront's sees anything
+  const int all_sure = c.parents ? it.context : it.context + it.m0 / p.group + 1;
+  const int end = !any ? 0 : it.context + (c.parents ? it.length : min(m0 + 31, rows.rows - 1) / p.group + 1);
+  const Spoiled<SIZE, DP, KT> spoiled{reinterpret_cast<uint32_t*>(lds + 4 * kTile), attn_exponent<TYPE>()};
+  spoiled.clear(threadIdx.x, 64 * WAVES);
+  RowTile<TYPE, Row, DP> tile;
+  tile.start(rows.q(p, c, it, kv_head), p.head_dim, p.scale * kAttnLog2e, lane);
+
+  const size_t layer = (size_t)c.layer * p.pages * p.kv_heads * p.head_dim * SIZE << p.page_shift;
+  const Loader loader{static_cast<const uint8_t*>(p.keys) + layer, static_cast<const uint8_t*>(p.values) + layer,
+                      p.kv_heads, kv_head, p.page_shift, p.head_dim, it.context + it.length - 1};
+  const int* table = c.table + it.sequence * c.table_stride;
+  const uint32_t base = lds_address(lds);
+  const int tiles = (it.key1 - it.key0 + KT - 1) / KT;
+  int pages = table[loader.entry(it.key0, lane)];
+  if (tiles > 0) loader.load(it.key0, pages, base, base + kTile, wave, WAVES, lane);
+  pages = table[loader.entry(it.key0 + KT, lane)];
+  for (int t = 0; t < tiles; ++t) {
+    wait_loads<0>();
+    __syncthreads();
+    const int key = it.key0 + t * KT;
+    const uint32_t now = base + (t & 1) * 2 * kTile, next = base + (~t & 1) * 2 * kTile;
+    if (t + 1 < tiles) {
+      loader.load(key + KT, pages, next, next + kTile, wave, WAVES, lane);
+      pages = table[loader.entry(key + 2 * KT, lane)];
+    }
+    const bool partly = key + KT > all_sure;  // for some row of the workgroup
+    if (partly) {
+      spoiled.scan(lds + (now - base) + kTile, threadIdx.x, 64 * WAVES);
+      __syncthreads();
+    }
+    if (key < end) {
+      uint32_t see[KB] = {};
+      if (partly)
+#pragma unroll
+        for (int b = 0; b < KB; ++b) see[b] = sight.bits(key + 32 * b);
+      tile.template tile<KB>(now, now + kTile, partly, see);
+      if (partly && spoiled.any()) tile.sums.template spoil<KB>(spoiled.bits, see, tile.half);
+    }
+    if (partly && spoiled.any()) {
+      __syncthreads();
+      spoiled.clear(threadIdx.x, 64 * WAVES);
+    }
+  }
+  const float sum = half_pair_sum(tile.sums.sum);
+  if (!rows.real) return;
+  if (it.part < 0) {
+    const float scale = 1.f / sum;
+    Row* y = rows.y(p, c, it, kv_head);
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = 32 * b + 8 * i + 4 * tile.half;
+        const floatx4 v{tile.sums.y[b][4 * i], tile.sums.y[b][4 * i + 1], tile.sums.y[b][4 * i + 2],
+                        tile.sums.y[b][4 * i + 3]};
+        if (d < p.head_dim) store4(y + d, v * scale);
+      }
+  } else {
+    const size_t row = ((size_t)it.part * p.kv_heads + kv_head) * (32 * WAVES) + 32 * wave + (lane & 31);
+    if (tile.half == 0) p.part_ml[row] = make_float2(tile.sums.reference, sum);
+    float* y = p.part_y + row * DP;
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<floatx4*>(y + 32 * b + 8 * i + 4 * tile.half) =
+            floatx4{tile.sums.y[b][4 * i], tile.sums.y[b][4 * i + 1], tile.sums.y[b][4 * i + 2],
+                    tile.sums.y[b][4 * i + 3]};
+  }
+}
+
+// Waves share 32 rows and take tiles of 32 keys in turn, each from LDS of its own; their sums are joined at the end.
+template <int TYPE, typename Row, int DP, int WAVES>
+struct SplitLds {
+  static constexpr int kTile = 32 * DP * attn_cell_bytes<TYPE>();
+  static constexpr int kWave = 4 * kTile;           // two tiles of keys and two of values
+  static constexpr int kRow = DP + 4;               // floats of a row of sums, in the same memory
+  static_assert(32 * kRow * 4 <= kWave, "a wavefront's sums fit its tiles");
+  static constexpr int kSpoiled = Spoiled<attn_cell_bytes<TYPE>(), DP, 32>::kBytes / 4;
+  static constexpr int kBytes = WAVES * kWave + WAVES * 64 * 4 + kAttnPageList * 4 + WAVES * kSpoiled * 4;
+};
+
+template <int TYPE, typename Row, int DP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 1) void attn_split_kernel(AttnPlan p, AttnCall c) {
+  constexpr int SIZE = attn_cell_bytes<TYPE>(), KT = 32;
+  typedef TileLoader<SIZE, DP, KT> Loader;
+  typedef SplitLds<TYPE, Row, DP, WAVES> M;
+  constexpr int kLoads = 2 * Loader::kLoads;
+  extern __shared__ __align__(16) uint8_t lds[];
+  float* const ml = reinterpret_cast<float*>(lds + WAVES * M::kWave);  // [WAVES][2][32]
+  int* const list = reinterpret_cast<int*>(ml + WAVES * 64);
+  const int index = blockIdx.x / p.kv_heads, kv_head = blockIdx.x % p.kv_heads;
+  if (index >= p.counts[0]) return;
+  const AttnItem it = p.items[index];
+  if (!p.run[it.sequence]) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const ItemRows<Row> rows(p, it, it.m0, lane);
+  const Sight sight = rows.sight(p, c, it);
+  const int sure = c.parents ? it.context : it.context + it.m0 / p.group + 1;
+  RowTile<TYPE, Row, DP> tile;
+  tile.start(rows.q(p, c, it, kv_head), p.head_dim, p.scale * kAttnLog2e, lane);
+
+  const size_t layer = (size_t)c.layer * p.pages * p.kv_heads * p.head_dim * SIZE << p.page_shift;
+  const Loader loader{static_cast<const uint8_t*>(p.keys) + layer, static_cast<const uint8_t*>(p.values) + layer,
+                      p.kv_heads, kv_head, p.page_shift, p.head_dim, it.context + it.length - 1};
+  const int* table = c.table + it.sequence * c.table_stride;
+  const uint32_t lds_base = lds_address(lds), base = lds_base + wave * M::kWave;
+  const Spoiled<SIZE, DP, KT> spoiled{reinterpret_cast<uint32_t*>(list + kAttnPageList) + wave * M::kSpoiled,
+                                      attn_exponent<TYPE>()};
+  // as many keys at a time as the list has pages for
+  const int stretch = kAttnPageList << p.page_shift;
+  for (int key0 = it.key0; key0 < it.key1;) {
+    const int first = key0 >> p.page_shift;
+    const int key1 = (int)min((int64_t)it.key1, ((int64_t)first << p.page_shift) + stretch);
+    const int entries = loader.entry(key1 - 1, 0) - first + 1;
+    __syncthreads();
+    for (int i = threadIdx.x; i < entries; i += 64 * WAVES) list[i] = table[first + i];
+    __syncthreads();
+    auto load = [&](int key, int buffer) {
+      const int pages = list[min(loader.entry(key, lane) - first, entries - 1)];
+      loader.load(key, pages, base + buffer * 2 * M::kTile, base + buffer * 2 * M::kTile + M::kTile, 0, 1, lane);
+    };
+    int key = key0 + KT * wave;
+    if (key < key1) load(key, 0);
+    for (int t = 0; key < key1; ++t, key += KT * WAVES) {
+      if (key + KT * WAVES < key1) {
+        load(key + KT * WAVES, ~t & 1);
+        wait_loads<kLoads <= 63 ? kLoads : 0>();
+      } else {
+        wait_loads<0>();
+      }
+      const uint32_t now = base + (t & 1) * 2 * M::kTile;
+      uint32_t see[1] = {};
+      const bool partly = key + KT > sure;
+      if (partly) {
+        see[0] = sight.bits(key);
+        spoiled.clear(lane, 64);
+        wave_lds_order();
+        spoiled.scan(lds + (now - lds_base) + M::kTile, lane, 64);
+        wave_lds_order();
+      }
+      tile.template tile<1>(now, now + M::kTile, partly, see);
+      if (partly && spoiled.any()) tile.sums.template spoil<1>(spoiled.bits, see, tile.half);
+      wave_lds_order();  // the next load into this tile's place follows its reads
+    }
+    key0 = key1;
+  }
+  const float sum = half_pair_sum(tile.sums.sum);
+  if (lane < 32) {
+    ml[wave * 64 + lane] = tile.sums.reference;
+    ml[wave * 64 + 32 + lane] = sum;
+  }
+  float* const own = reinterpret_cast<float*>(lds + wave * M::kWave) + (lane & 31) * M::kRow;
+#pragma unroll
+  for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<floatx4*>(own + 32 * b + 8 * i + 4 * tile.half) =
+          floatx4{tile.sums.y[b][4 * i], tile.sums.y[b][4 * i + 1], tile.sums.y[b][4 * i + 2],
+                  tile.sums.y[b][4 * i + 3]};
+  __syncthreads();
+  const int count = min(32, rows.rows - it.m0), pieces = p.head_dim / 4;
+  for (int i = threadIdx.x; i < count * pieces; i += 64 * WAVES) {
+    const int r = i / pieces, d = 4 * (i % pieces);
+    float reference = -__builtin_inff();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) reference = fmaxf(reference, ml[w * 64 + r]);
+    floatx4 v{};
+    float total = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      // a wavefront that saw nothing for this row has zeros
+      const float mine = ml[w * 64 + r];
+      const float weight = mine == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(mine - reference);
+      total += weight * ml[w * 64 + 32 + r];
+      v += weight * *reinterpret_cast<const floatx4*>(lds + w * M::kWave + (r * M::kRow + d) * 4);
+    }
+    if (it.part < 0) {
+      const int m = it.m0 + r;
+      Row* y = static_cast<Row*>(c.y) + (it.begin + m / p.group) * c.y_stride +
+               (kv_head * p.group + m % p.group) * p.head_dim;
+      store4(y + d, v * (1.f / total));
+    } else {
+      const size_t row = ((size_t)it.part * p.kv_heads + kv_head) * 32 + r;
+      if (d == 0) p.part_ml[row] = make_float2(reference, total);
+      *reinterpret_cast<floatx4*>(p.part_y + row * DP + d) = v;
+    }
+  }
+}
+
+// ------------------------------------------------------------------ launches
+template <typename Kernel>
+hipError_t attn_launch(Kernel k, uint32_t grid, int threads, int lds, hipStream_t s, const AttnPlan& p,
+                       const AttnCall& c) {
+  if (lds > 65536) {
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL(k, dim3(grid), dim3(threads), lds, s, p, c);
+  return hipGetLastError();
+}
+
+// Waves of a workgroup that share tiles: eight, two to a SIMD, where rows, sums and probabilities fit 256 registers.
+template <int TYPE, typename Row, int DP>
+constexpr int attn_shared_waves() {
+  return DP == 256 || (TYPE == kAttnBF16 && sizeof(Row) == 4 && DP == 128) ? 4 : 8;
+}
+// Waves that split keys: what LDS holds of their tiles.
+template <int TYPE, int DP>
+constexpr int attn_split_waves() {
+  return DP * attn_cell_bytes<TYPE>() <= 256 ? 4 : DP * attn_cell_bytes<TYPE>() == 512 ? 2 : 1;
+}
+
+template <int TYPE, typename Row, int DP>
+hipError_t attn_attend(const AttnPlan& p, const AttnCall& c, const AttnCut& cut, uint32_t grid, hipStream_t s) {
+  if (cut.shared) {
+    constexpr int W = attn_shared_waves<TYPE, Row, DP>(), KT = DP * attn_cell_bytes<TYPE>() <= 512 ? 64 : 32;
+    return attn_launch(attn_shared_kernel<TYPE, Row, DP, W, KT>, grid, 64 * W, 
+                       4 * KT * DP * attn_cell_bytes<TYPE>() + Spoiled<attn_cell_bytes<TYPE>(), DP, KT>::kBytes, s, p, c);
+  }
+  constexpr int W = attn_split_waves<TYPE, DP>();
+  return attn_launch(attn_split_kernel<TYPE, Row, DP, W>, grid, 64 * W, SplitLds<TYPE, Row, DP, W>::kBytes, s, p, c);
+}
+
+template <int TYPE, typename Row>
+hipError_t attn_attend_width(const AttnPlan& p, const AttnCall& c, const AttnCut& cut, uint32_t grid, hipStream_t s) {
+  switch (attn_padded(p.head_dim)) {
+    case 64: return attn_attend<TYPE, Row, 64>(p, c, cut, grid, s);
+    case 128: return attn_attend<TYPE, Row, 128>(p, c, cut, grid, s);
+    default: return attn_attend<TYPE, Row, 256>(p, c, cut, grid, s);
+  }
+}
+
+}  // namespace llhip

@@ -110,6 +110,28 @@ class SsmDesc(ctypes.Structure):
     ]
 
 
+class AttentionDesc(ctypes.Structure):
+    """llambda_hip_attention_desc."""
+    _fields_ = [
+        ("heads", c_i64), ("kv_heads", c_i64), ("head_dim", c_i64), ("scale", ctypes.c_float),
+        ("row_type", c_int), ("cache_type", c_int), ("layers", c_i64), ("page_tokens", c_i64),
+        ("pages", c_i64), ("max_context", c_i64), ("max_tokens", c_i64), ("max_sequences", c_i64),
+        ("key_pages", c_void_p), ("value_pages", c_void_p),
+    ]
+
+
+class AttentionRows(ctypes.Structure):
+    """llambda_hip_attention_rows."""
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("output", c_void_p),
+                ("q_stride", c_i64), ("k_stride", c_i64), ("v_stride", c_i64), ("output_stride", c_i64)]
+
+
+class AttentionBatch(ctypes.Structure):
+    """llambda_hip_attention_batch."""
+    _fields_ = [("tokens", c_size), ("sequences", c_size), ("offsets", c_void_p), ("context", c_void_p),
+                ("table", c_void_p), ("table_stride", c_size), ("parents", c_void_p)]
+
+
 class RouterDesc(ctypes.Structure):
     """llambda_hip_router_desc."""
     _fields_ = [
@@ -204,6 +226,20 @@ SIGNATURES = {
     "llambda_hip_ssm_session_reset": (c_int, [c_void_p, c_i64]),
     "llambda_hip_ssm_session_write_state": (c_int, [c_void_p, c_i64, c_void_p, c_void_p, c_int]),
     "llambda_hip_ssm_session_read_state": (c_int, [c_void_p, c_i64, c_void_p, c_void_p]),
+    "llambda_hip_attention_session_create": (c_int, [ctypes.POINTER(AttentionDesc),
+                                                     ctypes.POINTER(c_void_p)]),
+    "llambda_hip_attention_session_destroy": (None, [c_void_p]),
+    "llambda_hip_attention_session_run_device": (c_int, [c_void_p, c_i64, ctypes.POINTER(AttentionRows),
+                                                         ctypes.POINTER(AttentionBatch), c_void_p]),
+    "llambda_hip_attention_session_run": (c_int, [c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_void_p,
+                                                  c_size, c_i64, c_void_p, c_void_p]),
+    "llambda_hip_attention_session_accept_device": (c_int, [c_void_p, c_void_p, c_void_p, c_size, c_void_p,
+                                                            c_size, c_void_p, c_size, c_void_p]),
+    "llambda_hip_attention_session_sync": (c_int, [c_void_p, c_void_p]),
+    "llambda_hip_attention_session_write": (c_int, [c_void_p, c_i64, c_void_p, c_i64, c_i64, c_void_p,
+                                                    c_void_p]),
+    "llambda_hip_attention_session_read": (c_int, [c_void_p, c_i64, c_void_p, c_i64, c_i64, c_void_p,
+                                                   c_void_p]),
     "llambda_hip_sampler_create": (c_int, [c_size, ctypes.POINTER(c_void_p)]),
     "llambda_hip_sampler_destroy": (None, [c_void_p]),
     "llambda_hip_sampler_sample": (c_int, [c_void_p, c_void_p, c_size, c_int,
