@@ -48,6 +48,7 @@ typedef struct llambda_hip_ssm_session llambda_hip_ssm_session;
 typedef struct llambda_hip_attention_session llambda_hip_attention_session;
 typedef struct llambda_hip_router llambda_hip_router;
 typedef struct llambda_hip_batch_sampler llambda_hip_batch_sampler;
+typedef struct llambda_hip_token_scorer llambda_hip_token_scorer;
 
 /* ---- probe, versions, errors -------------------------------------- */
 
@@ -731,6 +732,42 @@ int llambda_hip_batch_sampler_sample_device(llambda_hip_batch_sampler* sampler,
 int llambda_hip_batch_sampler_sample(llambda_hip_batch_sampler* sampler, const float* logits,
                                      size_t count, size_t rows,
                                      const llambda_hip_batch_sampling* params, int64_t* tokens);
+
+/* ---- scores of tokens ------------------------------------------------------- */
+
+/* Where a call's results go, each NULL for none (device memory for the device form, host
+ * memory for the host form). */
+typedef struct llambda_hip_token_scores {
+  float* log_probs;           /* [rows][givens], of the given tokens */
+  float* entropy;             /* [rows] */
+  int32_t* top_tokens;        /* [rows][top]: the highest logits, the lower index first among equals */
+  float* top_log_probs;       /* [rows][top], theirs */
+} llambda_hip_token_scores;
+
+/* Workspace for up to max_rows rows of up to `vocab` logits (at most 262144) and max_top (at
+ * most 64) top tokens: 12 bytes for 1000 logits of a row, 256 more with top tokens.  No
+ * counterpart in the reference, which returns tokens alone. */
+int llambda_hip_token_scorer_create(size_t vocab, size_t max_rows, size_t max_top,
+                                    llambda_hip_token_scorer** result);
+void llambda_hip_token_scorer_destroy(llambda_hip_token_scorer* scorer);
+
+/* Natural logarithms of softmax(logits) at given[rows][givens] (at most 4096 a row) and at the
+ * `top` most likely tokens of each row, and the row's entropy, of logits [rows][count], `stride`
+ * from row to row (0: count).  Exponentials are in single precision, their sums in 64 bits.
+ * Logits of -inf have no probability and are no top token; places left over hold (-1, -inf).
+ * A row with a logit that is NaN or +inf, or with none above -inf, has NaN everywhere and no top
+ * tokens (-1); a given token outside 0..count - 1 has NaN.  Device memory, enqueued on `stream`
+ * (null = the scorer's), not waited for, with no allocation.  The calls of a scorer share its
+ * workspace and are ordered as llambda_hip_ssm_session_run_device's, under capture too. */
+int llambda_hip_token_scorer_score_device(llambda_hip_token_scorer* scorer, const float* logits,
+                                          size_t stride, size_t count, size_t rows,
+                                          const int32_t* given, size_t givens, size_t top,
+                                          const llambda_hip_token_scores* scores, void* stream);
+
+/* Host pointers, dense rows, synchronous; given tokens out of range are errors. */
+int llambda_hip_token_scorer_score(llambda_hip_token_scorer* scorer, const float* logits,
+                                   size_t count, size_t rows, const int32_t* given, size_t givens,
+                                   size_t top, const llambda_hip_token_scores* scores);
 
 /* ---- GGUF files ------------------------------------------------------------ */
 

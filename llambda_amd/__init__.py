@@ -9,7 +9,7 @@ Modules:
   moe          routed-MoE layer sessions and routers
   ssm          Mamba-2 mixer sessions
   attention    attention sessions over a paged cache
-  sampling     a token from logits, of one row or of a batch
+  sampling     a token from logits, of one row or of a batch; scores of tokens
   accelerator  the backend descriptor protocol
   projection   the tensor-indexed binding store with runtime fallback
   ggml         type tags and block geometry

@@ -32,7 +32,7 @@ HIP_FLAGS = [
 VGPR_FLAGS = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall"]
 
-HIP_SOURCES = ["gemv.hip", "gemv_mfma.hip", "gemm.hip", "moe.hip", "moe_mfma.hip", "moe_f16.hip", "decoder.hip", "sample.hip", "sample_batch.hip", "ssm.hip", "route.hip",
+HIP_SOURCES = ["gemv.hip", "gemv_mfma.hip", "gemm.hip", "moe.hip", "moe_mfma.hip", "moe_f16.hip", "decoder.hip", "sample.hip", "sample_batch.hip", "score.hip", "ssm.hip", "route.hip",
                "attention.hip", "attention_f16.hip", "attention_bf16.hip", "attention_f32.hip", "abi.hip"]
 # wavefronts of 512 registers keep sums in the accumulation registers
 ACCUMULATION_SOURCES = ["attention_f16.hip", "attention_bf16.hip", "attention_f32.hip"]

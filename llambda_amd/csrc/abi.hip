@@ -29,6 +29,7 @@
 #include "moe.h"
 #include "sample.h"
 #include "sample_batch.h"
+#include "score.h"
 #include "sha256.h"
 #include "ssm.h"
 
@@ -2640,6 +2641,142 @@ int llambda_hip_batch_sampler_sample(llambda_hip_batch_sampler* s, const float* 
     for (size_t i = 0; i < rows; ++i)
       if (got[i] < 0) failf("Row %zu: a NaN logit, or none above minus infinity.", i);
     for (size_t i = 0; i < rows; ++i) tokens[i] = got[i];
+  });
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------- token scores
+
+struct llambda_hip_token_scorer {
+  std::mutex run_mutex;
+  int device = 0;
+  hipStream_t stream = nullptr;
+  size_t vocab = 0, max_rows = 0, max_top = 0;
+  DevBuf parts, candidates;
+  DevBuf logits, given, results;  // device staging of the host-pointer runs
+  size_t staged_logits = 0, staged_given = 0, staged_results = 0;
+  // recorded after every call; the next one, which shares the workspace, waits
+  hipEvent_t done = nullptr;
+  ~llambda_hip_token_scorer() {
+    if (done) (void)hipEventDestroy(done);
+    if (stream) (void)hipStreamDestroy(stream);
+  }
+};
+
+namespace {
+
+void token_score_enqueue(llambda_hip_token_scorer* s, ScoreRows r, hipStream_t st) {
+  r.parts = s->parts.as<ScorePart>();
+  r.candidates = s->candidates.as<ScoreCandidate>();
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  HIPC(hipStreamIsCapturing(st, &capture));
+  const bool ordered = capture == hipStreamCaptureStatusNone;
+  if (ordered) HIPC(hipStreamWaitEvent(st, s->done, 0));
+  HIPC(score_rows_launch(r, st));
+  if (ordered) HIPC(hipEventRecord(s->done, st));
+}
+
+void check_token_score(const llambda_hip_token_scorer* s, const char* what, const void* logits, size_t count,
+                       size_t rows, const void* given, size_t givens, size_t top,
+                       const llambda_hip_token_scores* out) {
+  if (!s) failf("%s: null scorer", what);
+  if (!logits || !out) failf("%s: null argument", what);
+  if (count == 0 || count > s->vocab)
+    failf("%s: %zu logits do not fit the scorer (vocab %zu)", what, count, s->vocab);
+  if (rows == 0 || rows > s->max_rows) failf("%s: %zu rows are not in 1..%zu", what, rows, s->max_rows);
+  if (top > s->max_top) failf("%s: %zu top tokens are not in 0..%zu", what, top, s->max_top);
+  if (givens > 4096) failf("%s: %zu given tokens of a row are not in 0..4096", what, givens);
+  if (givens && (!given || !out->log_probs)) failf("%s: null given tokens or log probabilities", what);
+  if (top && !out->top_tokens && !out->top_log_probs) failf("%s: null top tokens and log probabilities", what);
+}
+
+}  // namespace
+
+extern "C" {
+
+int llambda_hip_token_scorer_create(size_t vocab, size_t max_rows, size_t max_top,
+                                    llambda_hip_token_scorer** result) {
+  return guarded([&] {
+    if (!result) failf("token_scorer_create: null result pointer");
+    *result = nullptr;
+    if (vocab == 0 || vocab > (size_t)kScoreMaxVocab)
+      failf("token_scorer_create: vocab %zu out of range (1..%d)", vocab, kScoreMaxVocab);
+    if (max_rows == 0 || max_rows > 65535)
+      failf("token_scorer_create: max_rows %zu out of range (1..65535)", max_rows);
+    if (max_top > (size_t)kScoreMaxTop) failf("token_scorer_create: max_top %zu out of range (0..%d)", max_top, kScoreMaxTop);
+    std::unique_ptr<llambda_hip_token_scorer> s(new llambda_hip_token_scorer());
+    s->device = current_device_checked();
+    s->vocab = vocab;
+    s->max_rows = max_rows;
+    s->max_top = max_top;
+    HIPC(hipStreamCreateWithFlags(&s->stream, hipStreamNonBlocking));
+    HIPC(hipEventCreateWithFlags(&s->done, hipEventDisableTiming));
+    const size_t chunks = max_rows * score_chunks((int64_t)vocab);
+    s->parts.alloc(chunks * sizeof(ScorePart), "score sums");
+    if (max_top) s->candidates.alloc(chunks * kScoreMaxTop * sizeof(ScoreCandidate), "score candidates");
+    *result = s.release();
+  });
+}
+
+void llambda_hip_token_scorer_destroy(llambda_hip_token_scorer* scorer) { delete scorer; }
+
+int llambda_hip_token_scorer_score_device(llambda_hip_token_scorer* s, const float* logits, size_t stride,
+                                          size_t count, size_t rows, const int32_t* given, size_t givens, size_t top,
+                                          const llambda_hip_token_scores* out, void* stream) {
+  return guarded([&] {
+    const char* what = "token_scorer_score_device";
+    check_token_score(s, what, logits, count, rows, given, givens, top, out);
+    if (!stride) stride = count;
+    if (stride < count || stride > INT32_MAX) failf("%s: rows of %zu logits at a stride of %zu", what, count, stride);
+    if ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(given) |
+         reinterpret_cast<uintptr_t>(out->log_probs) | reinterpret_cast<uintptr_t>(out->entropy) |
+         reinterpret_cast<uintptr_t>(out->top_tokens) | reinterpret_cast<uintptr_t>(out->top_log_probs)) & 3u)
+      failf("%s: pointers must be 4-byte aligned", what);
+    std::lock_guard<std::mutex> lock(s->run_mutex);
+    DeviceScope scope(s->device);
+    ScoreRows r{logits, (int64_t)stride, (int)count, (int)rows, given, (int)givens, (int)top,
+                givens ? out->log_probs : nullptr, out->entropy, out->top_tokens, out->top_log_probs, nullptr, nullptr};
+    token_score_enqueue(s, r, stream ? static_cast<hipStream_t>(stream) : s->stream);
+  });
+}
+
+int llambda_hip_token_scorer_score(llambda_hip_token_scorer* s, const float* logits, size_t count, size_t rows,
+                                   const int32_t* given, size_t givens, size_t top,
+                                   const llambda_hip_token_scores* out) {
+  return guarded([&] {
+    const char* what = "token_scorer_score";
+    check_token_score(s, what, logits, count, rows, given, givens, top, out);
+    for (size_t i = 0; i < rows * givens; ++i)
+      if (given[i] < 0 || (size_t)given[i] >= count)
+        failf("%s: given token %d of row %zu is not in 0..%zu", what, given[i], i / givens, count - 1);
+    std::lock_guard<std::mutex> lock(s->run_mutex);
+    DeviceScope scope(s->device);
+    auto room = [](DevBuf& b, size_t& have, size_t need, const char* name) {
+      if (need <= have) return;
+      have = 0;
+      b.alloc(need * sizeof(float), name);
+      have = need;
+    };
+    const size_t g = rows * givens, n = rows * top;
+    room(s->logits, s->staged_logits, rows * count, "logits");
+    room(s->given, s->staged_given, g, "given tokens");
+    room(s->results, s->staged_results, g + rows + 2 * n, "token scores");
+    HIPC(hipMemcpyAsync(s->logits.ptr, logits, rows * count * sizeof(float), hipMemcpyHostToDevice, s->stream));
+    if (g) HIPC(hipMemcpyAsync(s->given.ptr, given, g * sizeof(int32_t), hipMemcpyHostToDevice, s->stream));
+    float* d = s->results.as<float>();
+    int* tokens = reinterpret_cast<int*>(d + g + rows);
+    ScoreRows r{s->logits.as<float>(), (int64_t)count, (int)count, (int)rows, s->given.as<int>(), (int)givens, (int)top,
+                g ? d : nullptr, d + g, tokens, d + g + rows + n, nullptr, nullptr};
+    token_score_enqueue(s, r, s->stream);
+    auto back = [&](void* to, const void* from, size_t elements) {
+      if (to && elements) HIPC(hipMemcpyAsync(to, from, elements * 4, hipMemcpyDeviceToHost, s->stream));
+    };
+    back(out->log_probs, d, g);
+    back(out->entropy, d + g, rows);
+    back(out->top_tokens, tokens, n);
+    back(out->top_log_probs, d + g + rows + n, n);
+    HIPC(hipStreamSynchronize(s->stream));
   });
 }
 

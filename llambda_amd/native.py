@@ -147,6 +147,12 @@ class BatchSampling(ctypes.Structure):
                 ("min_p", c_void_p), ("random_value", c_void_p)]
 
 
+class TokenScores(ctypes.Structure):
+    """llambda_hip_token_scores."""
+    _fields_ = [("log_probs", c_void_p), ("entropy", c_void_p), ("top_tokens", c_void_p),
+                ("top_log_probs", c_void_p)]
+
+
 class GgufTensor(ctypes.Structure):
     """llambda_hip_gguf_tensor."""
     _fields_ = [("name", c_void_p), ("name_length", c_size), ("dimension_count", ctypes.c_uint32),
@@ -253,6 +259,12 @@ SIGNATURES = {
                                                         c_void_p]),
     "llambda_hip_batch_sampler_sample": (c_int, [c_void_p, c_void_p, c_size, c_size,
                                                  ctypes.POINTER(BatchSampling), c_void_p]),
+    "llambda_hip_token_scorer_create": (c_int, [c_size, c_size, c_size, ctypes.POINTER(c_void_p)]),
+    "llambda_hip_token_scorer_destroy": (None, [c_void_p]),
+    "llambda_hip_token_scorer_score_device": (c_int, [c_void_p, c_void_p, c_size, c_size, c_size, c_void_p,
+                                                      c_size, c_size, ctypes.POINTER(TokenScores), c_void_p]),
+    "llambda_hip_token_scorer_score": (c_int, [c_void_p, c_void_p, c_size, c_size, c_void_p, c_size, c_size,
+                                               ctypes.POINTER(TokenScores)]),
     "llambda_hip_gguf_open": (c_int, [c_char_p, ctypes.POINTER(c_void_p)]),
     "llambda_hip_gguf_close": (None, [c_void_p]),
     "llambda_hip_gguf_header": (c_int, [c_void_p, ctypes.POINTER(ctypes.c_uint32),

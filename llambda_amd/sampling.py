@@ -8,6 +8,7 @@ random-value in [0, 1) -- and its argument errors.
 from __future__ import annotations
 
 import ctypes
+from dataclasses import dataclass
 from typing import Optional, Sequence
 
 import numpy as np
@@ -170,3 +171,82 @@ class HipBatchSampler:
                                                          ctypes.byref(p), out.ctypes.data) != 0:
             raise SamplingError(native.last_error())
         return out
+
+
+@dataclass
+class TokenScores:
+    """Of each row: natural logarithms of the given tokens' probabilities, the entropy, and the most likely tokens
+    with their log probabilities (-1, -inf where there are no more)."""
+    log_probs: np.ndarray       # float32 [rows][givens]
+    entropy: np.ndarray         # float32 [rows]
+    top_tokens: np.ndarray      # int32 [rows][top]
+    top_log_probs: np.ndarray   # float32 [rows][top]
+
+
+class HipTokenScorer:
+    """Log probabilities of given tokens, entropy and top alternatives of rows of logits
+    (llambda_hip_token_scorer_*)."""
+
+    def __init__(self, vocab: int, max_rows: int, max_top: int = 0):
+        self._h = None
+        for name, value in (("vocab", vocab), ("max_rows", max_rows), ("max_top", max_top)):
+            if value < 0:
+                raise SamplingError(f"{name} {value} is negative")
+        handle = ctypes.c_void_p()
+        if native.lib().llambda_hip_token_scorer_create(vocab, max_rows, max_top, ctypes.byref(handle)) != 0:
+            raise SamplingError(native.last_error())
+        self._h = handle
+        self.vocab = vocab
+        self.max_rows = max_rows
+        self.max_top = max_top
+
+    def close(self) -> None:
+        if getattr(self, "_h", None):
+            native.lib().llambda_hip_token_scorer_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:  # noqa: BLE001 - interpreter shutdown
+            pass
+
+    def score_device(self, logits_ptr: int, rows: int, *, given_ptr: int = 0, given: int = 0, top: int = 0,
+                     log_probs_ptr: int = 0, entropy_ptr: int = 0, top_tokens_ptr: int = 0,
+                     top_log_probs_ptr: int = 0, count: Optional[int] = None, stride: int = 0,
+                     stream: int = 0) -> None:
+        """Device pointers: logits [rows][count] (the vocabulary by default), stride elements from row to row (0:
+        dense), int32 given tokens [rows][given]; results as in TokenScores, 0 = not wanted.  Not waited for."""
+        out = native.TokenScores(log_probs_ptr or None, entropy_ptr or None, top_tokens_ptr or None,
+                                 top_log_probs_ptr or None)
+        if native.lib().llambda_hip_token_scorer_score_device(
+                self._h, logits_ptr or None, stride, self.vocab if count is None else count, rows,
+                given_ptr or None, given, top, ctypes.byref(out), stream or None) != 0:
+            raise SamplingError(native.last_error())
+
+    def score(self, logits, given=None, top: int = 0) -> TokenScores:
+        """Scores of host logits [rows][count]; given: tokens of each row, [rows] or [rows][givens]."""
+        a = np.ascontiguousarray(logits, dtype=np.float32)
+        if a.ndim != 2:
+            raise SamplingError(f"logits have {a.ndim} dimensions, not 2")
+        if top < 0:
+            raise SamplingError(f"top {top} is negative")
+        rows = a.shape[0]
+        g = np.empty((rows, 0), dtype=np.int32)
+        if given is not None:
+            v = np.asarray(given)
+            if v.dtype.kind not in "iu":
+                raise SamplingError(f"given tokens must be whole numbers, got {v.dtype}")
+            if v.shape[:1] != (rows,) or v.ndim > 2:
+                raise SamplingError(f"given tokens of shape {v.shape} for {rows} rows")
+            if v.size and (int(v.min()) < 0 or int(v.max()) >= a.shape[1]):
+                raise SamplingError(f"given tokens are not all in 0..{a.shape[1] - 1}")
+            g = np.ascontiguousarray(v.reshape(rows, v.size // rows if rows else 0), dtype=np.int32)
+        r = TokenScores(np.empty(g.shape, np.float32), np.empty(rows, np.float32),
+                        np.empty((rows, top), np.int32), np.empty((rows, top), np.float32))
+        out = native.TokenScores(r.log_probs.ctypes.data, r.entropy.ctypes.data, r.top_tokens.ctypes.data,
+                                 r.top_log_probs.ctypes.data)
+        if native.lib().llambda_hip_token_scorer_score(self._h, a.ctypes.data, a.shape[1], rows, g.ctypes.data,
+                                                       g.shape[1], top, ctypes.byref(out)) != 0:
+            raise SamplingError(native.last_error())
+        return r
