@@ -26,16 +26,14 @@ ARCH = "gfx950"
 HIP_FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++20", "-fPIC", "-Wall",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+    # MFMA results in ordinary VGPRs: the kernels scale and add them with
+    # VALU instructions, which cannot read the accumulation registers
+    "-mllvm", "-amdgpu-mfma-vgpr-form=1",
 ]
-# MFMA results in ordinary VGPRs: the kernels scale and add them with
-# VALU instructions, which cannot read the accumulation registers
-VGPR_FLAGS = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall"]
 
 HIP_SOURCES = ["gemv.hip", "gemv_mfma.hip", "gemm.hip", "moe.hip", "moe_mfma.hip", "moe_f16.hip", "decoder.hip", "sample.hip", "sample_batch.hip", "score.hip", "ssm.hip", "route.hip",
                "attention.hip", "attention_f16.hip", "attention_bf16.hip", "attention_f32.hip", "abi.hip"]
-# wavefronts of 512 registers keep sums in the accumulation registers
-ACCUMULATION_SOURCES = ["attention_f16.hip", "attention_bf16.hip", "attention_f32.hip"]
 CXX_SOURCES = ["sha256.cpp", "gguf.cpp"]
 
 
@@ -56,8 +54,7 @@ def build(verbose: bool = False, defines=(), obj_dir: str = OBJ, lib_path: str =
     jobs = []
     for src in HIP_SOURCES:
         obj = os.path.join(obj_dir, src + ".o")
-        forms = [] if src in ACCUMULATION_SOURCES else VGPR_FLAGS
-        jobs.append([HIPCC, *HIP_FLAGS, *forms, *[f"-D{d}" for d in defines], "-c",
+        jobs.append([HIPCC, *HIP_FLAGS, *[f"-D{d}" for d in defines], "-c",
                      os.path.join(CSRC, src), "-o", obj])
     for src in CXX_SOURCES:
         obj = os.path.join(obj_dir, src + ".o")

@@ -191,26 +191,29 @@ struct RowSums {
   floatx16 y[DP / 32];
   float reference;  // the exponent that p is taken against; -inf: no key yet
   float sum;        // of this lane's keys
+  uint32_t bad[DP / 32];
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int b = 0; b < DP / 32; ++b) y[b] = floatx16{};
+    for (int b = 0; b < DP / 32; ++b) y[b] = floatx16{}, bad[b] = 0;
     reference = -__builtin_inff();
     sum = 0.f;
   }
+  // Notes the elements that are no numbers in keys that the row sees.
   template <int KB>
-  __device__ __forceinline__ void spoil(const uint32_t* bits, const uint32_t (&sight)[KB], int half) {
-    uint32_t bad[DP / 32] = {};
+  __device__ __forceinline__ void spoil(const uint32_t* bits, const uint32_t (&sight)[KB]) {
 #pragma unroll
     for (int b = 0; b < KB; ++b)
       for (int k = 0; k < 32; ++k)
         if (sight[b] >> k & 1)
 #pragma unroll
           for (int d = 0; d < DP / 32; ++d) bad[d] |= bits[(32 * b + k) * (DP / 32) + d];
+  }
+  // y's rows 32 b + 8 i + 4 half + 0..3.
+  __device__ __forceinline__ floatx4 piece(int b, int i, int half) const {
+    floatx4 v;
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        y[d][i] = bad[d] >> (8 * (i / 4) + 4 * half + i % 4) & 1 ? __builtin_nanf("") : y[d][i];
+    for (int k = 0; k < 4; ++k) v[k] = bad[b] >> (8 * i + 4 * half + k) & 1 ? __builtin_nanf("") : y[b][4 * i + k];
+    return v;
   }
   // The scores s of KB blocks of 32 keys become probabilities.
   template <int KB>
@@ -471,6 +474,13 @@ constexpr uint32_t attn_exponent() {
 // LDS accesses of this wavefront so far are done before those that follow.
 __device__ __forceinline__ void wave_lds_order() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
+// An item, in scalar registers.
+__device__ __forceinline__ AttnItem uniform_item(const AttnItem* item) {
+  const int* v = reinterpret_cast<const int*>(item);
+  auto at = [&](int i) { return __builtin_amdgcn_readfirstlane(v[i]); };
+  return AttnItem{at(0), at(1), at(2), at(3), at(4), at(5), at(6), at(7)};
+}
+
 // What an item's rows are, for one of its wavefronts (32 rows from m on).
 template <typename Row>
 struct ItemRows {
@@ -509,7 +519,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_shared_kernel(Attn
   extern __shared__ __align__(16) uint8_t lds[];
   const int index = blockIdx.x / p.kv_heads, kv_head = blockIdx.x % p.kv_heads;
   if (index >= p.counts[0]) return;
-  const AttnItem it = p.items[index];
+  const AttnItem it = uniform_item(p.items + index);
   if (!p.run[it.sequence]) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m0 = it.m0 + 32 * wave;
@@ -553,7 +563,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_shared_kernel(Attn
 #pragma unroll
         for (int b = 0; b < KB; ++b) see[b] = sight.bits(key + 32 * b);
       tile.template tile<KB>(now, now + kTile, partly, see);
-      if (partly && spoiled.any()) tile.sums.template spoil<KB>(spoiled.bits, see, tile.half);
+      if (partly && spoiled.any()) tile.sums.template spoil<KB>(spoiled.bits, see);
     }
     if (partly && spoiled.any()) {
       __syncthreads();
@@ -570,9 +580,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_shared_kernel(Attn
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int d = 32 * b + 8 * i + 4 * tile.half;
-        const floatx4 v{tile.sums.y[b][4 * i], tile.sums.y[b][4 * i + 1], tile.sums.y[b][4 * i + 2],
-                        tile.sums.y[b][4 * i + 3]};
-        if (d < p.head_dim) store4(y + d, v * scale);
+        if (d < p.head_dim) store4(y + d, tile.sums.piece(b, i, tile.half) * scale);
       }
   } else {
     const size_t row = ((size_t)it.part * p.kv_heads + kv_head) * (32 * WAVES) + 32 * wave + (lane & 31);
@@ -582,9 +590,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_shared_kernel(Attn
     for (int b = 0; b < DP / 32; ++b)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<floatx4*>(y + 32 * b + 8 * i + 4 * tile.half) =
-            floatx4{tile.sums.y[b][4 * i], tile.sums.y[b][4 * i + 1], tile.sums.y[b][4 * i + 2],
-                    tile.sums.y[b][4 * i + 3]};
+        *reinterpret_cast<floatx4*>(y + 32 * b + 8 * i + 4 * tile.half) = tile.sums.piece(b, i, tile.half);
   }
 }
 
@@ -610,7 +616,7 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attn_split_kernel(AttnPlan p, A
   int* const list = reinterpret_cast<int*>(ml + WAVES * 64);
   const int index = blockIdx.x / p.kv_heads, kv_head = blockIdx.x % p.kv_heads;
   if (index >= p.counts[0]) return;
-  const AttnItem it = p.items[index];
+  const AttnItem it = uniform_item(p.items + index);
   if (!p.run[it.sequence]) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const ItemRows<Row> rows(p, it, it.m0, lane);
@@ -659,7 +665,7 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attn_split_kernel(AttnPlan p, A
         wave_lds_order();
       }
       tile.template tile<1>(now, now + M::kTile, partly, see);
-      if (partly && spoiled.any()) tile.sums.template spoil<1>(spoiled.bits, see, tile.half);
+      if (partly && spoiled.any()) tile.sums.template spoil<1>(spoiled.bits, see);
       wave_lds_order();  // the next load into this tile's place follows its reads
     }
     key0 = key1;
@@ -674,9 +680,7 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attn_split_kernel(AttnPlan p, A
   for (int b = 0; b < DP / 32; ++b)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<floatx4*>(own + 32 * b + 8 * i + 4 * tile.half) =
-          floatx4{tile.sums.y[b][4 * i], tile.sums.y[b][4 * i + 1], tile.sums.y[b][4 * i + 2],
-                  tile.sums.y[b][4 * i + 3]};
+      *reinterpret_cast<floatx4*>(own + 32 * b + 8 * i + 4 * tile.half) = tile.sums.piece(b, i, tile.half);
   __syncthreads();
   const int count = min(32, rows.rows - it.m0), pieces = p.head_dim / 4;
   for (int i = threadIdx.x; i < count * pieces; i += 64 * WAVES) {
@@ -724,6 +728,11 @@ template <int TYPE, typename Row, int DP>
 constexpr int attn_shared_waves() {
   return DP == 256 || (TYPE == kAttnBF16 && sizeof(Row) == 4 && DP == 128) ? 4 : 8;
 }
+// Keys of a shared tile: what registers hold of their scores.
+template <int TYPE, int DP>
+constexpr int attn_shared_keys() {
+  return DP == 256 ? 32 : 64;
+}
 // Waves that split keys: what LDS holds of their tiles.
 template <int TYPE, int DP>
 constexpr int attn_split_waves() {
@@ -733,7 +742,7 @@ constexpr int attn_split_waves() {
 template <int TYPE, typename Row, int DP>
 hipError_t attn_attend(const AttnPlan& p, const AttnCall& c, const AttnCut& cut, uint32_t grid, hipStream_t s) {
   if (cut.shared) {
-    constexpr int W = attn_shared_waves<TYPE, Row, DP>(), KT = DP * attn_cell_bytes<TYPE>() <= 512 ? 64 : 32;
+    constexpr int W = attn_shared_waves<TYPE, Row, DP>(), KT = attn_shared_keys<TYPE, DP>();
     return attn_launch(attn_shared_kernel<TYPE, Row, DP, W, KT>, grid, 64 * W, 
                        4 * KT * DP * attn_cell_bytes<TYPE>() + Spoiled<attn_cell_bytes<TYPE>(), DP, KT>::kBytes, s, p, c);
   }
