@@ -16,6 +16,8 @@ namespace llhip {
 
 constexpr int kAttnMaxHeadDim = 256;
 constexpr int kAttnTreeNodes = 256;                    // nodes of a tree, at most
+constexpr int kAttnFewSequences = 256;  // of a call that needs no launch before the attend kernel
+constexpr int kAttnFewTokens = 256;
 constexpr int kAttnTreeWords = kAttnTreeNodes / 32;
 
 enum AttnType : int { kAttnF32 = 0, kAttnF16 = 1, kAttnBF16 = 30 };  // GGML's tags
@@ -35,7 +37,7 @@ struct AttnItem {
   int m0, key0, key1;
   int part;                              // -1: all it sees; else where in the partial results it goes
 };
-// Rows whose range of positions several items share.
+// Rows whose range of positions several items share (with fewer than two parts: nothing to join).
 struct AttnJoin {
   int begin, length, m0, parts, part0, sequence;
 };
@@ -103,6 +105,7 @@ struct AttnCut {
   int rows;         // of an item
   int min_keys;     // of a part
   int slots;        // parts over all kv heads come to about this many workgroups
+  bool few;         // the attend kernel makes the plan and puts the new rows into the cache
 };
 // The kernels of one cache type (attention_f16.hip, attention_bf16.hip, attention_f32.hip).
 hipError_t attn_attend_f16(const AttnPlan& p, const AttnCall& c, const AttnCut& cut, uint32_t grid, hipStream_t s);

@@ -8,7 +8,7 @@
 // share what is read of the cache), and the positions that a tile sees in parts
 // where the tiles alone would not fill the device or one would outlast the rest.
 // The attend kernel does the items; attn_join_kernel adds up parts.
-#include "attention.h"
+#include "attention_cut.h"
 
 #include <algorithm>
 #include <climits>
@@ -93,12 +93,6 @@ __device__ int block_scan(int v, int* lds, int& total) {
   return v + before;
 }
 
-__device__ __forceinline__ int seen_keys(const AttnPlan& p, const AttnCall& c, const AttnCut& cut, int m0, int length,
-                                         int context) {
-  if (c.parents) return context + length;
-  return context + min(length, (m0 + cut.rows - 1) / p.group + 1);
-}
-
 // Items and joins.  Tiles of many keys come first within a sequence.
 __device__ void plan(const AttnPlan& p, const AttnCall& c, const AttnCut& cut) {
   __shared__ int scan[kPlanThreads / 64], ends[kPlanThreads], lengths[kPlanThreads], contexts[kPlanThreads],
@@ -112,7 +106,7 @@ __device__ void plan(const AttnPlan& p, const AttnCall& c, const AttnCut& cut) {
     return;
   }
   if (threadIdx.x == 0) keys = 0;
-  int64_t chunk = 0;
+  int chunk = 0;
   int items = 0, joins = 0, parts = 0;
   for (int pass = 0; pass < 2; ++pass) {
     for (int i0 = 0; i0 < c.sequences; i0 += kPlanThreads) {
@@ -138,7 +132,7 @@ __device__ void plan(const AttnPlan& p, const AttnCall& c, const AttnCut& cut) {
             else which = mid + 1;
           }
           m0 = (ends[which] - 1 - t) * cut.rows;
-          seen = seen_keys(p, c, cut, m0, lengths[which], contexts[which]);
+          seen = attn_seen_keys(p, c, cut, m0, lengths[which], contexts[which]);
         }
         if (pass == 0) {
           unsigned long long v = seen;
@@ -147,16 +141,16 @@ __device__ void plan(const AttnPlan& p, const AttnCall& c, const AttnCut& cut) {
           if ((threadIdx.x & 63) == 0) atomicAdd(&keys, v);
           continue;
         }
-        if (t < tiles) n = ceil_div(seen, chunk);
+        if (t < tiles) n = (seen + chunk - 1) / chunk;
         int all_items, all_joins, all_parts;
         const int item = items + block_scan(n, scan, all_items) - n;
         const int join = joins + block_scan(n > 1, scan, all_joins) - (n > 1);
         const int part = parts + block_scan(n > 1 ? n : 0, scan, all_parts) - (n > 1 ? n : 0);
-        // equal parts, of whole tiles
-        const int size = n > 0 ? ceil_div(ceil_div(seen, n), 64) * 64 : 0;
-        for (int k = 0; k < n; ++k)
-          p.items[item + k] = AttnItem{i0 + which, begins[which], lengths[which], contexts[which], m0,
-                                       min(k * size, seen), min((k + 1) * size, seen), n > 1 ? part + k : -1};
+        AttnItem it{i0 + which, begins[which], lengths[which], contexts[which], m0, 0, 0, 0};
+        for (int k = 0; k < n; ++k) {
+          attn_part(it, seen, n, k, part);
+          p.items[item + k] = it;
+        }
         if (n > 1) p.joins[join] = AttnJoin{begins[which], lengths[which], m0, n, part, i0 + which};
         items += all_items;
         joins += all_joins;
@@ -166,9 +160,7 @@ __device__ void plan(const AttnPlan& p, const AttnCall& c, const AttnCut& cut) {
     }
     if (pass == 0) {
       __syncthreads();
-      // parts of about the work over the device's workgroups
-      chunk = (int64_t)((keys * p.kv_heads + cut.slots - 1) / cut.slots);
-      chunk = (max(chunk, (int64_t)cut.min_keys) + 63) / 64 * 64;
+      chunk = attn_chunk(p, cut, (int64_t)keys);
     }
   }
   if (threadIdx.x == 0) {
@@ -178,22 +170,6 @@ __device__ void plan(const AttnPlan& p, const AttnCall& c, const AttnCut& cut) {
 }
 
 // ------------------------------------------------------------- keys and values
-template <typename To, typename From>
-__device__ __forceinline__ void put8(To* to, const From* from) {
-  typedef From From8 __attribute__((ext_vector_type(8)));
-  typedef To To8 __attribute__((ext_vector_type(8)));
-  const From8 v = *reinterpret_cast<const From8*>(from);
-  // to the nearest; what is beyond the type becomes an infinity
-  if constexpr (sizeof(From) == sizeof(To)) *reinterpret_cast<To8*>(to) = __builtin_bit_cast(To8, v);
-  else *reinterpret_cast<To8*>(to) = __builtin_convertvector(v, To8);
-}
-
-// Element 0 of position `pos` of kv head 0 (heads are 1 << page_shift rows apart).
-__device__ __forceinline__ size_t cell(const AttnPlan& p, int layer, int page, int pos) {
-  return ((((size_t)layer * p.pages + page) * p.kv_heads << p.page_shift) + (pos & ((1 << p.page_shift) - 1))) *
-         p.head_dim;
-}
-
 // Workgroup 0 makes the plan; `share` workgroups take the rows of each sequence.
 template <typename Row, typename T>
 __global__ __launch_bounds__(kPlanThreads) void attn_prepare_kernel(AttnPlan p, AttnCall c, AttnCut cut, int share) {
@@ -228,20 +204,20 @@ __global__ __launch_bounds__(kPlanThreads) void attn_prepare_kernel(AttnPlan p, 
   const int pieces = p.kv_heads * p.head_dim / 8, per_head = p.head_dim / 8;
   for (int r = part; r < s.length; r += share) {
     const int pos = s.context + r;
-    const size_t at = cell(p, c.layer, c.table[i * c.table_stride + (pos >> p.page_shift)], pos);
+    const size_t at = attn_cell(p, c.layer, c.table[i * c.table_stride + (pos >> p.page_shift)], pos);
     const Row* k = static_cast<const Row*>(c.k) + (s.begin + r) * c.k_stride;
     const Row* v = static_cast<const Row*>(c.v) + (s.begin + r) * c.v_stride;
     for (int e = threadIdx.x; e < 2 * pieces; e += kPlanThreads) {
       const bool value = e >= pieces;
       const int piece = value ? e - pieces : e;
       const size_t to = at + ((size_t)(piece / per_head) << p.page_shift) * p.head_dim + piece % per_head * 8;
-      put8(static_cast<T*>(value ? p.values : p.keys) + to, (value ? v : k) + 8 * piece);
+      attn_put8(static_cast<T*>(value ? p.values : p.keys) + to, (value ? v : k) + 8 * piece);
     }
   }
 }
 
 // ----------------------------------------------------------------------- joins
-// Row m of a join: parts' sums taken to one reference.  A wavefront per row.
+// Row m of a join: parts' sums taken to one reference.  A wavefront per row; eight parts' sums are on their way at once.
 template <typename Row>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnPlan p, AttnCall c, AttnCut cut, int padded, int blocks) {
   const int index = blockIdx.x / (p.kv_heads * blocks), rest = blockIdx.x % (p.kv_heads * blocks);
@@ -249,23 +225,38 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnPlan p, AttnCall c, 
   const AttnJoin j = p.joins[index];
   const int kv_head = rest / blocks, lane = threadIdx.x & 63;
   const int r = rest % blocks * 4 + (threadIdx.x >> 6);
-  if (r >= cut.rows || j.m0 + r >= j.length * p.group || !p.run[j.sequence]) return;
+  if (j.parts < 2 || r >= cut.rows || j.m0 + r >= j.length * p.group || (!cut.few && !p.run[j.sequence])) return;
   const size_t step = (size_t)p.kv_heads * cut.rows;
   const size_t row = ((size_t)j.part0 * p.kv_heads + kv_head) * cut.rows + r;
   float reference = -__builtin_inff();
   for (int k = lane; k < j.parts; k += 64) reference = fmaxf(reference, p.part_ml[row + k * step].x);
   reference = wave_max(reference);
-  const int d = 4 * lane;
+  const int d = min(4 * lane, padded - 4);
   floatx4 v{};
   float total = 0.f;
-  for (int k = 0; k < j.parts; ++k) {
-    const float2 ml = p.part_ml[row + k * step];
-    // a part of which the row sees nothing has zeros
-    const float weight = ml.x == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(ml.x - reference);
-    total += weight * ml.y;
-    if (d < p.head_dim) v += weight * *reinterpret_cast<const floatx4*>(p.part_y + (row + k * step) * padded + d);
+  for (int k0 = 0; k0 < j.parts; k0 += 64) {
+    float weight = 0.f;
+    if (k0 + lane < j.parts) {
+      const float2 ml = p.part_ml[row + (k0 + lane) * step];
+      // a part of which the row sees nothing has zeros
+      weight = ml.x == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(ml.x - reference);
+      total += weight * ml.y;
+    }
+    const int count = min(64, j.parts - k0);
+    for (int k = 0; k < count; k += 8) {
+      floatx4 y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        y[i] = *reinterpret_cast<const floatx4*>(p.part_y + (row + (k0 + min(k + i, count - 1)) * step) * padded + d);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), k + i));
+        if (k + i < count) v += w * y[i];
+      }
+    }
   }
-  if (d >= p.head_dim) return;
+  total = wave_total(total);
+  if (4 * lane >= p.head_dim) return;
   const int m = j.m0 + r;
   Row* y = static_cast<Row*>(c.y) + (j.begin + m / p.group) * c.y_stride +
            (kv_head * p.group + m % p.group) * p.head_dim + d;
@@ -312,8 +303,8 @@ __global__ __launch_bounds__(kPlanThreads) void attn_accept_kernel(AttnPlan p, A
       const int from = context + path[j], to = context + j;
       if (from == to) continue;
       const u32x4 v = *reinterpret_cast<const u32x4*>(
-          pool + cell(p, blockIdx.y, table[from >> p.page_shift], from) + in);
-      *reinterpret_cast<u32x4*>(pool + cell(p, blockIdx.y, table[to >> p.page_shift], to) + in) = v;
+          pool + attn_cell(p, blockIdx.y, table[from >> p.page_shift], from) + in);
+      *reinterpret_cast<u32x4*>(pool + attn_cell(p, blockIdx.y, table[to >> p.page_shift], to) + in) = v;
     }
   }
 }
@@ -326,6 +317,13 @@ __global__ void attn_take_error_kernel(int* error) {
 // ------------------------------------------------------------------------ host
 
 constexpr int kCus = 256;
+#ifndef RT
+#define SLS 256
+#define MINS 256
+#define SLP 512
+#define MINP 256
+#define RT 160
+#endif
 
 static int shared_waves(const AttnPlan& p) {
   const int padded = attn_padded(p.head_dim);
@@ -333,16 +331,18 @@ static int shared_waves(const AttnPlan& p) {
 }
 
 static AttnCut cut_as(const AttnPlan& p, bool shared) {
-  AttnCut cut;
+  AttnCut cut{};
   cut.shared = shared;
   cut.rows = shared ? 32 * shared_waves(p) : 32;
-  cut.min_keys = shared ? 256 : 128;
-  cut.slots = shared ? kCus : 2 * kCus;
+  cut.min_keys = shared ? MINS : MINP;
+  cut.slots = shared ? SLS : SLP;
   return cut;
 }
-static AttnCut cut_of(const AttnPlan& p, int64_t tokens, int64_t sequences) {
+static AttnCut cut_of(const AttnPlan& p, const AttnCall& c) {
   // rows of a kv head in a sequence, on average; the lengths are on the device
-  return cut_as(p, ceil_div(tokens * p.group, sequences) > 32);
+  AttnCut cut = cut_as(p, ceil_div((int64_t)c.tokens * p.group, c.sequences) > RT);
+  cut.few = !cut.shared && c.tokens <= kAttnFewTokens && c.sequences <= kAttnFewSequences;
+  return cut;
 }
 
 // Items of a call at most: a tile for each cut.rows rows, one more for each sequence, and parts that are no shorter
@@ -362,6 +362,9 @@ AttnSizes attn_sizes(const AttnPlan& p) {
     const int64_t split = cut.slots / p.kv_heads;
     s.items = std::max(s.items, tiles + split);
     s.joins = std::max(s.joins, std::min(tiles, split));
+    if (!shared)  // of a call of few rows one for each tile
+      s.joins = std::max(s.joins, tiles_of(p, std::min(p.max_tokens, kAttnFewTokens),
+                                           std::min(p.max_sequences, kAttnFewSequences), cut.rows));
     // n > 1 parts are at most twice the n - 1 that come beside the tile's own
     s.part_rows = std::max(s.part_rows, 2 * split * p.kv_heads * cut.rows);
   }
@@ -379,11 +382,11 @@ static int64_t join_blocks(const AttnCut& cut, const AttnPlan& p, const AttnCall
 }
 static int64_t join_grid(const AttnPlan& p, const AttnCall& c, const AttnCut& cut) {
   const int64_t tiles = tiles_of(p, c.tokens, c.sequences, cut.rows);
-  return std::min<int64_t>(tiles, cut.slots / p.kv_heads) * p.kv_heads * join_blocks(cut, p, c);
+  return (cut.few ? tiles : std::min<int64_t>(tiles, cut.slots / p.kv_heads)) * p.kv_heads * join_blocks(cut, p, c);
 }
 
 bool attn_call_fits(const AttnPlan& p, const AttnCall& c) {
-  const AttnCut cut = cut_of(p, c.tokens, c.sequences);
+  const AttnCut cut = cut_of(p, c);
   const int64_t most = UINT32_MAX / 512;
   return items_of(p, c.tokens, c.sequences, cut) * p.kv_heads <= most &&
          1 + c.sequences * prepare_share(p, c) <= most && join_grid(p, c, cut) <= most;
@@ -398,9 +401,10 @@ static hipError_t prepare(const AttnPlan& p, const AttnCall& c, const AttnCut& c
 }
 
 hipError_t attn_run_launch(const AttnPlan& p, const AttnCall& c, hipStream_t s) {
-  const AttnCut cut = cut_of(p, c.tokens, c.sequences);
-  hipError_t e;
-  if (p.row_type == kAttnF16) e = prepare<_Float16, _Float16>(p, c, cut, s);
+  const AttnCut cut = cut_of(p, c);
+  hipError_t e = hipSuccess;
+  if (cut.few) {
+  } else if (p.row_type == kAttnF16) e = prepare<_Float16, _Float16>(p, c, cut, s);
   else if (p.row_type == kAttnBF16) e = prepare<__bf16, __bf16>(p, c, cut, s);
   else if (p.cache_type == kAttnF16) e = prepare<float, _Float16>(p, c, cut, s);
   else if (p.cache_type == kAttnBF16) e = prepare<float, __bf16>(p, c, cut, s);

@@ -13,7 +13,7 @@
 // Operands.  A cache in 16 bits is an operand as it is.  fp32 rows, and the fp32
 // probabilities of such rows, are split into parts of the cache's type whose
 // products are added: two of f16 (22 bits; q times a power of two for each row, p
-// times 2^15, so that the parts stay normal), three of bf16 (24 bits).  Rows in 16
+// times 2^9, so that the parts stay normal), three of bf16 (24 bits).  Rows in 16
 // bits are one part, and so are their probabilities: rounding those to 8 or 11 bits
 // costs what rounding the output costs.  An fp32 cache uses the fp32 products.
 //
@@ -21,7 +21,7 @@
 // pieces permuted so that neither read meets a bank twice.
 #pragma once
 
-#include "attention.h"
+#include "attention_cut.h"
 #include "mfma.h"
 
 namespace llhip {
@@ -44,10 +44,15 @@ __device__ __forceinline__ float half_pair_max(float v) {
 template <int TYPE>
 struct Cell;
 template <>
+struct Cell<kAttnF32> {
+  typedef float T;
+};
+template <>
 struct Cell<kAttnF16> {
   typedef _Float16 T;
   typedef halfx8 Frag;
-  static constexpr float kLift = 15.f;  // p times 2^15: down to 2^-29 its first part is a normal number
+  // p times 2^9, 2^15 at most: down to 2^-23 of the reference its first part is a normal number
+  static constexpr float kLift = 9.f;
   static __device__ __forceinline__ floatx16 mfma(Frag a, Frag b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -94,6 +99,23 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&out)[N])
   }
 }
 
+// COUNT fragments read from LDS, each AHEAD of its use, in this order: left to itself the compiler reads one ahead, and
+// every product waits for the LDS.
+template <int COUNT, int AHEAD, typename Frag, typename Read, typename Use>
+__device__ __forceinline__ void read_ahead(Read&& read, Use&& use) {
+  Frag f[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) f[i] = read(i);
+#pragma unroll
+  for (int i = 0; i < COUNT; ++i) {
+    __builtin_amdgcn_sched_barrier(0);
+    use(i, f[i % AHEAD]);
+    __builtin_amdgcn_sched_barrier(0);
+    if (i + AHEAD < COUNT) f[i % AHEAD] = read(i + AHEAD);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 template <typename Row>
 __device__ __forceinline__ void load8(const Row* p, float (&v)[8]) {
   if constexpr (sizeof(Row) == 4) {
@@ -137,33 +159,44 @@ template <int SIZE, int DP, int KT>
 struct TileLoader {
   typedef TileLayout<SIZE, DP> L;
   static constexpr int kLoads = KT / L::kRowsPerLoad;  // of keys, and of values, by one wavefront
-  const uint8_t* keys;
+  const uint8_t* keys;    // of the head in page 0
   const uint8_t* values;
-  int kv_heads, head, page_shift, head_dim;
+  uint64_t page_bytes;    // of all heads
+  int page_shift, head_dim;
   int last;  // the sequence's last position; tiles past it hold rows near it again
+  __device__ __forceinline__ TileLoader(const AttnPlan& p, int layer, int kv_head, const AttnItem& it)
+      : page_bytes(((uint64_t)p.kv_heads * p.head_dim * SIZE) << p.page_shift),
+        page_shift(p.page_shift),
+        head_dim(p.head_dim),
+        last(it.context + it.length - 1) {
+    const uint64_t at = (uint64_t)layer * p.pages * page_bytes + (((uint64_t)kv_head * p.head_dim * SIZE) << page_shift);
+    keys = static_cast<const uint8_t*>(p.keys) + at;
+    values = static_cast<const uint8_t*>(p.values) + at;
+  }
 
   // Lane l's page: the one of position base + l.
   __device__ __forceinline__ int entry(int base, int lane) const {
     return min(base + lane, last) >> page_shift;
   }
-  // Loads [from, kLoads) in steps of `step`, of tile `base`; pages: entry()'s, by lane.
-  __device__ __forceinline__ void load(int base, int pages, uint32_t lds_k, uint32_t lds_v, int from, int step,
-                                       int lane) const {
+  // Of the loads of the keys, or values, of tile `base` to LDS every STEP-th from `from` on; pages: entry()'s, by lane.
+  // What depends on the lane alone is the same for every tile.
+  template <bool VALUES, int STEP>
+  __device__ __forceinline__ void load(int base, int pages, uint32_t to, int from, int lane) const {
     constexpr int R = L::kRowsPerLoad;
+    static_assert(kLoads % STEP == 0, "as many loads for every wavefront");
     const int row = lane / L::kPieces, piece = lane % L::kPieces;
-    const int bytes = head_dim * SIZE;
-    for (int i = from; i < kLoads; i += step) {
-      const int r0 = i * R;
-      const int pos = min(base + r0, last & ~(R - 1));
-      const int page = __builtin_amdgcn_readlane(pages, r0);
-      const int64_t at =
-          ((((int64_t)page * kv_heads + head) << page_shift) + (pos & ((1 << page_shift) - 1))) * bytes;
-      int pk = piece ^ L::key_swizzle(r0 + row), pv = piece ^ L::value_swizzle(r0 + row);
+    const uint32_t bytes = head_dim * SIZE;
+    const uint32_t in_page = (1u << page_shift) - 1;
+#pragma unroll
+    for (int j = 0; j < kLoads / STEP; ++j) {
+      const int i = from + j * STEP, r0 = i * R;
+      uint32_t source = 16 * (piece ^ (VALUES ? L::value_swizzle(r0 + row) : L::key_swizzle(r0 + row)));
       // a row shorter than the tile's: its first piece again (the row's q has zeros there, its y is not stored)
-      if (16 * pk >= bytes) pk = 0;
-      if (16 * pv >= bytes) pv = 0;
-      load_lds16(keys + at, (uint32_t)(row * bytes + 16 * pk), lds_k + 1024u * i);
-      load_lds16(values + at, (uint32_t)(row * bytes + 16 * pv), lds_v + 1024u * i);
+      if (source >= bytes) source = 0;
+      const uint32_t pos = min(base + r0, last & ~(R - 1));
+      const uint32_t page = __builtin_amdgcn_readlane(pages, r0);
+      load_lds16((VALUES ? values : keys) + (uint64_t)page * page_bytes + (pos & in_page) * bytes, row * bytes + source,
+                 to + 1024u * i);
     }
   }
 };
@@ -184,6 +217,9 @@ struct Sight {
     return (uint32_t)((((uint64_t)hi << 32) | lo) >> s);
   }
 };
+
+// How far a row's maximum may grow, in powers of two, before its sums are scaled.
+constexpr float kSlack = 6.f;
 
 // Sums of 32 rows over the keys so far: y holds rows 32 b + 8 (i / 4) + 4 (lane / 32) + i % 4 of Y^T, column lane % 32.
 template <int DP>
@@ -215,7 +251,7 @@ struct RowSums {
     for (int k = 0; k < 4; ++k) v[k] = bad[b] >> (8 * i + 4 * half + k) & 1 ? __builtin_nanf("") : y[b][4 * i + k];
     return v;
   }
-  // The scores s of KB blocks of 32 keys become probabilities.
+  // The scores s of KB blocks of 32 keys become probabilities, 2^lift for the reference's.
   template <int KB>
   __device__ __forceinline__ void softmax(floatx16 (&s)[KB], float factor, float lift) {
     float top = s[0][0];
@@ -224,7 +260,8 @@ struct RowSums {
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
     top = half_pair_max(top) * factor;
-    if (__ballot(top > reference)) {
+    // the sums are scaled again only where a maximum has grown by more than the probabilities' range leaves room for
+    if (__ballot(top > reference + kSlack)) {
       const float next = fmaxf(reference, top);
       // a row that has seen nothing has nothing to scale (and no reference)
       const float scale = next == reference ? 1.f : __builtin_amdgcn_exp2f(reference - next);
@@ -301,6 +338,7 @@ struct RowTile {
   typedef typename C::Frag Frag;
   typedef TileLayout<2, DP> L;
   static constexpr int N = attn_parts<TYPE, Row>(), kSteps = DP / 16, kBlocks = DP / 32;
+  static constexpr int kAhead = N == 1 ? 4 : 3;  // what registers are left for
   Frag q[N][kSteps];
   RowSums<DP> sums;
   float factor;  // of the products, into exponents of two
@@ -352,43 +390,54 @@ struct RowTile {
     }
   }
 
-  // KB blocks of 32 keys at LDS addresses lds_k, lds_v; sight: what each lane's row sees of them, if masked.
+  // A tile of KB blocks of 32 keys between its steps: scores, then packed probabilities.
   template <int KB>
-  __device__ __forceinline__ void tile(uint32_t lds_k, uint32_t lds_v, bool masked, const uint32_t (&sight)[KB]) {
+  struct Work {
     floatx16 s[KB];
+    u32x4 p[KB][2][N];
+  };
+  template <int KB>
+  __device__ __forceinline__ void scores(Work<KB>& w, uint32_t lds_k) const {
 #pragma unroll
-    for (int b = 0; b < KB; ++b) {
-      s[b] = floatx16{};
+    for (int b = 0; b < KB; ++b) w.s[b] = floatx16{};
+    // the blocks in turn: a product does not follow one of the same sum
+    read_ahead<KB * kSteps, kAhead, Frag>(
+        [&](int i) {
+          return *reinterpret_cast<const __attribute__((address_space(3))) Frag*>(
+              lds_at(lds_k + (key_at ^ (32u * (i / KB)))) + 32 * (i % KB) * L::kRow);
+        },
+        [&](int i, const Frag& k) {
 #pragma unroll
-      for (int t = 0; t < kSteps; ++t) {
-        const Frag k = *reinterpret_cast<const __attribute__((address_space(3))) Frag*>(
-            lds_at(lds_k + (key_at ^ (32u * t))) + 32 * b * L::kRow);
-#pragma unroll
-        for (int n = 0; n < N; ++n) s[b] = C::mfma(k, q[n][t], s[b]);
-      }
-    }
-    if (masked) mask_scores(s, sight, half);
-    sums.softmax(s, factor, C::kLift);
+          for (int n = 0; n < N; ++n) w.s[i % KB] = C::mfma(k, q[n][i / KB], w.s[i % KB]);
+        });
+  }
+  // sight: what each lane's row sees of the tile, if masked.
+  template <int KB>
+  __device__ __forceinline__ void softmax(Work<KB>& w, bool masked, const uint32_t (&sight)[KB]) {
+    if (masked) mask_scores(w.s, sight, half);
+    sums.softmax(w.s, factor, C::kLift);
 #pragma unroll
     for (int b = 0; b < KB; ++b)
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        u32x4 packed[N];
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          uint32_t p[N];
-          split_pair<TYPE, N>(s[b][8 * t + 2 * i], s[b][8 * t + 2 * i + 1], p);
+          uint32_t part[N];
+          split_pair<TYPE, N>(w.s[b][8 * t + 2 * i], w.s[b][8 * t + 2 * i + 1], part);
 #pragma unroll
-          for (int n = 0; n < N; ++n) packed[n][i] = p[n];
+          for (int n = 0; n < N; ++n) w.p[b][t][n][i] = part[n];
         }
-#pragma unroll
-        for (int d = 0; d < kBlocks; ++d) {
-          const Frag v = __builtin_bit_cast(Frag, value(lds_v, 32 * b + 16 * t, d));
+  }
+  template <int KB>
+  __device__ __forceinline__ void add(const Work<KB>& w, uint32_t lds_v) {
+    read_ahead<KB * 2 * kBlocks, kAhead, Frag>(
+        [&](int i) { return __builtin_bit_cast(Frag, value(lds_v, i / kBlocks * 16, i % kBlocks)); },
+        [&](int i, const Frag& v) {
+          const int d = i % kBlocks, step = i / kBlocks;
 #pragma unroll
           for (int n = 0; n < N; ++n)
-            sums.y[d] = C::mfma(v, __builtin_bit_cast(Frag, packed[n]), sums.y[d]);
-        }
-      }
+            sums.y[d] = C::mfma(v, __builtin_bit_cast(Frag, w.p[step / 2][step % 2][n]), sums.y[d]);
+        });
   }
 
   // Keys key .. key + 15, elements 32 d .. 32 d + 31: lane l holds element l % 32 of keys 4 (l / 32) + 0..3 and
@@ -429,28 +478,37 @@ struct RowTile<kAttnF32, Row, DP> {
       q[s] = row && 8 * s < head_dim ? *reinterpret_cast<const floatx4*>(row + 8 * s + 4 * half) : floatx4{};
   }
   template <int KB>
-  __device__ __forceinline__ void tile(uint32_t lds_k, uint32_t lds_v, bool masked, const uint32_t (&sight)[KB]) {
+  struct Work {
     floatx16 s[KB];
+  };
+  template <int KB>
+  __device__ __forceinline__ void scores(Work<KB>& w, uint32_t lds_k) const {
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
-      s[b] = floatx16{};
+      w.s[b] = floatx16{};
 #pragma unroll
       for (int t = 0; t < kSteps; ++t) {
         const floatx4 k = *reinterpret_cast<const __attribute__((address_space(3))) floatx4*>(
             lds_at(lds_k + (key_at ^ (32u * t))) + 32 * b * L::kRow);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[b] = mfma(k[i], q[t][i], s[b]);
+        for (int i = 0; i < 4; ++i) w.s[b] = mfma(k[i], q[t][i], w.s[b]);
       }
     }
-    if (masked) mask_scores(s, sight, half);
-    sums.softmax(s, factor, 0.f);
+  }
+  template <int KB>
+  __device__ __forceinline__ void softmax(Work<KB>& w, bool masked, const uint32_t (&sight)[KB]) {
+    if (masked) mask_scores(w.s, sight, half);
+    sums.softmax(w.s, factor, 0.f);
+  }
+  template <int KB>
+  __device__ __forceinline__ void add(const Work<KB>& w, uint32_t lds_v) {
 #pragma unroll
     for (int b = 0; b < KB; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i)
 #pragma unroll
         for (int d = 0; d < kBlocks; ++d)
-          sums.y[d] = mfma(value(lds_v, 32 * b + 8 * (i / 4) + i % 4, d), s[b][i], sums.y[d]);
+          sums.y[d] = mfma(value(lds_v, 32 * b + 8 * (i / 4) + i % 4, d), w.s[b][i], sums.y[d]);
   }
   __device__ __forceinline__ float value(uint32_t lds_v, int key, int d) const {
     return *reinterpret_cast<const __attribute__((address_space(3))) float*>(lds_at(lds_v + value_at) +
@@ -512,7 +570,7 @@ struct ItemRows {
 
 // Waves share tiles of KT keys, two of which are in LDS; each has 32 rows of its own.
 template <int TYPE, typename Row, int DP, int WAVES, int KT>
-__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_shared_kernel(AttnPlan p, AttnCall c) {
+__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_shared_kernel(AttnPlan p, AttnCall c, AttnCut) {
   constexpr int SIZE = attn_cell_bytes<TYPE>(), KB = KT / 32;
   typedef TileLoader<SIZE, DP, KT> Loader;
   constexpr uint32_t kTile = KT * DP * SIZE;
@@ -526,50 +584,80 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_shared_kernel(Attn
   const ItemRows<Row> rows(p, it, m0, lane);
   const bool any = m0 < rows.rows;
   const Sight sight = rows.sight(p, c, it);
-  // below all_sure every row of the item sees everything, from end on none of this wavefront's sees anything
+  // below all_sure every row of the item sees everything
   const int all_sure = c.parents ? it.context : it.context + it.m0 / p.group + 1;
-  const int end = !any ? 0 : it.context + (c.parents ? it.length : min(m0 + 31, rows.rows - 1) / p.group + 1);
   const Spoiled<SIZE, DP, KT> spoiled{reinterpret_cast<uint32_t*>(lds + 4 * kTile), attn_exponent<TYPE>()};
   spoiled.clear(threadIdx.x, 64 * WAVES);
   RowTile<TYPE, Row, DP> tile;
   tile.start(rows.q(p, c, it, kv_head), p.head_dim, p.scale * kAttnLog2e, lane);
 
-  const size_t layer = (size_t)c.layer * p.pages * p.kv_heads * p.head_dim * SIZE << p.page_shift;
-  const Loader loader{static_cast<const uint8_t*>(p.keys) + layer, static_cast<const uint8_t*>(p.values) + layer,
-                      p.kv_heads, kv_head, p.page_shift, p.head_dim, it.context + it.length - 1};
+  const Loader loader(p, c.layer, kv_head, it);
   const int* table = c.table + it.sequence * c.table_stride;
   const uint32_t base = lds_address(lds);
   const int tiles = (it.key1 - it.key0 + KT - 1) / KT;
-  int pages = table[loader.entry(it.key0, lane)];
-  if (tiles > 0) loader.load(it.key0, pages, base, base + kTile, wave, WAVES, lane);
-  pages = table[loader.entry(it.key0 + KT, lane)];
-  for (int t = 0; t < tiles; ++t) {
-    wait_loads<0>();
-    __syncthreads();
-    const int key = it.key0 + t * KT;
-    const uint32_t now = base + (t & 1) * 2 * kTile, next = base + (~t & 1) * 2 * kTile;
-    if (t + 1 < tiles) {
-      loader.load(key + KT, pages, next, next + kTile, wave, WAVES, lane);
-      pages = table[loader.entry(key + 2 * KT, lane)];
+  auto key_of = [&](int t) { return it.key0 + t * KT; };
+  auto keys_at = [&](int t) { return base + (t & 1) * kTile; };
+  auto values_at = [&](int t) { return base + (2 + (t & 1)) * kTile; };
+  auto pages_of = [&](int t) { return table[loader.entry(key_of(t), lane)]; };
+  auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+  // the pages of tiles t and t + 1 when loads(t) is next
+  int pages = pages_of(0), next_pages = pages_of(1);
+  auto loads = [&](int t) {
+    if (t + 1 < tiles) loader.template load<false, WAVES>(key_of(t + 1), next_pages, keys_at(t + 1), wave, lane);
+    if (t < tiles) loader.template load<true, WAVES>(key_of(t), pages, values_at(t), wave, lane);
+    pages = next_pages;
+    next_pages = pages_of(t + 2);
+  };
+  // after the loads of tile t's values have ended, before they are read
+  auto look = [&](int t) {
+    if (t >= tiles || key_of(t) + KT <= all_sure) return;
+    spoiled.scan(lds + (values_at(t) - base), threadIdx.x, 64 * WAVES);
+    barrier();
+    if (spoiled.any()) {
+      uint32_t see[KB];
+#pragma unroll
+      for (int b = 0; b < KB; ++b) see[b] = sight.bits(key_of(t) + 32 * b);
+      tile.sums.template spoil<KB>(spoiled.bits, see);
+      barrier();
+      spoiled.clear(threadIdx.x, 64 * WAVES);
     }
-    const bool partly = key + KT > all_sure;  // for some row of the workgroup
-    if (partly) {
-      spoiled.scan(lds + (now - base) + kTile, threadIdx.x, 64 * WAVES);
-      __syncthreads();
+  };
+  typename RowTile<TYPE, Row, DP>::template Work<KB> work;
+  if (tiles > 0) loader.template load<false, WAVES>(it.key0, pages, keys_at(0), wave, lane);
+  wait_loads<0>();
+  barrier();
+  // Two phases a tile: products (of the probabilities before and of this tile's scores), then the softmax.  Waves 4 to
+  // 7, which share the SIMDs of waves 0 to 3, are a phase behind, so that one's products run beside the other's softmax.
+  const bool behind = WAVES > 4 && wave >= 4;
+  if (behind) {
+    loads(0);
+    barrier();
+  }
+  for (int t = 0; t <= tiles; ++t) {
+    if (!behind) loads(t);
+    if (any) {
+      if (t > 0) tile.add(work, values_at(t - 1));
+      if (t < tiles) tile.scores(work, keys_at(t));
     }
-    if (key < end) {
+    if (behind) wait_loads<0>();
+    barrier();
+    if (behind) {
+      look(t);
+      loads(t + 1);
+    }
+    if (any && t < tiles) {
+      const bool partly = key_of(t) + KT > all_sure;  // for some row of the workgroup
       uint32_t see[KB] = {};
       if (partly)
 #pragma unroll
-        for (int b = 0; b < KB; ++b) see[b] = sight.bits(key + 32 * b);
-      tile.template tile<KB>(now, now + kTile, partly, see);
-      if (partly && spoiled.any()) tile.sums.template spoil<KB>(spoiled.bits, see);
+        for (int b = 0; b < KB; ++b) see[b] = sight.bits(key_of(t) + 32 * b);
+      tile.softmax(work, partly, see);
     }
-    if (partly && spoiled.any()) {
-      __syncthreads();
-      spoiled.clear(threadIdx.x, 64 * WAVES);
-    }
+    if (!behind) wait_loads<0>();
+    barrier();
+    if (!behind) look(t);
   }
+  if (WAVES > 4 && !behind) barrier();
   const float sum = half_pair_sum(tile.sums.sum);
   if (!rows.real) return;
   if (it.part < 0) {
@@ -594,6 +682,169 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_shared_kernel(Attn
   }
 }
 
+// A call of few rows, of at most kAttnFewSequences sequences, needs no launch before the attend kernel: each of its
+// workgroups makes the plan for itself, checks its sequence, and puts those of the new rows' keys and values that it
+// is about to read into their pages.  (Others that read them put the same bytes there.)
+struct FewLds {
+  static constexpr int kParents = kAttnTreeNodes;
+  int lengths[kAttnFewSequences], contexts[kAttnFewSequences];
+  uint64_t waves[4];
+  int found[4];  // sequence, which of its items, its first tile, its first part
+  int parents[kParents];
+  uint32_t tree[32][kAttnTreeWords];
+};
+
+// Packed counts of tiles, items and parts: 20 bits each.
+__device__ __forceinline__ uint64_t few_counts(const AttnPlan& p, const AttnCall& c, const AttnCut& cut, int length,
+                                               int context, int chunk, int64_t& keys) {
+  uint64_t counts = 0;
+  for (int m0 = 0; m0 < length * p.group; m0 += cut.rows) {
+    const int seen = attn_seen_keys(p, c, cut, m0, length, context);
+    const int n = chunk ? (seen + chunk - 1) / chunk : 0;
+    keys += seen;
+    counts += 1 | (uint64_t)n << 20 | (uint64_t)(n > 1 ? n : 0) << 40;
+  }
+  return counts;
+}
+
+// Whether there is an item `index` to do; by a workgroup of 64 WAVES threads.
+template <int WAVES>
+__device__ __forceinline__ bool few_item(const AttnPlan& p, const AttnCall& c, const AttnCut& cut, FewLds& m, int index,
+                                         int kv_head, AttnItem& it) {
+  constexpr int B = 64 * WAVES;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  bool ascend = true;
+  int64_t keys = 0;
+  for (int i = t; i < c.sequences; i += B) {
+    int begin = i, length = 1;
+    if (c.offsets) {
+      begin = c.offsets[i];
+      const int end = c.offsets[i + 1];
+      ascend = ascend && begin >= 0 && end >= begin && end <= c.tokens;
+      length = end - begin;
+    }
+    int context = c.context[i];
+    if (context < 0 || (int64_t)context + length > p.max_context) {
+      if (ascend && length > 0 && index == 0 && kv_head == 0) atomicOr(p.error, kAttnErrContext);
+      context = length = 0;
+    }
+    m.lengths[i] = length;
+    m.contexts[i] = context;
+    if (ascend) few_counts(p, c, cut, length, context, 0, keys);
+  }
+  if (!__syncthreads_and(ascend)) {
+    if (t == 0 && index == 0 && kv_head == 0) {
+      atomicOr(p.error, kAttnErrOffsets);
+      p.counts[1] = 0;
+    }
+    return false;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) keys += __shfl_xor(keys, o, 64);
+  if (lane == 0) m.waves[wave] = keys;
+  if (t == 0) m.found[0] = -1;
+  __syncthreads();
+  keys = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) keys += m.waves[w];
+  const int chunk = attn_chunk(p, cut, keys);
+  uint64_t before = 0;
+  for (int i0 = 0; i0 < c.sequences; i0 += B) {
+    const int i = i0 + t;
+    int64_t unused = 0;
+    const uint64_t mine = i < c.sequences ? few_counts(p, c, cut, m.lengths[i], m.contexts[i], chunk, unused) : 0;
+    uint64_t sum = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint64_t u = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += u;
+    }
+    __syncthreads();
+    if (lane == 63) m.waves[wave] = sum;
+    __syncthreads();
+    uint64_t all = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      if (w < wave) sum += m.waves[w];
+      all += m.waves[w];
+    }
+    sum += before;
+    before += all;
+    const int last = (int)(sum >> 20 & 0xFFFFF), first = last - (int)(mine >> 20 & 0xFFFFF);
+    if (index >= first && index < last) {
+      m.found[0] = i;
+      m.found[1] = index - first;
+      m.found[2] = (int)((sum - mine) & 0xFFFFF);
+      m.found[3] = (int)((sum - mine) >> 40);
+    }
+  }
+  if (t == 0 && index == 0 && kv_head == 0) p.counts[1] = (int)(before & 0xFFFFF);
+  __syncthreads();
+  auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  it.sequence = uniform(m.found[0]);
+  if (it.sequence < 0) return false;
+  it.begin = c.offsets ? uniform(c.offsets[it.sequence]) : it.sequence;
+  it.length = uniform(m.lengths[it.sequence]);
+  it.context = uniform(m.contexts[it.sequence]);
+  int which = uniform(m.found[1]), tile = uniform(m.found[2]), part = uniform(m.found[3]), seen = 0, n = 0;
+  for (it.m0 = 0;; it.m0 += cut.rows, ++tile) {
+    seen = attn_seen_keys(p, c, cut, it.m0, it.length, it.context);
+    n = (seen + chunk - 1) / chunk;
+    if (which < n) break;
+    which -= n;
+    part += n > 1 ? n : 0;
+  }
+  attn_part(it, seen, n, which, part);
+  // what only a look at the whole sequence shows
+  const int* table = c.table + it.sequence * c.table_stride;
+  int bad = 0;
+  for (int e = t; e <= (it.context + it.length - 1) >> p.page_shift; e += B)
+    if ((uint32_t)table[e] >= (uint32_t)p.pages) bad = kAttnErrPage;
+  if (c.parents) {
+    if (it.length > kAttnTreeNodes) bad |= kAttnErrTree;
+    else
+      for (int j = t; j < it.length; j += B) {
+        m.parents[j] = c.parents[it.begin + j];
+        if (m.parents[j] < -1 || m.parents[j] >= j) bad |= kAttnErrTree;
+      }
+  }
+  if (bad) atomicOr(p.error, bad);
+  const bool refused = __syncthreads_or(bad);
+  if (t == 0 && kv_head == 0 && which == 0)
+    p.joins[tile] = AttnJoin{it.begin, it.length, it.m0, refused ? 0 : n, part, it.sequence};
+  return !refused;
+}
+
+// The new keys and values of an item's positions, and the ancestors of its rows' tokens.
+template <int TYPE, typename Row, int WAVES>
+__device__ __forceinline__ void few_new_rows(const AttnPlan& p, const AttnCall& c, const AttnItem& it, int kv_head,
+                                             FewLds& m) {
+  typedef typename Cell<TYPE>::T T;
+  const int pieces = p.head_dim / 8, first = max(it.key0, it.context), rows = it.key1 - first;
+  const int* table = c.table + it.sequence * c.table_stride;
+  for (int e = threadIdx.x; e < rows * 2 * pieces; e += 64 * WAVES) {
+    const int pos = first + e / (2 * pieces), piece = e % pieces;
+    const bool value = e / pieces & 1;
+    const size_t to = attn_cell(p, c.layer, table[pos >> p.page_shift], pos) +
+                      ((size_t)kv_head << p.page_shift) * p.head_dim + piece * 8;
+    const int64_t row = it.begin + pos - it.context;
+    const Row* from = static_cast<const Row*>(value ? c.v : c.k) + row * (value ? c.v_stride : c.k_stride) +
+                      kv_head * p.head_dim + piece * 8;
+    attn_put8(static_cast<T*>(value ? p.values : p.keys) + to, from);
+  }
+  if (c.parents && threadIdx.x < 32) {
+    const int token = it.m0 / p.group + threadIdx.x;
+    if (token < it.length) {
+      uint32_t* words = m.tree[threadIdx.x];
+#pragma unroll
+      for (int w = 0; w < kAttnTreeWords; ++w) words[w] = 0;
+      for (int n = token; n >= 0; n = m.parents[n]) words[n >> 5] |= 1u << (n & 31);
+    }
+  }
+  wait_loads<0>();  // and stores: what the loads below read is there
+  __syncthreads();
+}
+
 // Waves share 32 rows and take tiles of 32 keys in turn, each from LDS of its own; their sums are joined at the end.
 template <int TYPE, typename Row, int DP, int WAVES>
 struct SplitLds {
@@ -602,11 +853,12 @@ struct SplitLds {
   static constexpr int kRow = DP + 4;               // floats of a row of sums, in the same memory
   static_assert(32 * kRow * 4 <= kWave, "a wavefront's sums fit its tiles");
   static constexpr int kSpoiled = Spoiled<attn_cell_bytes<TYPE>(), DP, 32>::kBytes / 4;
-  static constexpr int kBytes = WAVES * kWave + WAVES * 64 * 4 + kAttnPageList * 4 + WAVES * kSpoiled * 4;
+  static constexpr int kSums = (WAVES * 64 + kAttnPageList + WAVES * kSpoiled + 1) / 2 * 8;  // the few's are 8-byte aligned
+  static constexpr int kBytes = WAVES * kWave + kSums + (int)sizeof(FewLds);
 };
 
 template <int TYPE, typename Row, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, 1) void attn_split_kernel(AttnPlan p, AttnCall c) {
+__global__ __launch_bounds__(64 * WAVES, 1) void attn_split_kernel(AttnPlan p, AttnCall c, AttnCut cut) {
   constexpr int SIZE = attn_cell_bytes<TYPE>(), KT = 32;
   typedef TileLoader<SIZE, DP, KT> Loader;
   typedef SplitLds<TYPE, Row, DP, WAVES> M;
@@ -615,19 +867,23 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attn_split_kernel(AttnPlan p, A
   float* const ml = reinterpret_cast<float*>(lds + WAVES * M::kWave);  // [WAVES][2][32]
   int* const list = reinterpret_cast<int*>(ml + WAVES * 64);
   const int index = blockIdx.x / p.kv_heads, kv_head = blockIdx.x % p.kv_heads;
-  if (index >= p.counts[0]) return;
-  const AttnItem it = uniform_item(p.items + index);
-  if (!p.run[it.sequence]) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  FewLds& few = *reinterpret_cast<FewLds*>(lds + WAVES * M::kWave + M::kSums);
+  AttnItem it;
+  if (cut.few) {
+    if (!few_item<WAVES>(p, c, cut, few, index, kv_head, it)) return;
+    few_new_rows<TYPE, Row, WAVES>(p, c, it, kv_head, few);
+  } else {
+    if (index >= p.counts[0]) return;
+    it = uniform_item(p.items + index);
+    if (!p.run[it.sequence]) return;
+  }
   const ItemRows<Row> rows(p, it, it.m0, lane);
-  const Sight sight = rows.sight(p, c, it);
+  Sight sight = rows.sight(p, c, it);
+  if (cut.few && c.parents) sight.tree = few.tree[rows.token - it.m0 / p.group];
   const int sure = c.parents ? it.context : it.context + it.m0 / p.group + 1;
-  RowTile<TYPE, Row, DP> tile;
-  tile.start(rows.q(p, c, it, kv_head), p.head_dim, p.scale * kAttnLog2e, lane);
-
-  const size_t layer = (size_t)c.layer * p.pages * p.kv_heads * p.head_dim * SIZE << p.page_shift;
-  const Loader loader{static_cast<const uint8_t*>(p.keys) + layer, static_cast<const uint8_t*>(p.values) + layer,
-                      p.kv_heads, kv_head, p.page_shift, p.head_dim, it.context + it.length - 1};
+  RowTile<TYPE, Row, DP> tile;  // started behind the first loads, which its rows need not wait for
+  const Loader loader(p, c.layer, kv_head, it);
   const int* table = c.table + it.sequence * c.table_stride;
   const uint32_t lds_base = lds_address(lds), base = lds_base + wave * M::kWave;
   const Spoiled<SIZE, DP, KT> spoiled{reinterpret_cast<uint32_t*>(list + kAttnPageList) + wave * M::kSpoiled,
@@ -638,15 +894,17 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attn_split_kernel(AttnPlan p, A
     const int first = key0 >> p.page_shift;
     const int key1 = (int)min((int64_t)it.key1, ((int64_t)first << p.page_shift) + stretch);
     const int entries = loader.entry(key1 - 1, 0) - first + 1;
-    __syncthreads();
+    if (key0 != it.key0) __syncthreads();
     for (int i = threadIdx.x; i < entries; i += 64 * WAVES) list[i] = table[first + i];
     __syncthreads();
     auto load = [&](int key, int buffer) {
       const int pages = list[min(loader.entry(key, lane) - first, entries - 1)];
-      loader.load(key, pages, base + buffer * 2 * M::kTile, base + buffer * 2 * M::kTile + M::kTile, 0, 1, lane);
+      loader.template load<false, 1>(key, pages, base + buffer * 2 * M::kTile, 0, lane);
+      loader.template load<true, 1>(key, pages, base + buffer * 2 * M::kTile + M::kTile, 0, lane);
     };
     int key = key0 + KT * wave;
     if (key < key1) load(key, 0);
+    if (key0 == it.key0) tile.start(rows.q(p, c, it, kv_head), p.head_dim, p.scale * kAttnLog2e, lane);
     for (int t = 0; key < key1; ++t, key += KT * WAVES) {
       if (key + KT * WAVES < key1) {
         load(key + KT * WAVES, ~t & 1);
@@ -664,7 +922,10 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attn_split_kernel(AttnPlan p, A
         spoiled.scan(lds + (now - lds_base) + M::kTile, lane, 64);
         wave_lds_order();
       }
-      tile.template tile<1>(now, now + M::kTile, partly, see);
+      typename RowTile<TYPE, Row, DP>::template Work<1> work;
+      tile.scores(work, now);
+      tile.softmax(work, partly, see);
+      tile.add(work, now + M::kTile);
       if (partly && spoiled.any()) tile.sums.template spoil<1>(spoiled.bits, see);
       wave_lds_order();  // the next load into this tile's place follows its reads
     }
@@ -714,12 +975,12 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attn_split_kernel(AttnPlan p, A
 // ------------------------------------------------------------------ launches
 template <typename Kernel>
 hipError_t attn_launch(Kernel k, uint32_t grid, int threads, int lds, hipStream_t s, const AttnPlan& p,
-                       const AttnCall& c) {
+                       const AttnCall& c, const AttnCut& cut) {
   if (lds > 65536) {
     hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(k, dim3(grid), dim3(threads), lds, s, p, c);
+  hipLaunchKernelGGL(k, dim3(grid), dim3(threads), lds, s, p, c, cut);
   return hipGetLastError();
 }
 
@@ -744,10 +1005,10 @@ hipError_t attn_attend(const AttnPlan& p, const AttnCall& c, const AttnCut& cut,
   if (cut.shared) {
     constexpr int W = attn_shared_waves<TYPE, Row, DP>(), KT = attn_shared_keys<TYPE, DP>();
     return attn_launch(attn_shared_kernel<TYPE, Row, DP, W, KT>, grid, 64 * W, 
-                       4 * KT * DP * attn_cell_bytes<TYPE>() + Spoiled<attn_cell_bytes<TYPE>(), DP, KT>::kBytes, s, p, c);
+                       4 * KT * DP * attn_cell_bytes<TYPE>() + Spoiled<attn_cell_bytes<TYPE>(), DP, KT>::kBytes, s, p, c, cut);
   }
   constexpr int W = attn_split_waves<TYPE, DP>();
-  return attn_launch(attn_split_kernel<TYPE, Row, DP, W>, grid, 64 * W, SplitLds<TYPE, Row, DP, W>::kBytes, s, p, c);
+  return attn_launch(attn_split_kernel<TYPE, Row, DP, W>, grid, 64 * W, SplitLds<TYPE, Row, DP, W>::kBytes, s, p, c, cut);
 }
 
 template <int TYPE, typename Row>

@@ -55,7 +55,7 @@ def attention(q, keys, values, visible, scale, row_kind, cache_kind):
     dim products, each at most u off at each of dim additions; two roundings by the factor.  A score's error e
     makes a probability's relative one e, and as much in their sum.  The exponential, the probabilities' split and
     the joins' factors: 16 u, and u of the exponent's argument; parts of f16 are off by 2^-25 at least, next to
-    2^15 for the row's largest probability.  Sums over n positions: no longer chain of additions than n / 8 + 64 (a lane adds
+    2^9 or more for the row's largest probability (a half of the smallest step, and as much of the second part).  Sums over n positions: no longer chain of additions than n / 8 + 64 (a lane adds
     every eighth probability; a product sums 16 at a time).  Probabilities of 16-bit rows are rounded once, and
     so is their output."""
     rows, heads, dim = q.shape
@@ -85,7 +85,7 @@ def attention(q, keys, values, visible, scale, row_kind, cache_kind):
             chain = visible.sum(1, keepdims=True) / 8 + 64
             bound[:, h] = (2 * e + (16 + chain) * u) * reach + 2 * u * far
             if cache_kind == "f16":
-                bound[:, h] += 2.0 ** -39 * visible @ np.abs(vf)
+                bound[:, h] += 2.0 ** -33 * visible @ np.abs(vf)
             if row_kind != "f32":
                 bound[:, h] += 1.001 * EPS[row_kind] / 2 * (reach + np.abs(y[:, h])) + 2.0 ** -24
     return y, bound
