@@ -2149,7 +2149,7 @@ int llambda_hip_attention_session_create(const llambda_hip_attention_desc* d,
     AttnPlan& p = s->plan;
     p.heads = (int)d->heads;
     p.kv_heads = (int)d->kv_heads;
-    p.group = (int)(d->heads / d->kv_heads);
+    p.group = attn_divisor((uint32_t)(d->heads / d->kv_heads));
     p.head_dim = (int)d->head_dim;
     p.row_type = d->row_type;
     p.cache_type = d->cache_type;

@@ -42,8 +42,24 @@ struct AttnJoin {
   int begin, length, m0, parts, part0, sequence;
 };
 
+// Quotients by a divisor of whole numbers below 2^31.
+struct AttnDivisor {
+  uint32_t divisor, factor, shift;
+};
+inline AttnDivisor attn_divisor(uint32_t d) {
+  uint32_t l = 0;
+  while ((1ull << l) < d) ++l;
+  return AttnDivisor{d, (uint32_t)((((1ull << l) - d) << 32) / d + 1), l};
+}
+__host__ __device__ __forceinline__ int operator/(int n, const AttnDivisor& d) {
+  const uint32_t high = (uint32_t)(((uint64_t)d.factor * (uint32_t)n) >> 32);
+  return (int)((high + (uint32_t)n) >> d.shift);
+}
+__host__ __device__ __forceinline__ int operator%(int n, const AttnDivisor& d) { return n - n / d * (int)d.divisor; }
+
 struct AttnPlan {
-  int heads, kv_heads, group, head_dim;
+  int heads, kv_heads, head_dim;
+  AttnDivisor group;       // heads to a kv head
   int row_type, cache_type;
   float scale;
   int layers, pages, page_shift;
@@ -104,7 +120,7 @@ struct AttnCut {
   bool shared;      // the waves of a workgroup share a tile of keys (and have rows of their own), or the reverse
   int rows;         // of an item
   int min_keys;     // of a part
-  int slots;        // parts over all kv heads come to about this many workgroups
+  int slots_log2;   // parts over all kv heads come to about this many workgroups
   bool few;         // the attend kernel makes the plan and puts the new rows into the cache
 };
 // The kernels of one cache type (attention_f16.hip, attention_bf16.hip, attention_f32.hip).

@@ -116,7 +116,7 @@ __device__ void plan(const AttnPlan& p, const AttnCall& c, const AttnCut& cut) {
       // a refused sequence's items do nothing; they only have to be few
       if (s.context < 0 || (int64_t)s.context + s.length > p.max_context) s.context = s.length = 0;
       int tiles;
-      ends[threadIdx.x] = block_scan(ceil_div((int64_t)s.length * p.group, cut.rows), scan, tiles);
+      ends[threadIdx.x] = block_scan((s.length * (int)p.group.divisor + cut.rows - 1) / cut.rows, scan, tiles);
       lengths[threadIdx.x] = s.length;
       contexts[threadIdx.x] = s.context;
       begins[threadIdx.x] = s.begin;
@@ -141,7 +141,7 @@ __device__ void plan(const AttnPlan& p, const AttnCall& c, const AttnCut& cut) {
           if ((threadIdx.x & 63) == 0) atomicAdd(&keys, v);
           continue;
         }
-        if (t < tiles) n = (seen + chunk - 1) / chunk;
+        if (t < tiles) n = attn_parts_of(seen, chunk);
         int all_items, all_joins, all_parts;
         const int item = items + block_scan(n, scan, all_items) - n;
         const int join = joins + block_scan(n > 1, scan, all_joins) - (n > 1);
@@ -225,7 +225,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnPlan p, AttnCall c, 
   const AttnJoin j = p.joins[index];
   const int kv_head = rest / blocks, lane = threadIdx.x & 63;
   const int r = rest % blocks * 4 + (threadIdx.x >> 6);
-  if (j.parts < 2 || r >= cut.rows || j.m0 + r >= j.length * p.group || (!cut.few && !p.run[j.sequence])) return;
+  if (j.parts < 2 || r >= cut.rows || j.m0 + r >= j.length * (int)p.group.divisor || (!cut.few && !p.run[j.sequence])) return;
   const size_t step = (size_t)p.kv_heads * cut.rows;
   const size_t row = ((size_t)j.part0 * p.kv_heads + kv_head) * cut.rows + r;
   float reference = -__builtin_inff();
@@ -259,7 +259,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnPlan p, AttnCall c, 
   if (4 * lane >= p.head_dim) return;
   const int m = j.m0 + r;
   Row* y = static_cast<Row*>(c.y) + (j.begin + m / p.group) * c.y_stride +
-           (kv_head * p.group + m % p.group) * p.head_dim + d;
+           (kv_head * (int)p.group.divisor + m % p.group) * p.head_dim + d;
   typedef Row Row4 __attribute__((ext_vector_type(4)));
   *reinterpret_cast<Row4*>(y) = __builtin_convertvector(v * (1.f / total), Row4);
 }
@@ -318,9 +318,9 @@ __global__ void attn_take_error_kernel(int* error) {
 
 constexpr int kCus = 256;
 #ifndef RT
-#define SLS 256
+#define SLS 8
 #define MINS 256
-#define SLP 512
+#define SLP 9
 #define MINP 256
 #define RT 160
 #endif
@@ -335,23 +335,23 @@ static AttnCut cut_as(const AttnPlan& p, bool shared) {
   cut.shared = shared;
   cut.rows = shared ? 32 * shared_waves(p) : 32;
   cut.min_keys = shared ? MINS : MINP;
-  cut.slots = shared ? SLS : SLP;
+  cut.slots_log2 = shared ? SLS : SLP;
   return cut;
 }
 static AttnCut cut_of(const AttnPlan& p, const AttnCall& c) {
   // rows of a kv head in a sequence, on average; the lengths are on the device
-  AttnCut cut = cut_as(p, ceil_div((int64_t)c.tokens * p.group, c.sequences) > RT);
+  AttnCut cut = cut_as(p, ceil_div((int64_t)c.tokens * p.group.divisor, c.sequences) > RT);
   cut.few = !cut.shared && c.tokens <= kAttnFewTokens && c.sequences <= kAttnFewSequences;
   return cut;
 }
 
 // Items of a call at most: a tile for each cut.rows rows, one more for each sequence, and parts that are no shorter
-// than the keys of all tiles over cut.slots.
+// than the keys of all tiles over 2^slots_log2.
 static int64_t tiles_of(const AttnPlan& p, int64_t tokens, int64_t sequences, int rows) {
-  return std::min(tokens * p.group / rows + sequences, tokens * p.group);
+  return std::min(tokens * p.group.divisor / rows + sequences, tokens * p.group.divisor);
 }
 static int64_t items_of(const AttnPlan& p, int64_t tokens, int64_t sequences, const AttnCut& cut) {
-  return tiles_of(p, tokens, sequences, cut.rows) + cut.slots / p.kv_heads;
+  return tiles_of(p, tokens, sequences, cut.rows) + (1 << cut.slots_log2) / p.kv_heads;
 }
 
 AttnSizes attn_sizes(const AttnPlan& p) {
@@ -359,7 +359,7 @@ AttnSizes attn_sizes(const AttnPlan& p) {
   for (int shared = 0; shared < 2; ++shared) {
     const AttnCut cut = cut_as(p, shared);
     const int64_t tiles = tiles_of(p, p.max_tokens, p.max_sequences, cut.rows);
-    const int64_t split = cut.slots / p.kv_heads;
+    const int64_t split = (1 << cut.slots_log2) / p.kv_heads;
     s.items = std::max(s.items, tiles + split);
     s.joins = std::max(s.joins, std::min(tiles, split));
     if (!shared)  // of a call of few rows one for each tile
@@ -378,11 +378,11 @@ static int64_t prepare_share(const AttnPlan& p, const AttnCall& c) {
 }
 static int64_t join_blocks(const AttnCut& cut, const AttnPlan& p, const AttnCall& c) {
   // 4 rows each; a step has only a group's
-  return ceil_div(c.offsets ? cut.rows : std::min(cut.rows, p.group), 4);
+  return ceil_div(c.offsets ? cut.rows : std::min<int>(cut.rows, p.group.divisor), 4);
 }
 static int64_t join_grid(const AttnPlan& p, const AttnCall& c, const AttnCut& cut) {
   const int64_t tiles = tiles_of(p, c.tokens, c.sequences, cut.rows);
-  return (cut.few ? tiles : std::min<int64_t>(tiles, cut.slots / p.kv_heads)) * p.kv_heads * join_blocks(cut, p, c);
+  return (cut.few ? tiles : std::min<int64_t>(tiles, (1 << cut.slots_log2) / p.kv_heads)) * p.kv_heads * join_blocks(cut, p, c);
 }
 
 bool attn_call_fits(const AttnPlan& p, const AttnCall& c) {

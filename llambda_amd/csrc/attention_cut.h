@@ -16,15 +16,19 @@ __device__ __forceinline__ int attn_seen_keys(const AttnPlan& p, const AttnCall&
 // Positions of a part, whole tiles: about the work of a kv head's rows (`keys`, over all tiles) over the workgroups
 // that the device holds.
 __device__ __forceinline__ int attn_chunk(const AttnPlan& p, const AttnCut& cut, int64_t keys) {
-  const int64_t share = (keys * p.kv_heads + cut.slots - 1) / cut.slots;
-  return (int)((min(max(share, (int64_t)cut.min_keys), (int64_t)1 << 30) + 63) / 64 * 64);
+  const int64_t share = ((keys * p.kv_heads - 1) >> cut.slots_log2) + 1;
+  return ((int)min(max(share, (int64_t)cut.min_keys), (int64_t)1 << 30) + 63) & ~63;
 }
 
-// Part k of n equal ones of the positions that a tile sees.
+// Parts of the positions that a tile sees, no longer than `chunk`.
+__device__ __forceinline__ int attn_parts_of(int seen, int chunk) {
+  return seen <= chunk ? 1 : (int)(((uint32_t)seen + chunk - 1) / (uint32_t)chunk);
+}
+// Part k of the n equal ones, of whole tiles.  (None is empty: they are no longer than the chunk that n came from.)
 __device__ __forceinline__ void attn_part(AttnItem& it, int seen, int n, int k, int part) {
-  const int64_t size = ((seen + n - 1) / n + 63) / 64 * 64;
-  it.key0 = (int)min(k * size, (int64_t)seen);
-  it.key1 = (int)min((k + 1) * size, (int64_t)seen);
+  const uint32_t size = n > 1 ? (((uint32_t)seen + n - 1) / n + 63) & ~63u : seen;
+  it.key0 = k * size;
+  it.key1 = min((k + 1) * size, (uint32_t)seen);
   it.part = n > 1 ? part + k : -1;
 }
 

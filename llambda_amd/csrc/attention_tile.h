@@ -117,19 +117,6 @@ __device__ __forceinline__ void read_ahead(Read&& read, Use&& use) {
 }
 
 template <typename Row>
-__device__ __forceinline__ void load8(const Row* p, float (&v)[8]) {
-  if constexpr (sizeof(Row) == 4) {
-    const floatx4 a = *reinterpret_cast<const floatx4*>(p), b = *reinterpret_cast<const floatx4*>(p + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
-  } else {
-    typedef Row Row8 __attribute__((ext_vector_type(8)));
-    const Row8 a = *reinterpret_cast<const Row8*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
-  }
-}
-template <typename Row>
 __device__ __forceinline__ void store4(Row* p, floatx4 v) {
   if constexpr (sizeof(Row) == 4) {
     *reinterpret_cast<floatx4*>(p) = v;
@@ -306,22 +293,28 @@ struct Spoiled {
   // The tile at `tile`, by `threads` threads; the words are clear.
   __device__ __forceinline__ void scan(uint8_t* tile, int thread, int threads) const {
     typedef TileLayout<SIZE, DP> L;
+    // an exponent of ones carries into the sign's place
+    constexpr uint32_t kSigns = SIZE == 4 ? 0x80000000u : 0x80008000u;
+#pragma unroll 4
     for (int i = thread; i < KT * L::kPieces; i += threads) {
       u32x4 v = *reinterpret_cast<const u32x4*>(tile + 16 * i);
-      const int key = i / L::kPieces;
-      const int d = ((i % L::kPieces) ^ L::value_swizzle(key)) * (16 / SIZE);
-      uint32_t bad = 0;
-      if constexpr (SIZE == 4) {
+      uint32_t carry = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if ((v[k] & 0x7F800000u) == 0x7F800000u) bad |= 1u << k, v[k] = 0;
-      } else {
+      for (int k = 0; k < 4; ++k) carry |= (v[k] & ~kSigns) + one;
+      if (carry & kSigns) {
+        const int key = i / L::kPieces;
+        const int d = ((i % L::kPieces) ^ L::value_swizzle(key)) * (16 / SIZE);
+        uint32_t bad = 0;
+        if constexpr (SIZE == 4) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if ((v[k / 2] >> (16 * (k & 1)) & exponent) == exponent)
-            bad |= 1u << k, v[k / 2] &= k & 1 ? 0xFFFFu : 0xFFFF0000u;
-      }
-      if (bad) {
+          for (int k = 0; k < 4; ++k)
+            if ((v[k] & ~kSigns) + one & kSigns) bad |= 1u << k, v[k] = 0;
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if ((v[k / 2] & ~kSigns) + one & (k & 1 ? 0x80000000u : 0x8000u))
+              bad |= 1u << k, v[k / 2] &= k & 1 ? 0xFFFFu : 0xFFFF0000u;
+        }
         *reinterpret_cast<u32x4*>(tile + 16 * i) = v;
         atomicOr(bits + key * kWords + d / 32, bad << (d % 32));
         bits[KT * kWords] = 1;
@@ -329,7 +322,7 @@ struct Spoiled {
     }
   }
   __device__ __forceinline__ bool any() const { return __builtin_amdgcn_readfirstlane(bits[KT * kWords]) != 0; }
-  uint32_t exponent;  // of 16 bits
+  uint32_t one;  // the lowest bit of an element's exponent, for each in 32 bits
 };
 
 template <int TYPE, typename Row, int DP>
@@ -345,22 +338,39 @@ struct RowTile {
   uint32_t key_at, value_at;
   int half;
 
-  // row: null for rows behind the last.  Lane l holds elements 16 s + 8 (l / 32) + 0..7 of row l % 32.
-  __device__ __forceinline__ void start(const Row* row, int head_dim, float scale_log2, int lane) {
+  // A row as it is on its way.  Lane l holds elements 16 s + 8 (l / 32) + 0..7 of row l % 32.
+  typedef Row Row8 __attribute__((ext_vector_type(8)));
+  struct Raw {
+    Row8 v[kSteps];
+  };
+  // row: null for rows behind the last.
+  __device__ __forceinline__ static void fetch(Raw& raw, const Row* row, int head_dim, int lane) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      raw.v[s] = Row8{};
+      if (row && 16 * s < head_dim) raw.v[s] = *reinterpret_cast<const Row8*>(row + 16 * s + 8 * (lane >> 5));
+    }
+  }
+  __device__ __forceinline__ void start(const Raw& raw, float scale_log2, int lane) {
     half = lane >> 5;
     sums.clear();
     const int r = lane & 31, j = lane & 15;
     key_at = r * L::kRow + 16 * (half ^ L::key_swizzle(r));
     value_at = (4 * half + (j >> 2)) * L::kRow + 16 * L::value_swizzle(j >> 2) + ((lane >> 4) & 1) * 32 + (j & 3) * 8;
+    if constexpr (N == 1) {
+      factor = scale_log2;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) q[0][s] = __builtin_bit_cast(Frag, raw.v[s]);
+      return;
+    }
     float v[kSteps][8], top = 0.f;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
+    for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[s][i] = 0.f;
-      if (row && 16 * s < head_dim) load8(row + 16 * s + 8 * half, v[s]);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[s][i]));
-    }
+      for (int i = 0; i < 8; ++i) {
+        v[s][i] = (float)raw.v[s][i];
+        top = fmaxf(top, fabsf(v[s][i]));
+      }
     float lift = 1.f;
     if (N == 2) {
       // the row's largest between 2^13 and 2^14 (rows next to zero, infinities and NaN as they are)
@@ -466,7 +476,17 @@ struct RowTile<kAttnF32, Row, DP> {
   static __device__ __forceinline__ floatx16 mfma(float a, float b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
   }
-  __device__ __forceinline__ void start(const Row* row, int head_dim, float scale_log2, int lane) {
+  struct Raw {
+    floatx4 v[kSteps];
+  };
+  __device__ __forceinline__ static void fetch(Raw& raw, const Row* row, int head_dim, int lane) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      raw.v[s] = floatx4{};
+      if (row && 8 * s < head_dim) raw.v[s] = *reinterpret_cast<const floatx4*>(row + 8 * s + 4 * (lane >> 5));
+    }
+  }
+  __device__ __forceinline__ void start(const Raw& raw, float scale_log2, int lane) {
     half = lane >> 5;
     sums.clear();
     const int r = lane & 31;
@@ -474,8 +494,7 @@ struct RowTile<kAttnF32, Row, DP> {
     value_at = 4 * half * L::kRow + 4 * r;
     factor = scale_log2;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-      q[s] = row && 8 * s < head_dim ? *reinterpret_cast<const floatx4*>(row + 8 * s + 4 * half) : floatx4{};
+    for (int s = 0; s < kSteps; ++s) q[s] = raw.v[s];
   }
   template <int KB>
   struct Work {
@@ -527,7 +546,7 @@ constexpr int attn_cell_bytes() {
 
 template <int TYPE>
 constexpr uint32_t attn_exponent() {
-  return TYPE == kAttnF16 ? 0x7C00u : 0x7F80u;
+  return TYPE == kAttnF16 ? 0x04000400u : TYPE == kAttnBF16 ? 0x00800080u : 0x00800000u;
 }
 // LDS accesses of this wavefront so far are done before those that follow.
 __device__ __forceinline__ void wave_lds_order() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
@@ -547,13 +566,13 @@ struct ItemRows {
   int token;   // its token, the last one's for rows behind it
   bool real;
   __device__ __forceinline__ ItemRows(const AttnPlan& p, const AttnItem& it, int m0, int lane) {
-    rows = it.length * p.group;
+    rows = it.length * (int)p.group.divisor;
     m = m0 + (lane & 31);
     real = m < rows;
     token = min(m, rows - 1) / p.group;
   }
   __device__ __forceinline__ int head(const AttnPlan& p, int kv_head) const {
-    return kv_head * p.group + min(m, rows - 1) % p.group;
+    return kv_head * (int)p.group.divisor + min(m, rows - 1) % p.group;
   }
   __device__ __forceinline__ const Row* q(const AttnPlan& p, const AttnCall& c, const AttnItem& it, int kv_head) const {
     return real ? static_cast<const Row*>(c.q) + (it.begin + token) * c.q_stride + head(p, kv_head) * p.head_dim
@@ -588,8 +607,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_shared_kernel(Attn
   const int all_sure = c.parents ? it.context : it.context + it.m0 / p.group + 1;
   const Spoiled<SIZE, DP, KT> spoiled{reinterpret_cast<uint32_t*>(lds + 4 * kTile), attn_exponent<TYPE>()};
   spoiled.clear(threadIdx.x, 64 * WAVES);
-  RowTile<TYPE, Row, DP> tile;
-  tile.start(rows.q(p, c, it, kv_head), p.head_dim, p.scale * kAttnLog2e, lane);
+  typedef RowTile<TYPE, Row, DP> Tile;
+  Tile tile;
 
   const Loader loader(p, c.layer, kv_head, it);
   const int* table = c.table + it.sequence * c.table_stride;
@@ -622,8 +641,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_shared_kernel(Attn
       spoiled.clear(threadIdx.x, 64 * WAVES);
     }
   };
-  typename RowTile<TYPE, Row, DP>::template Work<KB> work;
+  typename Tile::template Work<KB> work;
   if (tiles > 0) loader.template load<false, WAVES>(it.key0, pages, keys_at(0), wave, lane);
+  typename Tile::Raw raw;
+  Tile::fetch(raw, rows.q(p, c, it, kv_head), p.head_dim, lane);
+  tile.start(raw, p.scale * kAttnLog2e, lane);
   wait_loads<0>();
   barrier();
   // Two phases a tile: products (of the probabilities before and of this tile's scores), then the softmax.  Waves 4 to
@@ -690,6 +712,7 @@ struct FewLds {
   int lengths[kAttnFewSequences], contexts[kAttnFewSequences];
   uint64_t waves[4];
   int found[4];  // sequence, which of its items, its first tile, its first part
+  int tile[3];   // the item's: its place among all, its parts and the first of them
   int parents[kParents];
   uint32_t tree[32][kAttnTreeWords];
 };
@@ -698,16 +721,16 @@ struct FewLds {
 __device__ __forceinline__ uint64_t few_counts(const AttnPlan& p, const AttnCall& c, const AttnCut& cut, int length,
                                                int context, int chunk, int64_t& keys) {
   uint64_t counts = 0;
-  for (int m0 = 0; m0 < length * p.group; m0 += cut.rows) {
+  for (int m0 = 0; m0 < length * (int)p.group.divisor; m0 += cut.rows) {
     const int seen = attn_seen_keys(p, c, cut, m0, length, context);
-    const int n = chunk ? (seen + chunk - 1) / chunk : 0;
+    const int n = chunk ? attn_parts_of(seen, chunk) : 0;
     keys += seen;
     counts += 1 | (uint64_t)n << 20 | (uint64_t)(n > 1 ? n : 0) << 40;
   }
   return counts;
 }
 
-// Whether there is an item `index` to do; by a workgroup of 64 WAVES threads.
+// Whether there is an item `index`; by a workgroup of 64 WAVES threads.
 template <int WAVES>
 __device__ __forceinline__ bool few_item(const AttnPlan& p, const AttnCall& c, const AttnCut& cut, FewLds& m, int index,
                                          int kv_head, AttnItem& it) {
@@ -789,60 +812,73 @@ __device__ __forceinline__ bool few_item(const AttnPlan& p, const AttnCall& c, c
   int which = uniform(m.found[1]), tile = uniform(m.found[2]), part = uniform(m.found[3]), seen = 0, n = 0;
   for (it.m0 = 0;; it.m0 += cut.rows, ++tile) {
     seen = attn_seen_keys(p, c, cut, it.m0, it.length, it.context);
-    n = (seen + chunk - 1) / chunk;
+    n = attn_parts_of(seen, chunk);
     if (which < n) break;
     which -= n;
     part += n > 1 ? n : 0;
   }
   attn_part(it, seen, n, which, part);
-  // what only a look at the whole sequence shows
-  const int* table = c.table + it.sequence * c.table_stride;
+  m.tile[0] = tile;
+  m.tile[1] = n;
+  m.tile[2] = part;
+  return true;
+}
+
+// Checks an item's sequence; then the new keys and values of its positions, the ancestors of its rows' tokens, and the
+// list of its first pages.
+template <int TYPE, typename Row, int WAVES>
+__device__ __forceinline__ bool few_checked(const AttnPlan& p, const AttnCall& c, const AttnItem& it, int kv_head,
+                                            FewLds& m, int* list) {
+  typedef typename Cell<TYPE>::T T;
+  constexpr int B = 64 * WAVES;
+  const int t = threadIdx.x, first_page = it.key0 >> p.page_shift;
   int bad = 0;
-  for (int e = t; e <= (it.context + it.length - 1) >> p.page_shift; e += B)
-    if ((uint32_t)table[e] >= (uint32_t)p.pages) bad = kAttnErrPage;
+  for (int e = t; e <= (it.context + it.length - 1) >> p.page_shift; e += B) {
+    const int page = c.table[it.sequence * c.table_stride + e];
+    if ((uint32_t)page >= (uint32_t)p.pages) bad = kAttnErrPage;
+    if ((uint32_t)(e - first_page) < (uint32_t)kAttnPageList) list[e - first_page] = page;
+  }
   if (c.parents) {
-    if (it.length > kAttnTreeNodes) bad |= kAttnErrTree;
-    else
+    if (it.length > kAttnTreeNodes) {
+      bad |= kAttnErrTree;
+    } else {
       for (int j = t; j < it.length; j += B) {
         m.parents[j] = c.parents[it.begin + j];
         if (m.parents[j] < -1 || m.parents[j] >= j) bad |= kAttnErrTree;
       }
+    }
   }
   if (bad) atomicOr(p.error, bad);
   const bool refused = __syncthreads_or(bad);
-  if (t == 0 && kv_head == 0 && which == 0)
-    p.joins[tile] = AttnJoin{it.begin, it.length, it.m0, refused ? 0 : n, part, it.sequence};
-  return !refused;
-}
-
-// The new keys and values of an item's positions, and the ancestors of its rows' tokens.
-template <int TYPE, typename Row, int WAVES>
-__device__ __forceinline__ void few_new_rows(const AttnPlan& p, const AttnCall& c, const AttnItem& it, int kv_head,
-                                             FewLds& m) {
-  typedef typename Cell<TYPE>::T T;
+  if (t == 0 && kv_head == 0 && it.key0 == 0)
+    p.joins[m.tile[0]] = AttnJoin{it.begin, it.length, it.m0, refused ? 0 : m.tile[1], m.tile[2], it.sequence};
+  if (refused) return false;
   const int pieces = p.head_dim / 8, first = max(it.key0, it.context), rows = it.key1 - first;
-  const int* table = c.table + it.sequence * c.table_stride;
-  for (int e = threadIdx.x; e < rows * 2 * pieces; e += 64 * WAVES) {
+  if (rows <= 0 && !c.parents) return true;
+  for (int e = t; e < rows * 2 * pieces; e += B) {
     const int pos = first + e / (2 * pieces), piece = e % pieces;
     const bool value = e / pieces & 1;
-    const size_t to = attn_cell(p, c.layer, table[pos >> p.page_shift], pos) +
+    const int entry = (pos >> p.page_shift) - first_page;
+    const int page = entry < kAttnPageList ? list[entry] : c.table[it.sequence * c.table_stride + first_page + entry];
+    const size_t to = attn_cell(p, c.layer, page, pos) +
                       ((size_t)kv_head << p.page_shift) * p.head_dim + piece * 8;
     const int64_t row = it.begin + pos - it.context;
     const Row* from = static_cast<const Row*>(value ? c.v : c.k) + row * (value ? c.v_stride : c.k_stride) +
                       kv_head * p.head_dim + piece * 8;
     attn_put8(static_cast<T*>(value ? p.values : p.keys) + to, from);
   }
-  if (c.parents && threadIdx.x < 32) {
-    const int token = it.m0 / p.group + threadIdx.x;
+  if (c.parents && t < 32) {
+    const int token = it.m0 / p.group + t;
     if (token < it.length) {
-      uint32_t* words = m.tree[threadIdx.x];
+      uint32_t* words = m.tree[t];
 #pragma unroll
       for (int w = 0; w < kAttnTreeWords; ++w) words[w] = 0;
       for (int n = token; n >= 0; n = m.parents[n]) words[n >> 5] |= 1u << (n & 31);
     }
   }
-  wait_loads<0>();  // and stores: what the loads below read is there
+  wait_loads<0>();  // and stores: what the tiles' loads read is there
   __syncthreads();
+  return true;
 }
 
 // Waves share 32 rows and take tiles of 32 keys in turn, each from LDS of its own; their sums are joined at the end.
@@ -869,20 +905,24 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attn_split_kernel(AttnPlan p, A
   const int index = blockIdx.x / p.kv_heads, kv_head = blockIdx.x % p.kv_heads;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   FewLds& few = *reinterpret_cast<FewLds*>(lds + WAVES * M::kWave + M::kSums);
+  typedef RowTile<TYPE, Row, DP> Tile;
   AttnItem it;
   if (cut.few) {
     if (!few_item<WAVES>(p, c, cut, few, index, kv_head, it)) return;
-    few_new_rows<TYPE, Row, WAVES>(p, c, it, kv_head, few);
   } else {
     if (index >= p.counts[0]) return;
     it = uniform_item(p.items + index);
     if (!p.run[it.sequence]) return;
   }
   const ItemRows<Row> rows(p, it, it.m0, lane);
+  typename Tile::Raw raw;
+  constexpr bool kEarly = DP < 256;  // wide rows would take the registers of the checks
+  if (kEarly) Tile::fetch(raw, rows.q(p, c, it, kv_head), p.head_dim, lane);
+  if (cut.few && !few_checked<TYPE, Row, WAVES>(p, c, it, kv_head, few, list)) return;
   Sight sight = rows.sight(p, c, it);
   if (cut.few && c.parents) sight.tree = few.tree[rows.token - it.m0 / p.group];
   const int sure = c.parents ? it.context : it.context + it.m0 / p.group + 1;
-  RowTile<TYPE, Row, DP> tile;  // started behind the first loads, which its rows need not wait for
+  Tile tile;  // started behind the first loads, which its rows need not wait for
   const Loader loader(p, c.layer, kv_head, it);
   const int* table = c.table + it.sequence * c.table_stride;
   const uint32_t lds_base = lds_address(lds), base = lds_base + wave * M::kWave;
@@ -894,9 +934,11 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attn_split_kernel(AttnPlan p, A
     const int first = key0 >> p.page_shift;
     const int key1 = (int)min((int64_t)it.key1, ((int64_t)first << p.page_shift) + stretch);
     const int entries = loader.entry(key1 - 1, 0) - first + 1;
-    if (key0 != it.key0) __syncthreads();
-    for (int i = threadIdx.x; i < entries; i += 64 * WAVES) list[i] = table[first + i];
-    __syncthreads();
+    if (!cut.few || key0 != it.key0) {
+      if (key0 != it.key0) __syncthreads();
+      for (int i = threadIdx.x; i < entries; i += 64 * WAVES) list[i] = table[first + i];
+      __syncthreads();
+    }
     auto load = [&](int key, int buffer) {
       const int pages = list[min(loader.entry(key, lane) - first, entries - 1)];
       loader.template load<false, 1>(key, pages, base + buffer * 2 * M::kTile, 0, lane);
@@ -904,7 +946,10 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attn_split_kernel(AttnPlan p, A
     };
     int key = key0 + KT * wave;
     if (key < key1) load(key, 0);
-    if (key0 == it.key0) tile.start(rows.q(p, c, it, kv_head), p.head_dim, p.scale * kAttnLog2e, lane);
+    if (key0 == it.key0) {
+      if (!kEarly) Tile::fetch(raw, rows.q(p, c, it, kv_head), p.head_dim, lane);
+      tile.start(raw, p.scale * kAttnLog2e, lane);
+    }
     for (int t = 0; key < key1; ++t, key += KT * WAVES) {
       if (key + KT * WAVES < key1) {
         load(key + KT * WAVES, ~t & 1);
@@ -922,7 +967,7 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attn_split_kernel(AttnPlan p, A
         spoiled.scan(lds + (now - lds_base) + M::kTile, lane, 64);
         wave_lds_order();
       }
-      typename RowTile<TYPE, Row, DP>::template Work<1> work;
+      typename Tile::template Work<1> work;
       tile.scores(work, now);
       tile.softmax(work, partly, see);
       tile.add(work, now + M::kTile);
@@ -962,7 +1007,7 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attn_split_kernel(AttnPlan p, A
     if (it.part < 0) {
       const int m = it.m0 + r;
       Row* y = static_cast<Row*>(c.y) + (it.begin + m / p.group) * c.y_stride +
-               (kv_head * p.group + m % p.group) * p.head_dim;
+               (kv_head * (int)p.group.divisor + m % p.group) * p.head_dim;
       store4(y + d, v * (1.f / total));
     } else {
       const size_t row = ((size_t)it.part * p.kv_heads + kv_head) * 32 + r;
