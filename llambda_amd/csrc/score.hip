@@ -31,6 +31,9 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
+// LDS accesses of this wavefront so far are done before those that follow.
+__device__ __forceinline__ void lds_order() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 // Lane l's logit 4 k + j is the chunk's 4 (l + 64 k) + j.
 struct ChunkOrder {
   int lane;
@@ -157,94 +160,166 @@ __global__ __launch_bounds__(64 * kScoreWaves) void score_chunk_kernel(ScoreRows
   if (lane == 0) *part = ScorePart{sum, all_weighted, top, found};
 }
 
-// A row's chunks.  Keys rank candidates by logit, then by index, and are distinct; 0 is none.
-constexpr int kRowThreads = 256;
-constexpr int kRowSlots = kScoreMaxChunks * kScoreMaxTop / kRowThreads;
+// A row's chunks, by one wavefront: lane l takes chunks l and l + 64.  Keys rank candidates by logit, then by index, and
+// are distinct; 0 is none.
+constexpr int kRowChosen = 512;
+constexpr int kRowKeys = 4096;  // candidates of a row that are kept in LDS
+static_assert(kScoreMaxChunks <= 128, "two chunks to a lane");
 
-__global__ __launch_bounds__(kRowThreads) void score_row_kernel(ScoreRows r, int chunks) {
-  __shared__ float tops[kRowThreads / 64];
-  __shared__ double sums[kRowThreads / 64][2];
-  __shared__ uint64_t keys[kRowThreads];
-  __shared__ uint64_t chosen[kScoreMaxTop * kRowSlots];
-  __shared__ uint64_t bound;
-  __shared__ int chosen_count;
-  const int row = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  static_assert(kScoreMaxChunks <= kRowThreads, "a thread for each chunk");
-  ScorePart part{0, 0, -__builtin_inff(), 0};
-  if (t < chunks) part = r.parts[(int64_t)row * chunks + t];
-  const bool nan = __syncthreads_or(part.top != part.top);
-  const float wave_top = wave_max(part.top);
-  if (lane == 0) tops[wave] = wave_top;
-  if (t == 0) {
-    bound = 0;
-    chosen_count = 0;
-  }
-  __syncthreads();
-  float top = tops[0];
+__device__ __forceinline__ uint64_t candidate_key(const ScoreCandidate& v) {
+  return (uint64_t)((uint32_t)ordered(v.logit) ^ 0x80000000u) << 32 | (uint32_t)~v.token;
+}
+__device__ __forceinline__ float key_logit(uint64_t key) {
+  const int o = (int)((uint32_t)(key >> 32) ^ 0x80000000u);
+  return __builtin_bit_cast(float, o ^ ((o >> 31) & 0x7FFFFFFF));
+}
+__device__ __forceinline__ uint64_t wave_max_key(uint64_t v) {
 #pragma unroll
-  for (int w = 1; w < kRowThreads / 64; ++w) top = fmaxf(top, tops[w]);
+  for (int o = 32; o > 0; o >>= 1) {
+    const uint64_t u = __shfl_xor(v, o, 64);
+    v = u > v ? u : v;
+  }
+  return v;
+}
+// use(key) for each candidate of a lane's two lists of n[0] and n[1], BATCH of which are on their way at once.
+template <int BATCH, typename Use>
+__device__ __forceinline__ void each_candidate(const ScoreCandidate* list, const int (&n)[2], Use&& use) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const ScoreCandidate* at = list + 64 * h * kScoreMaxTop;
+    for (int i = 0; i < n[h]; i += BATCH) {
+      ScoreCandidate v[BATCH];
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) v[k] = at[min(i + k, n[h] - 1)];
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k)
+        if (i + k < n[h]) use(candidate_key(v[k]));
+    }
+  }
+}
+
+// RANKED: more than one top token (a wavefront to a workgroup then, for the LDS's sake).
+template <bool RANKED>
+__global__ __launch_bounds__(RANKED ? 64 : 256) void score_row_kernel(ScoreRows r, int chunks) {
+  __shared__ uint64_t kept[RANKED ? kRowKeys : 1], chosen[RANKED ? kRowChosen : 1];
+  __shared__ int chosen_count;
+  const int lane = threadIdx.x & 63, row = blockIdx.x * (RANKED ? 1 : 4) + (threadIdx.x >> 6);
+  if (row >= r.rows) return;
+  const float* x = r.logits + row * r.stride;
+  const int* given = r.given + (int64_t)row * r.givens;
+  auto given_logit = [&](int g) {
+    const int token = given[g];
+    return token >= 0 && token < r.count ? x[token] : __builtin_nanf("");
+  };
+  const float first_given = lane < r.givens ? given_logit(lane) : 0.f;  // on its way beside the sums
+  ScorePart part[2] = {{0, 0, -__builtin_inff(), 0}, {0, 0, -__builtin_inff(), 0}};
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    if (lane + 64 * h < chunks) part[h] = r.parts[(int64_t)row * chunks + lane + 64 * h];
+  const bool nan = __ballot(part[0].top != part[0].top || part[1].top != part[1].top) != 0;
+  const float top = wave_max(fmaxf(part[0].top, part[1].top));
   const bool empty = nan || top == -__builtin_inff();  // no distribution
-  const double lead = empty || part.top == -__builtin_inff() ? 0.0 : (double)top - (double)part.top;
-  const double scale = part.sum > 0 ? exp(-lead) : 0.0;
-  const double sum = wave_sum(scale * part.sum);
-  const double weighted = wave_sum(part.sum > 0 ? scale * (part.weighted + lead * part.sum) : 0.0);
-  if (lane == 0) sums[wave][0] = sum, sums[wave][1] = weighted;
-  __syncthreads();
   double s = 0, w = 0;
 #pragma unroll
-  for (int i = 0; i < kRowThreads / 64; ++i) s += sums[i][0], w += sums[i][1];
+  for (int h = 0; h < 2; ++h)
+    if (part[h].sum > 0) {
+      const double lead = (double)top - (double)part[h].top, scale = exp(-lead);
+      s += scale * part[h].sum;
+      w += scale * (part[h].weighted + lead * part[h].sum);
+    }
+  s = wave_sum(s);
+  w = wave_sum(w);
   const double log_sum = log(s);
-  const float* x = r.logits + row * r.stride;
   auto log_prob = [&](float logit) {
     return empty ? __builtin_nanf("") : (float)((double)logit - (double)top - log_sum);
   };
-  if (t == 0 && r.entropy) r.entropy[row] = empty ? __builtin_nanf("") : (float)(log_sum + w / s);
+  if (lane == 0 && r.entropy) r.entropy[row] = empty ? __builtin_nanf("") : (float)(log_sum + w / s);
   if (r.log_probs)
-    for (int g = t; g < r.givens; g += kRowThreads) {
-      const int token = r.given[(int64_t)row * r.givens + g];
-      r.log_probs[(int64_t)row * r.givens + g] =
-          token >= 0 && token < r.count ? log_prob(x[token]) : __builtin_nanf("");
-    }
+    for (int g = lane; g < r.givens; g += 64)
+      r.log_probs[(int64_t)row * r.givens + g] = log_prob(g == lane ? first_given : given_logit(g));
   if (r.top == 0) return;
+  auto place_token = [&](int place, uint64_t key) {
+    const int token = (int)~(uint32_t)key;
+    if (r.top_tokens) r.top_tokens[(int64_t)row * r.top + place] = token;
+    if (r.top_log_probs) r.top_log_probs[(int64_t)row * r.top + place] = log_prob(key_logit(key));
+  };
   int filled = 0;
   if (!empty) {
-    uint64_t best = 0, own[kRowSlots];
+    const ScoreCandidate* list = r.candidates + ((int64_t)row * chunks + lane) * kScoreMaxTop;
+    const int n[2] = {part[0].candidates, part[1].candidates};
+    uint64_t best = 0;
+    if constexpr (!RANKED) {
+      each_candidate<2>(list, n, [&](uint64_t key) { best = key > best ? key : best; });
+      best = wave_max_key(best);
+      if (lane == 0) place_token(0, best);
+      filled = 1;
+    } else {
+      int end = n[0] + n[1];
 #pragma unroll
-    for (int k = 0; k < kRowSlots; ++k) {
-      own[k] = 0;
-      const int slot = t + kRowThreads * k, c = slot / kScoreMaxTop;
-      if (c < chunks && slot % kScoreMaxTop < r.parts[(int64_t)row * chunks + c].candidates) {
-        const ScoreCandidate v = r.candidates[(int64_t)row * chunks * kScoreMaxTop + slot];
-        own[k] = (uint64_t)((uint32_t)ordered(v.logit) ^ 0x80000000u) << 32 | (uint32_t)~v.token;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(end, o, 64);
+        if (lane >= o) end += u;
       }
-      best = own[k] > best ? own[k] : best;
-    }
-    keys[t] = best;
-    __syncthreads();
-    // the key that `top` threads' best reach
-    int rank = 0;
-    for (int i = 0; i < kRowThreads; ++i) rank += keys[i] > best;
-    if (best && rank == r.top - 1) bound = best;
-    __syncthreads();
+      const int total = __builtin_amdgcn_readlane(end, 63);
+      const bool keep = total <= kRowKeys;
+      int at = end - n[0] - n[1];
+      each_candidate<16>(list, n, [&](uint64_t key) {
+        best = key > best ? key : best;
+        if (keep) kept[at++] = key;
+      });
+      if (lane == 0) chosen_count = 0;
+      chosen[lane] = best;
+      lds_order();
+      auto each = [&](auto&& use) {
+        if (keep) {
+#pragma unroll 8
+          for (int i = lane; i < total; i += 64) use(kept[i]);
+        } else {
+          each_candidate<16>(list, n, use);
+        }
+      };
+      // the key that `top` lanes' best reach; if there are not so many lanes, or more keys reach it than there is room
+      // for, one that enough keys reach
+      int rank = 0;
+#pragma unroll 8
+      for (int i = 0; i < 64; ++i) rank += chosen[i] > best;
+      const uint64_t bests = __ballot(best && rank == r.top - 1);
+      uint64_t bound = 1;
+      if (bests) bound = __shfl(best, __ffsll((unsigned long long)bests) - 1, 64);
+      auto reach = [&](uint64_t least) {
+        int count = 0;
+        each([&](uint64_t key) { count += key >= least; });
 #pragma unroll
-    for (int k = 0; k < kRowSlots; ++k)
-      if (own[k] && own[k] >= bound) chosen[atomicAdd(&chosen_count, 1)] = own[k];
-    __syncthreads();
-    const int n = chosen_count;
-    filled = min(n, r.top);
-    for (int i = t; i < n; i += kRowThreads) {
-      const uint64_t key = chosen[i];
-      int place = 0;
-      for (int j = 0; j < n; ++j) place += chosen[j] > key;
-      if (place < r.top) {
-        const int token = (int)~(uint32_t)key;
-        if (r.top_tokens) r.top_tokens[(int64_t)row * r.top + place] = token;
-        if (r.top_log_probs) r.top_log_probs[(int64_t)row * r.top + place] = log_prob(x[token]);
+        for (int o = 32; o > 0; o >>= 1) count += __shfl_xor(count, o, 64);
+        return count;
+      };
+      filled = reach(bound);
+      if (filled > kRowChosen) {
+        uint64_t hi = wave_max_key(best);
+        while (hi > bound && filled > kRowChosen) {
+          const uint64_t mid = bound + (hi - bound + 1) / 2;
+          const int count = reach(mid);
+          if (count >= r.top) bound = mid, filled = count;
+          else hi = mid - 1;
+        }
       }
+      lds_order();
+      each([&](uint64_t key) {
+        if (key >= bound) chosen[atomicAdd(&chosen_count, 1)] = key;
+      });
+      lds_order();
+      for (int i = lane; i < filled; i += 64) {
+        const uint64_t key = chosen[i];
+        int place = 0;
+#pragma unroll 4
+        for (int j = 0; j < filled; ++j) place += chosen[j] > key;
+        if (place < r.top) place_token(place, key);
+      }
+      filled = min(filled, r.top);
     }
   }
   // places without a token
-  for (int i = filled + t; i < r.top; i += kRowThreads) {
+  for (int i = filled + lane; i < r.top; i += 64) {
     if (r.top_tokens) r.top_tokens[(int64_t)row * r.top + i] = -1;
     if (r.top_log_probs) r.top_log_probs[(int64_t)row * r.top + i] = empty ? __builtin_nanf("") : -__builtin_inff();
   }
@@ -256,7 +331,8 @@ hipError_t score_rows_launch(const ScoreRows& r, hipStream_t s) {
   hipLaunchKernelGGL(score_chunk_kernel, dim3((uint32_t)blocks), dim3(64 * kScoreWaves), 0, s, r, chunks);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(score_row_kernel, dim3(r.rows), dim3(kRowThreads), 0, s, r, chunks);
+  if (r.top > 1) hipLaunchKernelGGL(score_row_kernel<true>, dim3(r.rows), dim3(64), 0, s, r, chunks);
+  else hipLaunchKernelGGL(score_row_kernel<false>, dim3((r.rows + 3) / 4), dim3(256), 0, s, r, chunks);
   return hipGetLastError();
 }
 
