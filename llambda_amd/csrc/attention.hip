@@ -93,10 +93,14 @@ __device__ int block_scan(int v, int* lds, int& total) {
   return v + before;
 }
 
-// Items and joins.  Tiles of many keys come first within a sequence.
+// Items and joins.  Long items come first, so that the short ones fill what they leave: a count of items by length, then
+// their places.  (The order of items of like length, and of the partial results' places, is that of the counters: no
+// result depends on it.)
+constexpr int kLengths = 16;
+
 __device__ void plan(const AttnPlan& p, const AttnCall& c, const AttnCut& cut) {
   __shared__ int scan[kPlanThreads / 64], ends[kPlanThreads], lengths[kPlanThreads], contexts[kPlanThreads],
-      begins[kPlanThreads];
+      begins[kPlanThreads], places[kLengths], joins, parts;
   __shared__ unsigned long long keys;
   if (!offsets_hold(c)) {
     if (threadIdx.x == 0) {
@@ -105,10 +109,10 @@ __device__ void plan(const AttnPlan& p, const AttnCall& c, const AttnCut& cut) {
     }
     return;
   }
-  if (threadIdx.x == 0) keys = 0;
+  if (threadIdx.x == 0) keys = joins = parts = 0;
+  if (threadIdx.x < kLengths) places[threadIdx.x] = 0;
   int chunk = 0;
-  int items = 0, joins = 0, parts = 0;
-  for (int pass = 0; pass < 2; ++pass) {
+  for (int pass = 0; pass < 3; ++pass) {
     for (int i0 = 0; i0 < c.sequences; i0 += kPlanThreads) {
       const int i = i0 + threadIdx.x;
       Sequence s{0, 0, 0};
@@ -121,52 +125,50 @@ __device__ void plan(const AttnPlan& p, const AttnCall& c, const AttnCut& cut) {
       contexts[threadIdx.x] = s.context;
       begins[threadIdx.x] = s.begin;
       __syncthreads();
-      for (int t0 = 0; t0 < tiles; t0 += kPlanThreads) {
-        const int t = t0 + threadIdx.x;
-        int which = 0, m0 = 0, seen = 0, n = 0;
-        if (t < tiles) {
-          int hi = kPlanThreads - 1;
-          while (which < hi) {  // the first sequence whose tiles end behind t
-            const int mid = (which + hi) / 2;
-            if (ends[mid] > t) hi = mid;
-            else which = mid + 1;
-          }
-          m0 = (ends[which] - 1 - t) * cut.rows;
-          seen = attn_seen_keys(p, c, cut, m0, lengths[which], contexts[which]);
+      for (int t = threadIdx.x; t < tiles; t += kPlanThreads) {
+        int which = 0;
+        for (int hi = kPlanThreads - 1; which < hi;) {  // the first sequence whose tiles end behind t
+          const int mid = (which + hi) / 2;
+          if (ends[mid] > t) hi = mid;
+          else which = mid + 1;
         }
+        const int m0 = (ends[which] - 1 - t) * cut.rows;
+        const int seen = attn_seen_keys(p, c, cut, m0, lengths[which], contexts[which]);
         if (pass == 0) {
-          unsigned long long v = seen;
-#pragma unroll
-          for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-          if ((threadIdx.x & 63) == 0) atomicAdd(&keys, v);
+          atomicAdd(&keys, (unsigned long long)seen);
           continue;
         }
-        if (t < tiles) n = attn_parts_of(seen, chunk);
-        int all_items, all_joins, all_parts;
-        const int item = items + block_scan(n, scan, all_items) - n;
-        const int join = joins + block_scan(n > 1, scan, all_joins) - (n > 1);
-        const int part = parts + block_scan(n > 1 ? n : 0, scan, all_parts) - (n > 1 ? n : 0);
+        const int n = attn_parts_of(seen, chunk);
         AttnItem it{i0 + which, begins[which], lengths[which], contexts[which], m0, 0, 0, 0};
+        attn_part(it, seen, n, 0, 0);
+        // all parts but the last have one length; the last takes its place among them
+        const int length = kLengths - 1 - (int)((int64_t)min(it.key1, chunk) * (kLengths - 1) / chunk);
+        const int at = atomicAdd(&places[length], n);
+        if (pass == 1) continue;
+        const int part = n > 1 ? atomicAdd(&parts, n) : 0;
         for (int k = 0; k < n; ++k) {
           attn_part(it, seen, n, k, part);
-          p.items[item + k] = it;
+          p.items[at + k] = it;
         }
-        if (n > 1) p.joins[join] = AttnJoin{begins[which], lengths[which], m0, n, part, i0 + which};
-        items += all_items;
-        joins += all_joins;
-        parts += all_parts;
+        if (n > 1) p.joins[atomicAdd(&joins, 1)] = AttnJoin{begins[which], lengths[which], m0, n, part, i0 + which};
       }
       __syncthreads();
     }
-    if (pass == 0) {
+    if (pass == 0) chunk = attn_chunk(p, cut, (int64_t)keys);
+    if (pass == 1) {
+      if (threadIdx.x == 0) {
+        int before = 0;
+        for (int l = 0; l < kLengths; ++l) {
+          const int n = places[l];
+          places[l] = before;
+          before += n;
+        }
+        p.counts[0] = before;
+      }
       __syncthreads();
-      chunk = attn_chunk(p, cut, (int64_t)keys);
     }
   }
-  if (threadIdx.x == 0) {
-    p.counts[0] = items;
-    p.counts[1] = joins;
-  }
+  if (threadIdx.x == 0) p.counts[1] = joins;
 }
 
 // ------------------------------------------------------------- keys and values
