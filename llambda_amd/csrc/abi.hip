@@ -1955,7 +1955,7 @@ struct llambda_hip_attention_session {
   int device = 0;
   hipStream_t stream = nullptr;
   AttnPlan plan{};
-  DevBuf pool_keys, pool_values, error, run, items, joins, counts, tree, part_y, part_ml;
+  DevBuf pool_keys, pool_values, error, run, tiles, workers, joins, counts, tree, part_y, part_ml;
   DevBuf q, k, v, y, lists;  // device staging of the host-pointer runs; lists: offsets, context, parents, table
   int64_t staged_tokens = 0;
   // recorded after every call that uses the workspace; the next one waits
@@ -2181,15 +2181,17 @@ int llambda_hip_attention_session_create(const llambda_hip_attention_desc* d,
     const AttnSizes sizes = attn_sizes(p);
     s->error.alloc(2 * sizeof(int), "error flags");
     s->run.alloc((size_t)p.max_sequences * sizeof(int), "sequences to run");
-    s->items.alloc((size_t)sizes.items * sizeof(AttnItem), "attention items");
-    s->joins.alloc((size_t)sizes.joins * sizeof(AttnJoin), "attention joins");
-    s->counts.alloc(2 * sizeof(int), "item counts");
+    s->tiles.alloc((size_t)sizes.tiles * sizeof(AttnTile), "attention tiles");
+    s->workers.alloc((size_t)sizes.workers * sizeof(AttnWorker), "attention shares");
+    s->joins.alloc((size_t)sizes.shares * sizeof(AttnJoin), "attention joins");
+    s->counts.alloc(2 * sizeof(int), "share counts");
     s->tree.alloc((size_t)p.max_tokens * kAttnTreeWords * sizeof(uint32_t), "ancestors");
     s->part_y.alloc((size_t)sizes.part_rows * attn_padded(p.head_dim) * sizeof(float), "partial results");
     s->part_ml.alloc((size_t)sizes.part_rows * sizeof(float2), "partial sums");
     p.error = s->error.as<int>();
     p.run = s->run.as<int>();
-    p.items = s->items.as<AttnItem>();
+    p.tiles = s->tiles.as<AttnTile>();
+    p.workers = s->workers.as<AttnWorker>();
     p.joins = s->joins.as<AttnJoin>();
     p.counts = s->counts.as<int>();
     p.tree = s->tree.as<uint32_t>();

@@ -30,16 +30,30 @@ enum AttnError : int {
   kAttnErrPath = 16,    // an accepted path that does not ascend
 };
 
-// Rows of one sequence and a range of its positions: a workgroup's work for one kv head.
-// Row m of a sequence's kv head is token m / group, head m % group of the group.
-struct AttnItem {
+// A call's work: rows of a sequence and kv head in tiles (row m is token m / group, head m % group of the group), each
+// with the positions that it sees in units of 2^AttnCut::unit_log2.  All kv heads' tiles are alike.
+struct AttnTile {
   int sequence, begin, length, context;  // the sequence's first row in the call, its rows, cached tokens
-  int m0, key0, key1;
-  int part;                              // -1: all it sees; else where in the partial results it goes
+  int m0, seen;
+  int64_t start;                         // its first unit among all, behind its overhead
 };
-// Rows whose range of positions several items share (with fewer than two parts: nothing to join).
+// A workgroup's share, for each kv head: units from .. to - 1, of tile `tile` and those that follow.  An end of it that lies
+// no further than `slack` from an end of a tile is taken to be there.
+struct AttnWorker {
+  int64_t from, to;
+  int tile, slack;
+};
+// What a workgroup does at a time: positions of a tile.
+struct AttnItem {
+  int sequence, begin, length, context;
+  int m0, key0, key1;
+  int part;  // -1: all that the tile sees; else where in the partial results it goes
+};
+// A tile that begins in a workgroup's share and ends in another's: its first part, and the place of the second, from
+// which on every other one is its.  parts 0: there is none.
 struct AttnJoin {
-  int begin, length, m0, parts, part0, sequence;
+  int begin, length, m0, parts, part0, part1;
+  int sequence;
 };
 
 // Quotients by a divisor of whole numbers below 2^31.
@@ -69,9 +83,10 @@ struct AttnPlan {
   int* error;  // [2]: AttnErrors of the calls since they were last taken, those taken
   // workspace of a call
   int* run;             // [max_sequences]: 0: refused, nothing of it is read or written
-  AttnItem* items;      // [attn_max_items]
-  AttnJoin* joins;      // [attn_max_joins]
-  int* counts;          // items, joins
+  AttnTile* tiles;      // [AttnSizes::tiles]
+  AttnWorker* workers;  // [AttnSizes::workers]
+  AttnJoin* joins;      // [AttnSizes::shares]
+  int* counts;          // workers, joins
   uint32_t* tree;       // [max_tokens][kAttnTreeWords]: a row's ancestors and itself
   float* part_y;        // [part][kv_heads][tile rows][padded head_dim]
   float2* part_ml;      // [part][kv_heads][tile rows]: reference exponent and sum
@@ -103,7 +118,7 @@ struct AttnAccept {
 
 // Workspace for calls of at most max_tokens and max_sequences.
 struct AttnSizes {
-  int64_t items, joins, part_rows;  // part_rows: rows of part_ml; part_y has attn_padded(head_dim) floats for each
+  int64_t tiles, workers, shares, part_rows;  // part_rows: rows of part_ml; part_y has attn_padded(head_dim) floats each
 };
 AttnSizes attn_sizes(const AttnPlan& p);
 inline int attn_padded(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
@@ -115,13 +130,15 @@ hipError_t attn_run_launch(const AttnPlan& p, const AttnCall& c, hipStream_t str
 hipError_t attn_accept_launch(const AttnPlan& p, const AttnAccept& a, hipStream_t stream);
 hipError_t attn_take_error_launch(const AttnPlan& p, hipStream_t stream);
 
-// How a call is cut: rows of an item, keys of a part at least, workgroups the device holds.
+// How a call is cut.
 struct AttnCut {
   bool shared;      // the waves of a workgroup share a tile of keys (and have rows of their own), or the reverse
-  int rows;         // of an item
-  int min_keys;     // of a part
-  int slots_log2;   // parts over all kv heads come to about this many workgroups
   bool few;         // the attend kernel makes the plan and puts the new rows into the cache
+  int rows;         // of a tile
+  int unit_log2;    // positions of a unit, whole tiles of keys
+  int overhead;     // units that a tile costs beside its own
+  int shares;       // for each kv head, of equal size, where tiles are divided
+  double each;      // 1 / shares
 };
 // The kernels of one cache type (attention_f16.hip, attention_bf16.hip, attention_f32.hip).
 hipError_t attn_attend_f16(const AttnPlan& p, const AttnCall& c, const AttnCut& cut, uint32_t grid, hipStream_t s);

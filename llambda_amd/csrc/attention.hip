@@ -3,11 +3,12 @@
 //
 // A call is three launches.  attn_prepare_kernel checks the sequences, rounds the
 // new rows' keys and values into their pages and notes each tree row's ancestors,
-// while one workgroup cuts the call into items: the rows of a sequence and kv head
-// in tiles (row m is token m / group, head m % group, so that the heads of a group
-// share what is read of the cache), and the positions that a tile sees in parts
-// where the tiles alone would not fill the device or one would outlast the rest.
-// The attend kernel does the items; attn_join_kernel adds up parts.
+// while one workgroup cuts the call into shares: the rows of a sequence and kv head
+// are taken in tiles (row m is token m / group, head m % group, so that the heads of
+// a group share what is read of the cache), and what all tiles see is dealt out
+// evenly, where tiles are few, over as many workgroups as the device has CUs.  The
+// attend kernel does the shares; attn_join_kernel adds up the parts of tiles that
+// lie in several.
 #include "attention_cut.h"
 
 #include <algorithm>
@@ -73,17 +74,18 @@ __device__ bool sequence_refused(const AttnPlan& p, const AttnCall& c, int i, co
 
 // ------------------------------------------------------------------- the cut
 // Inclusive sum over the workgroup; `total` receives all of it.
-__device__ int block_scan(int v, int* lds, int& total) {
+template <typename T>
+__device__ T block_scan(T v, T* lds, T& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(v, o, 64);
+    const T u = __shfl_up(v, o, 64);
     if (lane >= o) v += u;
   }
   if (lane == 63) lds[wave] = v;
   __syncthreads();
   total = 0;
-  int before = 0;
+  T before = 0;
 #pragma unroll
   for (int w = 0; w < kPlanThreads / 64; ++w) {
     if (w < wave) before += lds[w];
@@ -93,15 +95,16 @@ __device__ int block_scan(int v, int* lds, int& total) {
   return v + before;
 }
 
-// Items and joins.  Long items come first, so that the short ones fill what they leave: a count of items by length, then
-// their places.  (The order of items of like length, and of the partial results' places, is that of the counters: no
-// result depends on it.)
-constexpr int kLengths = 16;
+// Tiles and shares.  Where tiles are few, or one is long, equal shares of all units (a tile that lies in several of
+// them has as many parts); where they are many, each tile is a share and the long ones come first, so that the short
+// ones fill what they leave.  (Tiles of like length are then in the order of a counter: no result depends on it.)
+constexpr int kLengths = 32;
+constexpr int kManyTiles = 2;  // for each share
 
 __device__ void plan(const AttnPlan& p, const AttnCall& c, const AttnCut& cut) {
   __shared__ int scan[kPlanThreads / 64], ends[kPlanThreads], lengths[kPlanThreads], contexts[kPlanThreads],
-      begins[kPlanThreads], places[kLengths], joins, parts;
-  __shared__ unsigned long long keys;
+      begins[kPlanThreads], places[kLengths], longest;
+  __shared__ int64_t scan_units[kPlanThreads / 64];
   if (!offsets_hold(c)) {
     if (threadIdx.x == 0) {
       atomicOr(p.error, kAttnErrOffsets);
@@ -109,23 +112,26 @@ __device__ void plan(const AttnPlan& p, const AttnCall& c, const AttnCut& cut) {
     }
     return;
   }
-  if (threadIdx.x == 0) keys = joins = parts = 0;
+  if (threadIdx.x == 0) longest = 0;
   if (threadIdx.x < kLengths) places[threadIdx.x] = 0;
-  int chunk = 0;
-  for (int pass = 0; pass < 3; ++pass) {
-    for (int i0 = 0; i0 < c.sequences; i0 += kPlanThreads) {
-      const int i = i0 + threadIdx.x;
-      Sequence s{0, 0, 0};
-      if (i < c.sequences) s = sequence_of(c, i);
-      // a refused sequence's items do nothing; they only have to be few
-      if (s.context < 0 || (int64_t)s.context + s.length > p.max_context) s.context = s.length = 0;
-      int tiles;
-      ends[threadIdx.x] = block_scan((s.length * (int)p.group.divisor + cut.rows - 1) / cut.rows, scan, tiles);
-      lengths[threadIdx.x] = s.length;
-      contexts[threadIdx.x] = s.context;
-      begins[threadIdx.x] = s.begin;
-      __syncthreads();
-      for (int t = threadIdx.x; t < tiles; t += kPlanThreads) {
+  int before = 0;
+  int64_t units = 0;
+  for (int i0 = 0; i0 < c.sequences; i0 += kPlanThreads) {
+    const int i = i0 + threadIdx.x;
+    Sequence s{0, 0, 0};
+    if (i < c.sequences) s = sequence_of(c, i);
+    // a refused sequence's tiles do nothing; they only have to be few
+    if (s.context < 0 || (int64_t)s.context + s.length > p.max_context) s.context = s.length = 0;
+    int tiles;
+    ends[threadIdx.x] = block_scan((s.length * (int)p.group.divisor + cut.rows - 1) / cut.rows, scan, tiles);
+    lengths[threadIdx.x] = s.length;
+    contexts[threadIdx.x] = s.context;
+    begins[threadIdx.x] = s.begin;
+    __syncthreads();
+    for (int t0 = 0; t0 < tiles; t0 += kPlanThreads) {
+      const int t = t0 + threadIdx.x;
+      AttnTile tile{};
+      if (t < tiles) {
         int which = 0;
         for (int hi = kPlanThreads - 1; which < hi;) {  // the first sequence whose tiles end behind t
           const int mid = (which + hi) / 2;
@@ -133,42 +139,69 @@ __device__ void plan(const AttnPlan& p, const AttnCall& c, const AttnCut& cut) {
           else which = mid + 1;
         }
         const int m0 = (ends[which] - 1 - t) * cut.rows;
-        const int seen = attn_seen_keys(p, c, cut, m0, lengths[which], contexts[which]);
-        if (pass == 0) {
-          atomicAdd(&keys, (unsigned long long)seen);
-          continue;
-        }
-        const int n = attn_parts_of(seen, chunk);
-        AttnItem it{i0 + which, begins[which], lengths[which], contexts[which], m0, 0, 0, 0};
-        attn_part(it, seen, n, 0, 0);
-        // all parts but the last have one length; the last takes its place among them
-        const int length = kLengths - 1 - (int)((int64_t)min(it.key1, chunk) * (kLengths - 1) / chunk);
-        const int at = atomicAdd(&places[length], n);
-        if (pass == 1) continue;
-        const int part = n > 1 ? atomicAdd(&parts, n) : 0;
-        for (int k = 0; k < n; ++k) {
-          attn_part(it, seen, n, k, part);
-          p.items[at + k] = it;
-        }
-        if (n > 1) p.joins[atomicAdd(&joins, 1)] = AttnJoin{begins[which], lengths[which], m0, n, part, i0 + which};
+        tile = AttnTile{i0 + which, begins[which], lengths[which], contexts[which], m0,
+                        attn_seen_keys(p, c, cut, m0, lengths[which], contexts[which]), 0};
       }
-      __syncthreads();
+      const int mine = t < tiles ? attn_units(cut, tile.seen) : 0;
+      int64_t all;
+      tile.start = units + block_scan((int64_t)(t < tiles ? mine + cut.overhead : 0), scan_units, all) - mine;
+      units += all;
+      if (t < tiles) p.tiles[before + t] = tile;
+      int most = mine;
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
+      if ((threadIdx.x & 63) == 0) atomicMax(&longest, most);
     }
-    if (pass == 0) chunk = attn_chunk(p, cut, (int64_t)keys);
-    if (pass == 1) {
-      if (threadIdx.x == 0) {
-        int before = 0;
-        for (int l = 0; l < kLengths; ++l) {
-          const int n = places[l];
-          places[l] = before;
-          before += n;
-        }
-        p.counts[0] = before;
+    before += tiles;
+    __syncthreads();
+  }
+  const int64_t share = attn_share(cut, units);
+  // (what this workgroup wrote is read back by other threads of it: the barriers order it)
+  if (before >= kManyTiles * cut.shares && longest <= 2 * share) {
+    for (int pass = 0; pass < 2; ++pass) {
+      for (int t = threadIdx.x; t < before; t += kPlanThreads) {
+        const AttnTile tile = p.tiles[t];
+        const int n = attn_units(cut, tile.seen);
+        const int at = atomicAdd(&places[kLengths - 1 - (int)((int64_t)n * (kLengths - 1) / longest)], 1);
+        if (pass == 1) p.workers[at] = AttnWorker{tile.start, tile.start + n, t, 0};
       }
       __syncthreads();
+      if (pass == 0) {
+        if (threadIdx.x == 0) {
+          int sum = 0;
+          for (int l = 0; l < kLengths; ++l) {
+            const int n = places[l];
+            places[l] = sum;
+            sum += n;
+          }
+        }
+        __syncthreads();
+      }
+    }
+    if (threadIdx.x == 0) {
+      p.counts[0] = before;
+      p.counts[1] = 0;
+    }
+    return;
+  }
+  const int shares = units ? attn_share_of(units - 1, share) + 1 : 0;
+  for (int w = threadIdx.x; w < shares; w += kPlanThreads) p.joins[w].parts = 0;
+  __syncthreads();
+  for (int t = threadIdx.x; t < before; t += kPlanThreads) {
+    const AttnTile tile = p.tiles[t];
+    const int n = attn_units(cut, tile.seen);
+    // shares that begin within the tile or its overhead, and the one before, which may end there
+    const int first = attn_share_of(tile.start - cut.overhead + share - 1, share);
+    const int last = attn_share_of(tile.start + n - 1, share);
+    for (int w = max(first - 1, 0); w <= last; ++w) {
+      const AttnWorker worker{w * share, min((w + 1) * share, units), t, attn_slack(share)};
+      if (w >= first) p.workers[w] = worker;
+      AttnItem it{tile.sequence, tile.begin, tile.length, tile.context, tile.m0, 0, 0, 0};
+      if (attn_item(cut, worker, w, tile.seen, tile.start, it) && it.key0 == 0 && it.part >= 0)
+        p.joins[w] = attn_join(cut, it, tile.seen, tile.start, share, w);
     }
   }
-  if (threadIdx.x == 0) p.counts[1] = joins;
+  if (threadIdx.x == 0) p.counts[0] = p.counts[1] = shares;
 }
 
 // ------------------------------------------------------------- keys and values
@@ -219,8 +252,8 @@ __global__ __launch_bounds__(kPlanThreads) void attn_prepare_kernel(AttnPlan p, 
 }
 
 // ----------------------------------------------------------------------- joins
-// Row m of a join: parts' sums taken to one reference.  A wavefront per row; eight parts' sums are on their way at once.
-template <typename Row>
+// Row m of a join: parts' sums taken to one reference.  A wavefront per row; BATCH parts' sums are on their way at once.
+template <typename Row, int BATCH>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnPlan p, AttnCall c, AttnCut cut, int padded, int blocks) {
   const int index = blockIdx.x / (p.kv_heads * blocks), rest = blockIdx.x % (p.kv_heads * blocks);
   if (index >= p.counts[1]) return;
@@ -228,10 +261,11 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnPlan p, AttnCall c, 
   const int kv_head = rest / blocks, lane = threadIdx.x & 63;
   const int r = rest % blocks * 4 + (threadIdx.x >> 6);
   if (j.parts < 2 || r >= cut.rows || j.m0 + r >= j.length * (int)p.group.divisor || (!cut.few && !p.run[j.sequence])) return;
-  const size_t step = (size_t)p.kv_heads * cut.rows;
-  const size_t row = ((size_t)j.part0 * p.kv_heads + kv_head) * cut.rows + r;
+  auto row = [&](int k) {
+    return ((size_t)(k == 0 ? j.part0 : j.part1 + 2 * (k - 1)) * p.kv_heads + kv_head) * cut.rows + r;
+  };
   float reference = -__builtin_inff();
-  for (int k = lane; k < j.parts; k += 64) reference = fmaxf(reference, p.part_ml[row + k * step].x);
+  for (int k = lane; k < j.parts; k += 64) reference = fmaxf(reference, p.part_ml[row(k)].x);
   reference = wave_max(reference);
   const int d = min(4 * lane, padded - 4);
   floatx4 v{};
@@ -239,19 +273,19 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnPlan p, AttnCall c, 
   for (int k0 = 0; k0 < j.parts; k0 += 64) {
     float weight = 0.f;
     if (k0 + lane < j.parts) {
-      const float2 ml = p.part_ml[row + (k0 + lane) * step];
+      const float2 ml = p.part_ml[row(k0 + lane)];
       // a part of which the row sees nothing has zeros
       weight = ml.x == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(ml.x - reference);
       total += weight * ml.y;
     }
     const int count = min(64, j.parts - k0);
-    for (int k = 0; k < count; k += 8) {
-      floatx4 y[8];
+    for (int k = 0; k < count; k += BATCH) {
+      floatx4 y[BATCH];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        y[i] = *reinterpret_cast<const floatx4*>(p.part_y + (row + (k0 + min(k + i, count - 1)) * step) * padded + d);
+      for (int i = 0; i < BATCH; ++i)
+        y[i] = *reinterpret_cast<const floatx4*>(p.part_y + row(k0 + min(k + i, count - 1)) * padded + d);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < BATCH; ++i) {
         const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), k + i));
         if (k + i < count) v += w * y[i];
       }
@@ -319,57 +353,53 @@ __global__ void attn_take_error_kernel(int* error) {
 // ------------------------------------------------------------------------ host
 
 constexpr int kCus = 256;
-#ifndef RT
-#define SLS 8
-#define MINS 256
-#define SLP 9
-#define MINP 256
-#define RT 160
+#ifndef UNS
+#define UNS 6
+#define OVS 3
+#define OVP 2
+#define UNP 8
 #endif
-
 static int shared_waves(const AttnPlan& p) {
   const int padded = attn_padded(p.head_dim);
   return padded == 256 || (p.cache_type == kAttnBF16 && p.row_type == kAttnF32 && padded == 128) ? 4 : 8;
 }
 
+// Rows of a kv head in a sequence, on average, up to which waves share rows and not keys.
+constexpr int kFewRows = 160;
+
 static AttnCut cut_as(const AttnPlan& p, bool shared) {
   AttnCut cut{};
   cut.shared = shared;
   cut.rows = shared ? 32 * shared_waves(p) : 32;
-  cut.min_keys = shared ? MINS : MINP;
-  cut.slots_log2 = shared ? SLS : SLP;
+  cut.unit_log2 = shared ? UNS : UNP;
+  cut.overhead = shared ? OVS : OVP;
+  cut.shares = std::max(1, kCus / p.kv_heads);
+  cut.each = 1.0 / cut.shares;
   return cut;
 }
 static AttnCut cut_of(const AttnPlan& p, const AttnCall& c) {
-  // rows of a kv head in a sequence, on average; the lengths are on the device
-  AttnCut cut = cut_as(p, ceil_div((int64_t)c.tokens * p.group.divisor, c.sequences) > RT);
+  AttnCut cut = cut_as(p, ceil_div((int64_t)c.tokens * p.group.divisor, c.sequences) > kFewRows);
   cut.few = !cut.shared && c.tokens <= kAttnFewTokens && c.sequences <= kAttnFewSequences;
   return cut;
 }
 
-// Items of a call at most: a tile for each cut.rows rows, one more for each sequence, and parts that are no shorter
-// than the keys of all tiles over 2^slots_log2.
+// Tiles of a call at most: one for each cut.rows rows and one more for each sequence.
 static int64_t tiles_of(const AttnPlan& p, int64_t tokens, int64_t sequences, int rows) {
   return std::min(tokens * p.group.divisor / rows + sequences, tokens * p.group.divisor);
 }
-static int64_t items_of(const AttnPlan& p, int64_t tokens, int64_t sequences, const AttnCut& cut) {
-  return tiles_of(p, tokens, sequences, cut.rows) + (1 << cut.slots_log2) / p.kv_heads;
+static int64_t workers_of(const AttnPlan& p, const AttnCall& c, const AttnCut& cut) {
+  return cut.few ? cut.shares : std::max<int64_t>(cut.shares, tiles_of(p, c.tokens, c.sequences, cut.rows));
 }
 
 AttnSizes attn_sizes(const AttnPlan& p) {
-  AttnSizes s{0, 0, 0};
+  AttnSizes s{0, 0, 0, 0};
   for (int shared = 0; shared < 2; ++shared) {
     const AttnCut cut = cut_as(p, shared);
-    const int64_t tiles = tiles_of(p, p.max_tokens, p.max_sequences, cut.rows);
-    const int64_t split = (1 << cut.slots_log2) / p.kv_heads;
-    s.items = std::max(s.items, tiles + split);
-    s.joins = std::max(s.joins, std::min(tiles, split));
-    if (!shared)  // of a call of few rows one for each tile
-      s.joins = std::max(s.joins, tiles_of(p, std::min(p.max_tokens, kAttnFewTokens),
-                                           std::min(p.max_sequences, kAttnFewSequences), cut.rows));
-    // n > 1 parts are at most twice the n - 1 that come beside the tile's own
-    s.part_rows = std::max(s.part_rows, 2 * split * p.kv_heads * cut.rows);
+    s.tiles = std::max(s.tiles, tiles_of(p, p.max_tokens, p.max_sequences, cut.rows));
+    s.shares = std::max<int64_t>(s.shares, cut.shares);
+    s.part_rows = std::max(s.part_rows, (int64_t)2 * cut.shares * p.kv_heads * cut.rows);
   }
+  s.workers = std::max(s.tiles, s.shares);
   return s;
 }
 
@@ -383,15 +413,24 @@ static int64_t join_blocks(const AttnCut& cut, const AttnPlan& p, const AttnCall
   return ceil_div(c.offsets ? cut.rows : std::min<int>(cut.rows, p.group.divisor), 4);
 }
 static int64_t join_grid(const AttnPlan& p, const AttnCall& c, const AttnCut& cut) {
-  const int64_t tiles = tiles_of(p, c.tokens, c.sequences, cut.rows);
-  return (cut.few ? tiles : std::min<int64_t>(tiles, (1 << cut.slots_log2) / p.kv_heads)) * p.kv_heads * join_blocks(cut, p, c);
+  return (int64_t)cut.shares * p.kv_heads * join_blocks(cut, p, c);
 }
 
 bool attn_call_fits(const AttnPlan& p, const AttnCall& c) {
   const AttnCut cut = cut_of(p, c);
   const int64_t most = UINT32_MAX / 512;
-  return items_of(p, c.tokens, c.sequences, cut) * p.kv_heads <= most &&
-         1 + c.sequences * prepare_share(p, c) <= most && join_grid(p, c, cut) <= most;
+  return workers_of(p, c, cut) * p.kv_heads <= most && 1 + c.sequences * prepare_share(p, c) <= most &&
+         join_grid(p, c, cut) <= most;
+}
+
+template <typename Row>
+static hipError_t join(const AttnPlan& p, const AttnCall& c, const AttnCut& cut, hipStream_t s) {
+  const dim3 grid((uint32_t)join_grid(p, c, cut));
+  const int padded = attn_padded(p.head_dim), blocks = (int)join_blocks(cut, p, c);
+  // tiles of many rows have few parts
+  if (cut.shared) hipLaunchKernelGGL((attn_join_kernel<Row, 2>), grid, dim3(256), 0, s, p, c, cut, padded, blocks);
+  else hipLaunchKernelGGL((attn_join_kernel<Row, 8>), grid, dim3(256), 0, s, p, c, cut, padded, blocks);
+  return hipGetLastError();
 }
 
 template <typename Row, typename T>
@@ -412,22 +451,17 @@ hipError_t attn_run_launch(const AttnPlan& p, const AttnCall& c, hipStream_t s) 
   else if (p.cache_type == kAttnBF16) e = prepare<float, __bf16>(p, c, cut, s);
   else e = prepare<float, float>(p, c, cut, s);
   if (e != hipSuccess) return e;
-  const uint32_t grid = (uint32_t)(items_of(p, c.tokens, c.sequences, cut) * p.kv_heads);
+  const uint32_t grid = (uint32_t)(workers_of(p, c, cut) * p.kv_heads);
   switch (p.cache_type) {
     case kAttnF16: e = attn_attend_f16(p, c, cut, grid, s); break;
     case kAttnBF16: e = attn_attend_bf16(p, c, cut, grid, s); break;
     default: e = attn_attend_f32(p, c, cut, grid, s); break;
   }
   if (e != hipSuccess) return e;
-  // where no sequence can have two parts there is nothing to join
-  if (p.max_context <= cut.min_keys) return hipSuccess;
-  const uint32_t joins = (uint32_t)join_grid(p, c, cut);
-  if (joins == 0) return hipSuccess;
-  const int padded = attn_padded(p.head_dim), blocks = (int)join_blocks(cut, p, c);
-  if (p.row_type == kAttnF16) hipLaunchKernelGGL(attn_join_kernel<_Float16>, dim3(joins), dim3(256), 0, s, p, c, cut, padded, blocks);
-  else if (p.row_type == kAttnBF16) hipLaunchKernelGGL(attn_join_kernel<__bf16>, dim3(joins), dim3(256), 0, s, p, c, cut, padded, blocks);
-  else hipLaunchKernelGGL(attn_join_kernel<float>, dim3(joins), dim3(256), 0, s, p, c, cut, padded, blocks);
-  return hipGetLastError();
+  if (p.max_context <= 1 << cut.unit_log2) return hipSuccess;  // no tile has parts to join
+  if (p.row_type == kAttnF16) return join<_Float16>(p, c, cut, s);
+  if (p.row_type == kAttnBF16) return join<__bf16>(p, c, cut, s);
+  return join<float>(p, c, cut, s);
 }
 
 hipError_t attn_accept_launch(const AttnPlan& p, const AttnAccept& a, hipStream_t s) {

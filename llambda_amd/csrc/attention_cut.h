@@ -4,6 +4,9 @@
 
 #include "attention.h"
 
+#ifndef SLK
+#define SLK 16
+#endif
 namespace llhip {
 
 // Positions that the rows m0 .. m0 + cut.rows - 1 of a sequence see.
@@ -13,23 +16,42 @@ __device__ __forceinline__ int attn_seen_keys(const AttnPlan& p, const AttnCall&
   return context + min(length, (m0 + cut.rows - 1) / p.group + 1);
 }
 
-// Positions of a part, whole tiles: about the work of a kv head's rows (`keys`, over all tiles) over the workgroups
-// that the device holds.
-__device__ __forceinline__ int attn_chunk(const AttnPlan& p, const AttnCut& cut, int64_t keys) {
-  const int64_t share = ((keys * p.kv_heads - 1) >> cut.slots_log2) + 1;
-  return ((int)min(max(share, (int64_t)cut.min_keys), (int64_t)1 << 30) + 63) & ~63;
+__device__ __forceinline__ int attn_units(const AttnCut& cut, int seen) { return ((seen - 1) >> cut.unit_log2) + 1; }
+
+// Units of a share, so that cut.shares of them hold `units`.
+__device__ __forceinline__ int64_t attn_share(const AttnCut& cut, int64_t units) {
+  return units <= cut.shares ? 1 : (int64_t)((double)units * cut.each) + 1;
+}
+// The share that unit `at` is in.
+__device__ __forceinline__ int attn_share_of(int64_t at, int64_t share) {
+  int64_t n = (int64_t)((double)at / (double)share);
+  while (n * share > at) --n;
+  while ((n + 1) * share <= at) ++n;
+  return (int)n;
 }
 
-// Parts of the positions that a tile sees, no longer than `chunk`.
-__device__ __forceinline__ int attn_parts_of(int seen, int chunk) {
-  return seen <= chunk ? 1 : (int)(((uint32_t)seen + chunk - 1) / (uint32_t)chunk);
+// How far an end of a share of `share` units may move to spare a tile a part.
+__device__ __forceinline__ int attn_slack(int64_t share) { return (int)min(share / SLK, (int64_t)1 << 20); }
+
+// The item that share `index` has of a tile of `seen` positions, whose units begin at `start`; false if none.  A share
+// has two places among the partial results: for the tile that it begins within, and for the one that it ends within.
+__device__ __forceinline__ bool attn_item(const AttnCut& cut, const AttnWorker& w, int index, int seen, int64_t start,
+                                          AttnItem& it) {
+  const int64_t end = start + attn_units(cut, seen);
+  auto near = [&](int64_t at) { return at <= start + w.slack ? start : at >= end - w.slack ? end : at; };
+  const int64_t lo = near(w.from), hi = near(w.to);
+  if (lo >= hi) return false;
+  it.key0 = (int)(lo - start) << cut.unit_log2;
+  it.key1 = (int)min((hi - start) << cut.unit_log2, (int64_t)seen);
+  it.part = lo == start && hi == end ? -1 : 2 * index + (lo == start && w.from < start - cut.overhead);
+  return true;
 }
-// Part k of the n equal ones, of whole tiles.  (None is empty: they are no longer than the chunk that n came from.)
-__device__ __forceinline__ void attn_part(AttnItem& it, int seen, int n, int k, int part) {
-  const uint32_t size = n > 1 ? (((uint32_t)seen + n - 1) / n + 63) & ~63u : seen;
-  it.key0 = k * size;
-  it.key1 = min((k + 1) * size, (uint32_t)seen);
-  it.part = n > 1 ? part + k : -1;
+// The join of a tile of which share `index` has the first units but not the last.
+__device__ __forceinline__ AttnJoin attn_join(const AttnCut& cut, const AttnItem& it, int seen, int64_t start,
+                                              int64_t share, int index) {
+  const int64_t end = start + attn_units(cut, seen);
+  return AttnJoin{it.begin, it.length, it.m0, attn_share_of(end - attn_slack(share) - 1, share) - index + 1, it.part,
+                  2 * (index + 1), it.sequence};
 }
 
 // Element 0 of position `pos` of kv head 0 (heads are 1 << page_shift rows apart).

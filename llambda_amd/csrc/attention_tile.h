@@ -551,11 +551,24 @@ constexpr uint32_t attn_exponent() {
 // LDS accesses of this wavefront so far are done before those that follow.
 __device__ __forceinline__ void wave_lds_order() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// An item, in scalar registers.
-__device__ __forceinline__ AttnItem uniform_item(const AttnItem* item) {
-  const int* v = reinterpret_cast<const int*>(item);
-  auto at = [&](int i) { return __builtin_amdgcn_readfirstlane(v[i]); };
-  return AttnItem{at(0), at(1), at(2), at(3), at(4), at(5), at(6), at(7)};
+// Hides where a pointer comes from.
+template <typename T>
+__device__ __forceinline__ const T* opaque_pointer(const T* p) {
+  asm("" : "+s"(p));
+  return p;
+}
+
+// A struct of the workspace, in scalar registers.
+template <typename T>
+__device__ __forceinline__ T uniform_load(const T* at) {
+  union {
+    T t;
+    int v[sizeof(T) / 4];
+  } u;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(T) / 4); ++i)
+    u.v[i] = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(at)[i]);
+  return u.t;
 }
 
 // What an item's rows are, for one of its wavefronts (32 rows from m on).
@@ -589,20 +602,19 @@ struct ItemRows {
 
 // Waves share tiles of KT keys, two of which are in LDS; each has 32 rows of its own.
 template <int TYPE, typename Row, int DP, int WAVES, int KT>
-__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_shared_kernel(AttnPlan p, AttnCall c, AttnCut) {
+__device__ __forceinline__ void shared_item(const AttnPlan& p, const AttnCall& c, const AttnItem& it, int kv_head,
+                                            uint8_t* lds) {
   constexpr int SIZE = attn_cell_bytes<TYPE>(), KB = KT / 32;
   typedef TileLoader<SIZE, DP, KT> Loader;
   constexpr uint32_t kTile = KT * DP * SIZE;
-  extern __shared__ __align__(16) uint8_t lds[];
-  const int index = blockIdx.x / p.kv_heads, kv_head = blockIdx.x % p.kv_heads;
-  if (index >= p.counts[0]) return;
-  const AttnItem it = uniform_item(p.items + index);
-  if (!p.run[it.sequence]) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m0 = it.m0 + 32 * wave;
-  const ItemRows<Row> rows(p, it, m0, lane);
-  const bool any = m0 < rows.rows;
-  const Sight sight = rows.sight(p, c, it);
+  const bool any = m0 < it.length * (int)p.group.divisor;
+  auto see_tile = [&](int key, uint32_t (&see)[KB]) {
+    const Sight sight = ItemRows<Row>(p, it, m0, (int)opaque((uint32_t)lane)).sight(p, c, it);
+#pragma unroll
+    for (int b = 0; b < KB; ++b) see[b] = sight.bits(key + 32 * b);
+  };
   // below all_sure every row of the item sees everything
   const int all_sure = c.parents ? it.context : it.context + it.m0 / p.group + 1;
   const Spoiled<SIZE, DP, KT> spoiled{reinterpret_cast<uint32_t*>(lds + 4 * kTile), attn_exponent<TYPE>()};
@@ -634,8 +646,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_shared_kernel(Attn
     barrier();
     if (spoiled.any()) {
       uint32_t see[KB];
-#pragma unroll
-      for (int b = 0; b < KB; ++b) see[b] = sight.bits(key_of(t) + 32 * b);
+      see_tile(key_of(t), see);
       tile.sums.template spoil<KB>(spoiled.bits, see);
       barrier();
       spoiled.clear(threadIdx.x, 64 * WAVES);
@@ -644,7 +655,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_shared_kernel(Attn
   typename Tile::template Work<KB> work;
   if (tiles > 0) loader.template load<false, WAVES>(it.key0, pages, keys_at(0), wave, lane);
   typename Tile::Raw raw;
-  Tile::fetch(raw, rows.q(p, c, it, kv_head), p.head_dim, lane);
+  Tile::fetch(raw, ItemRows<Row>(p, it, m0, lane).q(p, c, it, kv_head), p.head_dim, lane);
   tile.start(raw, p.scale * kAttnLog2e, lane);
   wait_loads<0>();
   barrier();
@@ -670,9 +681,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_shared_kernel(Attn
     if (any && t < tiles) {
       const bool partly = key_of(t) + KT > all_sure;  // for some row of the workgroup
       uint32_t see[KB] = {};
-      if (partly)
-#pragma unroll
-        for (int b = 0; b < KB; ++b) see[b] = sight.bits(key_of(t) + 32 * b);
+      if (partly) see_tile(key_of(t), see);
       tile.softmax(work, partly, see);
     }
     if (!behind) wait_loads<0>();
@@ -681,6 +690,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_shared_kernel(Attn
   }
   if (WAVES > 4 && !behind) barrier();
   const float sum = half_pair_sum(tile.sums.sum);
+  // made again, so that the loop's registers need not hold it
+  const ItemRows<Row> rows(p, it, m0, (int)opaque((uint32_t)lane));
   if (!rows.real) return;
   if (it.part < 0) {
     const float scale = 1.f / sum;
@@ -704,123 +715,97 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_shared_kernel(Attn
   }
 }
 
+template <int TYPE, typename Row, int DP, int WAVES, int KT>
+__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_shared_kernel(AttnPlan p, AttnCall c, AttnCut cut) {
+  extern __shared__ __align__(16) uint8_t lds[];
+  const int index = blockIdx.x / p.kv_heads, kv_head = blockIdx.x % p.kv_heads;
+  if (index >= p.counts[0]) return;
+  for (int t = uniform_load(p.workers + index).tile;; ++t) {
+    // read again for every item, so that no register holds it meanwhile
+    const AttnWorker worker = uniform_load(opaque_pointer(p.workers) + index);
+    const AttnTile tile = uniform_load(p.tiles + t);
+    const bool last = tile.start + attn_units(cut, tile.seen) >= worker.to;
+    AttnItem it{tile.sequence, tile.begin, tile.length, tile.context, tile.m0, 0, 0, 0};
+    if (attn_item(cut, worker, index, tile.seen, tile.start, it) && p.run[it.sequence])
+      shared_item<TYPE, Row, DP, WAVES, KT>(p, c, it, kv_head, lds);
+    if (last) break;
+  }
+}
+
 // A call of few rows, of at most kAttnFewSequences sequences, needs no launch before the attend kernel: each of its
 // workgroups makes the plan for itself, checks its sequence, and puts those of the new rows' keys and values that it
 // is about to read into their pages.  (Others that read them put the same bytes there.)
 struct FewLds {
-  static constexpr int kParents = kAttnTreeNodes;
+  int64_t ends[kAttnFewSequences];  // units of a sequence's tiles and those before
+  int64_t waves[4];
   int lengths[kAttnFewSequences], contexts[kAttnFewSequences];
-  uint64_t waves[4];
-  int found[4];  // sequence, which of its items, its first tile, its first part
-  int tile[3];   // the item's: its place among all, its parts and the first of them
-  int parents[kParents];
+  int first;                        // the sequence of the share's first unit
+  int parents[kAttnTreeNodes];
   uint32_t tree[32][kAttnTreeWords];
 };
 
-// Packed counts of tiles, items and parts: 20 bits each.
-__device__ __forceinline__ uint64_t few_counts(const AttnPlan& p, const AttnCall& c, const AttnCut& cut, int length,
-                                               int context, int chunk, int64_t& keys) {
-  uint64_t counts = 0;
-  for (int m0 = 0; m0 < length * (int)p.group.divisor; m0 += cut.rows) {
-    const int seen = attn_seen_keys(p, c, cut, m0, length, context);
-    const int n = chunk ? attn_parts_of(seen, chunk) : 0;
-    keys += seen;
-    counts += 1 | (uint64_t)n << 20 | (uint64_t)(n > 1 ? n : 0) << 40;
-  }
-  return counts;
-}
-
-// Whether there is an item `index`; by a workgroup of 64 WAVES threads.
+// Share `index` of the call, by a workgroup of 64 WAVES threads; whether it has one.
 template <int WAVES>
-__device__ __forceinline__ bool few_item(const AttnPlan& p, const AttnCall& c, const AttnCut& cut, FewLds& m, int index,
-                                         int kv_head, AttnItem& it) {
+__device__ __forceinline__ bool few_share(const AttnPlan& p, const AttnCall& c, const AttnCut& cut, FewLds& m, int index,
+                                          int kv_head, int64_t& from, int64_t& to, int64_t& share) {
   constexpr int B = 64 * WAVES;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const bool speaks = index == 0 && kv_head == 0;
   bool ascend = true;
-  int64_t keys = 0;
-  for (int i = t; i < c.sequences; i += B) {
-    int begin = i, length = 1;
-    if (c.offsets) {
-      begin = c.offsets[i];
-      const int end = c.offsets[i + 1];
-      ascend = ascend && begin >= 0 && end >= begin && end <= c.tokens;
-      length = end - begin;
-    }
-    int context = c.context[i];
-    if (context < 0 || (int64_t)context + length > p.max_context) {
-      if (ascend && length > 0 && index == 0 && kv_head == 0) atomicOr(p.error, kAttnErrContext);
-      context = length = 0;
-    }
-    m.lengths[i] = length;
-    m.contexts[i] = context;
-    if (ascend) few_counts(p, c, cut, length, context, 0, keys);
-  }
-  if (!__syncthreads_and(ascend)) {
-    if (t == 0 && index == 0 && kv_head == 0) {
-      atomicOr(p.error, kAttnErrOffsets);
-      p.counts[1] = 0;
-    }
-    return false;
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) keys += __shfl_xor(keys, o, 64);
-  if (lane == 0) m.waves[wave] = keys;
-  if (t == 0) m.found[0] = -1;
-  __syncthreads();
-  keys = 0;
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) keys += m.waves[w];
-  const int chunk = attn_chunk(p, cut, keys);
-  uint64_t before = 0;
+  int64_t units = 0;
   for (int i0 = 0; i0 < c.sequences; i0 += B) {
     const int i = i0 + t;
-    int64_t unused = 0;
-    const uint64_t mine = i < c.sequences ? few_counts(p, c, cut, m.lengths[i], m.contexts[i], chunk, unused) : 0;
-    uint64_t sum = mine;
+    int64_t mine = 0;
+    if (i < c.sequences) {
+      int begin = i, length = 1;
+      if (c.offsets) {
+        begin = c.offsets[i];
+        const int end = c.offsets[i + 1];
+        ascend = ascend && begin >= 0 && end >= begin && end <= c.tokens;
+        length = ascend ? end - begin : 0;
+      }
+      int context = c.context[i];
+      if (context < 0 || (int64_t)context + length > p.max_context) {
+        if (speaks && length > 0) atomicOr(p.error, kAttnErrContext);
+        context = length = 0;
+      }
+      m.lengths[i] = length;
+      m.contexts[i] = context;
+      for (int m0 = 0; m0 < length * (int)p.group.divisor; m0 += cut.rows)
+        mine += attn_units(cut, attn_seen_keys(p, c, cut, m0, length, context)) + cut.overhead;
+    }
+    int64_t sum = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-      const uint64_t u = __shfl_up(sum, o, 64);
+      const int64_t u = __shfl_up(sum, o, 64);
       if (lane >= o) sum += u;
     }
-    __syncthreads();
+    if (i0) __syncthreads();
     if (lane == 63) m.waves[wave] = sum;
     __syncthreads();
-    uint64_t all = 0;
+    int64_t all = 0;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
       if (w < wave) sum += m.waves[w];
       all += m.waves[w];
     }
-    sum += before;
-    before += all;
-    const int last = (int)(sum >> 20 & 0xFFFFF), first = last - (int)(mine >> 20 & 0xFFFFF);
-    if (index >= first && index < last) {
-      m.found[0] = i;
-      m.found[1] = index - first;
-      m.found[2] = (int)((sum - mine) & 0xFFFFF);
-      m.found[3] = (int)((sum - mine) >> 40);
-    }
+    if (i < c.sequences) m.ends[i] = units + sum;
+    units += all;
   }
-  if (t == 0 && index == 0 && kv_head == 0) p.counts[1] = (int)(before & 0xFFFFF);
+  const bool holds = __syncthreads_and(ascend);
+  if (speaks && t == 0) {
+    if (!holds) atomicOr(p.error, kAttnErrOffsets);
+    p.counts[1] = holds ? cut.shares : 0;
+  }
+  if (!holds) return false;
+  share = attn_share(cut, units);
+  from = index * share;
+  to = min(from + share, units);
+  if (t == 0 && kv_head == 0) p.joins[index].parts = 0;
+  if (from >= units) return false;
+  for (int i = t; i < c.sequences; i += B)
+    if (m.ends[i] > from && (i == 0 || m.ends[i - 1] <= from)) m.first = i;
   __syncthreads();
-  auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-  it.sequence = uniform(m.found[0]);
-  if (it.sequence < 0) return false;
-  it.begin = c.offsets ? uniform(c.offsets[it.sequence]) : it.sequence;
-  it.length = uniform(m.lengths[it.sequence]);
-  it.context = uniform(m.contexts[it.sequence]);
-  int which = uniform(m.found[1]), tile = uniform(m.found[2]), part = uniform(m.found[3]), seen = 0, n = 0;
-  for (it.m0 = 0;; it.m0 += cut.rows, ++tile) {
-    seen = attn_seen_keys(p, c, cut, it.m0, it.length, it.context);
-    n = attn_parts_of(seen, chunk);
-    if (which < n) break;
-    which -= n;
-    part += n > 1 ? n : 0;
-  }
-  attn_part(it, seen, n, which, part);
-  m.tile[0] = tile;
-  m.tile[1] = n;
-  m.tile[2] = part;
   return true;
 }
 
@@ -849,10 +834,7 @@ __device__ __forceinline__ bool few_checked(const AttnPlan& p, const AttnCall& c
     }
   }
   if (bad) atomicOr(p.error, bad);
-  const bool refused = __syncthreads_or(bad);
-  if (t == 0 && kv_head == 0 && it.key0 == 0)
-    p.joins[m.tile[0]] = AttnJoin{it.begin, it.length, it.m0, refused ? 0 : m.tile[1], m.tile[2], it.sequence};
-  if (refused) return false;
+  if (__syncthreads_or(bad)) return false;
   const int pieces = p.head_dim / 8, first = max(it.key0, it.context), rows = it.key1 - first;
   if (rows <= 0 && !c.parents) return true;
   for (int e = t; e < rows * 2 * pieces; e += B) {
@@ -893,32 +875,24 @@ struct SplitLds {
   static constexpr int kBytes = WAVES * kWave + kSums + (int)sizeof(FewLds);
 };
 
+// Whether the item was done: not if its sequence is refused.
 template <int TYPE, typename Row, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, 1) void attn_split_kernel(AttnPlan p, AttnCall c, AttnCut cut) {
+__device__ __forceinline__ bool split_item(const AttnPlan& p, const AttnCall& c, const AttnCut& cut, const AttnItem& it,
+                                           int kv_head, uint8_t* lds) {
   constexpr int SIZE = attn_cell_bytes<TYPE>(), KT = 32;
   typedef TileLoader<SIZE, DP, KT> Loader;
   typedef SplitLds<TYPE, Row, DP, WAVES> M;
+  typedef RowTile<TYPE, Row, DP> Tile;
   constexpr int kLoads = 2 * Loader::kLoads;
-  extern __shared__ __align__(16) uint8_t lds[];
   float* const ml = reinterpret_cast<float*>(lds + WAVES * M::kWave);  // [WAVES][2][32]
   int* const list = reinterpret_cast<int*>(ml + WAVES * 64);
-  const int index = blockIdx.x / p.kv_heads, kv_head = blockIdx.x % p.kv_heads;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   FewLds& few = *reinterpret_cast<FewLds*>(lds + WAVES * M::kWave + M::kSums);
-  typedef RowTile<TYPE, Row, DP> Tile;
-  AttnItem it;
-  if (cut.few) {
-    if (!few_item<WAVES>(p, c, cut, few, index, kv_head, it)) return;
-  } else {
-    if (index >= p.counts[0]) return;
-    it = uniform_item(p.items + index);
-    if (!p.run[it.sequence]) return;
-  }
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const ItemRows<Row> rows(p, it, it.m0, lane);
   typename Tile::Raw raw;
   constexpr bool kEarly = DP < 256;  // wide rows would take the registers of the checks
   if (kEarly) Tile::fetch(raw, rows.q(p, c, it, kv_head), p.head_dim, lane);
-  if (cut.few && !few_checked<TYPE, Row, WAVES>(p, c, it, kv_head, few, list)) return;
+  if (cut.few && !few_checked<TYPE, Row, WAVES>(p, c, it, kv_head, few, list)) return false;
   Sight sight = rows.sight(p, c, it);
   if (cut.few && c.parents) sight.tree = few.tree[rows.token - it.m0 / p.group];
   const int sure = c.parents ? it.context : it.context + it.m0 / p.group + 1;
@@ -1014,6 +988,60 @@ __global__ __launch_bounds__(64 * WAVES, 1) void attn_split_kernel(AttnPlan p, A
       if (d == 0) p.part_ml[row] = make_float2(reference, total);
       *reinterpret_cast<floatx4*>(p.part_y + row * DP + d) = v;
     }
+  }
+  return true;
+}
+
+template <int TYPE, typename Row, int DP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 1) void attn_split_kernel(AttnPlan p, AttnCall c, AttnCut cut) {
+  typedef SplitLds<TYPE, Row, DP, WAVES> M;
+  extern __shared__ __align__(16) uint8_t lds[];
+  const int index = blockIdx.x / p.kv_heads, kv_head = blockIdx.x % p.kv_heads;
+  if (!cut.few) {
+    if (index >= p.counts[0]) return;
+    const AttnWorker worker = uniform_load(p.workers + index);
+    int64_t end = worker.from;
+    for (int t = worker.tile; end < worker.to; ++t) {
+      const AttnTile tile = uniform_load(p.tiles + t);
+      end = tile.start + attn_units(cut, tile.seen);
+      AttnItem it{tile.sequence, tile.begin, tile.length, tile.context, tile.m0, 0, 0, 0};
+      if (!attn_item(cut, worker, index, tile.seen, tile.start, it) || !p.run[it.sequence]) continue;
+      split_item<TYPE, Row, DP, WAVES>(p, c, cut, it, kv_head, lds);
+      __syncthreads();  // the sums have been read
+    }
+    return;
+  }
+  FewLds& few = *reinterpret_cast<FewLds*>(lds + WAVES * M::kWave + M::kSums);
+  int64_t from, to, share;
+  if (!few_share<WAVES>(p, c, cut, few, index, kv_head, from, to, share)) return;
+  auto uniform = [](int64_t v) {
+    return (int64_t)((uint64_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 |
+                     (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+  };
+  AttnItem it;
+  it.sequence = __builtin_amdgcn_readfirstlane(few.first);
+  int64_t start = it.sequence ? uniform(few.ends[it.sequence - 1]) : 0;  // of a tile's overhead
+  const AttnWorker worker{uniform(from), uniform(to), 0, attn_slack(uniform(share))};
+  it.m0 = 0;
+  while (start < worker.to) {
+    it.length = __builtin_amdgcn_readfirstlane(few.lengths[it.sequence]);
+    it.context = __builtin_amdgcn_readfirstlane(few.contexts[it.sequence]);
+    if (it.m0 >= it.length * (int)p.group.divisor) {
+      ++it.sequence;
+      it.m0 = 0;
+      continue;
+    }
+    const int seen = attn_seen_keys(p, c, cut, it.m0, it.length, it.context), units = attn_units(cut, seen);
+    start += cut.overhead;
+    if (attn_item(cut, worker, index, seen, start, it)) {
+      it.begin = c.offsets ? __builtin_amdgcn_readfirstlane(c.offsets[it.sequence]) : it.sequence;
+      const bool done = split_item<TYPE, Row, DP, WAVES>(p, c, cut, it, kv_head, lds);
+      if (done && it.key0 == 0 && it.part >= 0 && threadIdx.x == 0 && kv_head == 0)
+        p.joins[index] = attn_join(cut, it, seen, start, share, index);
+      __syncthreads();  // the sums have been read
+    }
+    start += units;
+    it.m0 += cut.rows;
   }
 }
 
