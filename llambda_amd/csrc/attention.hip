@@ -252,8 +252,9 @@ __global__ __launch_bounds__(kPlanThreads) void attn_prepare_kernel(AttnPlan p, 
 }
 
 // ----------------------------------------------------------------------- joins
-// Row m of a join: parts' sums taken to one reference.  A wavefront per row; BATCH parts' sums are on their way at once.
-template <typename Row, int BATCH>
+// Row m of a join: parts' sums taken to one reference.  A wavefront per row; kJoinParts parts' sums are on their way at once.
+constexpr int kJoinParts = 8;
+template <typename Row>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnPlan p, AttnCall c, AttnCut cut, int padded, int blocks) {
   const int index = blockIdx.x / (p.kv_heads * blocks), rest = blockIdx.x % (p.kv_heads * blocks);
   if (index >= p.counts[1]) return;
@@ -279,13 +280,13 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnPlan p, AttnCall c, 
       total += weight * ml.y;
     }
     const int count = min(64, j.parts - k0);
-    for (int k = 0; k < count; k += BATCH) {
-      floatx4 y[BATCH];
+    for (int k = 0; k < count; k += kJoinParts) {
+      floatx4 y[kJoinParts];
 #pragma unroll
-      for (int i = 0; i < BATCH; ++i)
+      for (int i = 0; i < kJoinParts; ++i)
         y[i] = *reinterpret_cast<const floatx4*>(p.part_y + row(k0 + min(k + i, count - 1)) * padded + d);
 #pragma unroll
-      for (int i = 0; i < BATCH; ++i) {
+      for (int i = 0; i < kJoinParts; ++i) {
         const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), k + i));
         if (k + i < count) v += w * y[i];
       }
@@ -300,9 +301,57 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnPlan p, AttnCall c, 
   *reinterpret_cast<Row4*>(y) = __builtin_convertvector(v * (1.f / total), Row4);
 }
 
+// The same where tiles have many rows, and few parts: four elements of two rows a thread.
+constexpr int kJoinAtOnce = 2;
+static __host__ __device__ __forceinline__ int join_rows(int padded) { return kJoinAtOnce * 256 / (padded / 4); }
+
+template <typename Row>
+__global__ __launch_bounds__(256) void attn_join_rows_kernel(AttnPlan p, AttnCall c, AttnCut cut, int padded, int blocks) {
+  const int index = blockIdx.x / (p.kv_heads * blocks), rest = blockIdx.x % (p.kv_heads * blocks);
+  if (index >= p.counts[1]) return;
+  const AttnJoin j = p.joins[index];
+  const int kv_head = rest / blocks, r0 = rest % blocks * join_rows(padded), rows = j.length * (int)p.group.divisor - j.m0;
+  if (j.parts < 2 || r0 >= rows || !p.run[j.sequence]) return;
+  const int pieces = padded / 4, d = threadIdx.x % pieces * 4, step = 256 / pieces;
+  auto place = [&](int k) {
+    return ((size_t)(k == 0 ? j.part0 : j.part1 + 2 * (k - 1)) * p.kv_heads + kv_head) * cut.rows;
+  };
+  const int r = r0 + threadIdx.x / pieces;
+  float reference[kJoinAtOnce], total[kJoinAtOnce] = {};
+  floatx4 v[kJoinAtOnce] = {};
+#pragma unroll
+  for (int i = 0; i < kJoinAtOnce; ++i) reference[i] = -__builtin_inff();
+  for (int k = 0; k < j.parts; ++k)
+#pragma unroll
+    for (int i = 0; i < kJoinAtOnce; ++i)
+      reference[i] = fmaxf(reference[i], p.part_ml[place(k) + r + i * step].x);
+  for (int k = 0; k < j.parts; ++k)
+#pragma unroll
+    for (int i = 0; i < kJoinAtOnce; ++i) {
+      const size_t row = place(k) + r + i * step;
+      const float2 ml = p.part_ml[row];
+      const floatx4 y = *reinterpret_cast<const floatx4*>(p.part_y + row * padded + d);
+      // a part of which the row sees nothing has zeros
+      const float weight = ml.x == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(ml.x - reference[i]);
+      total[i] += weight * ml.y;
+      v[i] += weight * y;
+    }
+#pragma unroll
+  for (int i = 0; i < kJoinAtOnce; ++i) {
+    const int row = r + i * step, m = j.m0 + row;
+    if (row >= rows || d >= p.head_dim) continue;
+    Row* y = static_cast<Row*>(c.y) + (j.begin + m / p.group) * c.y_stride +
+             (kv_head * (int)p.group.divisor + m % p.group) * p.head_dim + d;
+    typedef Row Row4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<Row4*>(y) = __builtin_convertvector(v[i] * (1.f / total[i]), Row4);
+  }
+}
+
 // ------------------------------------------------------------------- accepting
-// A workgroup per sequence and layer.  Node n_j goes to place j: n_0 < n_1 < ... has n_j >= j, so that in order no
-// place is written before it is read; a thread moves its own 16 bytes of every node.
+// Workgroups per sequence and layer, each with a share of the elements.  Node n_j goes to place j: n_0 < n_1 < ... has
+// n_j >= j, so that no place is written before it is read if nodes are taken in order, some at a time; a thread moves
+// its own 16 bytes of every node.
+constexpr int kAcceptAtOnce = 8;
 template <typename T>
 __global__ __launch_bounds__(kPlanThreads) void attn_accept_kernel(AttnPlan p, AttnAccept a) {
   const int i = blockIdx.x, count = a.counts[i], context = a.context[i];
@@ -329,18 +378,28 @@ __global__ __launch_bounds__(kPlanThreads) void attn_accept_kernel(AttnPlan p, A
   }
   if (bad) atomicOr(p.error, bad);
   if (__syncthreads_or(bad)) return;
+  __shared__ size_t from[kAttnTreeNodes], to[kAttnTreeNodes];
+  static_assert(kAttnTreeNodes <= kPlanThreads, "a thread for each node");
+  if ((int)threadIdx.x < count) {
+    const int source = context + path[threadIdx.x], place = context + threadIdx.x;
+    from[threadIdx.x] = attn_cell(p, blockIdx.y, table[source >> p.page_shift], source);
+    to[threadIdx.x] = attn_cell(p, blockIdx.y, table[place >> p.page_shift], place);
+  }
+  __syncthreads();
   constexpr int E = 16 / sizeof(T);
   const int pieces = p.kv_heads * p.head_dim / E, per_head = p.head_dim / E;
-  for (int e = threadIdx.x; e < 2 * pieces; e += kPlanThreads) {
+  for (int e = blockIdx.z * kPlanThreads + threadIdx.x; e < 2 * pieces; e += gridDim.z * kPlanThreads) {
     T* const pool = static_cast<T*>(e >= pieces ? p.values : p.keys);
     const int piece = e >= pieces ? e - pieces : e;
     const size_t in = ((size_t)(piece / per_head) << p.page_shift) * p.head_dim + piece % per_head * E;
-    for (int j = 0; j < count; ++j) {
-      const int from = context + path[j], to = context + j;
-      if (from == to) continue;
-      const u32x4 v = *reinterpret_cast<const u32x4*>(
-          pool + attn_cell(p, blockIdx.y, table[from >> p.page_shift], from) + in);
-      *reinterpret_cast<u32x4*>(pool + attn_cell(p, blockIdx.y, table[to >> p.page_shift], to) + in) = v;
+    for (int j = 0; j < count; j += kAcceptAtOnce) {
+      u32x4 v[kAcceptAtOnce];
+#pragma unroll
+      for (int i = 0; i < kAcceptAtOnce; ++i)
+        v[i] = *reinterpret_cast<const u32x4*>(pool + from[min(j + i, count - 1)] + in);
+#pragma unroll
+      for (int i = 0; i < kAcceptAtOnce; ++i)
+        if (j + i < count) *reinterpret_cast<u32x4*>(pool + to[j + i] + in) = v[i];
     }
   }
 }
@@ -353,12 +412,6 @@ __global__ void attn_take_error_kernel(int* error) {
 // ------------------------------------------------------------------------ host
 
 constexpr int kCus = 256;
-#ifndef UNS
-#define UNS 6
-#define OVS 3
-#define OVP 2
-#define UNP 8
-#endif
 static int shared_waves(const AttnPlan& p) {
   const int padded = attn_padded(p.head_dim);
   return padded == 256 || (p.cache_type == kAttnBF16 && p.row_type == kAttnF32 && padded == 128) ? 4 : 8;
@@ -371,8 +424,12 @@ static AttnCut cut_as(const AttnPlan& p, bool shared) {
   AttnCut cut{};
   cut.shared = shared;
   cut.rows = shared ? 32 * shared_waves(p) : 32;
-  cut.unit_log2 = shared ? UNS : UNP;
-  cut.overhead = shared ? OVS : OVP;
+  // A unit is a tile of keys, or four for each wavefront, which with fewer costs a step of one sequence more in its
+  // join than it gains (4096 tokens: units of 128 positions 30 us, of 256 20).  What else a tile costs, about 8 us to
+  // load its rows, to fill the pipeline and to store, is taken for 2 or 3 of them (prompts of 2311 tokens: for one 149 us,
+  // 2 145, 3 133; 1501 tokens in fp32, whose units take twice as long: for 2 131, 3 139).
+  cut.unit_log2 = shared ? 6 : 8;
+  cut.overhead = shared && p.cache_type != kAttnF32 ? 3 : 2;
   cut.shares = std::max(1, kCus / p.kv_heads);
   cut.each = 1.0 / cut.shares;
   return cut;
@@ -409,6 +466,7 @@ static int64_t prepare_share(const AttnPlan& p, const AttnCall& c) {
   return std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, 2), 8 * kCus / c.sequences));
 }
 static int64_t join_blocks(const AttnCut& cut, const AttnPlan& p, const AttnCall& c) {
+  if (cut.shared) return cut.rows / join_rows(attn_padded(p.head_dim));
   // 4 rows each; a step has only a group's
   return ceil_div(c.offsets ? cut.rows : std::min<int>(cut.rows, p.group.divisor), 4);
 }
@@ -427,9 +485,8 @@ template <typename Row>
 static hipError_t join(const AttnPlan& p, const AttnCall& c, const AttnCut& cut, hipStream_t s) {
   const dim3 grid((uint32_t)join_grid(p, c, cut));
   const int padded = attn_padded(p.head_dim), blocks = (int)join_blocks(cut, p, c);
-  // tiles of many rows have few parts
-  if (cut.shared) hipLaunchKernelGGL((attn_join_kernel<Row, 2>), grid, dim3(256), 0, s, p, c, cut, padded, blocks);
-  else hipLaunchKernelGGL((attn_join_kernel<Row, 8>), grid, dim3(256), 0, s, p, c, cut, padded, blocks);
+  if (cut.shared) hipLaunchKernelGGL(attn_join_rows_kernel<Row>, grid, dim3(256), 0, s, p, c, cut, padded, blocks);
+  else hipLaunchKernelGGL(attn_join_kernel<Row>, grid, dim3(256), 0, s, p, c, cut, padded, blocks);
   return hipGetLastError();
 }
 
@@ -465,7 +522,7 @@ hipError_t attn_run_launch(const AttnPlan& p, const AttnCall& c, hipStream_t s) 
 }
 
 hipError_t attn_accept_launch(const AttnPlan& p, const AttnAccept& a, hipStream_t s) {
-  const dim3 grid(a.sequences, p.layers);
+  const dim3 grid(a.sequences, p.layers, (2 * p.kv_heads * p.head_dim * (p.cache_type == kAttnF32 ? 4 : 2) + 16 * kPlanThreads - 1) / (16 * kPlanThreads));
   if (p.cache_type == kAttnF32) hipLaunchKernelGGL(attn_accept_kernel<float>, grid, dim3(kPlanThreads), 0, s, p, a);
   else hipLaunchKernelGGL(attn_accept_kernel<uint16_t>, grid, dim3(kPlanThreads), 0, s, p, a);
   return hipGetLastError();

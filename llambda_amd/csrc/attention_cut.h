@@ -4,9 +4,6 @@
 
 #include "attention.h"
 
-#ifndef SLK
-#define SLK 16
-#endif
 namespace llhip {
 
 // Positions that the rows m0 .. m0 + cut.rows - 1 of a sequence see.
@@ -31,7 +28,7 @@ __device__ __forceinline__ int attn_share_of(int64_t at, int64_t share) {
 }
 
 // How far an end of a share of `share` units may move to spare a tile a part.
-__device__ __forceinline__ int attn_slack(int64_t share) { return (int)min(share / SLK, (int64_t)1 << 20); }
+__device__ __forceinline__ int attn_slack(int64_t share) { return (int)min(share / 16, (int64_t)1 << 20); }
 
 // The item that share `index` has of a tile of `seen` positions, whose units begin at `start`; false if none.  A share
 // has two places among the partial results: for the tile that it begins within, and for the one that it ends within.
