@@ -27,15 +27,18 @@ __device__ __forceinline__ int attn_share_of(int64_t at, int64_t share) {
   return (int)n;
 }
 
-// How far an end of a share of `share` units may move to spare a tile a part.
+// How far an end of a share of `share` units may move to spare a tile a part; in a tile of `units`, less than half of
+// them, so that an end behind the tile stays behind it.
 __device__ __forceinline__ int attn_slack(int64_t share) { return (int)min(share / 16, (int64_t)1 << 20); }
+__device__ __forceinline__ int attn_slack_in(int slack, int units) { return min(slack, (units - 1) / 2); }
 
 // The item that share `index` has of a tile of `seen` positions, whose units begin at `start`; false if none.  A share
 // has two places among the partial results: for the tile that it begins within, and for the one that it ends within.
 __device__ __forceinline__ bool attn_item(const AttnCut& cut, const AttnWorker& w, int index, int seen, int64_t start,
                                           AttnItem& it) {
-  const int64_t end = start + attn_units(cut, seen);
-  auto near = [&](int64_t at) { return at <= start + w.slack ? start : at >= end - w.slack ? end : at; };
+  const int units = attn_units(cut, seen), slack = attn_slack_in(w.slack, units);
+  const int64_t end = start + units;
+  auto near = [&](int64_t at) { return at <= start + slack ? start : at >= end - slack ? end : at; };
   const int64_t lo = near(w.from), hi = near(w.to);
   if (lo >= hi) return false;
   it.key0 = (int)(lo - start) << cut.unit_log2;
@@ -46,9 +49,10 @@ __device__ __forceinline__ bool attn_item(const AttnCut& cut, const AttnWorker& 
 // The join of a tile of which share `index` has the first units but not the last.
 __device__ __forceinline__ AttnJoin attn_join(const AttnCut& cut, const AttnItem& it, int seen, int64_t start,
                                               int64_t share, int index) {
-  const int64_t end = start + attn_units(cut, seen);
-  return AttnJoin{it.begin, it.length, it.m0, attn_share_of(end - attn_slack(share) - 1, share) - index + 1, it.part,
-                  2 * (index + 1), it.sequence};
+  const int units = attn_units(cut, seen);
+  const int64_t last = start + units - attn_slack_in(attn_slack(share), units) - 1;  // the last part begins by here
+  return AttnJoin{it.begin, it.length, it.m0, attn_share_of(last, share) - index + 1, it.part, 2 * (index + 1),
+                  it.sequence};
 }
 
 // Element 0 of position `pos` of kv head 0 (heads are 1 << page_shift rows apart).

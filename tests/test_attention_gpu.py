@@ -630,3 +630,42 @@ def test_pages_shared_by_sequences(hip):
     p.call(session, step=True)
     session.sync()
     p.check()
+
+
+@pytest.mark.parametrize("kinds", [("f32", "f16"), ("f32", "f32"), ("bf16", "bf16")], ids="-".join)
+def test_many_tiles_to_a_share(hip, kinds):
+    """Shares of many tiles, whose ends lie near those of tiles, in tiles shorter than that is near, and behind them."""
+    rng = np.random.default_rng(22)
+    few = dict(heads=8, kv_heads=8, head_dim=16, kinds=kinds)
+    for lengths, cached, more in [
+            ([1] * 256, [300] * 256, few),
+            ([1] * 256, rng.integers(0, 900, size=256).tolist(), few),
+            ([1] * 200, rng.integers(0, 60, size=200).tolist(), dict(few, heads=64, kv_heads=64)),
+            (rng.integers(0, 3, size=120).tolist(), rng.integers(0, 700, size=120).tolist(),
+             dict(few, heads=80, kv_heads=2)),
+            # too many for a workgroup's own plan, one of them long
+            ([1] * 400, [30000] + [9] * 300 + [600] * 99, dict(few, heads=16, kv_heads=16))]:
+        p = Problem(rng, lengths, cached, **more)
+        session = p.open()
+        p.call(session, step=max(lengths) == 1)
+        session.sync()
+        p.check()
+        p.y.fill_(77)
+        p.call(session)  # with offsets, the same
+        session.sync()
+        p.check()
+
+
+@pytest.mark.parametrize("kinds", [("f32", "f16"), ("f32", "f32"), ("bf16", "bf16")], ids="-".join)
+@pytest.mark.parametrize("lengths, cached, heads, kv_heads", [
+    ([300] + [200] * 11 + [90, 257, 1, 512], [6000] + [0] * 15, 32, 32),  # a long one: in shares
+    ([200] * 12 + [130, 257, 0, 512, 700], [0] * 17, 64, 64),              # each tile a share
+    ([64] * 40 + [2, 0, 130], [0] * 20 + [33] * 23, 128, 32),
+    ([170] * 3 + [1200], [0, 90, 1000, 64], 4, 1)])
+def test_prompts_of_many_heads(hip, kinds, lengths, cached, heads, kv_heads):
+    rng = np.random.default_rng(23)
+    p = Problem(rng, lengths, cached, heads=heads, kv_heads=kv_heads, head_dim=16, kinds=kinds)
+    session = p.open()
+    p.call(session)
+    session.sync()
+    p.check()
