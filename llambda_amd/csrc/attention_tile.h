@@ -19,6 +19,18 @@
 //
 // Keys and values pass through LDS, loaded there directly, a tile ahead, 16-byte
 // pieces permuted so that neither read meets a bank twice.
+//
+// Two kernels.  Where a sequence has many rows, eight wavefronts with 32 rows each
+// share every tile (attn_shared_kernel): a tile's bytes serve 256 rows, and the two
+// wavefronts of a SIMD are a phase apart, one's products beside the other's softmax
+// (all at once: 2311 tokens of prompts 133 -> 127 us).  Bound by the products: 8192
+// tokens, 32 heads of 128, fp32 rows over f16, 550 GFLOP as two parts, 970 us or
+// 1130 TFLOP/s of products, next to 1070 of a large library product of f16 (random
+// operands hold the card to about 1500 from registers alone); 6000 tokens of bf16,
+// one part, 375 us or 790 TFLOP/s, for there the softmax weighs as much.  Where a
+// sequence has few rows, wavefronts share 32 of them and take a tile of keys each
+// (attn_split_kernel), so that the keys' way through the device is all that counts:
+// a step of 48 sequences, 614 MB, in 125 us, 4.9 TB/s (a large copy 5.1).
 #pragma once
 
 #include "attention_cut.h"
@@ -1062,10 +1074,11 @@ template <int TYPE, typename Row, int DP>
 constexpr int attn_shared_waves() {
   return DP == 256 || (TYPE == kAttnBF16 && sizeof(Row) == 4 && DP == 128) ? 4 : 8;
 }
-// Keys of a shared tile: what registers hold of their scores.
-template <int TYPE, int DP>
+// Keys of a shared tile: what registers hold of their scores.  (16 trees of 61 nodes, heads of 256 in bf16: tiles of 32
+// 127 us, of 64 118; with rows of fp32 64 do not fit.)
+template <typename Row, int DP>
 constexpr int attn_shared_keys() {
-  return DP == 256 ? 32 : 64;
+  return DP == 256 && sizeof(Row) == 4 ? 32 : 64;
 }
 // Waves that split keys: what LDS holds of their tiles.
 template <int TYPE, int DP>
@@ -1076,8 +1089,8 @@ constexpr int attn_split_waves() {
 template <int TYPE, typename Row, int DP>
 hipError_t attn_attend(const AttnPlan& p, const AttnCall& c, const AttnCut& cut, uint32_t grid, hipStream_t s) {
   if (cut.shared) {
-    constexpr int W = attn_shared_waves<TYPE, Row, DP>(), KT = attn_shared_keys<TYPE, DP>();
-    return attn_launch(attn_shared_kernel<TYPE, Row, DP, W, KT>, grid, 64 * W, 
+    constexpr int W = attn_shared_waves<TYPE, Row, DP>(), KT = attn_shared_keys<Row, DP>();
+    return attn_launch(attn_shared_kernel<TYPE, Row, DP, W, KT>, grid, 64 * W,
                        4 * KT * DP * attn_cell_bytes<TYPE>() + Spoiled<attn_cell_bytes<TYPE>(), DP, KT>::kBytes, s, p, c, cut);
   }
   constexpr int W = attn_split_waves<TYPE, DP>();
