@@ -421,9 +421,13 @@ static int shared_waves(const AttnPlan& p) {
   return padded == 256 || (p.cache_type == kAttnBF16 && p.row_type == kAttnF32 && padded == 128) ? 4 : 8;
 }
 
-// Rows of a kv head in a sequence, on average, up to which waves share rows and not keys: fewer than five wavefronts'
-// rows leave more of the other kernel idle than reading the keys once for each 32 costs.
-constexpr int kFewRows = 160;
+// Rows of a kv head in a sequence, on average, up to which waves share rows and not keys: those of two wavefronts, for
+// with fewer than three of eight at work the other kernel loses more than reading the keys for each 32 rows costs (us, 16
+// trees behind 2000 tokens, 8 kv heads of 128, fp32 rows over f16: 32 rows 53 against 69, 64 rows 68 and 72, 80 rows 86
+// and 72; over fp32 157 and 193, 248 and 207, 353 and 211).  A call without a launch before has more to lose (one tree
+// behind 4000 tokens: 160 rows 42 and 60; behind 30000, 160 rows 88 and 96, 224 rows 153 and 106), but not over
+// fp32 (30000 tokens, 128 rows: 347 and 192).
+constexpr int kFewRows = 64, kFewRowsAlone = 160;
 
 static AttnCut cut_as(const AttnPlan& p, bool shared) {
   AttnCut cut{};
@@ -440,8 +444,10 @@ static AttnCut cut_as(const AttnPlan& p, bool shared) {
   return cut;
 }
 static AttnCut cut_of(const AttnPlan& p, const AttnCall& c) {
-  AttnCut cut = cut_as(p, ceil_div((int64_t)c.tokens * p.group.divisor, c.sequences) > kFewRows);
-  cut.few = !cut.shared && c.tokens <= kAttnFewTokens && c.sequences <= kAttnFewSequences;
+  const bool alone = c.tokens <= kAttnFewTokens && c.sequences <= kAttnFewSequences;
+  const int64_t rows = ceil_div((int64_t)c.tokens * p.group.divisor, c.sequences);
+  AttnCut cut = cut_as(p, rows > (alone && p.cache_type != kAttnF32 ? kFewRowsAlone : kFewRows));
+  cut.few = !cut.shared && alone;
   return cut;
 }
 
