@@ -614,8 +614,9 @@ void llambda_hip_attention_session_destroy(llambda_hip_attention_session* sessio
  * written: offsets (nothing of the call is run); a sequence's tokens beyond max_context, its
  * pages outside the pool, its parents (the sequence is not run: its rows and pages stay as they
  * are).  llambda_hip_attention_session_sync reports them.  Counts of cached tokens are the
- * caller's: they are not changed.  The calls of a session are ordered as
- * llambda_hip_ssm_session_run_device's, under capture too. */
+ * caller's: they are not changed.  A call is refused, with nothing of it enqueued, where its
+ * sequences and tiles of 32 to 256 rows, times kv_heads, are 2^23 or more.  The calls of a
+ * session are ordered as llambda_hip_ssm_session_run_device's, under capture too. */
 int llambda_hip_attention_session_run_device(llambda_hip_attention_session* session, int64_t layer,
                                              const llambda_hip_attention_rows* rows,
                                              const llambda_hip_attention_batch* batch, void* stream);
@@ -644,7 +645,8 @@ int llambda_hip_attention_session_sync(llambda_hip_attention_session* session, v
 
 /* Copy positions [first, first + count) of a sequence whose table row is `table` (host memory)
  * into or out of the pages: keys and values [count][kv_heads][head_dim] of the cache's type, host
- * memory.  Synchronous; waits for the session's calls, whatever stream they ran on. */
+ * memory.  Synchronous; waits for the session's calls, whatever stream they ran on (a graph's
+ * replays are the caller's to wait for). */
 int llambda_hip_attention_session_write(llambda_hip_attention_session* session, int64_t layer,
                                         const int32_t* table, int64_t first, int64_t count,
                                         const void* keys, const void* values);

@@ -11,7 +11,7 @@
 // several.  A call of few rows has no first launch (attention_tile.h), and so a step
 // of one sequence is two: 13 + 5 us behind 4096 tokens, bound by latency (44 with the
 // first launch and shares of 64 tokens).  Around the 97 us of attending 2311 tokens of
-// prompts lie 9 of preparing and 8 of joining; moving the accepted nodes of 16 trees
+// prompts lie 9 of preparing and 13 of joining; moving the accepted nodes of 16 trees
 // takes 4.5.
 #include "attention_cut.h"
 

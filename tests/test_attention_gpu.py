@@ -669,3 +669,63 @@ def test_prompts_of_many_heads(hip, kinds, lengths, cached, heads, kv_heads):
     p.call(session)
     session.sync()
     p.check()
+
+
+@pytest.mark.parametrize("heads, kv_heads", [(1024, 1), (300, 300), (1024, 1024), (1, 1)])
+def test_ends_of_the_ranges(hip, heads, kv_heads):
+    """One head and the most; sequences that fill the context; a context that ends inside a page."""
+    rng = np.random.default_rng(24)
+    for lengths, cached, step in [([1, 1, 1], [0, 85, 36], True), ([3, 0, 1], [83, 0, 85], False)]:
+        p = Problem(rng, lengths, cached, heads=heads, kv_heads=kv_heads, head_dim=16)
+        p.table = p.table[:, :6].copy()
+        p.d_table = p.d_table[:, :6].contiguous()
+        p.width = 6
+        import torch
+        torch.cuda.synchronize()
+        session = p.open(max_context=86, max_tokens=p.tokens)
+        p.call(session, step=step)
+        session.sync()
+        p.check()
+
+
+def test_two_threads_and_one_session(hip):
+    """Host calls of several threads on sequences of their own, and scores beside them."""
+    from concurrent.futures import ThreadPoolExecutor
+    from llambda_amd.sampling import HipTokenScorer
+    layout = AttentionLayout(4, 2, 32)
+    session = HipAttentionSession(layout, pages=40, page_tokens=16, max_context=150, max_tokens=60)
+    scorer = HipTokenScorer(3001, 4, 4)
+
+    def one(i):
+        rng = np.random.default_rng(100 + i)
+        table = list(range(10 * i, 10 * i + 10))
+        k, v = (np.empty((0, 2, 32), np.float32) for _ in range(2))
+        for n in (40, 1, 60, 1, 1):
+            q, nk, nv = (rng.normal(size=(n, h, 32)).astype(np.float32) for h in (4, 2, 2))
+            y = session.run(q, nk, nv, table, len(k))
+            k, v = np.concatenate([k, ref.rounded(nk, "f16")]), np.concatenate([v, ref.rounded(nv, "f16")])
+            want, bound = ref.attention(q, k, v, ref.sees(n, len(k) - n), np.float32(1 / np.sqrt(32)), "f32", "f16")
+            assert np.all(np.abs(y - want) <= bound)
+            x = rng.normal(size=(2, 3001)).astype(np.float32)
+            top = scorer.score(x, top=1).top_tokens[:, 0]
+            assert np.array_equal(top, x.argmax(1))
+        return True
+
+    with ThreadPoolExecutor(4) as pool:
+        assert all(pool.map(one, range(4)))
+
+
+def test_calls_of_too_many_launches_are_refused(hip):
+    import torch
+    n, kv = 65535, 256
+    row = torch.zeros(n * kv * 16, dtype=torch.float32, device="cuda")
+    lists = torch.zeros(n, dtype=torch.int32, device="cuda")
+    session = HipAttentionSession(AttentionLayout(kv, kv, 16), pages=1, page_tokens=16, max_context=16, max_tokens=n,
+                                  max_sequences=n)
+    y = torch.full_like(row, 77)
+    torch.cuda.synchronize()
+    with pytest.raises(HipBackendError, match="65535 tokens of 65535 sequences are too many for one call"):
+        session.run_device(row.data_ptr(), row.data_ptr(), row.data_ptr(), y.data_ptr(), n, lists.data_ptr(),
+                           lists.data_ptr(), n)
+    session.sync()
+    assert torch.all(y == 77)
