@@ -729,3 +729,14 @@ def test_calls_of_too_many_launches_are_refused(hip):
                            lists.data_ptr(), n)
     session.sync()
     assert torch.all(y == 77)
+
+
+@pytest.mark.parametrize("kinds", [("f32", "f16"), ("bf16", "bf16")], ids="-".join)
+def test_a_million_tokens_in_one_page(hip, kinds):
+    rng = np.random.default_rng(25)
+    for lengths, cached in [([1], [2 ** 20 - 1]), ([100], [10 ** 6])]:
+        p = Problem(rng, lengths, cached, heads=1, kv_heads=1, head_dim=16, kinds=kinds, page=2 ** 20, extra_pages=0)
+        session = p.open()
+        p.call(session)
+        session.sync()
+        p.check()
