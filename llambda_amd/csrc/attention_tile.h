@@ -100,13 +100,15 @@ constexpr int attn_parts() {
 // (a, b) as N packed pairs whose sums they are.
 template <int TYPE, int N>
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&out)[N]) {
+  float minus = -1.f;  // hidden, so that an f16's conversion becomes part of the (exact) difference
+  asm("" : "+s"(minus));
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     out[n] = Cell<TYPE>::pack(a, b);
     if (n + 1 < N) {
       const floatx2 u = Cell<TYPE>::unpack(out[n]);
-      a -= u.x;
-      b -= u.y;
+      a = fmaf(u.x, minus, a);
+      b = fmaf(u.y, minus, b);
     }
   }
 }
