@@ -740,3 +740,57 @@ def test_a_million_tokens_in_one_page(hip, kinds):
         p.call(session)
         session.sync()
         p.check()
+
+
+@pytest.mark.parametrize("kinds", [("f32", "f16"), ("bf16", "bf16")], ids="-".join)
+@pytest.mark.parametrize("spare", [3, 700])
+def test_calls_without_a_row(hip, kinds, spare):
+    """Rows that belong to no sequence only, and one sequence among many empty ones."""
+    rng = np.random.default_rng(26)
+    for lengths in ([0, 0], [0] * 300 + [2] + [0] * 30):
+        p = Problem(rng, lengths, [5] * len(lengths), kinds=kinds, spare=spare)
+        session = p.open()
+        p.call(session)
+        session.sync()
+        p.check()
+
+
+@pytest.mark.parametrize("kinds", KINDS, ids="-".join)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("rows", [9, 150])
+def test_queries_that_are_no_numbers_spoil_their_own_rows(hip, kinds, bad, rows):
+    import torch
+    rng = np.random.default_rng(27)
+    p = Problem(rng, [rows], [70], kinds=kinds, heads=4, kv_heads=2)
+    p.q[3, 1, 5] = bad
+    p.d[0].copy_(torch.from_numpy(p.q.reshape(rows, -1)).to(p.d[0].dtype))
+    torch.cuda.synchronize()
+    session = p.open()
+    p.call(session)
+    session.sync()
+    torch.cuda.synchronize()
+    y = p.y.float().cpu().numpy().reshape(rows, 4, 64)
+    assert not np.any(np.isfinite(y[3, 1]))
+    p.q[3, 1, 5] = 0
+    page, at = p.places(0)
+    for pool, new in ((p.keys, p.k), (p.values, p.v)):
+        pool[0, page[70:], :, at[70:]] = ref.rounded(new, kinds[1])
+    want, bound = ref.attention(p.q, *(pool[0, page, :, at] for pool in (p.keys, p.values)), ref.sees(rows, 70),
+                                np.float32(p.scale), *kinds)
+    good = np.ones((rows, 4), dtype=bool)
+    good[3, 1] = False
+    assert np.all((np.abs(y - want) <= bound)[good])
+
+
+def test_a_page_read_twice_by_a_sequence(hip):
+    rng = np.random.default_rng(28)
+    p = Problem(rng, [1, 30], [70, 64], heads=4, kv_heads=2)
+    for i in range(2):
+        p.table[i, 1] = p.table[i, 0]
+        p.d_table[i, 1] = p.d_table[i, 0]
+    import torch
+    torch.cuda.synchronize()
+    session = p.open()
+    p.call(session)
+    session.sync()
+    p.check()
