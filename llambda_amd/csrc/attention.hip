@@ -250,7 +250,8 @@ __global__ __launch_bounds__(kPlanThreads) void attn_prepare_kernel(AttnPlan p, 
       const bool value = e >= pieces;
       const int piece = value ? e - pieces : e;
       const size_t to = at + ((size_t)(piece / per_head) << p.page_shift) * p.head_dim + piece % per_head * 8;
-      attn_put8(static_cast<T*>(value ? p.values : p.keys) + to, (value ? v : k) + 8 * piece);
+      attn_put8(static_cast<T*>(value ? p.values : p.keys) + to,
+                *reinterpret_cast<const attn_eight<Row>*>((value ? v : k) + 8 * piece));
     }
   }
 }

@@ -62,11 +62,11 @@ __device__ __forceinline__ size_t attn_cell(const AttnPlan& p, int layer, int pa
 }
 
 // Eight elements in the cache's type, to the nearest; what is beyond it becomes an infinity.
+template <typename T>
+using attn_eight = T __attribute__((ext_vector_type(8)));
 template <typename To, typename From>
-__device__ __forceinline__ void attn_put8(To* to, const From* from) {
-  typedef From From8 __attribute__((ext_vector_type(8)));
-  typedef To To8 __attribute__((ext_vector_type(8)));
-  const From8 v = *reinterpret_cast<const From8*>(from);
+__device__ __forceinline__ void attn_put8(To* to, const attn_eight<From>& v) {
+  typedef attn_eight<To> To8;
   if constexpr (sizeof(From) == sizeof(To)) *reinterpret_cast<To8*>(to) = __builtin_bit_cast(To8, v);
   else *reinterpret_cast<To8*>(to) = __builtin_convertvector(v, To8);
 }
