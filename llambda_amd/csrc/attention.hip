@@ -9,10 +9,9 @@
 // evenly, where tiles are few, over as many workgroups as the device has CUs.  The
 // attend kernel does the shares; the join adds up the parts of tiles that lie in
 // several.  A call of few rows has no first launch (attention_tile.h), and so a step
-// of one sequence is two: 13 + 5 us behind 4096 tokens, bound by latency (44 with the
-// first launch and shares of 64 tokens).  Around the 97 us of attending 2311 tokens of
-// prompts lie 9 of preparing and 13 of joining; moving the accepted nodes of 16 trees
-// takes 4.5.
+// of one sequence is two: 13 + 5 us behind 4096 tokens, bound by latency.  Around the
+// 97 us of attending 2311 tokens of prompts lie 9 of preparing and 13 of joining;
+// moving the accepted nodes of 16 trees takes 4.5.
 #include "attention_cut.h"
 
 #include <algorithm>
@@ -434,12 +433,13 @@ static AttnCut cut_as(const AttnPlan& p, bool shared) {
   AttnCut cut{};
   cut.shared = shared;
   cut.rows = shared ? 32 * shared_waves(p) : 32;
-  // A unit is a tile of keys, or four for each wavefront, which with fewer costs a step of one sequence more in its
-  // join than it gains (4096 tokens: units of 128 positions 30 us, of 256 20).  What else a tile costs, about 8 us to
-  // load its rows, to fill the pipeline and to store, is taken for 2 or 3 of them (prompts of 2311 tokens: for one 149 us,
-  // 2 145, 3 133; 1501 tokens in fp32, whose units take twice as long: for 2 131, 3 139).
+  // A unit is a tile of keys, or two for each wavefront (a step of one sequence 20 us, with twice as many 22, a tree of 26
+  // nodes 35 and 38).  What else a tile costs, about 8 us to load its rows, to fill the pipeline and to store, is taken for
+  // some of them: (us for 2, 3, 4 and 5) prompts of 2311 tokens over f16 145, 129, 120, 126; 12 of 2000, heads of 256 and
+  // fp32 rows, whose units take twice as long, 105, 98, 106, 107; 1501 tokens in fp32, four times, 124, 131, 131, 138.
   cut.unit_log2 = shared ? 6 : 8;
-  cut.overhead = shared && p.cache_type != kAttnF32 ? 3 : 2;
+  const bool wide = attn_padded(p.head_dim) == 256 && p.row_type == kAttnF32;
+  cut.overhead = !shared || p.cache_type == kAttnF32 ? 2 : wide ? 3 : 4;
   cut.shares = std::max(1, kCus / p.kv_heads);
   cut.each = 1.0 / cut.shares;
   return cut;
