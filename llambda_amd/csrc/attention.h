@@ -121,6 +121,12 @@ struct AttnSizes {
   int64_t tiles, workers, shares, part_rows;  // part_rows: rows of part_ml; part_y has attn_padded(head_dim) floats each
 };
 AttnSizes attn_sizes(const AttnPlan& p);
+// Keys of a tile that wavefronts share: what registers hold of their scores.  (Rows of 16 bits.  16 trees of 61 nodes, heads
+// of 256: 32 keys 127 us, 64 118.  Heads of 64, 28 over 4: 3 prompts of 600 tokens behind 2000 64 keys 101 us, 128 89, one of
+// 5000 161 and 153, 16 of 500 77 and 80.  Heads of 128: the same kind 160 and 153, 270 and 273, 120 and 137.)
+constexpr int attn_shared_keys(int padded, int row_bytes) {
+  return row_bytes == 2 && padded == 64 ? 128 : row_bytes == 4 && padded == 256 ? 32 : 64;
+}
 inline int attn_padded(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 inline int attn_table_width(const AttnPlan& p) { return (p.max_context + (1 << p.page_shift) - 1) >> p.page_shift; }
 

@@ -433,13 +433,13 @@ static AttnCut cut_as(const AttnPlan& p, bool shared) {
   AttnCut cut{};
   cut.shared = shared;
   cut.rows = shared ? 32 * shared_waves(p) : 32;
-  // A unit is a tile of keys, or two for each wavefront (a step of one sequence 20 us, with twice as many 22, a tree of 26
+  // A unit is a tile of keys (two, where it has 32), or two for each wavefront (a step of one sequence 20 us, with twice as many 22, a tree of 26
   // nodes 35 and 38).  What else a tile costs, about 8 us to load its rows, to fill the pipeline and to store, is taken for
   // some of them: (us for 2, 3, 4 and 5) prompts of 2311 tokens over f16 145, 129, 120, 126; 12 of 2000, heads of 256 and
   // fp32 rows, whose units take twice as long, 105, 98, 106, 107; 1501 tokens in fp32, four times, 124, 131, 131, 138.
-  cut.unit_log2 = shared ? 6 : 8;
-  const bool wide = attn_padded(p.head_dim) == 256 && p.row_type == kAttnF32;
-  cut.overhead = !shared || p.cache_type == kAttnF32 ? 2 : wide ? 3 : 4;
+  const int keys = attn_shared_keys(attn_padded(p.head_dim), p.row_type == kAttnF32 ? 4 : 2);
+  cut.unit_log2 = !shared ? 8 : keys == 128 ? 7 : 6;
+  cut.overhead = !shared || p.cache_type == kAttnF32 || keys == 128 ? 2 : keys == 32 ? 3 : 4;
   cut.shares = std::max(1, kCus / p.kv_heads);
   cut.each = 1.0 / cut.shares;
   return cut;

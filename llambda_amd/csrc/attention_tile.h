@@ -175,9 +175,11 @@ struct TileLoader {
     values = static_cast<const uint8_t*>(p.values) + at;
   }
 
-  // Lane l's page: the one of position base + l.
+  // Lane l's page: the one of position base + kApart l.
+  static constexpr int kApart = KT > 64 ? KT / 64 : 1;
+  static_assert(kApart == 1 || L::kRowsPerLoad % kApart == 0, "a load begins at a position whose page a lane has");
   __device__ __forceinline__ int entry(int base, int lane) const {
-    return min(base + lane, last) >> page_shift;
+    return min(base + lane * kApart, last) >> page_shift;
   }
   // Of the loads of the keys, or values, of tile `base` to LDS every STEP-th from `from` on; pages: entry()'s, by lane.
   // What depends on the lane alone is the same for every tile.
@@ -195,7 +197,7 @@ struct TileLoader {
       // a row shorter than the tile's: its first piece again (the row's q has zeros there, its y is not stored)
       if (source >= bytes) source = 0;
       const uint32_t pos = min(base + r0, last & ~(R - 1));
-      const uint32_t page = __builtin_amdgcn_readlane(pages, r0);
+      const uint32_t page = __builtin_amdgcn_readlane(pages, r0 / kApart);
       load_lds16((VALUES ? values : keys) + (uint64_t)page * page_bytes + (pos & in_page) * bytes, row * bytes + source,
                  to + 1024u * i);
     }
@@ -1097,12 +1099,6 @@ template <int TYPE, typename Row, int DP>
 constexpr int attn_shared_waves() {
   return DP == 256 || (TYPE == kAttnBF16 && sizeof(Row) == 4 && DP == 128) ? 4 : 8;
 }
-// Keys of a shared tile: what registers hold of their scores.  (16 trees of 61 nodes, heads of 256 in bf16: tiles of 32
-// 127 us, of 64 118; with rows of fp32 64 do not fit.)
-template <typename Row, int DP>
-constexpr int attn_shared_keys() {
-  return DP == 256 && sizeof(Row) == 4 ? 32 : 64;
-}
 // Waves that split keys: what LDS holds of their tiles.
 template <int TYPE, int DP>
 constexpr int attn_split_waves() {
@@ -1112,7 +1108,7 @@ constexpr int attn_split_waves() {
 template <int TYPE, typename Row, int DP>
 hipError_t attn_attend(const AttnPlan& p, const AttnCall& c, const AttnCut& cut, uint32_t grid, hipStream_t s) {
   if (cut.shared) {
-    constexpr int W = attn_shared_waves<TYPE, Row, DP>(), KT = attn_shared_keys<Row, DP>();
+    constexpr int W = attn_shared_waves<TYPE, Row, DP>(), KT = attn_shared_keys(DP, sizeof(Row));
     return attn_launch(attn_shared_kernel<TYPE, Row, DP, W, KT>, grid, 64 * W,
                        4 * KT * DP * attn_cell_bytes<TYPE>() + Spoiled<attn_cell_bytes<TYPE>(), DP, KT>::kBytes, s, p, c, cut);
   }
