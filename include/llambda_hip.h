@@ -548,7 +548,9 @@ enum {                          /* GGML's tags */
  * over the positions j that the row sees: j <= c + r.  Rows are taken as they are:
  * a model that rotates queries and keys does so before.  fp32 rows keep single precision
  * throughout; rows in 16 bits have their probabilities rounded to that type.  Values
- * that are infinite or NaN reach only the rows that see them (as either).
+ * that are infinite or NaN reach only the rows that see them (as either).  Keys that are
+ * infinite give scores: one of -inf has no weight, and a row with one of +inf, one that is no
+ * number, or none above -inf is NaN.
  *
  * The cache is a pool of pages, key_pages and value_pages [layers][pages][kv_heads]
  * [page_tokens][head_dim]; position j of sequence i is row j % page_tokens of page

@@ -496,7 +496,7 @@ struct RowTile {
 template <typename Row, int DP>
 struct RowTile<kAttnF32, Row, DP> {
   typedef TileLayout<4, DP> L;
-  static constexpr int kSteps = DP / 8, kBlocks = DP / 32;
+  static constexpr int N = 1, kSteps = DP / 8, kBlocks = DP / 32;
   floatx4 q[kSteps];  // elements 8 s + 4 (lane / 32) + 0..3
   RowSums<DP> sums;
   float factor;
@@ -588,6 +588,18 @@ __device__ __forceinline__ const T* opaque_pointer(const T* p) {
   return p;
 }
 
+// The kernel's first arguments, read again: where they are rarely needed, no register holds them meanwhile.
+struct AttnArgs {
+  AttnPlan p;
+  AttnCall c;
+};
+__device__ __forceinline__ const AttnArgs& args_again() {
+  typedef const __attribute__((address_space(4))) AttnArgs* Args;
+  Args a = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(a));
+  return *(const AttnArgs*)a;
+}
+
 // A struct of the workspace, in scalar registers.
 template <typename T>
 __device__ __forceinline__ T uniform_load(const T* at) {
@@ -629,6 +641,84 @@ struct ItemRows {
     return Sight{it.context + token + 1, nullptr};
   }
 };
+
+// Row m of a tile of ROWS by its definition, by one wavefront.  Parts of q are of either sign or zero, so that their products
+// with a key's infinity make no number of a score that is -inf and has no weight; and an element next to the end of fp32 has a
+// first part that is infinite.  A row whose sum is no number is formed anew here, in fp32, with products of whole elements:
+// twice over its keys, for the largest score and for the sums, or as far as a score that is +inf or no number.  (5000 tokens,
+// 32 heads of 128, one infinite key: 25 ms in place of 0.43.  A mend of the scores within the loop would cost every call.)
+// tree: the ancestors of the item's tokens in LDS, null where they are in the workspace.
+template <int TYPE, typename Row, int DP, int ROWS>
+__device__ __forceinline__ void whole_row(const AttnPlan& p, const AttnCall& c, const AttnItem& it, int kv_head, int m,
+                                          const uint32_t* tree) {
+  typedef typename Cell<TYPE>::T T;
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  typedef float float8 __attribute__((ext_vector_type(8)));
+  const int lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));
+  const ItemRows<Row> rows(p, it, m, 0);
+  Sight sight = rows.sight(p, c, it);
+  if (tree && c.parents) sight.tree = tree + (rows.token - it.m0 / p.group) * kAttnTreeWords;
+  const Row* const q = rows.q(p, c, it, kv_head);
+  const int* const table = c.table + it.sequence * c.table_stride;
+  const float factor = p.scale * kAttnLog2e;
+  auto cells = [&](void* pool, int page, int pos) {
+    return static_cast<const T*>(pool) + attn_cell(p, c.layer, page, pos) + ((size_t)kv_head << p.page_shift) * p.head_dim;
+  };
+  auto sees = [&](int base) { return base + lane < it.key1 && (sight.bits(base + (lane & 32)) >> (lane & 31) & 1); };
+  int page = 0;
+  auto score = [&](int base) {  // of key base + lane, in exponents of two
+    if (!sees(base)) return -__builtin_inff();
+    page = table[(base + lane) >> p.page_shift];
+    const T* const key = cells(p.keys, page, base + lane);
+    float v = 0.f;
+#pragma unroll 1
+    for (int d = 0; d < p.head_dim; d += 8) {
+      const float8 a = *reinterpret_cast<const float8*>(q + d);
+      const float8 b = __builtin_convertvector(*reinterpret_cast<const attn_eight<T>*>(key + d), float8);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v = fmaf(a[i], b[i], v);
+    }
+    return v * factor;
+  };
+  float reference = -__builtin_inff(), sum = 0.f;
+  floatx4 y{};
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    const float shift = Cell<TYPE>::kLift - (reference == -__builtin_inff() ? 0.f : reference);
+    for (int base = it.key0; base < it.key1; base += 64) {
+      const float v = score(base);
+      if (pass == 0) {
+        reference = fmaxf(reference, v);
+        if (!__ballot(!(v < __builtin_inff()))) continue;
+        sum = __builtin_nanf("");
+        break;
+      }
+      const float weight = __builtin_amdgcn_exp2f(v + shift);
+      sum += weight;
+      floatx4 some{};  // of 64 keys, then of all: no long chains
+      for (uint64_t left = __ballot(sees(base)); left; left &= left - 1) {
+        const int k = __builtin_ctzll(left);
+        const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), k));
+        const T* const value = cells(p.values, __builtin_amdgcn_readlane(page, k), base + k);
+        if (4 * lane < p.head_dim) some += w * __builtin_convertvector(*reinterpret_cast<const T4*>(value + 4 * lane), floatx4);
+      }
+      y += some;
+    }
+    reference = wave_max(reference);
+    if (__ballot(sum != sum)) {  // no softmax
+      reference = -__builtin_inff();
+      break;
+    }
+  }
+  sum = wave_total(sum);
+  if (it.part < 0) {
+    if (4 * lane < p.head_dim) store4(rows.y(p, c, it, kv_head) + 4 * lane, y * (1.f / sum));
+  } else {
+    const size_t row = ((size_t)it.part * p.kv_heads + kv_head) * ROWS + m - it.m0;
+    if (lane == 0) p.part_ml[row] = make_float2(reference, sum);
+    if (4 * lane < DP) *reinterpret_cast<floatx4*>(p.part_y + row * DP + 4 * lane) = y;
+  }
+}
 
 // Waves share tiles of KT keys, two of which are in LDS; each has 32 rows of its own.
 template <int TYPE, typename Row, int DP, int WAVES, int KT>
@@ -727,8 +817,9 @@ __device__ __forceinline__ void shared_item(const AttnPlan& p, const AttnCall& c
   const float sum = half_pair_sum(tile.sums.sum);
   // made again, so that the loop's registers need not hold it
   const ItemRows<Row> rows(p, it, m0, (int)opaque((uint32_t)lane));
-  if (!rows.real) return;
-  if (it.part < 0) {
+  const bool again = Tile::N > 1 && rows.real && sum != sum;
+  if (!rows.real || again) {
+  } else if (it.part < 0) {
     const float scale = 1.f / sum;
     Row* y = rows.y(p, c, it, kv_head);
 #pragma unroll
@@ -748,6 +839,11 @@ __device__ __forceinline__ void shared_item(const AttnPlan& p, const AttnCall& c
       for (int i = 0; i < 4; ++i)
         *reinterpret_cast<floatx4*>(y + 32 * b + 8 * i + 4 * tile.half) = tile.sums.piece(b, i, tile.half);
   }
+  if constexpr (Tile::N > 1)
+    for (uint32_t left = (uint32_t)__ballot(again); left; left &= left - 1) {
+      const AttnArgs& args = args_again();
+      whole_row<TYPE, Row, DP, 32 * WAVES>(args.p, args.c, it, kv_head, m0 + __builtin_ctz(left), nullptr);
+    }
 }
 
 template <int TYPE, typename Row, int DP, int WAVES, int KT>
@@ -1018,6 +1114,7 @@ __device__ __forceinline__ bool split_item(const AttnPlan& p, const AttnCall& c,
       *reinterpret_cast<floatx4*>(own + 32 * b + 8 * i + 4 * tile.half) = tile.sums.piece(b, i, tile.half);
   __syncthreads();
   const int count = min(32, rows.rows - it.m0);
+  uint32_t again = 0;
 #pragma unroll 2
   for (int i = threadIdx.x; i < count * (DP / 4); i += 64 * WAVES) {
     const int r = i / (DP / 4), d = 4 * (i % (DP / 4));
@@ -1035,6 +1132,10 @@ __device__ __forceinline__ bool split_item(const AttnPlan& p, const AttnCall& c,
       total += weight * ml[w * 64 + 32 + r];
       v += weight * *reinterpret_cast<const floatx4*>(lds + w * M::kWave + (r * M::kRow + d) * 4);
     }
+    if (Tile::N > 1 && total != total) {  // formed anew below (a row's threads are one wavefront's)
+      again |= 1u << r;
+      continue;
+    }
     if (it.part < 0) {
       const int m = it.m0 + r;
       Row* y = static_cast<Row*>(c.y) + (it.begin + m / p.group) * c.y_stride +
@@ -1045,6 +1146,14 @@ __device__ __forceinline__ bool split_item(const AttnPlan& p, const AttnCall& c,
       if (d == 0) p.part_ml[row] = make_float2(reference, total);
       *reinterpret_cast<floatx4*>(p.part_y + row * DP + d) = v;
     }
+  }
+  if constexpr (Tile::N > 1) {
+    if (__builtin_expect(__ballot(again != 0) != 0, 0))
+      for (int r = 0; r < count; ++r) {
+        if (!__ballot(again >> r & 1)) continue;
+        const AttnArgs& args = args_again();
+        whole_row<TYPE, Row, DP, 32>(args.p, args.c, it, kv_head, it.m0 + r, cut.few ? few.tree[0] : nullptr);
+      }
   }
   return true;
 }

@@ -8,9 +8,6 @@ from test_attention_gpu import KINDS, Problem, random_tree
 
 pytestmark = pytest.mark.gpu
 
-# rows that are an operand as they are
-WHOLE = [k for k in KINDS if k not in (("f32", "f16"), ("f32", "bf16"))]
-
 
 def put(p, bad):
     """Infinities in keys: bad lists (sequence, position, kv head, element, value), at cached positions and new ones."""
@@ -68,7 +65,7 @@ def run(p, step=False):
 WIDTHS = [16, 48, 64, 80, 112, 128, 208, 256]
 
 
-@pytest.mark.parametrize("kinds", WHOLE, ids="-".join)
+@pytest.mark.parametrize("kinds", KINDS, ids="-".join)
 @pytest.mark.parametrize("head_dim", WIDTHS)
 @pytest.mark.parametrize("shape", ["steps", "prompts", "many"])
 def test_infinite_keys(hip, kinds, head_dim, shape):
@@ -90,7 +87,7 @@ def test_infinite_keys(hip, kinds, head_dim, shape):
     run(p, step=shape == "steps")
 
 
-@pytest.mark.parametrize("kinds", WHOLE, ids="-".join)
+@pytest.mark.parametrize("kinds", KINDS, ids="-".join)
 @pytest.mark.parametrize("head_dim", [64, 80, 256])
 def test_infinite_keys_of_long_contexts(hip, kinds, head_dim):
     """Positions in parts that are joined, rows that share keys and rows that do not."""
@@ -104,7 +101,7 @@ def test_infinite_keys_of_long_contexts(hip, kinds, head_dim):
     run(p)
 
 
-@pytest.mark.parametrize("kinds", WHOLE, ids="-".join)
+@pytest.mark.parametrize("kinds", KINDS, ids="-".join)
 @pytest.mark.parametrize("nodes", [20, 200])
 def test_infinite_keys_of_trees(hip, kinds, nodes):
     rng = np.random.default_rng(42)
@@ -115,7 +112,16 @@ def test_infinite_keys_of_trees(hip, kinds, nodes):
     run(p)
 
 
-@pytest.mark.parametrize("kinds", WHOLE, ids="-".join)
+@pytest.mark.parametrize("kinds", [("f32", "f16")], ids="-".join)
+def test_keys_beyond_the_caches_range(hip, kinds):
+    """Rows in single precision whose keys become infinities in the cache."""
+    rng = np.random.default_rng(43)
+    p = Problem(rng, [90], [20], heads=8, kv_heads=2, head_dim=64, kinds=kinds)
+    put(p, [(0, 25, 0, 9, np.float32(1e5)), (0, 60, 1, 33, np.float32(-3e30))])
+    run(p)
+
+
+@pytest.mark.parametrize("kinds", KINDS, ids="-".join)
 def test_every_score_is_infinite(hip, kinds):
     """A row that has no weight left has no result, wherever its keys are; zeros times infinities are no numbers."""
     import torch
