@@ -58,6 +58,7 @@ struct Cell;
 template <>
 struct Cell<kAttnF32> {
   typedef float T;
+  static constexpr float kLift = 0.f;
 };
 template <>
 struct Cell<kAttnF16> {
@@ -237,6 +238,9 @@ struct Sight {
 
 // How far a row's maximum may grow, in powers of two, before its sums are scaled.
 constexpr float kSlack = 6.f;
+// Exponents from here on are off by one half and more, as products with the row's factor are rounded, and more than f16 has
+// room for beside the slack; from 2^31 on by more than fp32 has.
+constexpr float kMostExponent = 0x1p22f;
 
 // Sums of 32 rows over the keys so far: y holds rows 32 b + 8 (i / 4) + 4 (lane / 32) + i % 4 of Y^T, column lane % 32.
 template <int DP>
@@ -282,8 +286,10 @@ struct RowSums {
       const float next = fmaxf(reference, top);
       // a row that has seen nothing has nothing to scale (and no reference)
       const float scale = next == reference ? 1.f : __builtin_amdgcn_exp2f(reference - next);
-      reference = next;
       sum *= scale;
+      // such a row is formed anew in the end (whole_row)
+      if (next != reference && fabsf(next) >= kMostExponent) sum = __builtin_nanf("");
+      reference = next;
 #pragma unroll
       for (int b = 0; b < DP / 32; ++b) y[b] *= scale;
     }
@@ -496,7 +502,7 @@ struct RowTile {
 template <typename Row, int DP>
 struct RowTile<kAttnF32, Row, DP> {
   typedef TileLayout<4, DP> L;
-  static constexpr int N = 1, kSteps = DP / 8, kBlocks = DP / 32;
+  static constexpr int kSteps = DP / 8, kBlocks = DP / 32;
   floatx4 q[kSteps];  // elements 8 s + 4 (lane / 32) + 0..3
   RowSums<DP> sums;
   float factor;
@@ -547,7 +553,7 @@ struct RowTile<kAttnF32, Row, DP> {
   template <int KB>
   __device__ __forceinline__ void softmax(Work<KB>& w, bool masked, const uint32_t (&sight)[KB]) {
     if (masked) mask_scores(w.s, sight, half);
-    sums.softmax(w.s, factor, 0.f);
+    sums.softmax(w.s, factor, Cell<kAttnF32>::kLift);
   }
   template <int KB>
   __device__ __forceinline__ void add(const Work<KB>& w, uint32_t lds_v) {
@@ -642,11 +648,15 @@ struct ItemRows {
   }
 };
 
-// Row m of a tile of ROWS by its definition, by one wavefront.  Parts of q are of either sign or zero, so that their products
-// with a key's infinity make no number of a score that is -inf and has no weight; and an element next to the end of fp32 has a
-// first part that is infinite.  A row whose sum is no number is formed anew here, in fp32, with products of whole elements:
-// twice over its keys, for the largest score and for the sums, or as far as a score that is +inf or no number.  (5000 tokens,
-// 32 heads of 128, one infinite key: 25 ms in place of 0.43.  A mend of the scores within the loop would cost every call.)
+// Row m of a tile of ROWS by its definition, by one wavefront: a row whose sum is no number is formed anew here, in fp32, with
+// products of whole elements and differences of scores before all else, twice over its keys: for the largest score and for
+// the sums, or as far as a score that is +inf or no number.  Such rows are those of
+//   parts of q, which are of either sign or zero, so that their products with a key's infinity make no number of a score that
+//   is -inf and has no weight; an element next to the end of fp32 has a first part that is infinite;
+//   exponents from kMostExponent on;
+//   and those that are no numbers by the definition.
+// (5000 tokens, 32 heads of 128 in fp32 over f16, one infinite key: 25 ms in place of 0.43.  A mend within the loop would cost
+// every call.)
 // tree: the ancestors of the item's tokens in LDS, null where they are in the workspace.
 template <int TYPE, typename Row, int DP, int ROWS>
 __device__ __forceinline__ void whole_row(const AttnPlan& p, const AttnCall& c, const AttnItem& it, int kv_head, int m,
@@ -673,7 +683,7 @@ __device__ __forceinline__ void whole_row(const AttnPlan& p, const AttnCall& c, 
     float v = 0.f;
 #pragma unroll 1
     for (int d = 0; d < p.head_dim; d += 8) {
-      const float8 a = *reinterpret_cast<const float8*>(q + d);
+      const float8 a = __builtin_convertvector(*reinterpret_cast<const attn_eight<Row>*>(q + d), float8);
       const float8 b = __builtin_convertvector(*reinterpret_cast<const attn_eight<T>*>(key + d), float8);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v = fmaf(a[i], b[i], v);
@@ -684,7 +694,7 @@ __device__ __forceinline__ void whole_row(const AttnPlan& p, const AttnCall& c, 
   floatx4 y{};
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
-    const float shift = Cell<TYPE>::kLift - (reference == -__builtin_inff() ? 0.f : reference);
+    const float least = reference == -__builtin_inff() ? 0.f : reference;
     for (int base = it.key0; base < it.key1; base += 64) {
       const float v = score(base);
       if (pass == 0) {
@@ -693,7 +703,7 @@ __device__ __forceinline__ void whole_row(const AttnPlan& p, const AttnCall& c, 
         sum = __builtin_nanf("");
         break;
       }
-      const float weight = __builtin_amdgcn_exp2f(v + shift);
+      const float weight = __builtin_amdgcn_exp2f(v - least + Cell<TYPE>::kLift);
       sum += weight;
       floatx4 some{};  // of 64 keys, then of all: no long chains
       for (uint64_t left = __ballot(sees(base)); left; left &= left - 1) {
@@ -817,7 +827,7 @@ __device__ __forceinline__ void shared_item(const AttnPlan& p, const AttnCall& c
   const float sum = half_pair_sum(tile.sums.sum);
   // made again, so that the loop's registers need not hold it
   const ItemRows<Row> rows(p, it, m0, (int)opaque((uint32_t)lane));
-  const bool again = Tile::N > 1 && rows.real && sum != sum;
+  const bool again = rows.real && sum != sum;
   if (!rows.real || again) {
   } else if (it.part < 0) {
     const float scale = 1.f / sum;
@@ -839,11 +849,10 @@ __device__ __forceinline__ void shared_item(const AttnPlan& p, const AttnCall& c
       for (int i = 0; i < 4; ++i)
         *reinterpret_cast<floatx4*>(y + 32 * b + 8 * i + 4 * tile.half) = tile.sums.piece(b, i, tile.half);
   }
-  if constexpr (Tile::N > 1)
-    for (uint32_t left = (uint32_t)__ballot(again); left; left &= left - 1) {
-      const AttnArgs& args = args_again();
-      whole_row<TYPE, Row, DP, 32 * WAVES>(args.p, args.c, it, kv_head, m0 + __builtin_ctz(left), nullptr);
-    }
+  for (uint32_t left = (uint32_t)__ballot(again); left; left &= left - 1) {
+    const AttnArgs& args = args_again();
+    whole_row<TYPE, Row, DP, 32 * WAVES>(args.p, args.c, it, kv_head, m0 + __builtin_ctz(left), nullptr);
+  }
 }
 
 template <int TYPE, typename Row, int DP, int WAVES, int KT>
@@ -1132,7 +1141,7 @@ __device__ __forceinline__ bool split_item(const AttnPlan& p, const AttnCall& c,
       total += weight * ml[w * 64 + 32 + r];
       v += weight * *reinterpret_cast<const floatx4*>(lds + w * M::kWave + (r * M::kRow + d) * 4);
     }
-    if (Tile::N > 1 && total != total) {  // formed anew below (a row's threads are one wavefront's)
+    if (total != total) {  // formed anew below (a row's threads are one wavefront's)
       again |= 1u << r;
       continue;
     }
@@ -1147,14 +1156,12 @@ __device__ __forceinline__ bool split_item(const AttnPlan& p, const AttnCall& c,
       *reinterpret_cast<floatx4*>(p.part_y + row * DP + d) = v;
     }
   }
-  if constexpr (Tile::N > 1) {
-    if (__builtin_expect(__ballot(again != 0) != 0, 0))
-      for (int r = 0; r < count; ++r) {
-        if (!__ballot(again >> r & 1)) continue;
-        const AttnArgs& args = args_again();
-        whole_row<TYPE, Row, DP, 32>(args.p, args.c, it, kv_head, it.m0 + r, cut.few ? few.tree[0] : nullptr);
-      }
-  }
+  if (__builtin_expect(__ballot(again != 0) != 0, 0))
+    for (int r = 0; r < count; ++r) {
+      if (!__ballot(again >> r & 1)) continue;
+      const AttnArgs& args = args_again();
+      whole_row<TYPE, Row, DP, 32>(args.p, args.c, it, kv_head, it.m0 + r, cut.few ? few.tree[0] : nullptr);
+    }
   return true;
 }
 
