@@ -550,7 +550,8 @@ enum {                          /* GGML's tags */
  * throughout; rows in 16 bits have their probabilities rounded to that type.  Values
  * that are infinite or NaN reach only the rows that see them (as either).  Keys that are
  * infinite give scores: one of -inf has no weight, and a row with one of +inf, one that is no
- * number, or none above -inf is NaN.
+ * number, or none above -inf is NaN.  (Finite values of 2^100 and more may overflow in sums that
+ * are divided at the end.)
  *
  * The cache is a pool of pages, key_pages and value_pages [layers][pages][kv_heads]
  * [page_tokens][head_dim]; position j of sequence i is row j % page_tokens of page

@@ -419,7 +419,11 @@ struct RowTile {
         factor = scale_log2;
       }
     } else {
-      factor = scale_log2;
+      // rows of less than 2^-64 times 2^64: the third part of a number below 2^-110 would be next to nothing
+      top = half_pair_max(top);
+      const bool small = top < 0x1p-64f;
+      lift = small ? 0x1p64f : 1.f;
+      factor = small ? scale_log2 * 0x1p-64f : scale_log2;
     }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {

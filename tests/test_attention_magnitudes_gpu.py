@@ -103,3 +103,22 @@ def test_scores_rise_from_far_below(hip, kinds, rows):
     p.k[...] = -np.abs(p.k) - np.ldexp(np.float32(1), 10)
     p.k[-1] = 0  # the last row has two
     check(p)
+
+
+@pytest.mark.parametrize("kinds", [("f32", "bf16"), ("f32", "f32")], ids="-".join)
+@pytest.mark.parametrize("q_size, k_size", [(3e38, 3e-38), (1e30, 1e-30), (1e-30, 1e30), (1e-36, 1e36), (1e-38, 3e37)])
+@pytest.mark.parametrize("rows", [9, 150])
+def test_small_rows_of_large_keys(hip, kinds, q_size, k_size, rows):
+    """Scores next to one, of queries and keys that are next to the ends of the type."""
+    import torch
+    rng = np.random.default_rng(53)
+    p = Problem(rng, [rows, 1], [70, 300], heads=4, kv_heads=2, kinds=kinds)
+    p.q = (np.clip(p.q / 6, -1, 1) * np.float32(q_size)).astype(np.float32)
+    p.k, p.keys = (ref.rounded(a * np.float32(k_size), kind) for a, kind in ((p.k, "f32"), (p.keys, kinds[1])))
+    for t, a in ((p.d[0], p.q), (p.d[1], p.k), (p.d_keys, p.keys)):
+        t.copy_(torch.from_numpy(a.reshape(t.shape)).to(t.dtype))
+    torch.cuda.synchronize()
+    session = p.open()
+    p.call(session)
+    session.sync()
+    p.check()
