@@ -116,8 +116,20 @@ class HipAttentionSession:
             raise HipBackendError(f"HIP attention {what} has {a.size} elements, not rows of {width}.")
         return a.reshape(-1, heads, self.layout.head_dim)
 
+    @staticmethod
+    def _whole(a, what: str, used: Optional[int] = None) -> np.ndarray:
+        """Whole numbers as int32; the first `used` (all, if None) have to fit it, the others are not read."""
+        a = np.asarray(a).reshape(-1)
+        if a.size and a.dtype.kind not in "iu":
+            raise HipBackendError(f"HIP attention {what} must be whole numbers, not {a.dtype}.")
+        ends = np.iinfo(np.int32)
+        far = (a[:used] < ends.min) | (a[:used] > ends.max)
+        if far.any():
+            raise HipBackendError(f"HIP attention {what} holds {a[:used][far][0]}, which does not fit 32 bits.")
+        return np.ascontiguousarray(a, dtype=np.int32)
+
     def _table(self, table: Sequence[int], positions: int) -> np.ndarray:
-        t = np.ascontiguousarray(table, dtype=np.int32).reshape(-1)
+        t = self._whole(table, "table", -(-max(positions, 0) // self.page_tokens))
         if positions > t.size * self.page_tokens:
             raise HipBackendError(f"HIP attention table of {t.size} pages does not hold {positions} tokens.")
         return t
@@ -134,7 +146,7 @@ class HipAttentionSession:
         t = self._table(table, context + len(q))
         p = None
         if parents is not None:
-            p = np.ascontiguousarray(parents, dtype=np.int32).reshape(-1)
+            p = self._whole(parents, "parents")
             if p.size != len(q):
                 raise HipBackendError(f"HIP attention has {p.size} parents of {len(q)} rows.")
         y = np.empty_like(q)
