@@ -49,7 +49,7 @@ class HipAttentionSession:
         for t in (layout.row_type, layout.cache_type):
             if t not in TYPE_TAGS:
                 raise HipBackendError(f"HIP attention has no type {t!r}; they are {', '.join(TYPE_TAGS)}.")
-        if layout.scale is not None and not layout.scale > 0:
+        if layout.scale is not None and not np.float32(layout.scale) > 0:  # 0 is the default's
             raise HipBackendError(f"HIP attention scale {layout.scale} is not positive.")
         d = native.AttentionDesc()
         d.heads, d.kv_heads, d.head_dim = layout.heads, layout.kv_heads, layout.head_dim

@@ -56,3 +56,9 @@ def test_lists_that_fit(session):
     assert session._table([], 0).size == 0
     with pytest.raises(HipBackendError, match="closed"):
         session.run(*ROWS, np.array([0, 1], np.int64), parents=np.array([-1, 0], np.int16))
+
+
+def test_a_scale_that_is_zero_in_single_precision():
+    """It would be taken for the default."""
+    with pytest.raises(HipBackendError, match="scale 1e-60 is not positive"):
+        HipAttentionSession(AttentionLayout(4, 2, 16, scale=1e-60), pages=1, max_context=16)
