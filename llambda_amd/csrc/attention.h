@@ -127,6 +127,11 @@ AttnSizes attn_sizes(const AttnPlan& p);
 constexpr int attn_shared_keys(int padded, int row_bytes) {
   return row_bytes == 2 && padded == 64 ? 128 : row_bytes == 4 && padded == 256 ? 32 : 64;
 }
+// Wavefronts that share a tile of keys: eight, two to a SIMD, where rows, sums and probabilities fit 256 registers.  A tile has
+// 32 rows for each, so that the plan and the kernels have to agree.
+constexpr int attn_shared_waves(int cache_type, int row_bytes, int padded) {
+  return padded == 256 || (cache_type == kAttnBF16 && row_bytes == 4 && padded == 128) ? 4 : 8;
+}
 inline int attn_padded(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 inline int attn_table_width(const AttnPlan& p) { return (p.max_context + (1 << p.page_shift) - 1) >> p.page_shift; }
 

@@ -416,11 +416,6 @@ __global__ void attn_take_error_kernel(int* error) {
 // ------------------------------------------------------------------------ host
 
 constexpr int kCus = 256;
-static int shared_waves(const AttnPlan& p) {
-  const int padded = attn_padded(p.head_dim);
-  return padded == 256 || (p.cache_type == kAttnBF16 && p.row_type == kAttnF32 && padded == 128) ? 4 : 8;
-}
-
 // Rows of a kv head in a sequence, on average, up to which waves share rows and not keys: those of two wavefronts, for
 // with fewer than three of eight at work the other kernel loses more than reading the keys for each 32 rows costs (us, 16
 // trees behind 2000 tokens, 8 kv heads of 128, fp32 rows over f16: 32 rows 53 against 69, 64 rows 68 and 72, 80 rows 86
@@ -430,14 +425,15 @@ static int shared_waves(const AttnPlan& p) {
 constexpr int kFewRows = 64, kFewRowsAlone = 160;
 
 static AttnCut cut_as(const AttnPlan& p, bool shared) {
+  const int padded = attn_padded(p.head_dim), row_bytes = p.row_type == kAttnF32 ? 4 : 2;
   AttnCut cut{};
   cut.shared = shared;
-  cut.rows = shared ? 32 * shared_waves(p) : 32;
+  cut.rows = shared ? 32 * attn_shared_waves(p.cache_type, row_bytes, padded) : 32;
   // A unit is a tile of keys (two, where it has 32), or two for each wavefront (a step of one sequence 20 us, with twice as many 22, a tree of 26
   // nodes 35 and 38).  What else a tile costs, about 8 us to load its rows, to fill the pipeline and to store, is taken for
   // some of them: (us for 2, 3, 4 and 5) prompts of 2311 tokens over f16 145, 129, 120, 126; 12 of 2000, heads of 256 and
   // fp32 rows, whose units take twice as long, 105, 98, 106, 107; 1501 tokens in fp32, four times, 124, 131, 131, 138.
-  const int keys = attn_shared_keys(attn_padded(p.head_dim), p.row_type == kAttnF32 ? 4 : 2);
+  const int keys = attn_shared_keys(padded, row_bytes);
   cut.unit_log2 = !shared ? 8 : keys == 128 ? 7 : 6;
   cut.overhead = !shared || p.cache_type == kAttnF32 || keys == 128 ? 2 : keys == 32 ? 3 : 4;
   cut.shares = std::max(1, kCus / p.kv_heads);

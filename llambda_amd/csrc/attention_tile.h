@@ -1234,11 +1234,6 @@ hipError_t attn_launch(Kernel k, uint32_t grid, int threads, int lds, hipStream_
   return hipGetLastError();
 }
 
-// Waves of a workgroup that share tiles: eight, two to a SIMD, where rows, sums and probabilities fit 256 registers.
-template <int TYPE, typename Row, int DP>
-constexpr int attn_shared_waves() {
-  return DP == 256 || (TYPE == kAttnBF16 && sizeof(Row) == 4 && DP == 128) ? 4 : 8;
-}
 // Waves that split keys: what LDS holds of their tiles.
 template <int TYPE, int DP>
 constexpr int attn_split_waves() {
@@ -1248,7 +1243,7 @@ constexpr int attn_split_waves() {
 template <int TYPE, typename Row, int DP>
 hipError_t attn_attend(const AttnPlan& p, const AttnCall& c, const AttnCut& cut, uint32_t grid, hipStream_t s) {
   if (cut.shared) {
-    constexpr int W = attn_shared_waves<TYPE, Row, DP>(), KT = attn_shared_keys(DP, sizeof(Row));
+    constexpr int W = attn_shared_waves(TYPE, sizeof(Row), DP), KT = attn_shared_keys(DP, sizeof(Row));
     return attn_launch(attn_shared_kernel<TYPE, Row, DP, W, KT>, grid, 64 * W,
                        4 * KT * DP * attn_cell_bytes<TYPE>() + Spoiled<attn_cell_bytes<TYPE>(), DP, KT>::kBytes, s, p, c, cut);
   }
