@@ -195,26 +195,13 @@ struct TileLoader {
     for (int j = 0; j < kLoads / STEP; ++j) {
       const int i = from + j * STEP, r0 = i * R;
       uint32_t source = 16 * (piece ^ (VALUES ? L::value_swizzle(r0 + row) : L::key_swizzle(r0 + row)));
-      // a row shorter than the tile's: its first piece again (a key's becomes zeros, a value's y is not stored)
+      // a row shorter than the tile's: its first piece again (the row's q has zeros there, its y is not stored; rows whose
+      // zeros meet an infinite key come to whole_row)
       if (source >= bytes) source = 0;
       const uint32_t pos = min(base + r0, last & ~(R - 1));
       const uint32_t page = __builtin_amdgcn_readlane(pages, r0 / kApart);
       load_lds16((VALUES ? values : keys) + (uint64_t)page * page_bytes + (pos & in_page) * bytes, row * bytes + source,
                  to + 1024u * i);
-    }
-  }
-  // Zeros behind the elements of the keys that load<false, STEP> brought to LDS at `tile` for this wavefront, where rows are
-  // shorter than the tile's: their products with q's zeros have to be zeros whatever the keys hold.
-  template <int STEP>
-  __device__ __forceinline__ void clear_padding(uint8_t* tile, int from, int lane) const {
-    if (head_dim == DP) return;
-    asm volatile("" : "+v"(lane));  // so that no register holds for every tile what depends on it
-    const int row = lane / L::kPieces, piece = lane % L::kPieces;
-#pragma unroll
-    for (int j = 0; j < kLoads / STEP; ++j) {
-      const int i = from + j * STEP;
-      if (16 * (piece ^ L::key_swizzle(i * L::kRowsPerLoad + row)) >= head_dim * SIZE)
-        *reinterpret_cast<u32x4*>(tile + 1024 * i + 16 * lane) = u32x4{};
     }
   }
 };
@@ -657,9 +644,11 @@ struct ItemRows {
 // the sums, or as far as a score that is +inf or no number.  Such rows are those of
 //   parts of q, which are of either sign or zero, so that their products with a key's infinity make no number of a score that
 //   is -inf and has no weight; an element next to the end of fp32 has a first part that is infinite;
+//   heads narrower than their tile, whose zeros behind q meet a key's infinity (zeros behind the keys instead, written by
+//   each wavefront behind its loads, took steps at width 80 from 53 to 60 us and at 192 from 135 to 163);
 //   exponents from kMostExponent on;
 //   and those that are no numbers by the definition.
-// (5000 tokens, 32 heads of 128 in fp32 over f16, one infinite key: 25 ms in place of 0.43.  A mend within the loop would cost
+// (5000 tokens, 32 heads of 128 in fp32 over f16, one infinite key: 25 ms in place of 0.43; a mend within the loop would cost
 // every call.)
 // tree: the ancestors of the item's tokens in LDS, null where they are in the workspace.
 template <int TYPE, typename Row, int DP, int ROWS>
@@ -773,11 +762,6 @@ __device__ __forceinline__ void shared_item(const AttnPlan& p, const AttnCall& c
     pages = next_pages;
     next_pages = pages_of(t + 2);
   };
-  // this wavefront's loads have ended, those of tile t's keys among them
-  auto wait = [&](int t) {
-    wait_loads<0>();
-    if (t < tiles) loader.template clear_padding<WAVES>(lds + (keys_at(t) - base), wave, lane);
-  };
   // after the loads of tile t's values have ended, before they are read
   auto look = [&](int t) {
     if (t >= tiles || key_of(t) + KT <= all_sure) return;
@@ -796,7 +780,7 @@ __device__ __forceinline__ void shared_item(const AttnPlan& p, const AttnCall& c
   typename Tile::Raw raw;
   Tile::fetch(raw, ItemRows<Row>(p, it, m0, lane).q(p, c, it, kv_head), p.head_dim, lane);
   tile.start(raw, p.scale * kAttnLog2e, lane);
-  wait(0);
+  wait_loads<0>();
   barrier();
   // Two phases a tile: products (of the probabilities before and of this tile's scores), then the softmax.  Waves 4 to
   // 7, which share the SIMDs of waves 0 to 3, are a phase behind, so that one's products run beside the other's softmax.
@@ -811,7 +795,7 @@ __device__ __forceinline__ void shared_item(const AttnPlan& p, const AttnCall& c
       if (t > 0) tile.add(work, values_at(t - 1));
       if (t < tiles) tile.scores(work, keys_at(t));
     }
-    if (behind) wait(t + 1);
+    if (behind) wait_loads<0>();
     barrier();
     if (behind) {
       look(t);
@@ -823,7 +807,7 @@ __device__ __forceinline__ void shared_item(const AttnPlan& p, const AttnCall& c
       if (partly) see_tile(key_of(t), see);
       tile.softmax(work, partly, see);
     }
-    if (!behind) wait(t + 1);
+    if (!behind) wait_loads<0>();
     barrier();
     if (!behind) look(t);
   }
@@ -1095,7 +1079,6 @@ __device__ __forceinline__ bool split_item(const AttnPlan& p, const AttnCall& c,
         wait_loads<0>();
       }
       const uint32_t now = base + (t & 1) * 2 * M::kTile;
-      loader.template clear_padding<1>(lds + (now - lds_base), 0, lane);
       uint32_t see[1] = {};
       const bool partly = key + KT > sure;
       if (partly) {
