@@ -15,15 +15,13 @@
 #include "attention_cut.h"
 
 #include <algorithm>
-#include <climits>
+#include <cstdint>
 
 #include "mfma.h"
 
 namespace llhip {
 
 constexpr int kPlanThreads = 256;
-typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
-typedef float float8_t __attribute__((ext_vector_type(8)));
 
 static __host__ __device__ __forceinline__ int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
@@ -429,9 +427,9 @@ static AttnCut cut_as(const AttnPlan& p, bool shared) {
   AttnCut cut{};
   cut.shared = shared;
   cut.rows = shared ? 32 * attn_shared_waves(p.cache_type, row_bytes, padded) : 32;
-  // A unit is a tile of keys (two, where it has 32), or two for each wavefront (a step of one sequence 20 us, with twice as many 22, a tree of 26
-  // nodes 35 and 38).  What else a tile costs, about 8 us to load its rows, to fill the pipeline and to store, is taken for
-  // some of them: (us for 2, 3, 4 and 5) prompts of 2311 tokens over f16 145, 129, 120, 126; 12 of 2000, heads of 256 and
+  // A unit is a tile of keys (two, where it has 32), or two for each wavefront (a step of one sequence 20 us, with twice
+  // as many 22, a tree of 26 nodes 35 and 38).  What else a tile costs, about 8 us to load its rows, to fill the pipeline
+  // and to store, is taken for some of them: (us for 2, 3, 4 and 5) prompts of 2311 tokens over f16 145, 129, 120, 126; 12 of 2000, heads of 256 and
   // fp32 rows, whose units take twice as long, 105, 98, 106, 107; 1501 tokens in fp32, four times, 124, 131, 131, 138.
   const int keys = attn_shared_keys(padded, row_bytes);
   cut.unit_log2 = !shared ? 8 : keys == 128 ? 7 : 6;
@@ -530,7 +528,8 @@ hipError_t attn_run_launch(const AttnPlan& p, const AttnCall& c, hipStream_t s) 
 }
 
 hipError_t attn_accept_launch(const AttnPlan& p, const AttnAccept& a, hipStream_t s) {
-  const dim3 grid(a.sequences, p.layers, (2 * p.kv_heads * p.head_dim * (p.cache_type == kAttnF32 ? 4 : 2) + 16 * kPlanThreads - 1) / (16 * kPlanThreads));
+  const int bytes = 2 * p.kv_heads * p.head_dim * (p.cache_type == kAttnF32 ? 4 : 2);
+  const dim3 grid(a.sequences, p.layers, ceil_div(bytes, 16 * kPlanThreads));
   if (p.cache_type == kAttnF32) hipLaunchKernelGGL(attn_accept_kernel<float>, grid, dim3(kPlanThreads), 0, s, p, a);
   else hipLaunchKernelGGL(attn_accept_kernel<uint16_t>, grid, dim3(kPlanThreads), 0, s, p, a);
   return hipGetLastError();

@@ -40,9 +40,7 @@ namespace llhip {
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
-typedef _Float16 halfx4 __attribute__((ext_vector_type(4)));
 typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) const uint8_t* lds_bytes;
 __device__ __forceinline__ lds_bytes lds_at(uint32_t address) { return reinterpret_cast<lds_bytes>(address); }
 

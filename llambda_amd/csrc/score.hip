@@ -12,8 +12,6 @@
 // row: 16 of them with a barrier between took 15 us for one row and 43 for 2048.
 #include "score.h"
 
-#include <cfloat>
-
 #include "mfma.h"
 
 namespace llhip {
