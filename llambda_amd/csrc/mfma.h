@@ -140,10 +140,13 @@ __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+// A wavefront-uniform pointer in scalar registers.  A load that takes its address from a scalar must come five wait states
+// behind the vector instruction that wrote it; the compiler does not see the loads above, so the wait is here.
 __device__ __forceinline__ const uint8_t* uniform_ptr(const uint8_t* p) {
   const uint64_t v = reinterpret_cast<uint64_t>(p);
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
-  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+  uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
+  uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+  asm("s_nop 4" : "+s"(lo), "+s"(hi));
   return reinterpret_cast<const uint8_t*>(((uint64_t)hi << 32) | lo);
 }
 
