@@ -86,7 +86,7 @@ class HipAttentionSession:
                    table_stride: int = 0, stream: int = 0) -> None:
         """Sequence i's rows [offsets[i], offsets[i + 1]) behind context[i] cached tokens (int32 lists
         on the device); no offsets: one row each.  parents: the rows are trees.  Strides in elements,
-        0 = dense."""
+        0 = dense.  Next tokens of many sequences and long prompts are faster in calls of their own."""
         rows = native.AttentionRows(q_ptr or None, k_ptr or None, v_ptr or None, output_ptr or None,
                                     q_stride, k_stride, v_stride, output_stride)
         batch = native.AttentionBatch(tokens, sequences, offsets_ptr or None, context_ptr or None,

@@ -10,8 +10,8 @@
 // attend kernel does the shares; the join adds up the parts of tiles that lie in
 // several.  A call of few rows has no first launch (attention_tile.h), and so a step
 // of one sequence is two: 13 + 5 us behind 4096 tokens, bound by latency.  Around the
-// 97 us of attending 2311 tokens of prompts lie 9 of preparing and 13 of joining;
-// moving the accepted nodes of 16 trees takes 4.5.
+// 97 us of attending 2311 tokens of prompts lie 9 of preparing and 10 of joining;
+// moving the accepted nodes of 16 trees takes 4.5.  (Averages; the least are a few percent below.)
 #include "attention_cut.h"
 
 #include <algorithm>

@@ -23,12 +23,15 @@
 // Two kernels.  Where a sequence has many rows, eight wavefronts with 32 rows each
 // share every tile (attn_shared_kernel): a tile's bytes serve 256 rows, and the two
 // wavefronts of a SIMD are a phase apart, one's products beside the other's softmax
-// (8192 tokens 1014 us, all in step 1105).  Bound by the products: those 8192 tokens,
-// 32 heads of 128, fp32 rows over f16, are 550 GFLOP in two parts, in 955 to 1015 us
-// 1080 to 1150 TFLOP/s of products, next to 1070 of a large library product of f16
-// (random operands hold the card to about 1500 from registers alone); 6000 tokens of
-// bf16, one part, 360 to 395 us or 750 to 820 TFLOP/s, for there the softmax weighs as
-// much.  Where a sequence has few rows, wavefronts share 32 of them and take a tile of
+// (8192 tokens 1014 us, all in step 1105).  Those 8192 tokens, 32 heads of 128, fp32
+// rows over f16, are 550 GFLOP in two parts, in 940 to 1015 us 1080 to 1170 TFLOP/s of
+// products, next to 1070 of a large library product of f16 (random operands hold the
+// card to about 1500 from registers alone): the matrix pipes are busy in 66% of the
+// cycles that wavefronts live, the VALU in 45%.  6000 tokens of bf16, one part, take
+// 357 to 395 us or 750 to 830 TFLOP/s, 43% and 45%: each fragment of 1 KB feeds one
+// product of 32 cycles there, so that the four SIMDs ask the LDS for all of its 128
+// bytes a cycle.  1501 tokens in fp32, 70% and 15%, read fragments where they are
+// needed.  Where a sequence has few rows, wavefronts share 32 of them and take a tile of
 // keys each (attn_split_kernel), so that the keys' way through the device is all that
 // counts: a step of 48 sequences, 614 MB, in 125 us, 4.9 TB/s (a large copy 5.1).
 #pragma once

@@ -8,7 +8,7 @@
 // leaves more than 64 (equal logits, or neighbours in one lane), the exact `top`
 // first are chosen instead.  score_row_kernel joins a row's chunks in 64 bits.
 // The first kernel is bound by the logits' traffic: 2048 rows of 128256, 1.05 GB, in
-// 190 us, 5.5 TB/s (the second 6.5); one row by latency, 6 + 8 us.  A wavefront joins a
+// 193 us, 5.4 TB/s, or 225 after a pause (the second 6.5); one row by latency, 6 + 8 us.  A wavefront joins a
 // row: 16 of them with a barrier between took 15 us for one row and 43 for 2048.
 #include "score.h"
 
