@@ -591,6 +591,7 @@ struct AttnArgs {
   AttnPlan p;
   AttnCall c;
 };
+static_assert(sizeof(AttnPlan) % alignof(AttnCall) == 0, "arguments follow each other as a struct's members do");
 __device__ __forceinline__ const AttnArgs& args_again() {
   typedef const __attribute__((address_space(4))) AttnArgs* Args;
   Args a = (Args)__builtin_amdgcn_kernarg_segment_ptr();
